@@ -415,7 +415,8 @@ int musapy_reduce_fused_noalloc_v1(int op, int dtype, const void* a, void* c, in
  * per-tile length reaches 2^31 elements (pass more tiles), 3 ndim outside [0, 32] or an axis
  * outside [0, ndim) (32 is the reference's MUSAPY_MAX_NDIM), 4 a cumsum with 2^32 or more rows
  * (or a dimension outside the scanned axis of 2^32 or more), 5 a no-alloc reduction whose slots
- * need more than the library's static scratch.  A wrapper that reports an error launches
+ * need more than the library's static scratch, 6 an argument of a gated recurrent block's operator that is
+ * out of range.  A wrapper that reports an error launches
  * nothing. */
 int musapy_kernels_take_error(void);
 
@@ -431,7 +432,7 @@ int musapy_kernels_take_error(void);
  * and a workspace here belongs to one stream, so a fault is reported to that stream only.
  * musapy_kernels_take_fault_ws(workspace, bytes, stream): call after synchronizing `stream` (the
  * stream the workspace's launches ran on); reads the fault word on `stream` and returns 0 (no
- * fault), a bit set of 1 (a reduction combiner gave up) and 2 (a scan wait gave up), or -1 on a
+ * fault), a bit set of 1 (a reduction combiner gave up), 2 (a scan wait gave up) and 4 (a gated scan's gave up), or -1 on a
  * HIP error.  A fault also zeroes the whole workspace (payload and word) on `stream` and waits
  * for that, since a block that published after its combiner gave up may have left a slot
  * behind; the workspace is then ready for reuse.
@@ -443,6 +444,116 @@ int musapy_kernels_take_error(void);
 int musapy_kernels_take_fault_ws(void* workspace, size_t workspace_bytes, hipStream_t stream);
 int musapy_kernels_take_fault(int device);
 uint32_t musapy_kernels_set_spin_limit(uint32_t polls);
+
+/* ---- operators of a gated recurrent block (new; no counterpart in kernels.rs) ----
+ * Element types are MUSAPY_DT_F32, _F16 or _BF16; all arithmetic and every carried state is f32 and
+ * a result is rounded once, when it is stored.  Strides are in elements and may be 0 or negative.
+ * Every entry point returns 0 when its work was launched (or there was none), -1 when an argument
+ * is out of range (wrapper error 6) or scratch is missing (wrapper error 1); nothing is launched
+ * then.
+ *
+ * Gated scan along `axis`, t = 0 .. shape[axis] - 1, each lane (coordinate of the other axes) on its own:
+ *   MUSAPY_SCAN_DECAY  h[t] = g[t] h[t-1] + x[t]
+ *   MUSAPY_SCAN_BLEND  h[t] = s h[t-1] + (1 - s) x[t], s = sigmoid(g[t])
+ * h[-1] is `first` (zeros when NULL), and counts as 0 at every t whose `reset` byte is not 0,
+ * whatever it holds.  Gates are finite; a gate that is not may give NaN where a step-by-step
+ * evaluation gives an infinity.  `last` receives h at the last step in f32 (`first` itself when the
+ * axis is empty); it may be NULL.
+ *
+ * Its gradient, from dh, dlast (the gradient of `last`; zeros when NULL), x, gate, h and first:
+ *   G[t] = dh[t] + c[t+1], c[t] = a[t] G[t] (0 at a reset), c[end] = dlast, with a = g or s
+ *   decay: dx = G, dgate = G h[t-1];   blend: dx = (1 - s) G, dgate = G (h[t-1] - x) s (1 - s)
+ * `last` receives c[0], the gradient of `first`; it may be NULL.  x is not read by DECAY and may be
+ * NULL there.
+ *
+ * x, gate, reset, h (grad) and dh are strided views of `shape` (stride 0 where one is broadcast);
+ * first, last and dlast are C-contiguous over the shape without `axis`; `out` (h, or dx) is
+ * C-contiguous over `shape`.  dgate is C-contiguous over `shape` in `dgate_dtype` (gate_dtype or
+ * F32) when `parts` is 0.  Where the gate is shared along the last axis (gate stride 0, last axis
+ * not `axis`), `parts` may be musapy_gated_scan_parts_v1(args): dgate is then f32 over `shape` with
+ * the last extent replaced by `parts`, and the sum over that extent is the shared gate's gradient.
+ *
+ * `scratch` (musapy_gated_scan_scratch_v1(args, grad) bytes, any contents, 8-byte aligned) holds the hand-over
+ * words of scans whose steps are split over workgroups; such a scan waits, bounded as the cumsum's
+ * look-back is, and reports an expired wait to the fault word of `workspace` (bit 4). */
+enum { MUSAPY_SCAN_DECAY = 0, MUSAPY_SCAN_BLEND = 1 };
+typedef struct {
+  int kind, dtype, gate_dtype, dgate_dtype;
+  int ndim, axis;
+  const size_t* shape;
+  const void* x;
+  const ssize_t* x_strides;
+  const void* gate;
+  const ssize_t* gate_strides;
+  const uint8_t* reset; /* NULL: none */
+  const ssize_t* reset_strides;
+  const void* h; /* grad only */
+  const ssize_t* h_strides;
+  const void* dh; /* grad only */
+  const ssize_t* dh_strides;
+  const float* first;
+  const float* dlast; /* grad only */
+  void* out;
+  void* dgate; /* grad only */
+  float* last;
+  size_t parts; /* grad only */
+} musapy_gated_scan_args;
+size_t musapy_gated_scan_scratch_v1(const musapy_gated_scan_args* args, int grad);
+size_t musapy_gated_scan_parts_v1(const musapy_gated_scan_args* args);
+int musapy_gated_scan_v1(const musapy_gated_scan_args* args, void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes, hipStream_t stream);
+int musapy_gated_scan_grad_v1(const musapy_gated_scan_args* args, void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Norms before and after a block, with its gate, dropout and residual scale, over rows of `width`:
+ *   n1 = norm(x), u = n1 post_weight, v = u act(gate), d = dropout(v), r = residual + scale d,
+ *   n2 = norm(r), y = n2 pre_weight
+ * norm is MUSAPY_NORM_RMS  v / sqrt(mean(v^2) + eps), MUSAPY_NORM_LAYER (v less its mean first) or
+ * MUSAPY_NORM_NONE (post: n1 = x; pre: no y).  act is the identity (gate NULL), MUSAPY_GATE_SILU
+ * g sigmoid(g) or MUSAPY_GATE_SIGMOID.  Weights (`weight_dtype`: F32 or dtype) are C-contiguous, 1 where NULL; the scale
+ * of a column is scale_value * scale[c].  y is formed from the unrounded r.
+ * The gradient takes r as the forward stored it, and dr and dy (either may be NULL: zeros):
+ *   D = dr + norm'(r)(dy pre_weight), dresidual = D, dv = dropout'(D scale), du = dv act(gate),
+ *   dx = norm'(x)(du post_weight), dgate = dv u act'(gate), and the column sums over all rows
+ *   dpost_weight = sum du n1, dscale = sum D d scale_value, dpre_weight = sum dy n2.
+ * Every output may be NULL but the forward's r.  Arrays of `stream_dtype` (dtype or F32): residual, r, dr, dresidual; all others are of
+ * `dtype`.  Inputs have unit-stride rows `*_pitch` elements apart; outputs are C-contiguous.
+ * Dropout keeps column c of a row where its 16-bit random number (musapy_dropout_v1) is at least
+ * `threshold`, times 65536 / (65536 - threshold); threshold 0 keeps all, 65536 drops all.
+ * The column sums go through `scratch` (musapy_norm_residual_scratch_v1 bytes, 16-byte aligned). */
+enum { MUSAPY_NORM_NONE = 0, MUSAPY_NORM_RMS = 1, MUSAPY_NORM_LAYER = 2 };
+enum { MUSAPY_GATE_SILU = 1, MUSAPY_GATE_SIGMOID = 2 };
+typedef struct {
+  int dtype, stream_dtype, weight_dtype;
+  int post, pre, gate_kind;
+  float eps, scale_value;
+  uint32_t threshold;
+  uint64_t seed, offset;
+  size_t rows, width;
+  const void* x;
+  size_t x_pitch;
+  const void* residual; /* forward: may be NULL (zeros); grad: the forward's r, read when pre is not NONE */
+  size_t residual_pitch;
+  const void* gate;
+  size_t gate_pitch;
+  const void* dr; /* grad only */
+  size_t dr_pitch;
+  const void* dy; /* grad only */
+  size_t dy_pitch;
+  const void *post_weight, *scale, *pre_weight;
+  void* r;  /* forward */
+  void* y;  /* forward */
+  void *dx, *dresidual, *dgate, *dpost_weight, *dscale, *dpre_weight; /* grad */
+} musapy_norm_residual_args;
+size_t musapy_norm_residual_scratch_v1(const musapy_norm_residual_args* args);
+int musapy_norm_residual_v1(const musapy_norm_residual_args* args, hipStream_t stream);
+int musapy_norm_residual_grad_v1(const musapy_norm_residual_args* args, void* scratch, size_t scratch_bytes, hipStream_t stream);
+
+/* Dropout of a strided view: out (C-contiguous) = a * 65536 / (65536 - threshold) where kept, else 0.
+ * The 16-bit number of column c (last axis) of row r (C-order index of the other axes) comes from
+ * Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011)
+ * with the key (seed low, seed high) and the counter (c / 8, r, offset low, offset high): column c
+ * takes half c % 8 of its four words, low half of word 0 first.  Fewer than 2^32 rows, and fewer
+ * than 2^35 columns. */
+int musapy_dropout_v1(const void* a, void* out, int dtype, int ndim, const size_t* shape, const ssize_t* strides, uint32_t threshold, uint64_t seed, uint64_t offset, hipStream_t stream);
 
 /* ---- planning helper (new; no counterpart in kernels.rs) ----
  * Tiles per output that the partial entry points should be given for this reduction on this

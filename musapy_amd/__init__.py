@@ -28,6 +28,7 @@ from ._core import (  # noqa: F401
     eq, ne, lt, gt, le, ge,
     sum, prod, max, min, mean, argmax, argmin, cumsum,
     transpose, flip, index_select, contiguous,
+    gated_scan, gated_scan_grad, norm_residual, norm_residual_grad, dropout,
     set_default_device, get_default_device, synchronize, device_count, device_info, mem_stats, empty_cache,
     Stream, stream, current_stream, set_debug, debug,
 )
@@ -36,7 +37,7 @@ __all__ = [
     "Array", "Dtype", "array", "from_numpy", "ones", "add", "sub", "mul", "div", "pow", "sin", "cos", "exp",
     "log", "abs", "sign", "neg", "clamp", "astype", "eq", "ne", "lt", "gt", "le", "ge", "sum", "prod", "max",
     "min", "mean", "argmax", "argmin", "cumsum", "transpose", "permute", "flip", "slice", "index_select",
-    "contiguous", "Stream", "stream", "current_stream", "synchronize", "from_dlpack", "set_debug", "debug",
+    "contiguous", "gated_scan", "gated_scan_grad", "norm_residual", "norm_residual_grad", "dropout", "Stream", "stream", "current_stream", "synchronize", "from_dlpack", "set_debug", "debug",
 ]
 
 # dtype constants: Dtype objects that compare equal to their names and aliases

@@ -39,9 +39,13 @@ HIP_SOURCES = [
     "kernels/reduce.hip",
     "kernels/reduce_int.hip",
     "kernels/scan.hip",
+    "kernels/gated_scan.hip",
+    "kernels/gated_scan_grad.hip",
+    "kernels/norm_residual.hip",
+    "kernels/dropout.hip",
     "runtime/hip_runtime.cpp",
 ]
-CXX_SOURCES = ["ops/core.cpp", "ops/ops.cpp", "ops/interop.cpp", "python/module.cpp"]
+CXX_SOURCES = ["ops/core.cpp", "ops/ops.cpp", "ops/blocks.cpp", "ops/interop.cpp", "python/module.cpp"]
 
 
 def _run(cmd: list[str]) -> None:

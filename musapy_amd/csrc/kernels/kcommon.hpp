@@ -249,7 +249,7 @@ __device__ inline T shfl_xor(T v, int m) {
 // 1 = cumsum scratch missing or too small, 2 = a reduction tile longer than 2^31 elements,
 // 3 = ndim outside [0, 32] or axis outside [0, ndim), 4 = a scan with 2^32 or more rows (or a
 // non-axis extent of 2^32 or more), 5 = a no-alloc reduction that needs more than the static
-// scratch holds.
+// scratch holds, 6 = an argument of a gated recurrent block's operator that is out of range.
 inline thread_local int g_wrapper_error = 0;
 
 // ---------------------------------------------------------------------------------------------
@@ -259,7 +259,7 @@ inline thread_local int g_wrapper_error = 0;
 // (or scratch) the launch was given, skip or finish their work, and exit normally -- so a grid
 // always drains.  The host reads and clears that word after synchronizing the stream
 // (musapy_kernels_take_fault_ws), so a fault is reported to the stream whose launch gave up.
-enum : uint32_t { kFaultReduceWait = 1u, kFaultScanWait = 2u };
+enum : uint32_t { kFaultReduceWait = 1u, kFaultScanWait = 2u, kFaultGatedScanWait = 4u };
 // polls a bounded wait may make (default 2^24; musapy_kernels_set_spin_limit)
 uint32_t wait_spin_limit();
 

@@ -358,6 +358,7 @@ void Stream::synchronize() {
       std::string what;
       if (fault & 1) what += "a single-launch reduction's combiner";
       if (fault & 2) what += std::string(what.empty() ? "" : " and ") + "a cumsum look-back";
+      if (fault & 4) what += std::string(what.empty() ? "" : " and ") + "a gated scan's look-back";
       throw KernelError("device wait expired in " + what + " on stream " + std::to_string(id_) +
                         ": results of the work queued on this stream since its last synchronize are invalid "
                         "(stream poisoned)" + failed);

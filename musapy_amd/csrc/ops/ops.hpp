@@ -43,6 +43,41 @@ Array arg_reduce_multi(const Array& a, const std::vector<ssize_t>* axes, bool ke
                        ReduceKernel k);
 Array cumsum_op(const Array& a, std::optional<size_t> axis, const Array* out);
 
+// Operators of a gated recurrent block (blocks.cpp); the formulas stand in musapy_kernels.h.
+// gated_scan returns (h, the state after the last step, f32); `gate` and `reset` broadcast to x.
+enum class ScanKind { Decay, Blend };
+std::pair<Array, Array> gated_scan(const Array& x, const Array& gate, const Array* h0, const Array* reset, ssize_t axis,
+                                   ScanKind kind, const Array* out, const Array* state_out);
+struct GatedScanGrad {
+  Array dx, dgate;
+  std::optional<Array> dh0;  // when h0 was given
+};
+GatedScanGrad gated_scan_grad(const Array& dh, const Array& x, const Array& gate, const Array& h, const Array* h0,
+                              const Array* reset, const Array* dstate, ssize_t axis, ScanKind kind, const Array* dx_out,
+                              const Array* dgate_out, const Array* dh0_out);
+enum class NormKind { None, Rms, Layer };
+enum class GateKind { Silu = 1, Sigmoid };
+struct NormOptions {
+  NormKind post = NormKind::Rms, pre = NormKind::Rms;
+  GateKind gate_kind = GateKind::Silu;
+  double eps = 1e-6, scale_value = 1.0, p = 0.0;
+  uint64_t seed = 0, offset = 0;
+};
+struct NormResidual {
+  Array r;
+  std::optional<Array> y;  // with a pre norm
+};
+NormResidual norm_residual(const Array& x, const Array* residual, const Array* gate, const Array* post_weight,
+                           const Array* scale, const Array* pre_weight, const NormOptions& o, const Array* r_out,
+                           const Array* y_out);
+struct NormResidualGrad {
+  std::optional<Array> dx, dresidual, dgate, dpost_weight, dscale, dpre_weight;
+};
+NormResidualGrad norm_residual_grad(const Array* dr, const Array* dy, const Array& x, const Array* r, const Array* gate,
+                                    const Array* post_weight, const Array* scale, const Array* pre_weight,
+                                    const NormOptions& o, const NormResidualGrad& outs);
+Array dropout(const Array& x, double p, uint64_t seed, uint64_t offset, const Array* out);
+
 // indexing.rs views + materialisation
 Array transpose(const Array& a, const std::vector<size_t>* axes);
 Array flip(const Array& a, size_t axis);

@@ -170,6 +170,65 @@ Array reduce_py(const Array& a, const py::object& axis, bool keepdims, const Arr
   return arg ? arg_reduce_multi(a, &*ax, keepdims, out, k) : reduce_multi(a, &*ax, keepdims, out, k);
 }
 
+// ---- arguments of the block operators ----
+// an array, or nothing for None
+const Array* opt_array(const py::object& o) { return o.is_none() ? nullptr : &o.cast<const Array&>(); }
+// the n arrays (or Nones) of an out= tuple
+std::vector<const Array*> out_arrays(const py::object& o, size_t n) {
+  std::vector<const Array*> r(n, nullptr);
+  if (o.is_none()) return r;
+  auto t = o.cast<py::sequence>();
+  if (py::isinstance<py::str>(o) || t.size() != n)
+    throw py::type_error("out= is a tuple of " + std::to_string(n) + " arrays or Nones");
+  for (size_t i = 0; i < n; ++i) r[i] = opt_array(t[i]);
+  return r;
+}
+ScanKind scan_kind(const std::string& s) {
+  if (s == "decay") return ScanKind::Decay;
+  if (s == "blend") return ScanKind::Blend;
+  throw py::value_error("kind is 'decay' or 'blend', not '" + s + "'");
+}
+NormKind norm_kind(const py::object& o) {
+  if (o.is_none()) return NormKind::None;
+  const std::string s = py::str(o);
+  if (s == "rms") return NormKind::Rms;
+  if (s == "layer") return NormKind::Layer;
+  throw py::value_error("a norm is 'rms', 'layer' or None, not '" + s + "'");
+}
+NormOptions norm_options(const py::object& post, const py::object& pre, const std::string& gate_kind, const py::object& scale,
+                         double eps, double p, uint64_t seed, uint64_t offset) {
+  NormOptions o;
+  o.post = norm_kind(post);
+  o.pre = norm_kind(pre);
+  if (gate_kind == "silu") o.gate_kind = GateKind::Silu;
+  else if (gate_kind == "sigmoid") o.gate_kind = GateKind::Sigmoid;
+  else throw py::value_error("gate_kind is 'silu' or 'sigmoid', not '" + gate_kind + "'");
+  if (!scale.is_none() && !py::isinstance<Array>(scale)) o.scale_value = scale.cast<double>();
+  o.eps = eps;
+  o.p = p;
+  o.seed = seed;
+  o.offset = offset;
+  return o;
+}
+const Array* scale_array(const py::object& scale) { return py::isinstance<Array>(scale) ? opt_array(scale) : nullptr; }
+std::optional<Array> opt_copy(const Array* a) { return a ? std::optional<Array>(*a) : std::nullopt; }
+
+// Runs a block operator and, in debug mode, records its OpContext on the stream of `first(result)`.
+template <class F, class G>
+auto traced_block(const char* name, std::initializer_list<const Array*> inputs, F&& f, G&& first) {
+  if (!is_debug()) return f();
+  capture_frame();
+  try {
+    auto r = f();
+    record_op(name, inputs, first(r));
+    set_debug_frame(nullptr);
+    return r;
+  } catch (...) {
+    set_debug_frame(nullptr);
+    throw;
+  }
+}
+
 py::dict plan_to_dict(const mpy::Plan& p) {
   py::dict d;
   py::list shape, strides;
@@ -493,6 +552,105 @@ PYBIND11_MODULE(_core, m) {
         return traced("cumsum", {&a}, [&] { return cumsum_op(a, resolve_axis(ax, a.ndim()), out); });
       },
       py::arg("a"), py::arg("axis") = py::none(), py::arg("out") = nullptr);
+
+  // operators of a gated recurrent block
+  m.def(
+      "gated_scan",
+      [](const Array& x, const Array& gate, const py::object& h0, const py::object& reset, ssize_t axis,
+         const std::string& kind, const Array* out, const Array* state_out) {
+        const ScanKind k = scan_kind(kind);
+        return traced_block(
+            "gated_scan", {&x, &gate},
+            [&] { return gated_scan(x, gate, opt_array(h0), opt_array(reset), axis, k, out, state_out); },
+            [](const std::pair<Array, Array>& r) -> const Array& { return r.first; });
+      },
+      py::arg("x"), py::arg("gate"), py::arg("h0") = py::none(), py::kw_only(), py::arg("reset") = py::none(),
+      py::arg("axis") = -2, py::arg("kind") = "decay", py::arg("out") = nullptr, py::arg("state_out") = nullptr,
+      "Gated linear recurrence along an axis: h[t] = g[t] h[t-1] + x[t] (kind 'decay'), or\n"
+      "h[t] = s h[t-1] + (1 - s) x[t] with s = sigmoid(g[t]) (kind 'blend').  Returns (h, state): h like x, and\n"
+      "the f32 state after the last step, which is the h0 of the next call.  x: f32, f16 or bf16; gate: x's\n"
+      "dtype or f32, broadcast to x; h0 (f32, x's shape without the axis): zeros when None; reset (bool,\n"
+      "broadcast to x): true where h[t-1] counts as 0, as at the first token of a packed sequence.");
+  m.def(
+      "gated_scan_grad",
+      [](const Array& dh, const Array& x, const Array& gate, const Array& h, const py::object& h0, const py::object& reset,
+         const py::object& dstate, ssize_t axis, const std::string& kind, const py::object& out) {
+        const ScanKind k = scan_kind(kind);
+        auto o = out_arrays(out, 3);
+        GatedScanGrad g = traced_block(
+            "gated_scan_grad", {&dh, &x, &gate, &h},
+            [&] {
+              return gated_scan_grad(dh, x, gate, h, opt_array(h0), opt_array(reset), opt_array(dstate), axis, k, o[0], o[1],
+                                     o[2]);
+            },
+            [](const GatedScanGrad& r) -> const Array& { return r.dx; });
+        return py::make_tuple(g.dx, g.dgate, g.dh0);
+      },
+      py::arg("dh"), py::arg("x"), py::arg("gate"), py::arg("h"), py::arg("h0") = py::none(), py::kw_only(),
+      py::arg("reset") = py::none(), py::arg("dstate") = py::none(), py::arg("axis") = -2, py::arg("kind") = "decay",
+      py::arg("out") = py::none(),
+      "Gradient of gated_scan: (dx, dgate, dh0) from dh, dstate (None: zeros) and the forward's x, gate, h, h0 and\n"
+      "reset.  dgate has the gate's own shape, summed over the axes it was broadcast along; dh0 is None without\n"
+      "h0.  out: a tuple of three arrays or Nones.");
+  m.def(
+      "norm_residual",
+      [](const Array& x, const py::object& residual, const py::object& gate, const py::object& post_weight,
+         const py::object& scale, const py::object& pre_weight, const py::object& post, const py::object& pre,
+         const std::string& gate_kind, double eps, double p, uint64_t seed, uint64_t offset, const py::object& out) {
+        const NormOptions opt = norm_options(post, pre, gate_kind, scale, eps, p, seed, offset);
+        auto o = out_arrays(out, 2);
+        NormResidual r = traced_block(
+            "norm_residual", {&x},
+            [&] {
+              return norm_residual(x, opt_array(residual), opt_array(gate), opt_array(post_weight), scale_array(scale),
+                                   opt_array(pre_weight), opt, o[0], o[1]);
+            },
+            [](const NormResidual& v) -> const Array& { return v.r; });
+        return py::make_tuple(r.r, r.y);
+      },
+      py::arg("x"), py::arg("residual") = py::none(), py::kw_only(), py::arg("gate") = py::none(),
+      py::arg("post_weight") = py::none(), py::arg("scale") = py::none(), py::arg("pre_weight") = py::none(),
+      py::arg("post") = "rms", py::arg("pre") = "rms", py::arg("gate_kind") = "silu", py::arg("eps") = 1e-6,
+      py::arg("p") = 0.0, py::arg("seed") = 0, py::arg("offset") = 0, py::arg("out") = py::none(),
+      "A block's way back to the residual stream and the next block's norm, over the last axis:\n"
+      "r = residual + scale * dropout(norm(x) * post_weight * act(gate)), y = norm(r) * pre_weight.  Returns (r, y).\n"
+      "post, pre: 'rms', 'layer' or None (no norm; without pre, y is None).  residual: x's dtype or f32, which is\n"
+      "r's; gate, y: x's dtype; weights: one dtype, f32 or x's; scale: a number or an array like the weights.\n"
+      "p, seed, offset: as for dropout.");
+  m.def(
+      "norm_residual_grad",
+      [](const py::object& dresidual, const py::object& dy, const Array& x, const py::object& residual_out,
+         const py::object& gate, const py::object& post_weight, const py::object& scale, const py::object& pre_weight,
+         const py::object& post, const py::object& pre, const std::string& gate_kind, double eps, double p, uint64_t seed,
+         uint64_t offset, const py::object& out) {
+        const NormOptions opt = norm_options(post, pre, gate_kind, scale, eps, p, seed, offset);
+        auto o = out_arrays(out, 6);
+        NormResidualGrad outs{opt_copy(o[0]), opt_copy(o[1]), opt_copy(o[2]), opt_copy(o[3]), opt_copy(o[4]), opt_copy(o[5])};
+        NormResidualGrad g = traced_block(
+            "norm_residual_grad", {&x},
+            [&] {
+              return norm_residual_grad(opt_array(dresidual), opt_array(dy), x, opt_array(residual_out), opt_array(gate),
+                                        opt_array(post_weight), scale_array(scale), opt_array(pre_weight), opt, outs);
+            },
+            [](const NormResidualGrad& v) -> const Array& { return *v.dx; });
+        return py::make_tuple(g.dx, g.dresidual, g.dgate, g.dpost_weight, g.dscale, g.dpre_weight);
+      },
+      py::arg("dresidual"), py::arg("dy"), py::arg("x"), py::arg("residual_out"), py::kw_only(), py::arg("gate") = py::none(),
+      py::arg("post_weight") = py::none(), py::arg("scale") = py::none(), py::arg("pre_weight") = py::none(),
+      py::arg("post") = "rms", py::arg("pre") = "rms", py::arg("gate_kind") = "silu", py::arg("eps") = 1e-6,
+      py::arg("p") = 0.0, py::arg("seed") = 0, py::arg("offset") = 0, py::arg("out") = py::none(),
+      "Gradient of norm_residual: (dx, dresidual, dgate, dpost_weight, dscale, dpre_weight) from the gradients of r and y\n"
+      "(either may be None), x, the forward's r and the same options; None for what was not given.  out: a\n"
+      "tuple of six arrays or Nones.");
+  m.def(
+      "dropout",
+      [](const Array& x, double p, uint64_t seed, uint64_t offset, const Array* out) {
+        return traced("dropout", {&x}, [&] { return dropout(x, p, seed, offset, out); });
+      },
+      py::arg("x"), py::arg("p"), py::arg("seed"), py::arg("offset") = 0, py::arg("out") = nullptr,
+      "x / (1 - p) where kept, 0 where dropped.  Which elements are kept follows from seed, offset and an\n"
+      "element's place in the array alone (Philox4x32-10), so the gradient is dropout(dy, p, seed, offset) and no mask is\n"
+      "stored.  p is rounded to a multiple of 2^-16.");
 
   // views
   m.def(
