@@ -50,6 +50,87 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_walk(GsArgs p) {
   }
 }
 
+// One tile (gated_scan.hpp) a workgroup; SPLIT: several tiles to a chain.
+template <class TX, class TG, bool BLEND, bool RESET, bool SPLIT, bool NT>
+__global__ __launch_bounds__(kGsBlock) void k_gs_tiles(GsArgs p, GsSplit sp) {
+  constexpr int V = 16 / int(sizeof(TX));
+  constexpr int S = kGsS;
+  constexpr uint32_t kSteps = kGsTileSteps;
+  __shared__ GsTile<V> sm;
+  uint32_t chain, tile;
+  if (!gs_take<SPLIT>(sp, sm.ticket, chain, tile)) return;
+  const GsPlace<V> at(p, chain);
+  const uint64_t t0 = uint64_t(tile) * kSteps + threadIdx.x / kGsLt * S;  // the thread's first step
+  const bool full = GsPlace<V>::whole(p, chain) && (uint64_t(tile) + 1) * kSteps <= p.T;
+  const int steps = full ? S : at.nl == 0 || t0 >= p.T ? 0 : p.T - t0 < uint64_t(S) ? int(p.T - t0) : S;
+  const TX* x = static_cast<const TX*>(p.x) + at.off[kGsX] + int64_t(t0) * p.ts[kGsX];
+  const TG* gate = static_cast<const TG*>(p.gate) + at.off[kGsGate] + int64_t(t0) * p.ts[kGsGate];
+  TX* out = static_cast<TX*>(p.out) + at.off[kGsOut] + int64_t(t0) * p.ts[kGsOut];
+
+  Vec<TX, V> wx[S];
+  Vec<TG, V> wg[S];
+  uint32_t cuts = 0;
+  auto load = [&](auto FULL) {
+    constexpr bool F = decltype(FULL)::value;
+    // steps and lanes that are not there leave the state alone: x = 0 and a factor of 1
+    gs_load_steps<F, NT>(wx, x, p.ts[kGsX], 1, at.nl, steps, TX(0.0f));
+    gs_load_steps<F, NT>(wg, gate, p.ts[kGsGate], p.ls[kGsGate], at.nl, steps, TG(BLEND ? __builtin_inff() : 1.0f));
+    if constexpr (RESET) {
+      const uint8_t* reset = p.reset + at.off[kGsReset] + int64_t(t0) * p.ts[kGsReset];
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (F || s < steps) cuts |= uint32_t(reset[s * p.ts[kGsReset]] != 0) << s;
+    }
+  };
+  if (full) load(std::true_type{});
+  else load(std::false_type{});
+
+  float P = 0.0f;
+  if (p.first && at.state_on) P = p.first[at.state];
+  float a[S][V], b[S][V], A[V], H[V], c[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    A[v] = 1.0f;
+    H[v] = 0.0f;
+  }
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const bool cut = RESET && ((cuts >> s) & 1);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      a[s][v] = float(wg[s].v[v]);
+      b[s][v] = float(wx[s].v[v]);
+      if constexpr (BLEND) {
+        float rest;
+        gs_sigmoid(a[s][v], a[s][v], rest);
+        b[s][v] *= rest;
+      }
+      H[v] = cut ? b[s][v] : __builtin_fmaf(a[s][v], H[v], b[s][v]);
+      A[v] = cut ? __builtin_nanf("") : A[v] * a[s][v];
+    }
+  }
+
+  gs_tile_state<V, SPLIT>(sm, A, H, c, P, sp, chain, tile);
+
+  auto finish = [&](auto FULL) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      if (!decltype(FULL)::value && s >= steps) continue;
+      const bool cut = RESET && ((cuts >> s) & 1);
+#pragma unroll
+      for (int v = 0; v < V; ++v) c[v] = cut ? b[s][v] : __builtin_fmaf(a[s][v], c[v], b[s][v]);
+      gs_store_step<decltype(FULL)::value, NT>(out + s * p.ts[kGsOut], at.nl, c);
+    }
+  };
+  if (full) finish(std::true_type{});
+  else finish(std::false_type{});
+  if (tile + 1 == sp.tiles && p.last && at.state_on) p.last[at.state] = P;
+}
+
+__global__ void k_gs_clear(uint64_t* w, uint64_t n) {
+  for (uint64_t i = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += uint64_t(gridDim.x) * blockDim.x) w[i] = 0;
+}
+
 // ---- planning -------------------------------------------------------------------------------------
 namespace {
 bool gs_bad() {
@@ -179,13 +260,66 @@ void gs_vectors(GsPlan& pl, int V) {
   pl.a.nvdiv = make_fastdiv(pl.a.nv ? pl.a.nv : 1);
 }
 
+constexpr uint64_t kGsHead = kGsShards * kGsCounterWords;  // words in front of the tiles': the ticket counters
+
+GsRoute gs_route(const GsPlan& pl, int V) {
+  GsRoute r;
+  if (!pl.lanes || pl.a.T <= 16) return r;
+  r.chains = (uint64_t(pl.a.nvec) + kGsLt - 1) / kGsLt;
+  r.tiles = (pl.a.T + kGsTileSteps - 1) / kGsTileSteps;
+  if (r.tiles > 1) {
+    const uint64_t lanes = kGsLt * uint64_t(V);
+    r.group_words = (r.tiles + kGsGroup - 1) / kGsGroup * r.chains * lanes;
+    r.words = kGsHead + r.chains * r.tiles * lanes + r.group_words;
+  }
+  r.walk = !grid_fits((r.chains + kGsShards) * r.tiles, kGsBlock);
+  if (r.walk) r.words = 0;
+  return r;
+}
+
+bool gs_split(GsSplit& sp, const GsRoute& r, void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes,
+              hipStream_t st) {
+  sp.chains = uint32_t(r.chains);
+  sp.tiles = uint32_t(r.tiles);
+  sp.shards = sp.chains < kGsShards ? sp.chains : kGsShards;
+  sp.per_shard = (sp.chains + sp.shards - 1) / sp.shards;
+  sp.sdiv = make_fastdiv(sp.shards);
+  sp.pdiv = make_fastdiv(sp.per_shard);
+  if (r.tiles == 1) return true;
+  WsSplit ws;
+  if (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 7) || scratch_bytes < r.words * 8 ||
+      !ws_split(workspace, workspace_bytes, ws)) {
+    g_wrapper_error = 1;
+    return false;
+  }
+  uint64_t* w = static_cast<uint64_t*>(scratch);
+  sp.counters = w;
+  sp.groups = w + kGsHead;
+  sp.words = sp.groups + r.group_words;
+  sp.fault = ws.fault;
+  sp.spin_limit = wait_spin_limit();
+  const uint64_t blocks = (r.words + 255) / 256;
+  k_gs_clear<<<unsigned(blocks < 2048 ? blocks : 2048), 256, 0, st>>>(w, r.words);
+  return true;
+}
+
 }  // namespace mpy
 
 using namespace mpy;
 
 extern "C" {
 
-size_t musapy_gated_scan_scratch_v1(const musapy_gated_scan_args* p, int grad) { return 0; }
+size_t musapy_gated_scan_scratch_v1(const musapy_gated_scan_args* p, int grad) {
+  GsPlan pl;
+  if (!gs_plan(p, grad != 0, pl)) {
+    g_wrapper_error = 0;  // the call itself reports it
+    return 0;
+  }
+  if (pl.rows == 0 || pl.a.D == 0 || !pl.lanes) return 0;
+  const int V = gs_vector(p->dtype);
+  gs_vectors(pl, V);
+  return gs_route(pl, V).words * 8;
+}
 
 size_t musapy_gated_scan_parts_v1(const musapy_gated_scan_args* p) {
   if (p == nullptr || p->shape == nullptr || p->gate_strides == nullptr || p->ndim < 2 || p->ndim > kMaxDims ||
@@ -208,7 +342,22 @@ int musapy_gated_scan_v1(const musapy_gated_scan_args* p, void* scratch, size_t 
   if (pl.rows == 0 || pl.a.D == 0) return 0;
   const int V = pl.lanes ? gs_vector(p->dtype) : 1;
   gs_vectors(pl, V);
+  const GsRoute r = gs_route(pl, V);
+  if (!r.walk) {
+    GsSplit sp{};
+    if (!gs_split(sp, r, scratch, scratch_bytes, workspace, workspace_bytes, st)) return -1;
+    const bool nt = uint64_t(pl.a.nvec) * pl.a.T * 16 >= kStreamLoadBytes;
+    gs_types(p->dtype, p->gate_dtype, [&](auto tx, auto tg) {
+      using TX = decltype(tx);
+      using TG = decltype(tg);
+      gs_flags([&](auto BLEND, auto RESET, auto SPLIT, auto NT) {
+        k_gs_tiles<TX, TG, BLEND.value, RESET.value, SPLIT.value, NT.value><<<gs_grid(sp), kGsBlock, 0, st>>>(pl.a, sp);
+      }, p->kind == MUSAPY_SCAN_BLEND, p->reset != nullptr, r.tiles > 1, nt);
+    });
+    return 0;
+  }
   const unsigned grid = unsigned((uint64_t(pl.a.nvec) + kGsBlock - 1) / kGsBlock);
+  if (!grid_fits(grid, kGsBlock)) return gs_bad() ? 0 : -1;
   gs_types(p->dtype, p->gate_dtype, [&](auto tx, auto tg) {
     using TX = decltype(tx);
     using TG = decltype(tg);

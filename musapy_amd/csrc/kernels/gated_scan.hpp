@@ -6,7 +6,10 @@
 // which is the same recurrence run over reversed time, with (a[t], a[t] dh[t]) for (a, b).
 #pragma once
 
+#include <tuple>
+
 #include "kcommon.hpp"
+#include "publish.hpp"
 
 namespace mpy {
 
@@ -85,6 +88,291 @@ __device__ inline void gs_store(T* p, int nl, const float (&x)[V]) {
   }
 }
 
+// The S steps of a thread as they lie in memory, `p` at the first one.  FULL: all steps and lanes are
+// there; else `steps` and `nl` of them, and `none` in the others' place.
+template <bool FULL, bool NT, class T, int V, int S>
+__device__ inline void gs_load_steps(Vec<T, V> (&w)[S], const T* p, int64_t ts, int64_t ls, int nl, int steps, T none) {
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const T* at = p + s * ts;
+    if (!FULL && (s >= steps || nl < V)) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) w[s].v[v] = s < steps && v < nl ? at[v * ls] : none;
+    } else if (ls == 0) {
+      const T e = *at;
+#pragma unroll
+      for (int v = 0; v < V; ++v) w[s].v[v] = e;
+    } else {
+      w[s] = vload_el<T, V, NT>(at);
+    }
+  }
+}
+// Hides where a value comes from, so that what was computed from it before is formed again instead
+// of being kept in registers.
+template <class T, int V>
+__device__ inline void gs_opaque(Vec<T, V>& w) {
+  uint32_t r[sizeof(w) / 4];
+  __builtin_memcpy(r, &w, sizeof(w));
+#pragma unroll
+  for (int i = 0; i < int(sizeof(w) / 4); ++i) asm volatile("" : "+v"(r[i]));
+  __builtin_memcpy(&w, r, sizeof(w));
+}
+// Stores one step; FULL: all lanes are there.
+template <bool FULL, bool NT, class T, int V>
+__device__ inline void gs_store_step(T* p, int nl, const float (&x)[V]) {
+  if (FULL || nl == V) {
+    Vec<T, V> w;
+#pragma unroll
+    for (int v = 0; v < V; ++v) w.v[v] = T(x[v]);
+    vstore_el<NT, T, V>(p, w);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (v < nl) p[v] = T(x[v]);
+  }
+}
+
+// ---- tiles of steps -------------------------------------------------------------------------------
+// A run of steps maps the state c in front of it to A c + H behind it, and two runs compose to
+// (A2 A1, A2 H1 + H2).  A = NaN says that the state in front does not matter (the run holds a
+// reset, or its H is NaN already); a state of 0 is not multiplied, so that a product of growing
+// gates that overflowed does not make it NaN.
+__device__ inline float gs_apply(float A, float H, float c) {
+  return c == 0.0f || A != A ? H : __builtin_fmaf(A, c, H);
+}
+
+// Tiles of 32 segments of 4 steps by 8 vectors of lanes: 128 bytes of x a step, every cache line one
+// tile's.  Thread (segment, vector) holds its segment's steps in registers.
+constexpr int kGsLt = 8;
+constexpr int kGsS = 4;                                  // steps of a segment
+constexpr int kGsTileSteps = kGsBlock / kGsLt * kGsS;    // 128
+
+template <int V>
+struct GsTile {
+  static constexpr int BS = kGsBlock;
+  static constexpr int kSegs = BS / kGsLt;
+  static constexpr int kLanes = kGsLt * V;              // 64 or 32
+  static constexpr int kParts = BS / kLanes;            // threads that scan one lane's segments
+  static constexpr int kPer = kSegs / kParts;           // segments of each
+  // element v of thread (segment, vector); the padding puts the v of a vector on banks of their own, so
+  // that both the threads' accesses and those lane by lane touch every bank once
+  float a[V][BS + kGsLt], h[V][BS + kGsLt];
+  float pa[kParts][kLanes], ph[kParts][kLanes], c[kParts][kLanes];
+  uint32_t ticket;
+};
+
+// Steps split over workgroups.  For each tile of each chain (a group of vectors) and lane, one word
+// holds the tile's (A, H); every kGsGroup tiles form a group, whose last tile publishes the group's
+// (A, H) too, and later, in the same word, the state behind the group as (NaN, state), which is the
+// map that gives that state whatever lies in front.  A word is 0 until it is published: (+0, +0)
+// goes as (-0, +0), which means the same.
+constexpr uint32_t kGsGroup = 4;
+constexpr int kGsWindow = 8;  // groups whose words the look-back reads at once
+struct GsSplit {
+  // Tickets: one counter for each shard of chains, a cache line apart.  One counter for all took
+  // 14 ns a ticket, the rate of atomics on one address: 239 us of the 16384 tiles of (65536, 2048).
+  uint64_t* counters;
+  uint32_t shards, per_shard;  // chain = number in the shard * shards + shard
+  FastDiv sdiv, pdiv;
+  uint64_t* words;   // [tile][chain][lane]
+  uint64_t* groups;  // [group][chain][lane]
+  uint32_t* fault;
+  uint32_t spin_limit;
+  uint32_t chains, tiles;
+};
+constexpr uint32_t kGsShards = 32;
+constexpr uint32_t kGsCounterWords = 16;
+
+__device__ inline uint64_t gs_pack(float A, float H) {
+  const uint64_t w = (uint64_t(__float_as_uint(A)) << 32) | __float_as_uint(H);
+  return w ? w : uint64_t(0x80000000u) << 32;
+}
+__device__ inline float gs_apply(uint64_t w, float c) {
+  return gs_apply(__uint_as_float(uint32_t(w >> 32)), __uint_as_float(uint32_t(w)), c);
+}
+
+// The state in front of `tile` for one lane, from the group in front's and the tiles of its own
+// group that lie between; that group's state from the nearest one published, through the (A, H) of the
+// groups between.  Every state is folded front to back over the same runs wherever the
+// look-back starts, so results are the same bits run to run.  (ta, th) is the tile's own map; the last
+// tile of a group publishes its group's.  A wait makes at most spin_limit polls, then records its
+// fault and goes on with 0, so every workgroup exits.
+template <int LANES>
+__device__ inline float gs_look_back(const GsSplit& sp, uint32_t chain, uint32_t tile, int lane, float first, float ta,
+                                     float th) {
+  const uint32_t group = tile / kGsGroup, in = tile % kGsGroup;
+  const uint64_t ws = uint64_t(sp.chains) * LANES;
+  uint64_t* const wt = sp.words + (uint64_t(tile) * sp.chains + chain) * LANES + lane;
+  uint64_t* const wg = sp.groups + (uint64_t(group) * sp.chains + chain) * LANES + lane;
+  const bool follow = tile + 1 < sp.tiles;            // a tile behind waits on this one,
+  const bool last = follow && in == kGsGroup - 1;     // or on its group
+  if (follow && !last) st_relaxed(wt, gs_pack(ta, th));
+  uint32_t spins = 0;
+  bool done = false;
+  // the tiles of the group in front of this one
+  uint64_t w[kGsGroup - 1];
+  for (; !done && spins < sp.spin_limit; ++spins) {
+    bool ok = true;
+#pragma unroll
+    for (uint32_t i = 0; i < kGsGroup - 1; ++i) {
+      w[i] = i < in ? ld_relaxed(wt - uint64_t(in - i) * ws) : gs_pack(1.0f, 0.0f);
+      ok = ok && w[i] != 0;
+    }
+    done = __all(ok);
+    if (!done) __builtin_amdgcn_s_sleep(1);
+  }
+  uint64_t mine = 0;
+  if (last) {
+    float ga = 1.0f, gh = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < kGsGroup - 1; ++i) {
+      gh = gs_apply(w[i], gh);
+      ga = ga * __uint_as_float(uint32_t(w[i] >> 32));
+    }
+    mine = gs_pack(ga * ta, gs_apply(ta, th, gh));
+    st_relaxed(wg, mine);
+  }
+  // the state behind the group in front
+  float P = first;
+  if (group > 0) {
+    done = false;
+    for (; !done && spins < sp.spin_limit; ++spins) {
+      uint64_t m[kGsWindow];
+      m[0] = ld_relaxed(wg - ws);
+      P = __uint_as_float(uint32_t(m[0]));
+      auto state = [](uint64_t x) { return uint32_t(x >> 32) << 1 > 0xff000000u; };  // A is NaN
+      done = __all(state(m[0]));
+      if (done) break;
+#pragma unroll
+      for (int d = 1; d < kGsWindow; ++d) m[d] = uint32_t(d) < group ? ld_relaxed(wg - uint64_t(d + 1) * ws) : 0;
+      bool have = false;
+      P = 0.0f;
+#pragma unroll
+      for (int d = kGsWindow - 1; d >= 0; --d) {
+        P = gs_apply(m[d], P);
+        have = (have || state(m[d])) && m[d] != 0;
+      }
+      done = __all(have);
+      if (!done) __builtin_amdgcn_s_sleep(1);
+    }
+  }
+  if (!done && (group > 0 || in > 0)) {
+    if (lane == 0) atomicOr(sp.fault, kFaultGatedScanWait);
+    P = 0.0f;
+  }
+  if (last) st_relaxed(wg, (uint64_t(0x7fc00000u) << 32) | __float_as_uint(gs_apply(mine, P)));
+#pragma unroll
+  for (uint32_t i = 0; i < kGsGroup - 1; ++i)
+    if (i < in) P = gs_apply(w[i], P);
+  return P;
+}
+
+// From each thread's segment (A, H) to the state c in front of it.  `P` (thread l: the tile's lane l)
+// is the state in front of the first tile; it becomes the one behind this tile.
+template <int V, bool SPLIT>
+__device__ inline void gs_tile_state(GsTile<V>& sm, const float (&A)[V], const float (&H)[V], float (&c)[V], float& P,
+                                     const GsSplit& sp, uint32_t chain, uint32_t tile) {
+  using G = GsTile<V>;
+  const int tid = threadIdx.x, lt = tid % kGsLt, seg = tid / kGsLt;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    sm.a[v][tid] = A[v];
+    sm.h[v][tid] = H[v];
+  }
+  lds_barrier();
+  // lane l of the tile: element l / 8 of vector l % 8
+  const int lane = tid % G::kLanes, part = tid / G::kLanes;
+  float* const la = &sm.a[lane / kGsLt][part * G::kPer * kGsLt + lane % kGsLt];
+  float* const lh = &sm.h[lane / kGsLt][part * G::kPer * kGsLt + lane % kGsLt];
+  float a[G::kPer], h[G::kPer];
+#pragma unroll
+  for (int i = 0; i < G::kPer; ++i) {
+    a[i] = la[i * kGsLt];
+    h[i] = lh[i * kGsLt];
+  }
+  float pa = 1.0f, ph = 0.0f;
+#pragma unroll
+  for (int i = 0; i < G::kPer; ++i) {
+    la[i * kGsLt] = pa;
+    lh[i * kGsLt] = ph;
+    ph = gs_apply(a[i], h[i], ph);
+    pa = pa * a[i];
+  }
+  sm.pa[part][lane] = pa;
+  sm.ph[part][lane] = ph;
+  lds_barrier();
+  if (tid < kWave) {  // (of 32 lanes, the wave's other half follows)
+    float xa[G::kParts], xh[G::kParts];
+#pragma unroll
+    for (int i = 0; i < G::kParts; ++i) {
+      xa[i] = sm.pa[i][lane];
+      xh[i] = sm.ph[i][lane];
+    }
+    float ta = xa[0], th = xh[0];
+#pragma unroll
+    for (int i = 1; i < G::kParts; ++i) {
+      th = gs_apply(xa[i], xh[i], th);
+      ta = ta * xa[i];
+    }
+    if constexpr (SPLIT) P = gs_look_back<G::kLanes>(sp, chain, tile, lane, P, ta, th);
+    float q = P;
+#pragma unroll
+    for (int i = 0; i < G::kParts; ++i) {
+      sm.c[i][lane] = q;
+      q = gs_apply(xa[i], xh[i], q);
+    }
+    P = q;
+  }
+  lds_barrier();
+  const int mine = seg / G::kPer;
+#pragma unroll
+  for (int v = 0; v < V; ++v) c[v] = gs_apply(sm.a[v][tid], sm.h[v][tid], sm.c[mine][v * kGsLt + lt]);
+}
+
+// The tile of a workgroup.  SPLIT: by ticket, in the order of the steps within a shard of chains, so
+// that every tile that one waits on was taken before it and is running or done.  false: none left.
+template <bool SPLIT>
+__device__ inline bool gs_take(const GsSplit& sp, uint32_t& ticket, uint32_t& chain, uint32_t& tile) {
+  chain = blockIdx.x;
+  tile = 0;
+  if constexpr (SPLIT) {
+    const uint32_t shard = blockIdx.x - fd_div(sp.sdiv, blockIdx.x) * sp.shards;
+    if (threadIdx.x == 0) ticket = atomicAdd(reinterpret_cast<uint32_t*>(sp.counters + shard * kGsCounterWords), 1u);
+    __syncthreads();
+    const uint32_t t = ticket;
+    tile = fd_div(sp.pdiv, t);
+    chain = (t - tile * sp.per_shard) * sp.shards + shard;
+    return chain < sp.chains;
+  }
+  return true;
+}
+
+// Where a thread of a tile works: its vector's first lane, and for thread l the tile lane l's state.
+template <int V>
+struct GsPlace {
+  int nl;                // lanes of the vector; 0: none
+  bool state_on;
+  int64_t off[kGsOps];
+  int64_t state;
+  __device__ GsPlace(const GsArgs& p, uint32_t chain) {
+    const uint32_t q = chain * kGsLt + threadIdx.x % kGsLt;
+    const uint32_t qc = q < p.nvec ? q : p.nvec - 1;  // threads past the last vector stand on it and touch nothing
+    const uint32_t row = fd_div(p.nvdiv, qc), col = (qc - row * p.nv) * V;
+    nl = q >= p.nvec ? 0 : p.D - col < uint32_t(V) ? int(p.D - col) : V;
+    row_offsets<kGsOps>(p.ix, row, off);
+#pragma unroll
+    for (int o = 0; o < kGsOps; ++o) off[o] += int64_t(col) * p.ls[o];
+    // thread l's vector is the one that lane l belongs to
+    const uint32_t e = threadIdx.x % (kGsLt * V) / kGsLt;
+    state_on = threadIdx.x < kWave && e < uint32_t(nl);
+    state = off[kGsState] + e;
+  }
+  // all lanes of the chain's vectors are there (the same for the whole workgroup)
+  static __device__ bool whole(const GsArgs& p, uint32_t chain) {
+    return p.D % V == 0 && (uint64_t(chain) + 1) * kGsLt <= p.nvec;
+  }
+};
+
 // ---- host side ----------------------------------------------------------------------------------
 struct GsPlan {
   GsArgs a;
@@ -109,6 +397,19 @@ inline int gs_part_shift(uint64_t D, int V) {
   return s;
 }
 
+// How the lanes' tiles are launched, and the scratch that takes.
+struct GsRoute {
+  bool walk = true;
+  uint64_t chains = 0, tiles = 0;
+  uint64_t words = 0, group_words = 0;  // of a split scan
+};
+GsRoute gs_route(const GsPlan& pl, int V);
+// Fills `sp` in and clears its words on `st`; false (wrapper error 1) without room for them.
+bool gs_split(GsSplit& sp, const GsRoute& r, void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes,
+              hipStream_t st);
+
+inline unsigned gs_grid(const GsSplit& sp) { return sp.tiles > 1 ? sp.shards * sp.per_shard * sp.tiles : sp.chains; }
+
 // Calls fn(TX{}, TG{}) with the element types of x and the gate.
 template <class Fn>
 inline void gs_types(int dtype, int gate_dtype, Fn&& fn) {
@@ -119,6 +420,21 @@ inline void gs_types(int dtype, int gate_dtype, Fn&& fn) {
   }
   if (gate_dtype == MUSAPY_DT_F32) return fn(f16{}, float{});
   return fn(f16{}, f16{});
+}
+
+// Calls fn with a std::bool_constant for each flag.
+template <class Fn, class... Known>
+inline void gs_flags_from(Fn&& fn, std::tuple<Known...> known) {
+  std::apply(fn, known);
+}
+template <class Fn, class... Known, class... More>
+inline void gs_flags_from(Fn&& fn, std::tuple<Known...> known, bool flag, More... more) {
+  if (flag) gs_flags_from(fn, std::tuple_cat(known, std::make_tuple(std::true_type{})), more...);
+  else gs_flags_from(fn, std::tuple_cat(known, std::make_tuple(std::false_type{})), more...);
+}
+template <class Fn, class... Flags>
+inline void gs_flags(Fn&& fn, Flags... flags) {
+  gs_flags_from(fn, std::tuple<>{}, flags...);
 }
 
 }  // namespace mpy

@@ -76,6 +76,123 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
   }
 }
 
+// One tile a workgroup, over reversed time: step k is t = T - 1 - k.  What was loaded stays as it was,
+// and the factors are formed twice, for the tile's map and for its results: registers are dearer here
+// than the second sigmoid.
+template <class TX, class TG, bool BLEND, bool RESET, bool SPLIT, bool NT>
+__global__ __launch_bounds__(kGsBlock) void k_gs_grad_tiles(GsArgs p, GsSplit sp) {
+  constexpr int V = 16 / int(sizeof(TX));
+  constexpr int S = kGsS;
+  constexpr uint32_t kSteps = kGsTileSteps;
+  __shared__ GsTile<V> sm;
+  uint32_t chain, tile;
+  if (!gs_take<SPLIT>(sp, sm.ticket, chain, tile)) return;
+  const GsPlace<V> at(p, chain);
+  const uint64_t k0 = uint64_t(tile) * kSteps + threadIdx.x / kGsLt * S;
+  // (t = 0 has no h[t-1], so its tile is not a full one)
+  const bool full = GsPlace<V>::whole(p, chain) && (uint64_t(tile) + 1) * kSteps < p.T;
+  const int steps = full ? S : at.nl == 0 || k0 >= p.T ? 0 : p.T - k0 < uint64_t(S) ? int(p.T - k0) : S;
+  const int64_t t0 = int64_t(p.T) - 1 - int64_t(k0);
+  auto from = [&](auto* base, int o, int64_t t) { return base + at.off[o] + t * p.ts[o]; };
+  Vec<TX, V> wd[S], wh[S], wx[S];
+  Vec<TG, V> wg[S];
+  uint32_t cuts = 0;
+  auto load = [&](auto FULL) {
+    constexpr bool F = decltype(FULL)::value;
+    // steps and lanes that are not there pass the flow on: dh = 0 and a factor of 1
+    gs_load_steps<F, NT>(wd, from(static_cast<const TX*>(p.dh), kGsDh, t0), -p.ts[kGsDh], 1, at.nl, steps, TX(0.0f));
+    gs_load_steps<F, NT>(wg, from(static_cast<const TG*>(p.gate), kGsGate, t0), -p.ts[kGsGate], p.ls[kGsGate], at.nl, steps,
+                         TG(BLEND ? __builtin_inff() : 1.0f));
+    const int hs = k0 + steps == p.T ? steps - 1 : steps;  // h[-1] is no element of h
+    gs_load_steps<F, NT>(wh, from(static_cast<const TX*>(p.h), kGsH, t0 - 1), -p.ts[kGsH], 1, at.nl, hs, TX(0.0f));
+    if constexpr (BLEND)
+      gs_load_steps<F, NT>(wx, from(static_cast<const TX*>(p.x), kGsX, t0), -p.ts[kGsX], 1, at.nl, steps, TX(0.0f));
+    if constexpr (RESET) {
+      const uint8_t* r = from(p.reset, kGsReset, t0);
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (F || s < steps) cuts |= uint32_t(r[-s * p.ts[kGsReset]] != 0) << s;
+    }
+  };
+  if (full) load(std::true_type{});
+  else load(std::false_type{});
+  float P = 0.0f;
+  if (p.first && at.state_on) P = p.first[at.state];
+  float A[V], H[V], c[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    A[v] = 1.0f;
+    H[v] = 0.0f;
+  }
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const bool cut = RESET && ((cuts >> s) & 1);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float a = float(wg[s].v[v]), rest;
+      if constexpr (BLEND) gs_sigmoid(a, a, rest);
+      H[v] = cut ? 0.0f : a * (float(wd[s].v[v]) + H[v]);
+      A[v] = cut ? __builtin_nanf("") : A[v] * a;
+    }
+  }
+
+  gs_tile_state<V, SPLIT>(sm, A, H, c, P, sp, chain, tile);
+
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    gs_opaque(wd[s]);
+    gs_opaque(wg[s]);
+  }
+  TX* dx = from(static_cast<TX*>(p.out), kGsOut, t0);
+  const int64_t dgate = at.off[kGsDgate] + t0 * p.ts[kGsDgate];
+  const uint32_t vec = chain * kGsLt + threadIdx.x % kGsLt;  // parts: rows are whole groups of vectors
+  const int parts = p.part_lanes < 0 ? 0 : 1 << p.part_lanes;
+  const uint32_t part = parts ? (vec - fd_div(p.nvdiv, vec) * p.nv) >> p.part_lanes : 0;
+  auto finish = [&](auto FULL) {
+    constexpr bool F = decltype(FULL)::value;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      if (!F && s >= steps && !parts) continue;
+      const bool cut = RESET && ((cuts >> s) & 1);
+      float ox[V], og[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float a = float(wg[s].v[v]), rest = 1.0f;
+        if constexpr (BLEND) gs_sigmoid(a, a, rest);
+        float hb = float(wh[s].v[v]);
+        if (!F && k0 + s + 1 == p.T && p.h_first && v < at.nl) hb = p.h_first[at.off[kGsState] + v];
+        if (cut) hb = 0.0f;
+        const float G = float(wd[s].v[v]) + c[v];
+        if constexpr (BLEND) {
+          ox[v] = rest * G;
+          og[v] = G * (hb - float(wx[s].v[v])) * (a * rest);
+        } else {
+          ox[v] = G;
+          og[v] = cut ? 0.0f : G * hb;
+        }
+        c[v] = cut ? 0.0f : a * G;
+      }
+      const bool in = F || s < steps;
+      if (in) gs_store_step<F, NT>(dx - s * p.ts[kGsOut], at.nl, ox);
+      const int64_t to = dgate - s * p.ts[kGsDgate];
+      if (parts) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum += F || v < at.nl ? og[v] : 0.0f;
+        for (int m = 1; m < parts; m <<= 1) sum += __shfl_xor(sum, m, kWave);
+        if (in && (vec & uint32_t(parts - 1)) == 0) static_cast<float*>(p.dgate)[to + part] = sum;
+      } else if (p.dgate_f32) {
+        gs_store_step<F, NT>(static_cast<float*>(p.dgate) + to, at.nl, og);
+      } else {
+        gs_store_step<F, NT>(static_cast<TG*>(p.dgate) + to, at.nl, og);
+      }
+    }
+  };
+  if (full) finish(std::true_type{});
+  else finish(std::false_type{});
+  if (tile + 1 == sp.tiles && p.last && at.state_on) p.last[at.state] = P;
+}
+
 }  // namespace mpy
 
 using namespace mpy;
@@ -89,7 +206,25 @@ int musapy_gated_scan_grad_v1(const musapy_gated_scan_args* p, void* scratch, si
   if (pl.rows == 0 || pl.a.D == 0) return 0;
   const int V = pl.lanes ? gs_vector(p->dtype) : 1;
   gs_vectors(pl, V);
+  const GsRoute r = gs_route(pl, V);
+  if (!r.walk) {
+    GsSplit sp{};
+    if (!gs_split(sp, r, scratch, scratch_bytes, workspace, workspace_bytes, st)) return -1;
+    const bool nt = uint64_t(pl.a.nvec) * pl.a.T * 16 >= kStreamLoadBytes;
+    gs_types(p->dtype, p->gate_dtype, [&](auto tx, auto tg) {
+      using TX = decltype(tx);
+      using TG = decltype(tg);
+      gs_flags([&](auto BLEND, auto RESET, auto SPLIT, auto NT) {
+        k_gs_grad_tiles<TX, TG, BLEND.value, RESET.value, SPLIT.value, NT.value><<<gs_grid(sp), kGsBlock, 0, st>>>(pl.a, sp);
+      }, p->kind == MUSAPY_SCAN_BLEND, p->reset != nullptr, r.tiles > 1, nt);
+    });
+    return 0;
+  }
   const unsigned grid = unsigned((uint64_t(pl.a.nvec) + kGsBlock - 1) / kGsBlock);
+  if (!grid_fits(grid, kGsBlock)) {
+    g_wrapper_error = 6;
+    return -1;
+  }
   gs_types(p->dtype, p->gate_dtype, [&](auto tx, auto tg) {
     using TX = decltype(tx);
     using TG = decltype(tg);
