@@ -18,21 +18,51 @@ struct DropArgs {
   float scale;
 };
 
-// One thread per group of eight columns: one call of the generator.
-template <class T>
+// A thread takes kDropGroups groups of eight columns, one call of the generator each, a workgroup's width
+// apart: their loads are all in flight before the first is used.  UNIT: the columns are unit-stride.
+constexpr int kDropGroups = 4;
+
+template <class T, bool UNIT, bool NT>
 __global__ __launch_bounds__(kDropBlock) void k_dropout(const T* __restrict__ a, T* __restrict__ out, DropArgs p) {
-  const uint64_t q = uint64_t(blockIdx.x) * kDropBlock + threadIdx.x;
-  if (q >= p.total) return;
-  const uint32_t row = fd_div(p.gdiv, uint32_t(q));
-  const uint32_t g = uint32_t(q) - row * p.groups;
-  const uint64_t col = uint64_t(g) * 8;
-  int64_t off[1];
-  row_offsets<1>(p.ix, row, off);
-  const T* in = a + off[0] + int64_t(col) * p.ls;
-  T* o = out + uint64_t(row) * p.width + col;
-  const uint32_t keep = philox_keep8(p.key, g, row, p.threshold);
-  const int n = p.width - col < 8 ? int(p.width - col) : 8;
-  for (int e = 0; e < n; ++e) o[e] = (keep >> e) & 1 ? T(float(in[e * p.ls]) * p.scale) : T(0.0f);
+  const uint64_t first = uint64_t(blockIdx.x) * (kDropBlock * kDropGroups) + threadIdx.x;
+  Vec<T, 8> w[kDropGroups];
+  uint32_t row[kDropGroups], g[kDropGroups];
+  int n[kDropGroups];
+#pragma unroll
+  for (int i = 0; i < kDropGroups; ++i) {
+    const uint64_t q = first + uint64_t(i) * kDropBlock;
+    n[i] = 0;
+    if (q >= p.total) continue;
+    row[i] = fd_div(p.gdiv, uint32_t(q));
+    g[i] = uint32_t(q) - row[i] * p.groups;
+    const uint64_t col = uint64_t(g[i]) * 8;
+    n[i] = p.width - col < 8 ? int(p.width - col) : 8;
+    int64_t off[1];
+    row_offsets<1>(p.ix, row[i], off);
+    const T* in = a + off[0] + int64_t(col) * p.ls;
+    if (UNIT && n[i] == 8) {
+      w[i] = vload_el<T, 8, NT>(in);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < n[i]) w[i].v[e] = in[e * p.ls];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kDropGroups; ++i) {
+    if (n[i] == 0) continue;
+    const uint32_t keep = philox_keep8(p.key, g[i], row[i], p.threshold);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[i].v[e] = (keep >> e) & 1 ? T(float(w[i].v[e]) * p.scale) : T(0.0f);
+    T* o = out + uint64_t(row[i]) * p.width + uint64_t(g[i]) * 8;
+    if (n[i] == 8) {
+      vstore_el<NT, T, 8>(o, w[i]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < n[i]) o[e] = w[i].v[e];
+    }
+  }
 }
 
 template <class T>
@@ -75,8 +105,13 @@ int launch_dropout(const void* a, void* out, int ndim, const size_t* shape, cons
   p.key = philox_key(seed, offset);
   p.threshold = threshold;
   p.scale = dropout_scale(threshold);
-  k_dropout<T><<<unsigned((uint64_t(p.total) + kDropBlock - 1) / kDropBlock), kDropBlock, 0, st>>>(
-      static_cast<const T*>(a), static_cast<T*>(out), p);
+  const unsigned grid = unsigned((uint64_t(p.total) + kDropBlock * kDropGroups - 1) / (kDropBlock * kDropGroups));
+  auto go = [&](auto UNIT, auto NT) {
+    k_dropout<T, UNIT.value, NT.value><<<grid, kDropBlock, 0, st>>>(static_cast<const T*>(a), static_cast<T*>(out), p);
+  };
+  if (p.ls != 1 && width > 1) go(std::false_type{}, std::false_type{});
+  else if (rows * width * sizeof(T) >= kStreamLoadBytes) go(std::true_type{}, std::true_type{});
+  else go(std::true_type{}, std::false_type{});
   return 0;
 }
 

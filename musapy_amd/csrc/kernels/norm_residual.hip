@@ -8,6 +8,9 @@
 #include "kcommon.hpp"
 #include "philox.hpp"
 
+#ifndef NRW
+#define NRW
+#endif
 namespace mpy {
 
 using bf16 = __bf16;
@@ -25,7 +28,8 @@ struct NrArgs {
   const void *x, *res, *gate, *dr, *dy, *w1, *scale, *w2;
   int64_t xp, resp, gatep, drp, dyp;
   void *r, *y, *dx, *dres, *dgate;
-  float* part;       // column sums of each block: [block][3][width] (dw1, ds, dw2)
+  float* part;       // column sums of each worker: [worker][3][width] (dw1, ds, dw2)
+  uint32_t workers;  // workgroups, or waves, that go from row to row
 };
 
 __device__ inline float nr_sigmoid(float g) {
@@ -35,7 +39,9 @@ __device__ inline float nr_sigmoid(float g) {
 }
 // act(g) and its derivative
 __device__ inline void nr_act(int kind, float g, float& a, float& slope) {
-  const float s = nr_sigmoid(g), rest = nr_sigmoid(-g);
+  const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(g));
+  const float r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
+  const float s = g >= 0.0f ? r : er, rest = g >= 0.0f ? er : r;
   if (kind == MUSAPY_GATE_SILU) {
     a = g * s;
     slope = __builtin_fmaf(a, rest, s);
@@ -62,6 +68,8 @@ __device__ inline float nr_block_sum(float v, float* sm) {
 
 constexpr int kNrBlock = 256;
 
+// ---- rows of any width ----------------------------------------------------------------------------
+// Rows that do not fit a workgroup's registers are read again for every sum: one workgroup a row.
 template <class T, class TS>
 struct NrRow {  // one row of a call, evaluated element by element
   const NrArgs& p;
@@ -208,22 +216,450 @@ __global__ __launch_bounds__(kNrBlock) void k_nr_grad(NrArgs p) {
   }
 }
 
-// Column sums over the blocks' partial sums, in the blocks' order.
+// ---- rows in registers ------------------------------------------------------------------------------
+// A thread holds NV vectors of eight columns of a row (the columns of one call of the random
+// generator), and a workgroup of as many waves as that takes goes from row to row.  With one vector
+// a thread (rows of up to 8192) the next row's loads are in flight while this one's is summed, and
+// weights stay in registers across rows, as the gradient's column sums always do; with two (up to 16384)
+// there is no room for that.  WAVE: rows of up to 512 columns, a wave each and no barriers.  LAYER: one
+// of the norms is a layer norm.
+
+// Hides where a value comes from, so that its conversion is done again instead of kept in registers.
 template <class T>
-__global__ __launch_bounds__(kNrBlock) void k_nr_columns(const float* part, uint32_t blocks, uint32_t width, bool f32, void* o0,
+__device__ inline void nr_opaque(Vec<T, 8>& w) {
+  uint32_t r[sizeof(w) / 4];
+  __builtin_memcpy(r, &w, sizeof(w));
+#pragma unroll
+  for (int i = 0; i < int(sizeof(w) / 4); ++i) asm volatile("" : "+v"(r[i]));
+  __builtin_memcpy(&w, r, sizeof(w));
+}
+
+// Sum over a wave, the same in every lane: DPP moves within rows of 16 lanes and across them.
+template <int CTRL, int MASK>
+__device__ inline float nr_dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, MASK, 0xf, false));
+}
+__device__ inline float nr_wave_sum(float v) {
+  v += nr_dpp<0x111, 0xf>(v);  // row_shr:1
+  v += nr_dpp<0x112, 0xf>(v);  // row_shr:2
+  v += nr_dpp<0x114, 0xf>(v);  // row_shr:4
+  v += nr_dpp<0x118, 0xf>(v);  // row_shr:8
+  v += nr_dpp<0x142, 0xa>(v);  // row_bcast:15
+  v += nr_dpp<0x143, 0xc>(v);  // row_bcast:31
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// Sums of N values over the threads of a row.  Every wave reads the (up to 16) waves' sums with one
+// load and adds them by rotations of 16 lanes.  The two halves of `sm` alternate, so that one barrier
+// a sum is enough.
+template <int N, bool WAVE>
+__device__ inline void nr_sums_of(float (&v)[N], float (*sm)[4][16], int& half, int waves) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = nr_wave_sum(v[i]);
+  if constexpr (!WAVE) {
+    const int wv = threadIdx.x / kWave, l = threadIdx.x % 16;
+    if (threadIdx.x % kWave == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) sm[half][i][wv] = v[i];
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = sm[half][i][l];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = l < waves ? v[i] : 0.0f;
+      v[i] += nr_dpp<0x128, 0xf>(v[i]);  // row_ror:8
+      v[i] += nr_dpp<0x124, 0xf>(v[i]);  // row_ror:4
+      v[i] += nr_dpp<0x122, 0xf>(v[i]);  // row_ror:2
+      v[i] += nr_dpp<0x121, 0xf>(v[i]);  // row_ror:1
+    }
+    half ^= 1;
+  }
+}
+// (the hardware's reciprocal square root is within 1 ulp)
+__device__ inline float nr_rsqrt(float v) { return __builtin_amdgcn_rsqf(v); }
+
+// Columns 8 j .. 8 j + n - 1 of a row; zeros where there are none.
+template <bool NT, class T>
+__device__ inline Vec<T, 8> nr_load(const T* row, uint32_t j, int n) {
+  if (n == 8) return vload_el<T, 8, NT>(row + uint64_t(j) * 8);
+  Vec<T, 8> w;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w.v[e] = e < n ? row[uint64_t(j) * 8 + e] : T(0.0f);
+  return w;
+}
+template <bool NT, class T>
+__device__ inline void nr_store(T* row, uint32_t j, int n, const float (&x)[8]) {
+  if (n == 8) {
+    Vec<T, 8> w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w.v[e] = T(x[e]);
+    vstore_el<NT, T, 8>(row + uint64_t(j) * 8, w);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) row[uint64_t(j) * 8 + e] = T(x[e]);
+  }
+}
+template <class T>
+__device__ inline void nr_load_weight(const void* w, bool f32, uint32_t j, int n, float (&o)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = e < n ? nr_weight<T>(w, f32, j * 8 + e) : 0.0f;
+}
+
+// Where a thread works: its row, the rows' step, and its vectors' widths.
+template <int NV, bool WAVE>
+struct NrPlace {
+  uint32_t t, threads, row, step;
+  int waves, n[NV];
+  __device__ explicit NrPlace(uint32_t width) {
+    threads = WAVE ? kWave : blockDim.x;
+    waves = int(threads / kWave);
+    t = WAVE ? threadIdx.x % kWave : threadIdx.x;
+    const uint32_t per = WAVE ? blockDim.x / kWave : 1;
+    row = blockIdx.x * per + (WAVE ? threadIdx.x / kWave : 0);
+    step = gridDim.x * per;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = vec(i) * 8;
+      n[i] = c >= width ? 0 : width - c < 8 ? int(width - c) : 8;
+    }
+  }
+  __device__ uint32_t vec(int i) const { return t + uint32_t(i) * threads; }
+};
+
+template <class T, class TS, int NV, int BS, bool WAVE, bool LAYER, bool NT>
+__global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
+  __shared__ float sm[2][4][16];
+  const NrPlace<NV, WAVE> at(p.width);
+  int half = 0;
+  constexpr bool kAhead = NV == 1;
+  float w1[8], sc[8], w2[8];
+  auto weights = [&](int i) {
+    nr_load_weight<T>(p.w1, p.weight_f32, at.vec(i), at.n[i], w1);
+    nr_load_weight<T>(p.scale, p.weight_f32, at.vec(i), at.n[i], sc);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sc[e] *= p.scale_value;
+  };
+  auto pre_weights = [&](int i) { nr_load_weight<T>(p.w2, p.weight_f32, at.vec(i), at.n[i], w2); };
+  if (kAhead) {
+    weights(0);
+    pre_weights(0);
+  }
+  Vec<T, 8> nx[NV], ng[NV];
+  Vec<TS, 8> nres[NV];
+  auto load = [&](uint32_t row) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      nx[i] = nr_load<NT>(static_cast<const T*>(p.x) + int64_t(row) * p.xp, at.vec(i), at.n[i]);
+      if (p.gate) ng[i] = nr_load<NT>(static_cast<const T*>(p.gate) + int64_t(row) * p.gatep, at.vec(i), at.n[i]);
+      if (p.res) nres[i] = nr_load<NT>(static_cast<const TS*>(p.res) + int64_t(row) * p.resp, at.vec(i), at.n[i]);
+    }
+  };
+  const float over = 1.0f / float(p.width);
+  if (kAhead && at.row < p.rows) load(at.row);
+  for (uint32_t row = at.row; row < p.rows; row += at.step) {
+    if (!kAhead) load(row);
+    Vec<T, 8> g[NV];
+    Vec<TS, 8> res[NV];
+    float u[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      g[i] = ng[i];
+      res[i] = nres[i];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[i][e] = float(nx[i].v[e]);
+    }
+    if (kAhead && row + at.step < p.rows) load(row + at.step);
+    // mean and 1 / deviation of `v`, which is left centred
+    auto stats = [&](int kind, float (&v)[NV][8]) {
+      if (LAYER && kind == MUSAPY_NORM_LAYER) {
+        float s[1] = {0.0f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[0] += v[i][e];
+        nr_sums_of<1, WAVE>(s, sm, half, at.waves);
+        const float mean = s[0] * over;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[i][e] = e < at.n[i] ? v[i][e] - mean : 0.0f;
+      }
+      float q[1] = {0.0f};
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[0] = __builtin_fmaf(v[i][e], v[i][e], q[0]);
+      nr_sums_of<1, WAVE>(q, sm, half, at.waves);
+      return nr_rsqrt(q[0] * over + p.eps);
+    };
+    const float inv1 = p.post != MUSAPY_NORM_NONE ? stats(p.post, u) : 1.0f;
+    const uint64_t base = uint64_t(row) * p.width;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (!kAhead) weights(i);
+      const uint32_t keep = p.threshold ? philox_keep8(p.key, at.vec(i), row, p.threshold) : 0xffu;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float v = u[i][e] * inv1 * w1[e];
+        if (p.gate) {
+          const float gv = float(g[i].v[e]), s = nr_sigmoid(gv);
+          v *= p.gate_kind == MUSAPY_GATE_SILU ? gv * s : s;
+        }
+        v = (keep >> e) & 1 ? v * p.keep_scale : 0.0f;
+        u[i][e] = __builtin_fmaf(sc[e], v, p.res ? float(res[i].v[e]) : 0.0f);
+      }
+      nr_store<NT>(static_cast<TS*>(p.r) + base, at.vec(i), at.n[i], u[i]);
+    }
+    if (p.y) {
+      const float inv2 = stats(p.pre, u);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (!kAhead) pre_weights(i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[i][e] = u[i][e] * inv2 * w2[e];
+        nr_store<NT>(static_cast<T*>(p.y) + base, at.vec(i), at.n[i], u[i]);
+      }
+    }
+  }
+}
+
+// The gradient.  With m the mean (0 for rms norms) the sums that depend on the row's inputs alone,
+// (x - m)^2, (r - m)^2, dy w2 (r - m) and dy w2, are formed in one round; those of the post norm's input
+// gradient, which need D, in a second.
+template <class T, class TS, int NV, int BS, bool WAVE, bool LAYER, bool NT>
+__global__ __launch_bounds__(BS) NRW void k_nr_grad_rows(NrArgs p) {
+  __shared__ float sm[2][4][16];
+  const NrPlace<NV, WAVE> at(p.width);
+  int half = 0;
+  constexpr bool kAhead = NV == 1;
+  float w1[8], sc[8], w2[8], a1[NV][8], as[NV][8], a2[NV][8];
+  auto weights = [&](int i) {
+    nr_load_weight<T>(p.w1, p.weight_f32, at.vec(i), at.n[i], w1);
+    nr_load_weight<T>(p.scale, p.weight_f32, at.vec(i), at.n[i], sc);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sc[e] *= p.scale_value * p.keep_scale;
+  };
+  auto pre_weights = [&](int i) { nr_load_weight<T>(p.w2, p.weight_f32, at.vec(i), at.n[i], w2); };
+  if (kAhead) {
+    weights(0);
+    pre_weights(0);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a1[i][e] = as[i][e] = a2[i][e] = 0.0f;
+  const bool pre = p.pre != MUSAPY_NORM_NONE;
+  Vec<T, 8> nx[NV], ng[NV], ny[NV];
+  Vec<TS, 8> nr[NV], nd[NV];
+  auto load = [&](uint32_t row) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      nx[i] = nr_load<NT>(static_cast<const T*>(p.x) + int64_t(row) * p.xp, at.vec(i), at.n[i]);
+      if (p.gate) ng[i] = nr_load<NT>(static_cast<const T*>(p.gate) + int64_t(row) * p.gatep, at.vec(i), at.n[i]);
+      if (pre) nr[i] = nr_load<NT>(static_cast<const TS*>(p.res) + int64_t(row) * p.resp, at.vec(i), at.n[i]);
+      if (p.dr) nd[i] = nr_load<NT>(static_cast<const TS*>(p.dr) + int64_t(row) * p.drp, at.vec(i), at.n[i]);
+      if (p.dy) ny[i] = nr_load<NT>(static_cast<const T*>(p.dy) + int64_t(row) * p.dyp, at.vec(i), at.n[i]);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i)  // what is not given is zero
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      nx[i].v[e] = ng[i].v[e] = ny[i].v[e] = T(0.0f);
+      nr[i].v[e] = nd[i].v[e] = TS(0.0f);
+    }
+  const float over = 1.0f / float(p.width);
+  if (kAhead && at.row < p.rows) load(at.row);
+  for (uint32_t row = at.row; row < p.rows; row += at.step) {
+    if (!kAhead) load(row);
+    Vec<T, 8> x[NV], g[NV], y[NV];
+    Vec<TS, 8> r[NV], d[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      x[i] = nx[i];
+      g[i] = ng[i];
+      y[i] = ny[i];
+      r[i] = nr[i];
+      d[i] = nd[i];
+    }
+    if (kAhead && row + at.step < p.rows) load(row + at.step);
+    float m1 = 0.0f, m2 = 0.0f;
+    if constexpr (LAYER) {
+      float s[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          s[0] += float(x[i].v[e]);
+          s[1] += float(r[i].v[e]);
+        }
+      nr_sums_of<2, WAVE>(s, sm, half, at.waves);
+      if (p.post == MUSAPY_NORM_LAYER) m1 = s[0] * over;
+      if (p.pre == MUSAPY_NORM_LAYER) m2 = s[1] * over;
+    }
+    // (columns that are not there hold zeros, and stay zeros when centred)
+    auto xc = [&](int i, int e) {
+      const float v = float(x[i].v[e]);
+      return !LAYER ? v : e < at.n[i] ? v - m1 : 0.0f;
+    };
+    auto rc = [&](int i, int e) {
+      const float v = float(r[i].v[e]);
+      return !LAYER ? v : e < at.n[i] ? v - m2 : 0.0f;
+    };
+    auto dy = [&](int i, int e) { return float(y[i].v[e]); };
+    float inv1 = 1.0f, inv2 = 1.0f, along2 = 0.0f, flat2 = 0.0f;
+    if (pre || p.post != MUSAPY_NORM_NONE) {
+      float s[LAYER ? 4 : 3] = {};
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (!kAhead) pre_weights(i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float a = xc(i, e), b = rc(i, e), q = dy(i, e) * w2[e];
+          s[0] = __builtin_fmaf(a, a, s[0]);
+          s[1] = __builtin_fmaf(b, b, s[1]);
+          s[2] = __builtin_fmaf(q, b, s[2]);
+          if constexpr (LAYER) s[3] += q;
+        }
+        nr_opaque(x[i]);
+        nr_opaque(r[i]);
+        nr_opaque(y[i]);
+      }
+      nr_sums_of<LAYER ? 4 : 3, WAVE>(s, sm, half, at.waves);
+      if (p.post != MUSAPY_NORM_NONE) inv1 = nr_rsqrt(s[0] * over + p.eps);
+      if (pre) {
+        inv2 = nr_rsqrt(s[1] * over + p.eps);
+        along2 = s[2] * inv2 * over;
+        if constexpr (LAYER)
+          if (p.pre == MUSAPY_NORM_LAYER) flat2 = s[3] * over;
+      }
+    }
+    const uint64_t base = uint64_t(row) * p.width;
+    float q1[NV][8], s2[LAYER ? 2 : 1] = {};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t keep = p.threshold ? philox_keep8(p.key, at.vec(i), row, p.threshold) : 0xffu;
+      float D[8], dg[8];
+      if (!kAhead) {
+        weights(i);
+        pre_weights(i);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float n1 = xc(i, e) * inv1, n2 = rc(i, e) * inv2, y1 = dy(i, e);
+        float q = __builtin_fmaf(-n2, along2, y1 * w2[e]);
+        if constexpr (LAYER) q = e < at.n[i] ? q - flat2 : 0.0f;
+        D[e] = __builtin_fmaf(inv2, q, float(d[i].v[e]));
+        const float Dk = (keep >> e) & 1 ? D[e] : 0.0f;
+        float act = 1.0f, slope = 0.0f;
+        if (p.gate) nr_act(p.gate_kind, float(g[i].v[e]), act, slope);
+        const float dv = Dk * sc[e], u = n1 * w1[e];
+        const float du = dv * act;
+        dg[e] = dv * u * slope;
+        a1[i][e] = __builtin_fmaf(du, n1, a1[i][e]);
+        as[i][e] = (keep >> e) & 1 ? __builtin_fmaf(Dk, u * act, as[i][e]) : as[i][e];
+        a2[i][e] = __builtin_fmaf(y1, n2, a2[i][e]);
+        q1[i][e] = du * w1[e];
+        s2[0] = __builtin_fmaf(q1[i][e], n1, s2[0]);
+        if constexpr (LAYER) s2[1] += q1[i][e];
+      }
+      if (p.dres) nr_store<NT>(static_cast<TS*>(p.dres) + base, at.vec(i), at.n[i], D);
+      if (p.dgate) nr_store<NT>(static_cast<T*>(p.dgate) + base, at.vec(i), at.n[i], dg);
+      nr_opaque(x[i]);
+    }
+    if (p.post != MUSAPY_NORM_NONE) {
+      nr_sums_of<LAYER ? 2 : 1, WAVE>(s2, sm, half, at.waves);
+      const float along1 = s2[0] * over * inv1;
+      float flat1 = 0.0f;
+      if constexpr (LAYER)
+        if (p.post == MUSAPY_NORM_LAYER) flat1 = s2[1] * over;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q1[i][e] = inv1 * (__builtin_fmaf(-xc(i, e), along1, q1[i][e]) - flat1);
+    }
+    if (p.dx)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) nr_store<NT>(static_cast<T*>(p.dx) + base, at.vec(i), at.n[i], q1[i]);
+  }
+  if (p.part) {
+    const uint32_t worker = WAVE ? blockIdx.x * (blockDim.x / kWave) + threadIdx.x / kWave : blockIdx.x;
+    if (worker >= p.workers) return;
+    float* const part = p.part + uint64_t(worker) * 3 * p.width;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) as[i][e] *= p.scale_value * p.keep_scale;
+      nr_store<false>(part, at.vec(i), at.n[i], a1[i]);
+      nr_store<false>(part + p.width, at.vec(i), at.n[i], as[i]);
+      nr_store<false>(part + 2 * uint64_t(p.width), at.vec(i), at.n[i], a2[i]);
+    }
+  }
+}
+
+// Column sums over the workers' partial sums: 64 columns a workgroup, each of its four waves a quarter of
+// the workers, joined in order.
+template <class T>
+__global__ __launch_bounds__(kNrBlock) void k_nr_columns(const float* part, uint32_t workers, uint32_t width, bool f32, void* o0,
                                                          void* o1, void* o2) {
-  const uint32_t c = blockIdx.x * kNrBlock + threadIdx.x;
+  __shared__ float sm[kNrBlock / kWave][kWave];
   void* const o = blockIdx.y == 0 ? o0 : blockIdx.y == 1 ? o1 : o2;
-  if (c >= width || o == nullptr) return;
-  float s = 0.0f;
-  for (uint32_t b = 0; b < blocks; ++b) s += part[(uint64_t(b) * 3 + blockIdx.y) * width + c];
-  if (f32) static_cast<float*>(o)[c] = s;
-  else static_cast<T*>(o)[c] = T(s);
+  if (o == nullptr) return;
+  const uint32_t l = threadIdx.x % kWave, wv = threadIdx.x / kWave;
+  const uint32_t c = blockIdx.x * kWave + l;
+  const uint32_t per = (workers + 3) / 4, from = wv * per, to = from + per < workers ? from + per : workers;
+  float s[8] = {};
+  if (c < width) {
+    const float* q = part + uint64_t(blockIdx.y) * width + c;
+    const uint64_t step = 3 * uint64_t(width);
+    uint32_t b = from;
+    for (; b + 8 <= to; b += 8)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += q[(b + i) * step];
+    for (; b < to; ++b) s[0] += q[b * step];
+  }
+  sm[wv][l] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+  __syncthreads();
+  if (wv != 0 || c >= width) return;
+  const float v = (sm[0][l] + sm[1][l]) + (sm[2][l] + sm[3][l]);
+  if (f32) static_cast<float*>(o)[c] = v;
+  else static_cast<T*>(o)[c] = T(v);
 }
 
 namespace {
 
-constexpr uint32_t kNrGradBlocks = 512;
+// How the rows of a call are spread: `threads` to a workgroup, `blocks` of them.
+struct NrRoute {
+  int nv = 0;  // vectors of eight columns to a thread; 0: the kernels for any width
+  bool wave = false;
+  unsigned threads = kNrBlock, blocks = 0;
+  uint32_t workers = 0;
+};
+NrRoute nr_route(const musapy_norm_residual_args* p, bool grad) {
+  NrRoute r;
+  const uint64_t vecs = (p->width + 7) / 8;
+  const uint64_t rows = p->rows;
+  if (vecs > 2048) {
+    r.blocks = r.workers = unsigned(grad ? (rows < 512 ? rows : 512) : rows);
+    return r;
+  }
+  if (vecs <= kWave) {
+    r.nv = 1;
+    r.wave = true;
+    const uint64_t most = grad ? 512 : 2048, want = (rows + 3) / 4;
+    r.blocks = unsigned(want < most ? want : most);
+    r.workers = uint32_t(rows < r.blocks * uint64_t(4) ? rows : r.blocks * uint64_t(4));
+    return r;
+  }
+  r.nv = vecs <= 1024 ? 1 : 2;
+  r.threads = unsigned((vecs + r.nv * kWave - 1) / (r.nv * kWave) * kWave);
+  // forward: about eight rows a workgroup, so that weights are loaded once for them; gradient: as many
+  // workgroups as the CUs hold at a time, since each leaves a row of column sums
+  const uint64_t most = grad ? uint64_t(256) * 1024 / r.threads : rows < 8192 ? rows < 1024 ? rows : 1024 : (rows + 7) / 8;
+  r.blocks = r.workers = unsigned(rows < most ? rows : most);
+  return r;
+}
 
 int nr_bad() {
   g_wrapper_error = 6;
@@ -286,8 +722,14 @@ void nr_types(int dtype, int stream_dtype, Fn&& fn) {
 
 bool nr_sums(const musapy_norm_residual_args* p) { return p->dpost_weight || p->dscale || p->dpre_weight; }
 
-uint32_t nr_grad_blocks(const musapy_norm_residual_args* p) {
-  return uint32_t(p->rows < kNrGradBlocks ? p->rows : kNrGradBlocks);
+// Calls fn with (NV, BS, WAVE) of the kernel for a route.
+template <class Fn>
+void nr_kernel(const NrRoute& r, Fn&& fn) {
+  using std::integral_constant;
+  if (r.wave) return fn(integral_constant<int, 1>{}, integral_constant<int, 256>{}, std::true_type{});
+  if (r.nv == 1 && r.threads <= 512) return fn(integral_constant<int, 1>{}, integral_constant<int, 512>{}, std::false_type{});
+  if (r.nv == 1) return fn(integral_constant<int, 1>{}, integral_constant<int, 1024>{}, std::false_type{});
+  return fn(integral_constant<int, 2>{}, integral_constant<int, 1024>{}, std::false_type{});
 }
 
 }  // namespace
@@ -300,7 +742,7 @@ extern "C" {
 
 size_t musapy_norm_residual_scratch_v1(const musapy_norm_residual_args* p) {
   if (p == nullptr || !nr_sums(p)) return 0;
-  return size_t(nr_grad_blocks(p)) * 3 * p->width * sizeof(float);
+  return size_t(nr_route(p, true).workers) * 3 * p->width * sizeof(float);
 }
 
 int musapy_norm_residual_v1(const musapy_norm_residual_args* p, hipStream_t st) {
@@ -308,8 +750,22 @@ int musapy_norm_residual_v1(const musapy_norm_residual_args* p, hipStream_t st) 
   if (nr_args(p, a) != 0) return -1;
   if (a.rows == 0 || a.width == 0) return 0;
   if (a.x == nullptr || a.r == nullptr) return nr_bad();
+  const NrRoute r = nr_route(p, false);
+  const bool layer = a.post == MUSAPY_NORM_LAYER || a.pre == MUSAPY_NORM_LAYER;
+  const bool nt = uint64_t(a.rows) * a.width * 8 >= kStreamLoadBytes;
   nr_types(p->dtype, p->stream_dtype, [&](auto t, auto ts) {
-    k_nr<decltype(t), decltype(ts)><<<a.rows, kNrBlock, 0, st>>>(a);
+    using T = decltype(t);
+    using TS = decltype(ts);
+    if (r.nv == 0) {
+      k_nr<T, TS><<<r.blocks, r.threads, 0, st>>>(a);
+      return;
+    }
+    nr_kernel(r, [&](auto NV, auto BS, auto WAVE) {
+      with_store_policy(nt, [&](auto NT) {
+        if (layer) k_nr_rows<T, TS, NV.value, BS.value, WAVE.value, true, NT.value><<<r.blocks, r.threads, 0, st>>>(a);
+        else k_nr_rows<T, TS, NV.value, BS.value, WAVE.value, false, NT.value><<<r.blocks, r.threads, 0, st>>>(a);
+      });
+    });
   });
   return 0;
 }
@@ -320,8 +776,10 @@ int musapy_norm_residual_grad_v1(const musapy_norm_residual_args* p, void* scrat
   if (a.width == 0) return 0;
   if (a.rows > 0 && (a.x == nullptr || (a.pre != MUSAPY_NORM_NONE && a.res == nullptr))) return nr_bad();
   if (a.pre == MUSAPY_NORM_NONE) a.dy = nullptr;
-  const uint32_t blocks = nr_grad_blocks(p);
-  if (nr_sums(p) && blocks > 0) {
+  const NrRoute r = nr_route(p, true);
+  const bool layer = a.post == MUSAPY_NORM_LAYER || a.pre == MUSAPY_NORM_LAYER;
+  a.workers = r.workers;
+  if (nr_sums(p) && r.workers > 0) {
     if (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 15) || scratch_bytes < musapy_norm_residual_scratch_v1(p)) {
       g_wrapper_error = 1;
       return -1;
@@ -329,10 +787,20 @@ int musapy_norm_residual_grad_v1(const musapy_norm_residual_args* p, void* scrat
     a.part = static_cast<float*>(scratch);
   }
   nr_types(p->dtype, p->stream_dtype, [&](auto t, auto ts) {
-    if (blocks > 0) k_nr_grad<decltype(t), decltype(ts)><<<blocks, kNrBlock, 0, st>>>(a);
+    using T = decltype(t);
+    using TS = decltype(ts);
+    const bool nt = uint64_t(a.rows) * a.width * 8 >= kStreamLoadBytes;
+    if (r.blocks > 0 && r.nv == 0) k_nr_grad<T, TS><<<r.blocks, r.threads, 0, st>>>(a);
+    else if (r.blocks > 0)
+      nr_kernel(r, [&](auto NV, auto BS, auto WAVE) {
+        with_store_policy(nt, [&](auto NT) {
+          if (layer) k_nr_grad_rows<T, TS, NV.value, BS.value, WAVE.value, true, NT.value><<<r.blocks, r.threads, 0, st>>>(a);
+          else k_nr_grad_rows<T, TS, NV.value, BS.value, WAVE.value, false, NT.value><<<r.blocks, r.threads, 0, st>>>(a);
+        });
+      });
     if (nr_sums(p))
-      k_nr_columns<decltype(t)><<<dim3((a.width + kNrBlock - 1) / kNrBlock, 3), kNrBlock, 0, st>>>(
-          a.part, blocks, a.width, a.weight_f32, p->dpost_weight, p->dscale, p->dpre_weight);
+      k_nr_columns<T><<<dim3((a.width + kWave - 1) / kWave, 3), kNrBlock, 0, st>>>(
+          a.part, r.workers, a.width, a.weight_f32, p->dpost_weight, p->dscale, p->dpre_weight);
   });
   return 0;
 }

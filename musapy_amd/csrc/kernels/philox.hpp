@@ -20,6 +20,8 @@ inline PhiloxKey philox_key(uint64_t seed, uint64_t offset) {
   return PhiloxKey{uint32_t(seed), uint32_t(seed >> 32), uint32_t(offset), uint32_t(offset >> 32)};
 }
 
+__device__ inline uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
+
 // The four words of the counter (c0, c1, c2, c3).  The 64-bit products are one v_mad_u64_u32 each,
 // and the mixing one three-operand v_bitop3 each; the keys are the same for all lanes and stay in
 // scalar registers.
@@ -28,9 +30,9 @@ __device__ inline void philox(const PhiloxKey& key, uint32_t c0, uint32_t c1, ui
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
     const uint64_t p = uint64_t(c0) * 0xD2511F53u, q = uint64_t(c2) * 0xCD9E8D57u;
-    c0 = uint32_t(q >> 32) ^ c1 ^ k0;
+    c0 = xor3(uint32_t(q >> 32), c1, k0);
     c1 = uint32_t(q);
-    c2 = uint32_t(p >> 32) ^ c3 ^ k1;
+    c2 = xor3(uint32_t(p >> 32), c3, k1);
     c3 = uint32_t(p);
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
