@@ -52,7 +52,7 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_walk(GsArgs p) {
 
 // One tile (gated_scan.hpp) a workgroup; SPLIT: several tiles to a chain.
 template <class TX, class TG, bool BLEND, bool RESET, bool SPLIT, bool NT>
-__global__ __launch_bounds__(kGsBlock) void k_gs_tiles(GsArgs p, GsSplit sp) {
+__global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(4))) void k_gs_tiles(GsArgs p, GsSplit sp) {
   constexpr int V = 16 / int(sizeof(TX));
   constexpr int S = kGsS;
   constexpr uint32_t kSteps = kGsTileSteps;
@@ -67,8 +67,8 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_tiles(GsArgs p, GsSplit sp) {
   const TG* gate = static_cast<const TG*>(p.gate) + at.off[kGsGate] + int64_t(t0) * p.ts[kGsGate];
   TX* out = static_cast<TX*>(p.out) + at.off[kGsOut] + int64_t(t0) * p.ts[kGsOut];
 
-  Vec<TX, V> wx[S];
-  Vec<TG, V> wg[S];
+  Pack<TX, V> wx[S];
+  Pack<TG, V> wg[S];
   uint32_t cuts = 0;
   auto load = [&](auto FULL) {
     constexpr bool F = decltype(FULL)::value;
@@ -98,8 +98,8 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_tiles(GsArgs p, GsSplit sp) {
     const bool cut = RESET && ((cuts >> s) & 1);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      a[s][v] = float(wg[s].v[v]);
-      b[s][v] = float(wx[s].v[v]);
+      a[s][v] = pack_get(wg[s], v);
+      b[s][v] = pack_get(wx[s], v);
       if constexpr (BLEND) {
         float rest;
         gs_sigmoid(a[s][v], a[s][v], rest);
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_tiles(GsArgs p, GsSplit sp) {
       const bool cut = RESET && ((cuts >> s) & 1);
 #pragma unroll
       for (int v = 0; v < V; ++v) c[v] = cut ? b[s][v] : __builtin_fmaf(a[s][v], c[v], b[s][v]);
-      gs_store_step<decltype(FULL)::value, NT>(out + s * p.ts[kGsOut], at.nl, c);
+      pack_store<NT>(out + s * p.ts[kGsOut], decltype(FULL)::value ? V : at.nl, c);
     }
   };
   if (full) finish(std::true_type{});

@@ -9,12 +9,10 @@
 #include <tuple>
 
 #include "kcommon.hpp"
+#include "pack.hpp"
 #include "publish.hpp"
 
 namespace mpy {
-
-using bf16 = __bf16;
-using f16 = _Float16;
 
 constexpr int kGsBlock = 256;
 
@@ -91,44 +89,13 @@ __device__ inline void gs_store(T* p, int nl, const float (&x)[V]) {
 // The S steps of a thread as they lie in memory, `p` at the first one.  FULL: all steps and lanes are
 // there; else `steps` and `nl` of them, and `none` in the others' place.
 template <bool FULL, bool NT, class T, int V, int S>
-__device__ inline void gs_load_steps(Vec<T, V> (&w)[S], const T* p, int64_t ts, int64_t ls, int nl, int steps, T none) {
+__device__ inline void gs_load_steps(Pack<T, V> (&w)[S], const T* p, int64_t ts, int64_t ls, int nl, int steps, T none) {
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     const T* at = p + s * ts;
-    if (!FULL && (s >= steps || nl < V)) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) w[s].v[v] = s < steps && v < nl ? at[v * ls] : none;
-    } else if (ls == 0) {
-      const T e = *at;
-#pragma unroll
-      for (int v = 0; v < V; ++v) w[s].v[v] = e;
-    } else {
-      w[s] = vload_el<T, V, NT>(at);
-    }
-  }
-}
-// Hides where a value comes from, so that what was computed from it before is formed again instead
-// of being kept in registers.
-template <class T, int V>
-__device__ inline void gs_opaque(Vec<T, V>& w) {
-  uint32_t r[sizeof(w) / 4];
-  __builtin_memcpy(r, &w, sizeof(w));
-#pragma unroll
-  for (int i = 0; i < int(sizeof(w) / 4); ++i) asm volatile("" : "+v"(r[i]));
-  __builtin_memcpy(&w, r, sizeof(w));
-}
-// Stores one step; FULL: all lanes are there.
-template <bool FULL, bool NT, class T, int V>
-__device__ inline void gs_store_step(T* p, int nl, const float (&x)[V]) {
-  if (FULL || nl == V) {
-    Vec<T, V> w;
-#pragma unroll
-    for (int v = 0; v < V; ++v) w.v[v] = T(x[v]);
-    vstore_el<NT, T, V>(p, w);
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v < nl) p[v] = T(x[v]);
+    if (!FULL && s >= steps) w[s] = pack_all<T, V>(none);
+    else if (ls == 0) w[s] = pack_all<T, V>(*at);
+    else w[s] = pack_load<NT, V>(at, FULL ? V : nl, none);
   }
 }
 

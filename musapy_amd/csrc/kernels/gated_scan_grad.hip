@@ -94,8 +94,8 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_tiles(GsArgs p, GsSplit sp
   const int steps = full ? S : at.nl == 0 || k0 >= p.T ? 0 : p.T - k0 < uint64_t(S) ? int(p.T - k0) : S;
   const int64_t t0 = int64_t(p.T) - 1 - int64_t(k0);
   auto from = [&](auto* base, int o, int64_t t) { return base + at.off[o] + t * p.ts[o]; };
-  Vec<TX, V> wd[S], wh[S], wx[S];
-  Vec<TG, V> wg[S];
+  Pack<TX, V> wd[S], wh[S], wx[S];
+  Pack<TG, V> wg[S];
   uint32_t cuts = 0;
   auto load = [&](auto FULL) {
     constexpr bool F = decltype(FULL)::value;
@@ -129,9 +129,9 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_tiles(GsArgs p, GsSplit sp
     const bool cut = RESET && ((cuts >> s) & 1);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float a = float(wg[s].v[v]), rest;
+      float a = pack_get(wg[s], v), rest;
       if constexpr (BLEND) gs_sigmoid(a, a, rest);
-      H[v] = cut ? 0.0f : a * (float(wd[s].v[v]) + H[v]);
+      H[v] = cut ? 0.0f : a * (pack_get(wd[s], v) + H[v]);
       A[v] = cut ? __builtin_nanf("") : A[v] * a;
     }
   }
@@ -140,8 +140,8 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_tiles(GsArgs p, GsSplit sp
 
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    gs_opaque(wd[s]);
-    gs_opaque(wg[s]);
+    pack_opaque(wd[s]);
+    pack_opaque(wg[s]);
   }
   TX* dx = from(static_cast<TX*>(p.out), kGsOut, t0);
   const int64_t dgate = at.off[kGsDgate] + t0 * p.ts[kGsDgate];
@@ -157,15 +157,15 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_tiles(GsArgs p, GsSplit sp
       float ox[V], og[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        float a = float(wg[s].v[v]), rest = 1.0f;
+        float a = pack_get(wg[s], v), rest = 1.0f;
         if constexpr (BLEND) gs_sigmoid(a, a, rest);
-        float hb = float(wh[s].v[v]);
+        float hb = pack_get(wh[s], v);
         if (!F && k0 + s + 1 == p.T && p.h_first && v < at.nl) hb = p.h_first[at.off[kGsState] + v];
         if (cut) hb = 0.0f;
-        const float G = float(wd[s].v[v]) + c[v];
+        const float G = pack_get(wd[s], v) + c[v];
         if constexpr (BLEND) {
           ox[v] = rest * G;
-          og[v] = G * (hb - float(wx[s].v[v])) * (a * rest);
+          og[v] = G * (hb - pack_get(wx[s], v)) * (a * rest);
         } else {
           ox[v] = G;
           og[v] = cut ? 0.0f : G * hb;
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_tiles(GsArgs p, GsSplit sp
         c[v] = cut ? 0.0f : a * G;
       }
       const bool in = F || s < steps;
-      if (in) gs_store_step<F, NT>(dx - s * p.ts[kGsOut], at.nl, ox);
+      if (in) pack_store<NT>(dx - s * p.ts[kGsOut], F ? V : at.nl, ox);
       const int64_t to = dgate - s * p.ts[kGsDgate];
       if (parts) {
         float sum = 0.0f;
@@ -182,9 +182,9 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_tiles(GsArgs p, GsSplit sp
         for (int m = 1; m < parts; m <<= 1) sum += __shfl_xor(sum, m, kWave);
         if (in && (vec & uint32_t(parts - 1)) == 0) static_cast<float*>(p.dgate)[to + part] = sum;
       } else if (p.dgate_f32) {
-        gs_store_step<F, NT>(static_cast<float*>(p.dgate) + to, at.nl, og);
+        pack_store<NT>(static_cast<float*>(p.dgate) + to, F ? V : at.nl, og);
       } else {
-        gs_store_step<F, NT>(static_cast<TG*>(p.dgate) + to, at.nl, og);
+        pack_store<NT>(static_cast<TG*>(p.dgate) + to, F ? V : at.nl, og);
       }
     }
   };

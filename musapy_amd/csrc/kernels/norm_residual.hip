@@ -6,15 +6,10 @@
 //   dg = dv u act'(g),  dw1 = sum du n1,  ds = sum D d,  dw2 = sum dy n2
 // with norm'(.)(q) = (q - n mean(q n) [- mean(q)]) / deviation, the bracket for layer norms.
 #include "kcommon.hpp"
+#include "pack.hpp"
 #include "philox.hpp"
 
-#ifndef NRW
-#define NRW
-#endif
 namespace mpy {
-
-using bf16 = __bf16;
-using f16 = _Float16;
 
 struct NrArgs {
   int post, pre, gate_kind;
@@ -37,18 +32,14 @@ __device__ inline float nr_sigmoid(float g) {
   const float r = __builtin_amdgcn_rcpf(1.0f + e);
   return g >= 0.0f ? r : e * r;
 }
-// act(g) and its derivative
+// act(g) and its derivative: with m = g (silu) or 1, act = s m and act' = s (1 - s) m [+ s for silu]
 __device__ inline void nr_act(int kind, float g, float& a, float& slope) {
   const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(g));
   const float r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
   const float s = g >= 0.0f ? r : er, rest = g >= 0.0f ? er : r;
-  if (kind == MUSAPY_GATE_SILU) {
-    a = g * s;
-    slope = __builtin_fmaf(a, rest, s);
-  } else {
-    a = s;
-    slope = s * rest;
-  }
+  const bool silu = kind == MUSAPY_GATE_SILU;
+  a = s * (silu ? g : 1.0f);
+  slope = __builtin_fmaf(a, rest, silu ? s : 0.0f);
 }
 
 template <class T>
@@ -217,22 +208,13 @@ __global__ __launch_bounds__(kNrBlock) void k_nr_grad(NrArgs p) {
 }
 
 // ---- rows in registers ------------------------------------------------------------------------------
-// A thread holds NV vectors of eight columns of a row (the columns of one call of the random
-// generator), and a workgroup of as many waves as that takes goes from row to row.  With one vector
-// a thread (rows of up to 8192) the next row's loads are in flight while this one's is summed, and
-// weights stay in registers across rows, as the gradient's column sums always do; with two (up to 16384)
-// there is no room for that.  WAVE: rows of up to 512 columns, a wave each and no barriers.  LAYER: one
-// of the norms is a layer norm.
-
-// Hides where a value comes from, so that its conversion is done again instead of kept in registers.
-template <class T>
-__device__ inline void nr_opaque(Vec<T, 8>& w) {
-  uint32_t r[sizeof(w) / 4];
-  __builtin_memcpy(r, &w, sizeof(w));
-#pragma unroll
-  for (int i = 0; i < int(sizeof(w) / 4); ++i) asm volatile("" : "+v"(r[i]));
-  __builtin_memcpy(&w, r, sizeof(w));
-}
+// A thread holds NV vectors of C columns of a row, and a workgroup of as many waves as that takes goes
+// from row to row.  With one vector a thread the next row's loads are in flight while this one's is
+// summed, and weights stay in registers across rows, as the gradient's column sums always do; with more
+// there is no room for that.  Forward C = 8, the columns of one call of the random generator; the
+// gradient, which holds five inputs, three weights and three sums of a column, C = 4: with 8 it took 180
+// registers, one workgroup of 512 a CU.  WAVE: rows that a wave holds, without barriers.  LAYER: one of
+// the norms is a layer norm.  FULL: the width is a multiple of C, so that every vector is a whole one.
 
 // Sum over a wave, the same in every lane: DPP moves within rows of 16 lanes and across them.
 template <int CTRL, int MASK>
@@ -278,36 +260,24 @@ __device__ inline void nr_sums_of(float (&v)[N], float (*sm)[4][16], int& half, 
 // (the hardware's reciprocal square root is within 1 ulp)
 __device__ inline float nr_rsqrt(float v) { return __builtin_amdgcn_rsqf(v); }
 
-// Columns 8 j .. 8 j + n - 1 of a row; zeros where there are none.
-template <bool NT, class T>
-__device__ inline Vec<T, 8> nr_load(const T* row, uint32_t j, int n) {
-  if (n == 8) return vload_el<T, 8, NT>(row + uint64_t(j) * 8);
-  Vec<T, 8> w;
+template <class T, int C>
+__device__ inline void nr_load_weight(const void* w, bool f32, uint64_t col, int n, float (&o)[C]) {
+  Pack<float, C> p = pack_all<float, C>(n ? 1.0f : 0.0f);
+  if (w != nullptr && n > 0) {
+    if (f32) {
+      p = pack_load<false, C>(static_cast<const float*>(w) + col, n, 0.0f);
+    } else {
+      const Pack<T, C> q = pack_load<false, C>(static_cast<const T*>(w) + col, n, T(0.0f));
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w.v[e] = e < n ? row[uint64_t(j) * 8 + e] : T(0.0f);
-  return w;
-}
-template <bool NT, class T>
-__device__ inline void nr_store(T* row, uint32_t j, int n, const float (&x)[8]) {
-  if (n == 8) {
-    Vec<T, 8> w;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w.v[e] = T(x[e]);
-    vstore_el<NT, T, 8>(row + uint64_t(j) * 8, w);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < n) row[uint64_t(j) * 8 + e] = T(x[e]);
+      for (int e = 0; e < C; ++e) p.w[e] = __builtin_bit_cast(uint32_t, pack_get(q, e));
+    }
   }
-}
-template <class T>
-__device__ inline void nr_load_weight(const void* w, bool f32, uint32_t j, int n, float (&o)[8]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = e < n ? nr_weight<T>(w, f32, j * 8 + e) : 0.0f;
+  for (int e = 0; e < C; ++e) o[e] = pack_get(p, e);
 }
 
 // Where a thread works: its row, the rows' step, and its vectors' widths.
-template <int NV, bool WAVE>
+template <int C, int NV, bool WAVE, bool FULL>
 struct NrPlace {
   uint32_t t, threads, row, step;
   int waves, n[NV];
@@ -316,58 +286,70 @@ struct NrPlace {
     waves = int(threads / kWave);
     t = WAVE ? threadIdx.x % kWave : threadIdx.x;
     const uint32_t per = WAVE ? blockDim.x / kWave : 1;
-    row = blockIdx.x * per + (WAVE ? threadIdx.x / kWave : 0);
+    // the same for the whole wave, which keeps it and the rows' addresses in scalar registers
+    row = WAVE ? blockIdx.x * per + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) : blockIdx.x;
     step = gridDim.x * per;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const uint32_t c = vec(i) * 8;
-      n[i] = c >= width ? 0 : width - c < 8 ? int(width - c) : 8;
+      const uint32_t c = col(i);
+      n[i] = c >= width ? 0 : !FULL && width - c < uint32_t(C) ? int(width - c) : C;
     }
   }
   __device__ uint32_t vec(int i) const { return t + uint32_t(i) * threads; }
+  __device__ bool has(int i) const { return n[i] != 0; }
+  __device__ int count(int i) const { return FULL ? C : n[i]; }  // where it has one
+  __device__ uint32_t col(int i) const { return vec(i) * C; }  // (widths in registers are small: 32-bit offsets)
 };
 
-template <class T, class TS, int NV, int BS, bool WAVE, bool LAYER, bool NT>
+template <class T, class TS, int NV, int BS, bool WAVE, bool LAYER, bool FULL, bool NT>
 __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
   __shared__ float sm[2][4][16];
-  const NrPlace<NV, WAVE> at(p.width);
+  const NrPlace<8, NV, WAVE, FULL> at(p.width);
   int half = 0;
   constexpr bool kAhead = NV == 1;
+  const int kind = p.gate ? p.gate_kind : MUSAPY_GATE_SIGMOID;
   float w1[8], sc[8], w2[8];
   auto weights = [&](int i) {
-    nr_load_weight<T>(p.w1, p.weight_f32, at.vec(i), at.n[i], w1);
-    nr_load_weight<T>(p.scale, p.weight_f32, at.vec(i), at.n[i], sc);
+    nr_load_weight<T>(p.w1, p.weight_f32, at.col(i), at.n[i], w1);
+    nr_load_weight<T>(p.scale, p.weight_f32, at.col(i), at.n[i], sc);
 #pragma unroll
     for (int e = 0; e < 8; ++e) sc[e] *= p.scale_value;
   };
-  auto pre_weights = [&](int i) { nr_load_weight<T>(p.w2, p.weight_f32, at.vec(i), at.n[i], w2); };
+  auto pre_weights = [&](int i) { nr_load_weight<T>(p.w2, p.weight_f32, at.col(i), at.n[i], w2); };
   if (kAhead) {
     weights(0);
     pre_weights(0);
   }
-  Vec<T, 8> nx[NV], ng[NV];
-  Vec<TS, 8> nres[NV];
+  Pack<T, 8> nx[NV], ng[NV];
+  Pack<TS, 8> nres[NV];
   auto load = [&](uint32_t row) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      nx[i] = nr_load<NT>(static_cast<const T*>(p.x) + int64_t(row) * p.xp, at.vec(i), at.n[i]);
-      if (p.gate) ng[i] = nr_load<NT>(static_cast<const T*>(p.gate) + int64_t(row) * p.gatep, at.vec(i), at.n[i]);
-      if (p.res) nres[i] = nr_load<NT>(static_cast<const TS*>(p.res) + int64_t(row) * p.resp, at.vec(i), at.n[i]);
+      if (!at.has(i)) continue;
+      nx[i] = pack_load<NT, 8>(static_cast<const T*>(p.x) + int64_t(row) * p.xp + at.col(i), at.count(i), T(0.0f));
+      if (p.gate) ng[i] = pack_load<NT, 8>(static_cast<const T*>(p.gate) + int64_t(row) * p.gatep + at.col(i), at.count(i), T(0.0f));
+      if (p.res) nres[i] = pack_load<NT, 8>(static_cast<const TS*>(p.res) + int64_t(row) * p.resp + at.col(i), at.count(i), TS(0.0f));
     }
   };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {  // what is not there is zero; no gate: one whose sigmoid is 1
+    nx[i] = pack_all<T, 8>(T(0.0f));
+    ng[i] = pack_all<T, 8>(T(p.gate ? 0.0f : __builtin_inff()));
+    nres[i] = pack_all<TS, 8>(TS(0.0f));
+  }
   const float over = 1.0f / float(p.width);
   if (kAhead && at.row < p.rows) load(at.row);
   for (uint32_t row = at.row; row < p.rows; row += at.step) {
     if (!kAhead) load(row);
-    Vec<T, 8> g[NV];
-    Vec<TS, 8> res[NV];
+    Pack<T, 8> g[NV];
+    Pack<TS, 8> res[NV];
     float u[NV][8];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       g[i] = ng[i];
       res[i] = nres[i];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) u[i][e] = float(nx[i].v[e]);
+      for (int e = 0; e < 8; ++e) u[i][e] = pack_get(nx[i], e);
     }
     if (kAhead && row + at.step < p.rows) load(row + at.step);
     // mean and 1 / deviation of `v`, which is left centred
@@ -402,14 +384,12 @@ __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float v = u[i][e] * inv1 * w1[e];
-        if (p.gate) {
-          const float gv = float(g[i].v[e]), s = nr_sigmoid(gv);
-          v *= p.gate_kind == MUSAPY_GATE_SILU ? gv * s : s;
-        }
+        const float gv = pack_get(g[i], e);
+        v *= nr_sigmoid(gv) * (kind == MUSAPY_GATE_SILU ? gv : 1.0f);
         v = (keep >> e) & 1 ? v * p.keep_scale : 0.0f;
-        u[i][e] = __builtin_fmaf(sc[e], v, p.res ? float(res[i].v[e]) : 0.0f);
+        u[i][e] = __builtin_fmaf(sc[e], v, pack_get(res[i], e));
       }
-      nr_store<NT>(static_cast<TS*>(p.r) + base, at.vec(i), at.n[i], u[i]);
+      if (at.has(i)) pack_store<NT>(static_cast<TS*>(p.r) + base + at.col(i), at.count(i), u[i]);
     }
     if (p.y) {
       const float inv2 = stats(p.pre, u);
@@ -418,7 +398,7 @@ __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
         if (!kAhead) pre_weights(i);
 #pragma unroll
         for (int e = 0; e < 8; ++e) u[i][e] = u[i][e] * inv2 * w2[e];
-        nr_store<NT>(static_cast<T*>(p.y) + base, at.vec(i), at.n[i], u[i]);
+        if (at.has(i)) pack_store<NT>(static_cast<T*>(p.y) + base + at.col(i), at.count(i), u[i]);
       }
     }
   }
@@ -427,20 +407,22 @@ __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
 // The gradient.  With m the mean (0 for rms norms) the sums that depend on the row's inputs alone,
 // (x - m)^2, (r - m)^2, dy w2 (r - m) and dy w2, are formed in one round; those of the post norm's input
 // gradient, which need D, in a second.
-template <class T, class TS, int NV, int BS, bool WAVE, bool LAYER, bool NT>
-__global__ __launch_bounds__(BS) NRW void k_nr_grad_rows(NrArgs p) {
+template <class T, class TS, int NV, int BS, bool WAVE, bool LAYER, bool FULL, bool NT>
+__global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
   __shared__ float sm[2][4][16];
-  const NrPlace<NV, WAVE> at(p.width);
+  constexpr int C = 4;
+  const NrPlace<C, NV, WAVE, FULL> at(p.width);
   int half = 0;
   constexpr bool kAhead = NV == 1;
-  float w1[8], sc[8], w2[8], a1[NV][8], as[NV][8], a2[NV][8];
+  const int kind = p.gate ? p.gate_kind : MUSAPY_GATE_SIGMOID;
+  float w1[C], sc[C], w2[C], a1[NV][C], as[NV][C], a2[NV][C];
   auto weights = [&](int i) {
-    nr_load_weight<T>(p.w1, p.weight_f32, at.vec(i), at.n[i], w1);
-    nr_load_weight<T>(p.scale, p.weight_f32, at.vec(i), at.n[i], sc);
+    nr_load_weight<T>(p.w1, p.weight_f32, at.col(i), at.n[i], w1);
+    nr_load_weight<T>(p.scale, p.weight_f32, at.col(i), at.n[i], sc);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sc[e] *= p.scale_value * p.keep_scale;
+    for (int e = 0; e < C; ++e) sc[e] *= p.scale_value * p.keep_scale;
   };
-  auto pre_weights = [&](int i) { nr_load_weight<T>(p.w2, p.weight_f32, at.vec(i), at.n[i], w2); };
+  auto pre_weights = [&](int i) { nr_load_weight<T>(p.w2, p.weight_f32, at.col(i), at.n[i], w2); };
   if (kAhead) {
     weights(0);
     pre_weights(0);
@@ -448,33 +430,38 @@ __global__ __launch_bounds__(BS) NRW void k_nr_grad_rows(NrArgs p) {
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) a1[i][e] = as[i][e] = a2[i][e] = 0.0f;
+    for (int e = 0; e < C; ++e) a1[i][e] = as[i][e] = a2[i][e] = 0.0f;
   const bool pre = p.pre != MUSAPY_NORM_NONE;
-  Vec<T, 8> nx[NV], ng[NV], ny[NV];
-  Vec<TS, 8> nr[NV], nd[NV];
+  Pack<T, C> nx[NV], ng[NV], ny[NV];
+  Pack<TS, C> nr[NV], nd[NV];
   auto load = [&](uint32_t row) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      nx[i] = nr_load<NT>(static_cast<const T*>(p.x) + int64_t(row) * p.xp, at.vec(i), at.n[i]);
-      if (p.gate) ng[i] = nr_load<NT>(static_cast<const T*>(p.gate) + int64_t(row) * p.gatep, at.vec(i), at.n[i]);
-      if (pre) nr[i] = nr_load<NT>(static_cast<const TS*>(p.res) + int64_t(row) * p.resp, at.vec(i), at.n[i]);
-      if (p.dr) nd[i] = nr_load<NT>(static_cast<const TS*>(p.dr) + int64_t(row) * p.drp, at.vec(i), at.n[i]);
-      if (p.dy) ny[i] = nr_load<NT>(static_cast<const T*>(p.dy) + int64_t(row) * p.dyp, at.vec(i), at.n[i]);
+      if (!at.has(i)) continue;
+      nx[i] = pack_load<NT, C>(static_cast<const T*>(p.x) + int64_t(row) * p.xp + at.col(i), at.count(i), T(0.0f));
+      if (p.gate) ng[i] = pack_load<NT, C>(static_cast<const T*>(p.gate) + int64_t(row) * p.gatep + at.col(i), at.count(i), T(0.0f));
+      if (pre) nr[i] = pack_load<NT, C>(static_cast<const TS*>(p.res) + int64_t(row) * p.resp + at.col(i), at.count(i), TS(0.0f));
+      if (p.dr) nd[i] = pack_load<NT, C>(static_cast<const TS*>(p.dr) + int64_t(row) * p.drp + at.col(i), at.count(i), TS(0.0f));
+      if (p.dy) ny[i] = pack_load<NT, C>(static_cast<const T*>(p.dy) + int64_t(row) * p.dyp + at.col(i), at.count(i), T(0.0f));
     }
   };
 #pragma unroll
-  for (int i = 0; i < NV; ++i)  // what is not given is zero
+  for (int i = 0; i < NV; ++i) {  // what is not there is zero; no gate: one whose sigmoid is 1
+    nx[i] = ny[i] = pack_all<T, C>(T(0.0f));
+    ng[i] = pack_all<T, C>(T(p.gate ? 0.0f : __builtin_inff()));
+    nr[i] = nd[i] = pack_all<TS, C>(TS(0.0f));
+  }
+  const int shift = at.t % 2 * C;
+  uint32_t keeps[NV], later[NV];
+  bool spare = false;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      nx[i].v[e] = ng[i].v[e] = ny[i].v[e] = T(0.0f);
-      nr[i].v[e] = nd[i].v[e] = TS(0.0f);
-    }
+  for (int i = 0; i < NV; ++i) keeps[i] = later[i] = 0xffu;
   const float over = 1.0f / float(p.width);
   if (kAhead && at.row < p.rows) load(at.row);
   for (uint32_t row = at.row; row < p.rows; row += at.step) {
     if (!kAhead) load(row);
-    Vec<T, 8> x[NV], g[NV], y[NV];
-    Vec<TS, 8> r[NV], d[NV];
+    Pack<T, C> x[NV], g[NV], y[NV];
+    Pack<TS, C> r[NV], d[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       x[i] = nx[i];
@@ -490,9 +477,9 @@ __global__ __launch_bounds__(BS) NRW void k_nr_grad_rows(NrArgs p) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          s[0] += float(x[i].v[e]);
-          s[1] += float(r[i].v[e]);
+        for (int e = 0; e < C; ++e) {
+          s[0] += pack_get(x[i], e);
+          s[1] += pack_get(r[i], e);
         }
       nr_sums_of<2, WAVE>(s, sm, half, at.waves);
       if (p.post == MUSAPY_NORM_LAYER) m1 = s[0] * over;
@@ -500,14 +487,14 @@ __global__ __launch_bounds__(BS) NRW void k_nr_grad_rows(NrArgs p) {
     }
     // (columns that are not there hold zeros, and stay zeros when centred)
     auto xc = [&](int i, int e) {
-      const float v = float(x[i].v[e]);
+      const float v = pack_get(x[i], e);
       return !LAYER ? v : e < at.n[i] ? v - m1 : 0.0f;
     };
     auto rc = [&](int i, int e) {
-      const float v = float(r[i].v[e]);
+      const float v = pack_get(r[i], e);
       return !LAYER ? v : e < at.n[i] ? v - m2 : 0.0f;
     };
-    auto dy = [&](int i, int e) { return float(y[i].v[e]); };
+    auto dy = [&](int i, int e) { return pack_get(y[i], e); };
     float inv1 = 1.0f, inv2 = 1.0f, along2 = 0.0f, flat2 = 0.0f;
     if (pre || p.post != MUSAPY_NORM_NONE) {
       float s[LAYER ? 4 : 3] = {};
@@ -515,16 +502,16 @@ __global__ __launch_bounds__(BS) NRW void k_nr_grad_rows(NrArgs p) {
       for (int i = 0; i < NV; ++i) {
         if (!kAhead) pre_weights(i);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < C; ++e) {
           const float a = xc(i, e), b = rc(i, e), q = dy(i, e) * w2[e];
           s[0] = __builtin_fmaf(a, a, s[0]);
           s[1] = __builtin_fmaf(b, b, s[1]);
           s[2] = __builtin_fmaf(q, b, s[2]);
           if constexpr (LAYER) s[3] += q;
         }
-        nr_opaque(x[i]);
-        nr_opaque(r[i]);
-        nr_opaque(y[i]);
+        pack_opaque(x[i]);
+        pack_opaque(r[i]);
+        pack_opaque(y[i]);
       }
       nr_sums_of<LAYER ? 4 : 3, WAVE>(s, sm, half, at.waves);
       if (p.post != MUSAPY_NORM_NONE) inv1 = nr_rsqrt(s[0] * over + p.eps);
@@ -535,25 +522,41 @@ __global__ __launch_bounds__(BS) NRW void k_nr_grad_rows(NrArgs p) {
           if (p.pre == MUSAPY_NORM_LAYER) flat2 = s[3] * over;
       }
     }
+    // A call of the generator covers two threads' columns: of each pair one forms this row's bits and the
+    // other the next row's, and both use both.
+    if (p.threshold) {
+      if (!spare) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const uint32_t k = philox_keep8(p.key, at.vec(i) / 2, at.t % 2 ? row + at.step : row, p.threshold);
+          keeps[i] = uint32_t(__builtin_amdgcn_update_dpp(0, int(k), 0xa0, 0xf, 0xf, true));  // quad_perm 0, 0, 2, 2
+          later[i] = uint32_t(__builtin_amdgcn_update_dpp(0, int(k), 0xf5, 0xf, 0xf, true));  // quad_perm 1, 1, 3, 3
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) keeps[i] = later[i];
+      }
+      spare = !spare;
+    }
     const uint64_t base = uint64_t(row) * p.width;
-    float q1[NV][8], s2[LAYER ? 2 : 1] = {};
+    float q1[NV][C], s2[LAYER ? 2 : 1] = {};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const uint32_t keep = p.threshold ? philox_keep8(p.key, at.vec(i), row, p.threshold) : 0xffu;
-      float D[8], dg[8];
+      const uint32_t keep = keeps[i] >> shift;
+      float D[C], dg[C];
       if (!kAhead) {
         weights(i);
         pre_weights(i);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < C; ++e) {
         const float n1 = xc(i, e) * inv1, n2 = rc(i, e) * inv2, y1 = dy(i, e);
         float q = __builtin_fmaf(-n2, along2, y1 * w2[e]);
         if constexpr (LAYER) q = e < at.n[i] ? q - flat2 : 0.0f;
-        D[e] = __builtin_fmaf(inv2, q, float(d[i].v[e]));
+        D[e] = __builtin_fmaf(inv2, q, pack_get(d[i], e));
         const float Dk = (keep >> e) & 1 ? D[e] : 0.0f;
-        float act = 1.0f, slope = 0.0f;
-        if (p.gate) nr_act(p.gate_kind, float(g[i].v[e]), act, slope);
+        float act, slope;
+        nr_act(kind, pack_get(g[i], e), act, slope);
         const float dv = Dk * sc[e], u = n1 * w1[e];
         const float du = dv * act;
         dg[e] = dv * u * slope;
@@ -564,9 +567,9 @@ __global__ __launch_bounds__(BS) NRW void k_nr_grad_rows(NrArgs p) {
         s2[0] = __builtin_fmaf(q1[i][e], n1, s2[0]);
         if constexpr (LAYER) s2[1] += q1[i][e];
       }
-      if (p.dres) nr_store<NT>(static_cast<TS*>(p.dres) + base, at.vec(i), at.n[i], D);
-      if (p.dgate) nr_store<NT>(static_cast<T*>(p.dgate) + base, at.vec(i), at.n[i], dg);
-      nr_opaque(x[i]);
+      if (p.dres && at.has(i)) pack_store<NT>(static_cast<TS*>(p.dres) + base + at.col(i), at.count(i), D);
+      if (p.dgate && at.has(i)) pack_store<NT>(static_cast<T*>(p.dgate) + base + at.col(i), at.count(i), dg);
+      pack_opaque(x[i]);
     }
     if (p.post != MUSAPY_NORM_NONE) {
       nr_sums_of<LAYER ? 2 : 1, WAVE>(s2, sm, half, at.waves);
@@ -577,11 +580,12 @@ __global__ __launch_bounds__(BS) NRW void k_nr_grad_rows(NrArgs p) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q1[i][e] = inv1 * (__builtin_fmaf(-xc(i, e), along1, q1[i][e]) - flat1);
+        for (int e = 0; e < C; ++e) q1[i][e] = inv1 * (__builtin_fmaf(-xc(i, e), along1, q1[i][e]) - flat1);
     }
     if (p.dx)
 #pragma unroll
-      for (int i = 0; i < NV; ++i) nr_store<NT>(static_cast<T*>(p.dx) + base, at.vec(i), at.n[i], q1[i]);
+      for (int i = 0; i < NV; ++i)
+        if (at.has(i)) pack_store<NT>(static_cast<T*>(p.dx) + base + at.col(i), at.count(i), q1[i]);
   }
   if (p.part) {
     const uint32_t worker = WAVE ? blockIdx.x * (blockDim.x / kWave) + threadIdx.x / kWave : blockIdx.x;
@@ -590,10 +594,11 @@ __global__ __launch_bounds__(BS) NRW void k_nr_grad_rows(NrArgs p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) as[i][e] *= p.scale_value * p.keep_scale;
-      nr_store<false>(part, at.vec(i), at.n[i], a1[i]);
-      nr_store<false>(part + p.width, at.vec(i), at.n[i], as[i]);
-      nr_store<false>(part + 2 * uint64_t(p.width), at.vec(i), at.n[i], a2[i]);
+      for (int e = 0; e < C; ++e) as[i][e] *= p.scale_value * p.keep_scale;
+      if (!at.has(i)) continue;
+      pack_store<false>(part + at.col(i), at.count(i), a1[i]);
+      pack_store<false>(part + p.width + at.col(i), at.count(i), as[i]);
+      pack_store<false>(part + 2 * uint64_t(p.width) + at.col(i), at.count(i), a2[i]);
     }
   }
 }
@@ -631,16 +636,16 @@ namespace {
 
 // How the rows of a call are spread: `threads` to a workgroup, `blocks` of them.
 struct NrRoute {
-  int nv = 0;  // vectors of eight columns to a thread; 0: the kernels for any width
+  int nv = 0;  // vectors to a thread; 0: the kernels for any width
   bool wave = false;
   unsigned threads = kNrBlock, blocks = 0;
   uint32_t workers = 0;
 };
 NrRoute nr_route(const musapy_norm_residual_args* p, bool grad) {
   NrRoute r;
-  const uint64_t vecs = (p->width + 7) / 8;
+  const uint64_t vecs = grad ? (p->width + 3) / 4 : (p->width + 7) / 8;
   const uint64_t rows = p->rows;
-  if (vecs > 2048) {
+  if (p->width > 16384) {
     r.blocks = r.workers = unsigned(grad ? (rows < 512 ? rows : 512) : rows);
     return r;
   }
@@ -652,7 +657,7 @@ NrRoute nr_route(const musapy_norm_residual_args* p, bool grad) {
     r.workers = uint32_t(rows < r.blocks * uint64_t(4) ? rows : r.blocks * uint64_t(4));
     return r;
   }
-  r.nv = vecs <= 1024 ? 1 : 2;
+  r.nv = vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : 4;
   r.threads = unsigned((vecs + r.nv * kWave - 1) / (r.nv * kWave) * kWave);
   // forward: about eight rows a workgroup, so that weights are loaded once for them; gradient: as many
   // workgroups as the CUs hold at a time, since each leaves a row of column sums
@@ -722,14 +727,26 @@ void nr_types(int dtype, int stream_dtype, Fn&& fn) {
 
 bool nr_sums(const musapy_norm_residual_args* p) { return p->dpost_weight || p->dscale || p->dpre_weight; }
 
-// Calls fn with (NV, BS, WAVE) of the kernel for a route.
-template <class Fn>
-void nr_kernel(const NrRoute& r, Fn&& fn) {
+// Calls fn with (NV, BS, WAVE, LAYER, FULL, NT) of the kernel for a call.
+template <int C, class Fn>
+void nr_kernel(const NrRoute& r, const NrArgs& a, Fn&& fn) {
+  using std::false_type;
   using std::integral_constant;
-  if (r.wave) return fn(integral_constant<int, 1>{}, integral_constant<int, 256>{}, std::true_type{});
-  if (r.nv == 1 && r.threads <= 512) return fn(integral_constant<int, 1>{}, integral_constant<int, 512>{}, std::false_type{});
-  if (r.nv == 1) return fn(integral_constant<int, 1>{}, integral_constant<int, 1024>{}, std::false_type{});
-  return fn(integral_constant<int, 2>{}, integral_constant<int, 1024>{}, std::false_type{});
+  using std::true_type;
+  const bool layer = a.post == MUSAPY_NORM_LAYER || a.pre == MUSAPY_NORM_LAYER;
+  const bool nt = uint64_t(a.rows) * a.width * 8 >= kStreamLoadBytes;
+  auto more = [&](auto nv, auto bs, auto wave) {
+    with_store_policy(layer, [&](auto LAYER) {
+      if (a.width % C) fn(nv, bs, wave, LAYER, false_type{}, false_type{});
+      else if (nt) fn(nv, bs, wave, LAYER, true_type{}, true_type{});
+      else fn(nv, bs, wave, LAYER, true_type{}, false_type{});
+    });
+  };
+  if (r.wave) more(integral_constant<int, 1>{}, integral_constant<int, 256>{}, true_type{});
+  else if (r.nv == 1 && r.threads <= 512) more(integral_constant<int, 1>{}, integral_constant<int, 512>{}, false_type{});
+  else if (r.nv == 1) more(integral_constant<int, 1>{}, integral_constant<int, 1024>{}, false_type{});
+  else if (r.nv == 2) more(integral_constant<int, 2>{}, integral_constant<int, 1024>{}, false_type{});
+  else if constexpr (C == 4) more(integral_constant<int, 4>{}, integral_constant<int, 1024>{}, false_type{});
 }
 
 }  // namespace
@@ -751,21 +768,14 @@ int musapy_norm_residual_v1(const musapy_norm_residual_args* p, hipStream_t st) 
   if (a.rows == 0 || a.width == 0) return 0;
   if (a.x == nullptr || a.r == nullptr) return nr_bad();
   const NrRoute r = nr_route(p, false);
-  const bool layer = a.post == MUSAPY_NORM_LAYER || a.pre == MUSAPY_NORM_LAYER;
-  const bool nt = uint64_t(a.rows) * a.width * 8 >= kStreamLoadBytes;
   nr_types(p->dtype, p->stream_dtype, [&](auto t, auto ts) {
     using T = decltype(t);
     using TS = decltype(ts);
-    if (r.nv == 0) {
-      k_nr<T, TS><<<r.blocks, r.threads, 0, st>>>(a);
-      return;
-    }
-    nr_kernel(r, [&](auto NV, auto BS, auto WAVE) {
-      with_store_policy(nt, [&](auto NT) {
-        if (layer) k_nr_rows<T, TS, NV.value, BS.value, WAVE.value, true, NT.value><<<r.blocks, r.threads, 0, st>>>(a);
-        else k_nr_rows<T, TS, NV.value, BS.value, WAVE.value, false, NT.value><<<r.blocks, r.threads, 0, st>>>(a);
+    if (r.nv == 0) k_nr<T, TS><<<r.blocks, r.threads, 0, st>>>(a);
+    else
+      nr_kernel<8>(r, a, [&](auto NV, auto BS, auto WAVE, auto LAYER, auto FULL, auto NT) {
+        k_nr_rows<T, TS, NV.value, BS.value, WAVE.value, LAYER.value, FULL.value, NT.value><<<r.blocks, r.threads, 0, st>>>(a);
       });
-    });
   });
   return 0;
 }
@@ -777,7 +787,6 @@ int musapy_norm_residual_grad_v1(const musapy_norm_residual_args* p, void* scrat
   if (a.rows > 0 && (a.x == nullptr || (a.pre != MUSAPY_NORM_NONE && a.res == nullptr))) return nr_bad();
   if (a.pre == MUSAPY_NORM_NONE) a.dy = nullptr;
   const NrRoute r = nr_route(p, true);
-  const bool layer = a.post == MUSAPY_NORM_LAYER || a.pre == MUSAPY_NORM_LAYER;
   a.workers = r.workers;
   if (nr_sums(p) && r.workers > 0) {
     if (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 15) || scratch_bytes < musapy_norm_residual_scratch_v1(p)) {
@@ -789,14 +798,11 @@ int musapy_norm_residual_grad_v1(const musapy_norm_residual_args* p, void* scrat
   nr_types(p->dtype, p->stream_dtype, [&](auto t, auto ts) {
     using T = decltype(t);
     using TS = decltype(ts);
-    const bool nt = uint64_t(a.rows) * a.width * 8 >= kStreamLoadBytes;
     if (r.blocks > 0 && r.nv == 0) k_nr_grad<T, TS><<<r.blocks, r.threads, 0, st>>>(a);
     else if (r.blocks > 0)
-      nr_kernel(r, [&](auto NV, auto BS, auto WAVE) {
-        with_store_policy(nt, [&](auto NT) {
-          if (layer) k_nr_grad_rows<T, TS, NV.value, BS.value, WAVE.value, true, NT.value><<<r.blocks, r.threads, 0, st>>>(a);
-          else k_nr_grad_rows<T, TS, NV.value, BS.value, WAVE.value, false, NT.value><<<r.blocks, r.threads, 0, st>>>(a);
-        });
+      nr_kernel<4>(r, a, [&](auto NV, auto BS, auto WAVE, auto LAYER, auto FULL, auto NT) {
+        k_nr_grad_rows<T, TS, NV.value, BS.value, WAVE.value, LAYER.value, FULL.value, NT.value>
+            <<<r.blocks, r.threads, 0, st>>>(a);
       });
     if (nr_sums(p))
       k_nr_columns<T><<<dim3((a.width + kWave - 1) / kWave, 3), kNrBlock, 0, st>>>(
