@@ -1,5 +1,5 @@
 // gated_scan.hip -- the gated scan's forward kernels and the planning of both directions, for gfx950.
-#include "gated_scan.hpp"
+#include "gated_scan_rows.hpp"
 
 namespace mpy {
 
@@ -127,6 +127,66 @@ __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(4))) v
   if (tile + 1 == sp.tiles && p.last && at.state_on) p.last[at.state] = P;
 }
 
+// Rows of unit-stride steps (gated_scan_rows.hpp).
+template <class TX, class TG, bool BLEND, bool RESET, int GW, bool SPLIT, bool NT>
+__global__ __launch_bounds__(kGsBlock) void k_gs_rows(GsArgs p, GsSplit sp) {
+  __shared__ GsRowTile sm;
+  uint32_t chain, tile;
+  int64_t off[kGsOps];
+  if (!gs_row_take<GW, SPLIT>(p, sp, sm, chain, tile, off)) return;
+  constexpr uint32_t kSteps = GW * kGsRun;
+  uint64_t t = uint64_t(tile) * kSteps + threadIdx.x % GW * kGsRun;  // the thread's first step
+  auto left = [&](uint64_t at) { return at >= p.T ? 0 : p.T - at < uint64_t(kGsRun) ? int(p.T - at) : kGsRun; };
+  Pack<TX, kGsRun> nx;
+  Pack<TG, kGsRun> ng;
+  uint32_t ncuts = 0;
+  auto load = [&](uint64_t at) {
+    const int n = left(at);
+    nx = gs_load_run<false, NT>(static_cast<const TX*>(p.x) + off[kGsX] + int64_t(at), 1, n, TX(0.0f));
+    ng = gs_load_run<false, NT>(static_cast<const TG*>(p.gate) + off[kGsGate] + int64_t(at) * p.ts[kGsGate], p.ts[kGsGate], n,
+                                TG(BLEND ? __builtin_inff() : 1.0f));
+    if constexpr (RESET)
+      ncuts = gs_load_cuts<false>(p.reset + off[kGsReset] + int64_t(at) * p.ts[kGsReset], p.ts[kGsReset], n);
+  };
+  load(t);
+  float P = p.first ? p.first[off[kGsState]] : 0.0f;
+  int half = 0;
+  for (;;) {
+    float a[kGsRun], b[kGsRun], A = 1.0f, H = 0.0f;
+    const uint32_t cuts = ncuts;
+#pragma unroll
+    for (int e = 0; e < kGsRun; ++e) {
+      a[e] = pack_get(ng, e);
+      b[e] = pack_get(nx, e);
+      if constexpr (BLEND) {
+        float rest;
+        gs_sigmoid(a[e], a[e], rest);
+        b[e] *= rest;
+      }
+      const bool cut = RESET && ((cuts >> e) & 1);
+      H = cut ? b[e] : __builtin_fmaf(a[e], H, b[e]);
+      A = cut ? __builtin_nanf("") : A * a[e];
+    }
+    if (!SPLIT && tile + 1 < sp.tiles) load(t + kSteps);
+    float c = gs_row_state<GW, SPLIT>(sm, half, A, H, P, sp, chain, tile);
+    float h[kGsRun];
+#pragma unroll
+    for (int e = 0; e < kGsRun; ++e) {
+      c = RESET && ((cuts >> e) & 1) ? b[e] : __builtin_fmaf(a[e], c, b[e]);
+      h[e] = c;
+    }
+    const int n = left(t);
+    if (n > 0) gs_store_run<false, NT>(static_cast<TX*>(p.out) + off[kGsOut] + int64_t(t), n, h);
+    if (tile + 1 >= sp.tiles) {
+      if (p.last && threadIdx.x % GW == 0) p.last[off[kGsState]] = P;
+      break;
+    }
+    if (SPLIT) break;
+    ++tile;
+    t += kSteps;
+  }
+}
+
 __global__ void k_gs_clear(uint64_t* w, uint64_t n) {
   for (uint64_t i = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += uint64_t(gridDim.x) * blockDim.x) w[i] = 0;
 }
@@ -233,6 +293,10 @@ bool gs_plan(const musapy_gated_scan_args* p, bool grad, GsPlan& out) {
   auto unit = [&](int o) { return a.ls[o] == 1 || a.D == 1; };
   out.lanes = (!reads_x || unit(kGsX)) && unit(kGsOut) && unit(kGsState) && (unit(kGsGate) || a.ls[kGsGate] == 0) &&
               (p->reset == nullptr || a.ls[kGsReset] == 0 || a.D == 1) && (!grad || (unit(kGsH) && unit(kGsDh)));
+  auto run = [&](int o) { return a.ts[o] == 1; };
+  out.steps = (!reads_x || run(kGsX)) && run(kGsOut) && (run(kGsGate) || a.ts[kGsGate] == 0) &&
+              (p->reset == nullptr || run(kGsReset) || a.ts[kGsReset] == 0) &&
+              (!grad || (run(kGsH) && run(kGsDh) && run(kGsDgate) && !parts));
   a.x = p->x;
   a.gate = p->gate;
   a.reset = p->reset;
@@ -254,26 +318,42 @@ bool gs_plan(const musapy_gated_scan_args* p, bool grad, GsPlan& out) {
   return true;
 }
 
+namespace {
 void gs_vectors(GsPlan& pl, int V) {
   pl.a.nv = (pl.a.D + uint32_t(V) - 1) / uint32_t(V);
   pl.a.nvec = uint32_t(pl.rows) * pl.a.nv;
   pl.a.nvdiv = make_fastdiv(pl.a.nv ? pl.a.nv : 1);
 }
+}  // namespace
 
 constexpr uint64_t kGsHead = kGsShards * kGsCounterWords;  // words in front of the tiles': the ticket counters
 
-GsRoute gs_route(const GsPlan& pl, int V) {
+GsRoute gs_route(GsPlan& pl, int dtype) {
   GsRoute r;
-  if (!pl.lanes || pl.a.T <= 16) return r;
-  r.chains = (uint64_t(pl.a.nvec) + kGsLt - 1) / kGsLt;
-  r.tiles = (pl.a.T + kGsTileSteps - 1) / kGsTileSteps;
-  if (r.tiles > 1) {
-    const uint64_t lanes = kGsLt * uint64_t(V);
+  const uint64_t T = pl.a.T;
+  auto words = [&](uint64_t lanes) {
     r.group_words = (r.tiles + kGsGroup - 1) / kGsGroup * r.chains * lanes;
     r.words = kGsHead + r.chains * r.tiles * lanes + r.group_words;
+  };
+  if (pl.steps && T > 1 && (!pl.lanes || pl.a.D == 1)) {
+    gs_vectors(pl, 1);
+    r.kind = GsRoute::kRows;
+    r.group = T <= 8 * kGsRun ? 8 : T <= uint64_t(kWave) * kGsRun ? kWave : kGsBlock;
+    r.chains = pl.a.nvec;
+    r.tiles = (T + r.group * kGsRun - 1) / (r.group * kGsRun);
+    // fewer rows than the GPU holds workgroups at a time: a workgroup to a tile
+    if (r.tiles > 1 && r.chains < 1024) words(1);
+    if (grid_fits((r.chains + kGsShards) * (r.words ? r.tiles : 1), kGsBlock)) return r;
+    r = GsRoute{};
   }
-  r.walk = !grid_fits((r.chains + kGsShards) * r.tiles, kGsBlock);
-  if (r.walk) r.words = 0;
+  r.V = pl.lanes ? gs_vector(dtype) : 1;
+  gs_vectors(pl, r.V);
+  if (!pl.lanes || T <= 16) return r;
+  r.chains = (uint64_t(pl.a.nvec) + kGsLt - 1) / kGsLt;
+  r.tiles = (T + kGsTileSteps - 1) / kGsTileSteps;
+  if (!grid_fits((r.chains + kGsShards) * r.tiles, kGsBlock)) return r;
+  r.kind = GsRoute::kTiles;
+  if (r.tiles > 1) words(kGsLt * uint64_t(r.V));
   return r;
 }
 
@@ -285,7 +365,7 @@ bool gs_split(GsSplit& sp, const GsRoute& r, void* scratch, size_t scratch_bytes
   sp.per_shard = (sp.chains + sp.shards - 1) / sp.shards;
   sp.sdiv = make_fastdiv(sp.shards);
   sp.pdiv = make_fastdiv(sp.per_shard);
-  if (r.tiles == 1) return true;
+  if (r.words == 0) return true;
   WsSplit ws;
   if (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 7) || scratch_bytes < r.words * 8 ||
       !ws_split(workspace, workspace_bytes, ws)) {
@@ -315,10 +395,8 @@ size_t musapy_gated_scan_scratch_v1(const musapy_gated_scan_args* p, int grad) {
     g_wrapper_error = 0;  // the call itself reports it
     return 0;
   }
-  if (pl.rows == 0 || pl.a.D == 0 || !pl.lanes) return 0;
-  const int V = gs_vector(p->dtype);
-  gs_vectors(pl, V);
-  return gs_route(pl, V).words * 8;
+  if (pl.rows == 0 || pl.a.D == 0) return 0;
+  return gs_route(pl, p->dtype).words * 8;
 }
 
 size_t musapy_gated_scan_parts_v1(const musapy_gated_scan_args* p) {
@@ -340,19 +418,26 @@ int musapy_gated_scan_v1(const musapy_gated_scan_args* p, void* scratch, size_t 
   GsPlan pl;
   if (!gs_plan(p, false, pl)) return -1;
   if (pl.rows == 0 || pl.a.D == 0) return 0;
-  const int V = pl.lanes ? gs_vector(p->dtype) : 1;
-  gs_vectors(pl, V);
-  const GsRoute r = gs_route(pl, V);
-  if (!r.walk) {
+  const GsRoute r = gs_route(pl, p->dtype);
+  const int V = r.V;
+  if (r.kind != GsRoute::kWalk) {
     GsSplit sp{};
     if (!gs_split(sp, r, scratch, scratch_bytes, workspace, workspace_bytes, st)) return -1;
-    const bool nt = uint64_t(pl.a.nvec) * pl.a.T * 16 >= kStreamLoadBytes;
+    const unsigned grid = gs_grid(r, sp);
+    const bool nt = pl.rows * pl.a.D * pl.a.T * (p->dtype == MUSAPY_DT_F32 ? 4 : 2) >= kStreamLoadBytes;
     gs_types(p->dtype, p->gate_dtype, [&](auto tx, auto tg) {
       using TX = decltype(tx);
       using TG = decltype(tg);
-      gs_flags([&](auto BLEND, auto RESET, auto SPLIT, auto NT) {
-        k_gs_tiles<TX, TG, BLEND.value, RESET.value, SPLIT.value, NT.value><<<gs_grid(sp), kGsBlock, 0, st>>>(pl.a, sp);
-      }, p->kind == MUSAPY_SCAN_BLEND, p->reset != nullptr, r.tiles > 1, nt);
+      gs_flags([&](auto BLEND, auto RESET, auto NT) {
+        if (r.kind == GsRoute::kRows)
+          gs_row_kernel(r, [&](auto GW, auto SPLIT) {
+            k_gs_rows<TX, TG, BLEND.value, RESET.value, GW.value, SPLIT.value, NT.value><<<grid, kGsBlock, 0, st>>>(pl.a, sp);
+          });
+        else if (r.words)
+          k_gs_tiles<TX, TG, BLEND.value, RESET.value, true, NT.value><<<grid, kGsBlock, 0, st>>>(pl.a, sp);
+        else
+          k_gs_tiles<TX, TG, BLEND.value, RESET.value, false, NT.value><<<grid, kGsBlock, 0, st>>>(pl.a, sp);
+      }, p->kind == MUSAPY_SCAN_BLEND, p->reset != nullptr, nt);
     });
     return 0;
   }

@@ -345,14 +345,12 @@ struct GsPlan {
   GsArgs a;
   uint64_t rows;  // rows of D lanes
   bool lanes;     // the lanes are unit-stride (gate: or shared), resets shared by the lanes
+  bool steps;     // the steps are unit-stride (gate, resets: or shared)
 };
 
 // Checks and normalises a call; false with the wrapper error set when an argument is out of range.
 // Empty calls (no lanes) come back with rows or D equal to 0.
 bool gs_plan(const musapy_gated_scan_args* p, bool grad, GsPlan& out);
-// Splits the lanes into vectors of V.
-void gs_vectors(GsPlan& pl, int V);
-
 inline int gs_vector(int dtype) { return dtype == MUSAPY_DT_F32 ? 4 : 8; }  // 16 bytes of x
 
 // The largest power of two of vectors, up to 8, that divides a row of vectors: neighbouring
@@ -364,18 +362,24 @@ inline int gs_part_shift(uint64_t D, int V) {
   return s;
 }
 
-// How the lanes' tiles are launched, and the scratch that takes.
+// How a call is launched, and the scratch that takes.
 struct GsRoute {
-  bool walk = true;
+  enum Kind { kWalk, kTiles, kRows } kind = kWalk;
+  int V = 1;                               // lanes of a thread
+  int group = 0;                           // kRows: threads of a row
   uint64_t chains = 0, tiles = 0;
-  uint64_t words = 0, group_words = 0;  // of a split scan
+  uint64_t words = 0, group_words = 0;     // of tiles that wait on each other
 };
-GsRoute gs_route(const GsPlan& pl, int V);
+// Chooses the route and splits the lanes into its vectors.
+GsRoute gs_route(GsPlan& pl, int dtype);
 // Fills `sp` in and clears its words on `st`; false (wrapper error 1) without room for them.
 bool gs_split(GsSplit& sp, const GsRoute& r, void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes,
               hipStream_t st);
 
-inline unsigned gs_grid(const GsSplit& sp) { return sp.tiles > 1 ? sp.shards * sp.per_shard * sp.tiles : sp.chains; }
+inline unsigned gs_grid(const GsRoute& r, const GsSplit& sp) {
+  if (r.words) return sp.shards * sp.per_shard * sp.tiles;
+  return r.kind == GsRoute::kRows ? unsigned((r.chains * r.group + kGsBlock - 1) / kGsBlock) : sp.chains;
+}
 
 // Calls fn(TX{}, TG{}) with the element types of x and the gate.
 template <class Fn>

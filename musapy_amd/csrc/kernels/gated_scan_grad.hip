@@ -1,5 +1,5 @@
 // gated_scan_grad.hip -- the gated scan's gradient kernels, for gfx950.
-#include "gated_scan.hpp"
+#include "gated_scan_rows.hpp"
 
 namespace mpy {
 
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
 // and the factors are formed twice, for the tile's map and for its results: registers are dearer here
 // than the second sigmoid.
 template <class TX, class TG, bool BLEND, bool RESET, bool SPLIT, bool NT>
-__global__ __launch_bounds__(kGsBlock) void k_gs_grad_tiles(GsArgs p, GsSplit sp) {
+__global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(3))) void k_gs_grad_tiles(GsArgs p, GsSplit sp) {
   constexpr int V = 16 / int(sizeof(TX));
   constexpr int S = kGsS;
   constexpr uint32_t kSteps = kGsTileSteps;
@@ -193,6 +193,89 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_tiles(GsArgs p, GsSplit sp
   if (tile + 1 == sp.tiles && p.last && at.state_on) p.last[at.state] = P;
 }
 
+// Rows of unit-stride steps (gated_scan_rows.hpp), over reversed time: step k is t = T - 1 - k.
+template <class TX, class TG, bool BLEND, bool RESET, int GW, bool SPLIT, bool NT>
+__global__ __launch_bounds__(kGsBlock) void k_gs_grad_rows(GsArgs p, GsSplit sp) {
+  __shared__ GsRowTile sm;
+  uint32_t chain, tile;
+  int64_t off[kGsOps];
+  if (!gs_row_take<GW, SPLIT>(p, sp, sm, chain, tile, off)) return;
+  constexpr uint32_t kSteps = GW * kGsRun;
+  uint64_t k = uint64_t(tile) * kSteps + threadIdx.x % GW * kGsRun;
+  auto left = [&](uint64_t at) { return at >= p.T ? 0 : p.T - at < uint64_t(kGsRun) ? int(p.T - at) : kGsRun; };
+  Pack<TX, kGsRun> nd, nh, nx;
+  Pack<TG, kGsRun> ng;
+  uint32_t ncuts = 0;
+  auto load = [&](uint64_t at) {
+    const int n = left(at);
+    const int64_t t = int64_t(p.T) - 1 - int64_t(at);
+    nd = gs_load_run<true, NT>(static_cast<const TX*>(p.dh) + off[kGsDh] + t, 1, n, TX(0.0f));
+    // (step t = 0 has no h[t-1])
+    nh = gs_load_run<true, NT>(static_cast<const TX*>(p.h) + off[kGsH] + t - 1, 1, at + n == p.T ? n - 1 : n, TX(0.0f));
+    if constexpr (BLEND) nx = gs_load_run<true, NT>(static_cast<const TX*>(p.x) + off[kGsX] + t, 1, n, TX(0.0f));
+    ng = gs_load_run<true, NT>(static_cast<const TG*>(p.gate) + off[kGsGate] + t * p.ts[kGsGate], p.ts[kGsGate], n,
+                               TG(BLEND ? __builtin_inff() : 1.0f));
+    if constexpr (RESET) ncuts = gs_load_cuts<true>(p.reset + off[kGsReset] + t * p.ts[kGsReset], p.ts[kGsReset], n);
+  };
+  load(k);
+  float P = p.first ? p.first[off[kGsState]] : 0.0f;
+  int half = 0;
+  for (;;) {
+    const uint32_t cuts = ncuts;
+    float a[kGsRun], rest[kGsRun], dh[kGsRun], hb[kGsRun], x[kGsRun], A = 1.0f, H = 0.0f;
+    const int n = left(k);
+#pragma unroll
+    for (int e = 0; e < kGsRun; ++e) {
+      const int j = gs_at<true>(e);
+      a[e] = pack_get(ng, j);
+      rest[e] = 1.0f;
+      dh[e] = pack_get(nd, j);
+      hb[e] = pack_get(nh, j);
+      if constexpr (BLEND) {
+        gs_sigmoid(a[e], a[e], rest[e]);
+        x[e] = pack_get(nx, j);
+      }
+      const bool cut = RESET && ((cuts >> e) & 1);
+      H = cut ? 0.0f : a[e] * (dh[e] + H);
+      A = cut ? __builtin_nanf("") : A * a[e];
+    }
+    if (k + n == p.T && n > 0) {
+      const float first = p.h_first ? p.h_first[off[kGsState]] : 0.0f;
+#pragma unroll
+      for (int e = 0; e < kGsRun; ++e) hb[e] = e == n - 1 ? first : hb[e];
+    }
+    if (!SPLIT && tile + 1 < sp.tiles) load(k + kSteps);
+    float c = gs_row_state<GW, SPLIT>(sm, half, A, H, P, sp, chain, tile);
+    float ox[kGsRun], og[kGsRun];
+#pragma unroll
+    for (int e = 0; e < kGsRun; ++e) {
+      const bool cut = RESET && ((cuts >> e) & 1);
+      const float G = dh[e] + c, h = cut ? 0.0f : hb[e];
+      if constexpr (BLEND) {
+        ox[e] = rest[e] * G;
+        og[e] = G * (h - x[e]) * (a[e] * rest[e]);
+      } else {
+        ox[e] = G;
+        og[e] = cut ? 0.0f : G * h;
+      }
+      c = cut ? 0.0f : a[e] * G;
+    }
+    if (n > 0) {
+      const int64_t t = int64_t(p.T) - 1 - int64_t(k);
+      gs_store_run<true, NT>(static_cast<TX*>(p.out) + off[kGsOut] + t, n, ox);
+      if (p.dgate_f32) gs_store_run<true, NT>(static_cast<float*>(p.dgate) + off[kGsDgate] + t, n, og);
+      else gs_store_run<true, NT>(static_cast<TG*>(p.dgate) + off[kGsDgate] + t, n, og);
+    }
+    if (tile + 1 >= sp.tiles) {
+      if (p.last && threadIdx.x % GW == 0) p.last[off[kGsState]] = P;
+      break;
+    }
+    if (SPLIT) break;
+    ++tile;
+    k += kSteps;
+  }
+}
+
 }  // namespace mpy
 
 using namespace mpy;
@@ -204,19 +287,27 @@ int musapy_gated_scan_grad_v1(const musapy_gated_scan_args* p, void* scratch, si
   GsPlan pl;
   if (!gs_plan(p, true, pl)) return -1;
   if (pl.rows == 0 || pl.a.D == 0) return 0;
-  const int V = pl.lanes ? gs_vector(p->dtype) : 1;
-  gs_vectors(pl, V);
-  const GsRoute r = gs_route(pl, V);
-  if (!r.walk) {
+  const GsRoute r = gs_route(pl, p->dtype);
+  const int V = r.V;
+  if (r.kind != GsRoute::kWalk) {
     GsSplit sp{};
     if (!gs_split(sp, r, scratch, scratch_bytes, workspace, workspace_bytes, st)) return -1;
-    const bool nt = uint64_t(pl.a.nvec) * pl.a.T * 16 >= kStreamLoadBytes;
+    const unsigned grid = gs_grid(r, sp);
+    const bool nt = pl.rows * pl.a.D * pl.a.T * (p->dtype == MUSAPY_DT_F32 ? 4 : 2) >= kStreamLoadBytes;
     gs_types(p->dtype, p->gate_dtype, [&](auto tx, auto tg) {
       using TX = decltype(tx);
       using TG = decltype(tg);
-      gs_flags([&](auto BLEND, auto RESET, auto SPLIT, auto NT) {
-        k_gs_grad_tiles<TX, TG, BLEND.value, RESET.value, SPLIT.value, NT.value><<<gs_grid(sp), kGsBlock, 0, st>>>(pl.a, sp);
-      }, p->kind == MUSAPY_SCAN_BLEND, p->reset != nullptr, r.tiles > 1, nt);
+      gs_flags([&](auto BLEND, auto RESET, auto NT) {
+        if (r.kind == GsRoute::kRows)
+          gs_row_kernel(r, [&](auto GW, auto SPLIT) {
+            k_gs_grad_rows<TX, TG, BLEND.value, RESET.value, GW.value, SPLIT.value, NT.value>
+                <<<grid, kGsBlock, 0, st>>>(pl.a, sp);
+          });
+        else if (r.words)
+          k_gs_grad_tiles<TX, TG, BLEND.value, RESET.value, true, NT.value><<<grid, kGsBlock, 0, st>>>(pl.a, sp);
+        else
+          k_gs_grad_tiles<TX, TG, BLEND.value, RESET.value, false, NT.value><<<grid, kGsBlock, 0, st>>>(pl.a, sp);
+      }, p->kind == MUSAPY_SCAN_BLEND, p->reset != nullptr, nt);
     });
     return 0;
   }
