@@ -466,7 +466,8 @@ uint32_t musapy_kernels_set_spin_limit(uint32_t polls);
  * `last` receives c[0], the gradient of `first`; it may be NULL.  x is not read by DECAY and may be
  * NULL there.
  *
- * x, gate, reset, h (grad) and dh are strided views of `shape` (stride 0 where one is broadcast);
+ * x, gate, reset, h (grad) and dh are strided views of `shape` (stride 0 where one is broadcast; up to
+ * 8 dims, or as many as merge to that);
  * first, last and dlast are C-contiguous over the shape without `axis`; `out` (h, or dx) is
  * C-contiguous over `shape`.  dgate is C-contiguous over `shape` in `dgate_dtype` (gate_dtype or
  * F32) when `parts` is 0.  Where the gate is shared along the last axis (gate stride 0, last axis

@@ -12,7 +12,7 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_walk(GsArgs p) {
   const uint32_t col = (uint32_t(q) - row * p.nv) * V;
   const int nl = p.D - col < uint32_t(V) ? int(p.D - col) : V;
   int64_t off[kGsOps];
-  row_offsets<kGsOps>(p.ix, row, off);
+  gs_row_offsets(p.ix, row, off);
 #pragma unroll
   for (int o = 0; o < kGsOps; ++o) off[o] += int64_t(col) * p.ls[o];
   const TX* x = static_cast<const TX*>(p.x) + off[kGsX];
@@ -276,6 +276,7 @@ bool gs_plan(const musapy_gated_scan_args* p, bool grad, GsPlan& out) {
     for (int o = 0; o < kGsOps; ++o) cst[o][0] = 1;
     n = 1;
   }
+  if (n > kGsRowDims + 1) return gs_bad();
   a.T = p->shape[axis];
   a.D = uint32_t(size[0]);
   out.rows = 1;

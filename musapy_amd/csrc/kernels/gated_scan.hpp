@@ -20,8 +20,28 @@ constexpr int kGsBlock = 256;
 // the scanned axis.
 enum GsOperand { kGsX, kGsGate, kGsReset, kGsOut, kGsState, kGsH, kGsDh, kGsDgate, kGsOps };
 
+// The rows: coalesced non-axis dims but the innermost, innermost first.  (Kernel arguments of a few
+// hundred bytes: with room for 32 dims they were 2.5 KB.)
+constexpr int kGsRowDims = 6;
+struct GsRows {
+  int nd;
+  FastDiv div[kGsRowDims];
+  int64_t stride[kGsOps][kGsRowDims];
+};
+__device__ inline void gs_row_offsets(const GsRows& ix, uint32_t row, int64_t (&off)[kGsOps]) {
+#pragma unroll
+  for (int o = 0; o < kGsOps; ++o) off[o] = 0;
+  for (int i = 0; i < ix.nd; ++i) {
+    const uint32_t q = fd_div(ix.div[i], row);
+    const uint32_t c = row - q * ix.div[i].d;
+    row = q;
+#pragma unroll
+    for (int o = 0; o < kGsOps; ++o) off[o] += int64_t(c) * ix.stride[o][i];
+  }
+}
+
 struct GsArgs {
-  RowIndexer<kGsOps> ix;     // the rows: coalesced non-axis dims but the innermost
+  GsRows ix;
   int64_t ts[kGsOps];        // strides along the scanned axis
   int64_t ls[kGsOps];        // strides along the lanes (the innermost non-axis dim)
   uint64_t T;                // steps
@@ -326,7 +346,7 @@ struct GsPlace {
     const uint32_t qc = q < p.nvec ? q : p.nvec - 1;  // threads past the last vector stand on it and touch nothing
     const uint32_t row = fd_div(p.nvdiv, qc), col = (qc - row * p.nv) * V;
     nl = q >= p.nvec ? 0 : p.D - col < uint32_t(V) ? int(p.D - col) : V;
-    row_offsets<kGsOps>(p.ix, row, off);
+    gs_row_offsets(p.ix, row, off);
 #pragma unroll
     for (int o = 0; o < kGsOps; ++o) off[o] += int64_t(col) * p.ls[o];
     // thread l's vector is the one that lane l belongs to

@@ -14,7 +14,7 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
   const uint32_t col = vec * V;
   const int nl = !on ? 0 : p.D - col < uint32_t(V) ? int(p.D - col) : V;
   int64_t off[kGsOps];
-  row_offsets<kGsOps>(p.ix, row, off);
+  gs_row_offsets(p.ix, row, off);
 #pragma unroll
   for (int o = 0; o < kGsOps; ++o) off[o] += int64_t(col) * p.ls[o];
   float c[V];

@@ -165,7 +165,7 @@ __device__ inline bool gs_row_take(const GsArgs& p, const GsSplit& sp, GsRowTile
     if (chain >= p.nvec) return false;  // a whole group: the others go on
   }
   const uint32_t row = fd_div(p.nvdiv, chain), col = chain - row * p.nv;
-  row_offsets<kGsOps>(p.ix, row, off);
+  gs_row_offsets(p.ix, row, off);
 #pragma unroll
   for (int o = 0; o < kGsOps; ++o) off[o] += int64_t(col) * p.ls[o];
   return true;

@@ -603,17 +603,19 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
   }
 }
 
-// Column sums over the workers' partial sums: 64 columns a workgroup, each of its four waves a quarter of
+// Column sums over the workers' partial sums: 64 columns a workgroup, each of its sixteen waves a part of
 // the workers, joined in order.
+constexpr int kNrColumnWaves = 16;
 template <class T>
-__global__ __launch_bounds__(kNrBlock) void k_nr_columns(const float* part, uint32_t workers, uint32_t width, bool f32, void* o0,
+__global__ __launch_bounds__(kNrColumnWaves * kWave) void k_nr_columns(const float* part, uint32_t workers, uint32_t width, bool f32, void* o0,
                                                          void* o1, void* o2) {
-  __shared__ float sm[kNrBlock / kWave][kWave];
+  __shared__ float sm[kNrColumnWaves][kWave];
   void* const o = blockIdx.y == 0 ? o0 : blockIdx.y == 1 ? o1 : o2;
   if (o == nullptr) return;
   const uint32_t l = threadIdx.x % kWave, wv = threadIdx.x / kWave;
   const uint32_t c = blockIdx.x * kWave + l;
-  const uint32_t per = (workers + 3) / 4, from = wv * per, to = from + per < workers ? from + per : workers;
+  const uint32_t per = (workers + kNrColumnWaves - 1) / kNrColumnWaves;
+  const uint32_t from = wv * per, to = from + per < workers ? from + per : workers;
   float s[8] = {};
   if (c < width) {
     const float* q = part + uint64_t(blockIdx.y) * width + c;
@@ -627,7 +629,9 @@ __global__ __launch_bounds__(kNrBlock) void k_nr_columns(const float* part, uint
   sm[wv][l] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
   __syncthreads();
   if (wv != 0 || c >= width) return;
-  const float v = (sm[0][l] + sm[1][l]) + (sm[2][l] + sm[3][l]);
+  float v = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kNrColumnWaves; ++i) v += sm[i][l];
   if (f32) static_cast<float*>(o)[c] = v;
   else static_cast<T*>(o)[c] = T(v);
 }
@@ -660,9 +664,11 @@ NrRoute nr_route(const musapy_norm_residual_args* p, bool grad) {
   r.nv = vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : 4;
   r.threads = unsigned((vecs + r.nv * kWave - 1) / (r.nv * kWave) * kWave);
   // forward: about eight rows a workgroup, so that weights are loaded once for them; gradient: as many
-  // workgroups as the CUs hold at a time, since each leaves a row of column sums
-  const uint64_t most = grad ? uint64_t(256) * 1024 / r.threads : rows < 8192 ? rows < 1024 ? rows : 1024 : (rows + 7) / 8;
-  r.blocks = r.workers = unsigned(rows < most ? rows : most);
+  // workgroups as the CUs hold at a time (1024 threads of its registers each), since each leaves a row of
+  // column sums.  Either way with as even a number of rows as there can be.
+  const uint64_t most = grad ? uint64_t(256) * (1024 / r.threads) : rows < 8192 ? 1024 : (rows + 7) / 8;
+  const uint64_t per = (rows + most - 1) / most;
+  r.blocks = r.workers = unsigned(per ? (rows + per - 1) / per : 0);
   return r;
 }
 
@@ -805,7 +811,7 @@ int musapy_norm_residual_grad_v1(const musapy_norm_residual_args* p, void* scrat
             <<<r.blocks, r.threads, 0, st>>>(a);
       });
     if (nr_sums(p))
-      k_nr_columns<T><<<dim3((a.width + kWave - 1) / kWave, 3), kNrBlock, 0, st>>>(
+      k_nr_columns<T><<<dim3((a.width + kWave - 1) / kWave, 3), kNrColumnWaves * kWave, 0, st>>>(
           a.part, r.workers, a.width, a.weight_f32, p->dpost_weight, p->dscale, p->dpre_weight);
   });
   return 0;

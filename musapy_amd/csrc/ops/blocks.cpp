@@ -170,6 +170,7 @@ Strides spread(const char* op, const char* what, const Array& a, const Shape& sh
 
 void check_scan(const char* op, const Array& x, const Array& gate, const Array* reset, const Array* state,
                 const char* state_name, size_t axis) {
+  if (x.ndim() > 8) throw ShapeError(std::string(op) + ": x has " + std::to_string(x.ndim()) + " dimensions (at most 8)");
   need_float(op, "x", x.dtype);
   need_dtype_or_f32(op, "gate", gate, x.dtype);
   if (reset) need_dtype(op, "reset", *reset, Dtype::Bool);
