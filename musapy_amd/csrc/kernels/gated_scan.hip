@@ -3,7 +3,8 @@
 
 namespace mpy {
 
-// One thread per V lanes, one step after the other; V = 1 takes any strides.
+// One thread per V lanes, in batches of steps whose loads are all in flight before the first is used;
+// V = 1 takes any strides.
 template <class TX, class TG, bool BLEND, int V>
 __global__ __launch_bounds__(kGsBlock) void k_gs_walk(GsArgs p) {
   const uint64_t q = uint64_t(blockIdx.x) * kGsBlock + threadIdx.x;
@@ -22,26 +23,36 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_walk(GsArgs p) {
   float h[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) h[v] = p.first && v < nl ? p.first[off[kGsState] + v] : 0.0f;
-  for (uint64_t t = 0; t < p.T; ++t) {
-    float b[V], g[V];
-    gs_load<TX, V>(x, p.ls[kGsX], nl, b);
-    gs_load<TG, V>(gate, p.ls[kGsGate], nl, g);
-    const bool cut = reset && *reset;
+  for (uint64_t t = 0; t < p.T; t += kGsBatch) {
+    const int steps = p.T - t < uint64_t(kGsBatch) ? int(p.T - t) : kGsBatch;
+    float b[kGsBatch][V], g[kGsBatch][V];
+    bool cuts[kGsBatch];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float a = g[v], in = b[v];
-      if constexpr (BLEND) {
-        float rest;
-        gs_sigmoid(g[v], a, rest);
-        in = rest * b[v];
-      }
-      h[v] = cut ? in : __builtin_fmaf(a, h[v], in);
+    for (int s = 0; s < kGsBatch; ++s) {
+      if (s >= steps) break;
+      gs_load<TX, V>(x + s * p.ts[kGsX], p.ls[kGsX], nl, b[s]);
+      gs_load<TG, V>(gate + s * p.ts[kGsGate], p.ls[kGsGate], nl, g[s]);
+      cuts[s] = reset && reset[s * p.ts[kGsReset]];
     }
-    gs_store<TX, V>(out, nl, h);
-    x += p.ts[kGsX];
-    gate += p.ts[kGsGate];
-    out += p.ts[kGsOut];
-    if (reset) reset += p.ts[kGsReset];
+#pragma unroll
+    for (int s = 0; s < kGsBatch; ++s) {
+      if (s >= steps) break;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float a = g[s][v], in = b[s][v];
+        if constexpr (BLEND) {
+          float rest;
+          gs_sigmoid(a, a, rest);
+          in = rest * in;
+        }
+        h[v] = cuts[s] ? in : __builtin_fmaf(a, h[v], in);
+      }
+      gs_store<TX, V>(out + s * p.ts[kGsOut], nl, h);
+    }
+    x += kGsBatch * p.ts[kGsX];
+    gate += kGsBatch * p.ts[kGsGate];
+    out += kGsBatch * p.ts[kGsOut];
+    if (reset) reset += kGsBatch * p.ts[kGsReset];
   }
   if (p.last) {
 #pragma unroll
@@ -425,7 +436,7 @@ int musapy_gated_scan_v1(const musapy_gated_scan_args* p, void* scratch, size_t 
     GsSplit sp{};
     if (!gs_split(sp, r, scratch, scratch_bytes, workspace, workspace_bytes, st)) return -1;
     const unsigned grid = gs_grid(r, sp);
-    const bool nt = pl.rows * pl.a.D * pl.a.T * (p->dtype == MUSAPY_DT_F32 ? 4 : 2) >= kStreamLoadBytes;
+    const bool nt = gs_stream(pl, r, p->dtype);
     gs_types(p->dtype, p->gate_dtype, [&](auto tx, auto tg) {
       using TX = decltype(tx);
       using TG = decltype(tg);

@@ -15,6 +15,7 @@
 namespace mpy {
 
 constexpr int kGsBlock = 256;
+constexpr int kGsBatch = 4;  // steps that a thread of the walks loads at a time
 
 // Operands, and their places in the strides.  kGsState is first / last / dlast: x's shape without
 // the scanned axis.
@@ -159,7 +160,9 @@ struct GsSplit {
   // Tickets: one counter for each shard of chains, a cache line apart.  One counter for all took
   // 14 ns a ticket, the rate of atomics on one address: 239 us of the 16384 tiles of (65536, 2048).
   uint64_t* counters;
-  uint32_t shards, per_shard;  // chain = number in the shard * shards + shard
+  // A shard is a run of neighbouring chains, and blocks go to the XCDs in turn: neighbours, which share
+  // cache lines where rows do not start on them, run on one XCD at about the same time.
+  uint32_t shards, per_shard;
   FastDiv sdiv, pdiv;
   uint64_t* words;   // [tile][chain][lane]
   uint64_t* groups;  // [group][chain][lane]
@@ -328,7 +331,7 @@ __device__ inline bool gs_take(const GsSplit& sp, uint32_t& ticket, uint32_t& ch
     __syncthreads();
     const uint32_t t = ticket;
     tile = fd_div(sp.pdiv, t);
-    chain = (t - tile * sp.per_shard) * sp.shards + shard;
+    chain = shard * sp.per_shard + (t - tile * sp.per_shard);
     return chain < sp.chains;
   }
   return true;
@@ -356,7 +359,9 @@ struct GsPlace {
   }
   // all lanes of the chain's vectors are there (the same for the whole workgroup)
   static __device__ bool whole(const GsArgs& p, uint32_t chain) {
-    return p.D % V == 0 && (uint64_t(chain) + 1) * kGsLt <= p.nvec;
+    if ((uint64_t(chain) + 1) * kGsLt > p.nvec) return false;
+    const uint32_t q = chain * kGsLt, at = q - fd_div(p.nvdiv, q) * p.nv;
+    return p.D % V == 0 || at + kGsLt < p.nv;  // (a row's last vector is a part of one)
   }
 };
 
@@ -396,6 +401,13 @@ GsRoute gs_route(GsPlan& pl, int dtype);
 bool gs_split(GsSplit& sp, const GsRoute& r, void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes,
               hipStream_t st);
 
+// Streaming accesses for large calls; not for tiles whose rows' ends share cache lines with their
+// neighbours', which the L2 should keep until those come.
+inline bool gs_stream(const GsPlan& pl, const GsRoute& r, int dtype) {
+  const uint64_t es = dtype == MUSAPY_DT_F32 ? 4 : 2;
+  if (r.kind == GsRoute::kTiles && pl.a.ts[kGsOut] * int64_t(es) % 128 != 0) return false;
+  return pl.rows * pl.a.D * pl.a.T * es >= kStreamLoadBytes;
+}
 inline unsigned gs_grid(const GsRoute& r, const GsSplit& sp) {
   if (r.words) return sp.shards * sp.per_shard * sp.tiles;
   return r.kind == GsRoute::kRows ? unsigned((r.chains * r.group + kGsBlock - 1) / kGsBlock) : sp.chains;

@@ -3,7 +3,8 @@
 
 namespace mpy {
 
-// One thread per V lanes, from the last step to the first; V = 1 takes any strides.
+// One thread per V lanes, from the last step to the first, in batches of steps whose loads are all in
+// flight before the first is used; V = 1 takes any strides.
 template <class TX, class TG, bool BLEND, int V>
 __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
   const uint64_t q = uint64_t(blockIdx.x) * kGsBlock + threadIdx.x;
@@ -20,26 +21,41 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
   float c[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) c[v] = p.first && v < nl ? p.first[off[kGsState] + v] : 0.0f;
-  for (uint64_t k = 0; k < p.T; ++k) {
-    const int64_t t = int64_t(p.T - 1 - k);
-    float dh[V], g[V], hb[V], x[V], dg[V], dx[V];
+  for (uint64_t k0 = 0; k0 < p.T; k0 += kGsBatch) {
+  const int steps = p.T - k0 < uint64_t(kGsBatch) ? int(p.T - k0) : kGsBatch;
+  float bd[kGsBatch][V], bg[kGsBatch][V], bh[kGsBatch][V], bx[kGsBatch][V];
+  bool cuts[kGsBatch];
 #pragma unroll
-    for (int v = 0; v < V; ++v) dh[v] = g[v] = hb[v] = x[v] = 0.0f;
-    bool cut = false;
-    if (on) {
-      gs_load<TX, V>(static_cast<const TX*>(p.dh) + off[kGsDh] + t * p.ts[kGsDh], p.ls[kGsDh], nl, dh);
-      gs_load<TG, V>(static_cast<const TG*>(p.gate) + off[kGsGate] + t * p.ts[kGsGate], p.ls[kGsGate], nl, g);
+  for (int s = 0; s < kGsBatch; ++s) {
+    const int64_t t = int64_t(p.T - 1 - k0) - s;
+#pragma unroll
+    for (int v = 0; v < V; ++v) bd[s][v] = bg[s][v] = bh[s][v] = bx[s][v] = 0.0f;
+    cuts[s] = false;
+    if (s < steps && on) {
+      gs_load<TX, V>(static_cast<const TX*>(p.dh) + off[kGsDh] + t * p.ts[kGsDh], p.ls[kGsDh], nl, bd[s]);
+      gs_load<TG, V>(static_cast<const TG*>(p.gate) + off[kGsGate] + t * p.ts[kGsGate], p.ls[kGsGate], nl, bg[s]);
       if constexpr (BLEND)
-        gs_load<TX, V>(static_cast<const TX*>(p.x) + off[kGsX] + t * p.ts[kGsX], p.ls[kGsX], nl, x);
-      cut = p.reset && p.reset[off[kGsReset] + t * p.ts[kGsReset]];
-      if (!cut) {
-        if (t > 0)
-          gs_load<TX, V>(static_cast<const TX*>(p.h) + off[kGsH] + (t - 1) * p.ts[kGsH], p.ls[kGsH], nl, hb);
-        else if (p.h_first)
+        gs_load<TX, V>(static_cast<const TX*>(p.x) + off[kGsX] + t * p.ts[kGsX], p.ls[kGsX], nl, bx[s]);
+      cuts[s] = p.reset && p.reset[off[kGsReset] + t * p.ts[kGsReset]];
+      if (t > 0)
+        gs_load<TX, V>(static_cast<const TX*>(p.h) + off[kGsH] + (t - 1) * p.ts[kGsH], p.ls[kGsH], nl, bh[s]);
+      else if (p.h_first)
 #pragma unroll
-          for (int v = 0; v < V; ++v) hb[v] = v < nl ? p.h_first[off[kGsState] + v] : 0.0f;
-      }
+        for (int v = 0; v < V; ++v) bh[s][v] = v < nl ? p.h_first[off[kGsState] + v] : 0.0f;
     }
+  }
+#pragma unroll
+  for (int s = 0; s < kGsBatch; ++s) {
+    if (s >= steps) break;
+    const int64_t t = int64_t(p.T - 1 - k0) - s;
+    const bool cut = cuts[s];
+    float dg[V], dx[V];
+    const float(&dh)[V] = bd[s];
+    const float(&g)[V] = bg[s];
+    const float(&x)[V] = bx[s];
+    float hb[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) hb[v] = cut ? 0.0f : bh[s][v];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const float G = dh[v] + c[v];
@@ -68,6 +84,7 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
       if (p.dgate_f32) gs_store<float, V>(static_cast<float*>(p.dgate) + at, nl, dg);
       else gs_store<TG, V>(static_cast<TG*>(p.dgate) + at, nl, dg);
     }
+  }
   }
   if (p.last) {
 #pragma unroll
@@ -293,7 +310,7 @@ int musapy_gated_scan_grad_v1(const musapy_gated_scan_args* p, void* scratch, si
     GsSplit sp{};
     if (!gs_split(sp, r, scratch, scratch_bytes, workspace, workspace_bytes, st)) return -1;
     const unsigned grid = gs_grid(r, sp);
-    const bool nt = pl.rows * pl.a.D * pl.a.T * (p->dtype == MUSAPY_DT_F32 ? 4 : 2) >= kStreamLoadBytes;
+    const bool nt = gs_stream(pl, r, p->dtype);
     gs_types(p->dtype, p->gate_dtype, [&](auto tx, auto tg) {
       using TX = decltype(tx);
       using TG = decltype(tg);

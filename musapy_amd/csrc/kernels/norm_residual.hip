@@ -210,8 +210,8 @@ __global__ __launch_bounds__(kNrBlock) void k_nr_grad(NrArgs p) {
 // ---- rows in registers ------------------------------------------------------------------------------
 // A thread holds NV vectors of C columns of a row, and a workgroup of as many waves as that takes goes
 // from row to row.  With one vector a thread the next row's loads are in flight while this one's is
-// summed, and weights stay in registers across rows, as the gradient's column sums always do; with more
-// there is no room for that.  Forward C = 8, the columns of one call of the random generator; the
+// summed, and weights and the gradient's column sums stay in registers across rows; with more
+// there is no room for that, and the sums stay in LDS.  Forward C = 8, the columns of one call of the random generator; the
 // gradient, which holds five inputs, three weights and three sums of a column, C = 4: with 8 it took 180
 // registers, one workgroup of 512 a CU.  WAVE: rows that a wave holds, without barriers.  LAYER: one of
 // the norms is a layer norm.  FULL: the width is a multiple of C, so that every vector is a whole one.
@@ -415,7 +415,28 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
   int half = 0;
   constexpr bool kAhead = NV == 1;
   const int kind = p.gate ? p.gate_kind : MUSAPY_GATE_SIGMOID;
-  float w1[C], sc[C], w2[C], a1[NV][C], as[NV][C], a2[NV][C];
+  // The column sums: in registers, or, with more vectors, each thread's in LDS.
+  constexpr bool kLds = NV > 1;
+  float w1[C], sc[C], w2[C], a1[C], as[C], a2[C];
+  __shared__ float4 s_sums[kLds ? 3 * NV : 1][kLds ? BS : 1];
+  auto sums = [&](int i, bool store) {
+    if constexpr (kLds) {
+      float* const to[3] = {a1, as, a2};
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        float4& q = s_sums[3 * i + j][threadIdx.x];
+        if (store) {
+          q = float4{to[j][0], to[j][1], to[j][2], to[j][3]};
+        } else {
+          const float4 v = q;
+          to[j][0] = v.x;
+          to[j][1] = v.y;
+          to[j][2] = v.z;
+          to[j][3] = v.w;
+        }
+      }
+    }
+  };
   auto weights = [&](int i) {
     nr_load_weight<T>(p.w1, p.weight_f32, at.col(i), at.n[i], w1);
     nr_load_weight<T>(p.scale, p.weight_f32, at.col(i), at.n[i], sc);
@@ -428,9 +449,11 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
     pre_weights(0);
   }
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
 #pragma unroll
-    for (int e = 0; e < C; ++e) a1[i][e] = as[i][e] = a2[i][e] = 0.0f;
+    for (int e = 0; e < C; ++e) a1[e] = as[e] = a2[e] = 0.0f;
+    sums(i, true);
+  }
   const bool pre = p.pre != MUSAPY_NORM_NONE;
   Pack<T, C> nx[NV], ng[NV], ny[NV];
   Pack<TS, C> nr[NV], nd[NV];
@@ -548,6 +571,7 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
         weights(i);
         pre_weights(i);
       }
+      sums(i, false);
 #pragma unroll
       for (int e = 0; e < C; ++e) {
         const float n1 = xc(i, e) * inv1, n2 = rc(i, e) * inv2, y1 = dy(i, e);
@@ -560,13 +584,14 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
         const float dv = Dk * sc[e], u = n1 * w1[e];
         const float du = dv * act;
         dg[e] = dv * u * slope;
-        a1[i][e] = __builtin_fmaf(du, n1, a1[i][e]);
-        as[i][e] = (keep >> e) & 1 ? __builtin_fmaf(Dk, u * act, as[i][e]) : as[i][e];
-        a2[i][e] = __builtin_fmaf(y1, n2, a2[i][e]);
+        a1[e] = __builtin_fmaf(du, n1, a1[e]);
+        as[e] = (keep >> e) & 1 ? __builtin_fmaf(Dk, u * act, as[e]) : as[e];
+        a2[e] = __builtin_fmaf(y1, n2, a2[e]);
         q1[i][e] = du * w1[e];
         s2[0] = __builtin_fmaf(q1[i][e], n1, s2[0]);
         if constexpr (LAYER) s2[1] += q1[i][e];
       }
+      sums(i, true);
       if (p.dres && at.has(i)) pack_store<NT>(static_cast<TS*>(p.dres) + base + at.col(i), at.count(i), D);
       if (p.dgate && at.has(i)) pack_store<NT>(static_cast<T*>(p.dgate) + base + at.col(i), at.count(i), dg);
       pack_opaque(x[i]);
@@ -593,12 +618,13 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
     float* const part = p.part + uint64_t(worker) * 3 * p.width;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      sums(i, false);
 #pragma unroll
-      for (int e = 0; e < C; ++e) as[i][e] *= p.scale_value * p.keep_scale;
+      for (int e = 0; e < C; ++e) as[e] *= p.scale_value * p.keep_scale;
       if (!at.has(i)) continue;
-      pack_store<false>(part + at.col(i), at.count(i), a1[i]);
-      pack_store<false>(part + p.width + at.col(i), at.count(i), as[i]);
-      pack_store<false>(part + 2 * uint64_t(p.width) + at.col(i), at.count(i), a2[i]);
+      pack_store<false>(part + at.col(i), at.count(i), a1);
+      pack_store<false>(part + p.width + at.col(i), at.count(i), as);
+      pack_store<false>(part + 2 * uint64_t(p.width) + at.col(i), at.count(i), a2);
     }
   }
 }
@@ -649,7 +675,7 @@ NrRoute nr_route(const musapy_norm_residual_args* p, bool grad) {
   NrRoute r;
   const uint64_t vecs = grad ? (p->width + 3) / 4 : (p->width + 7) / 8;
   const uint64_t rows = p->rows;
-  if (p->width > 16384) {
+  if (p->width > (grad ? 12288 : 16384)) {
     r.blocks = r.workers = unsigned(grad ? (rows < 512 ? rows : 512) : rows);
     return r;
   }
@@ -661,7 +687,7 @@ NrRoute nr_route(const musapy_norm_residual_args* p, bool grad) {
     r.workers = uint32_t(rows < r.blocks * uint64_t(4) ? rows : r.blocks * uint64_t(4));
     return r;
   }
-  r.nv = vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : 4;
+  r.nv = int((vecs + 1023) / 1024);
   r.threads = unsigned((vecs + r.nv * kWave - 1) / (r.nv * kWave) * kWave);
   // forward: about eight rows a workgroup, so that weights are loaded once for them; gradient: as many
   // workgroups as the CUs hold at a time (1024 threads of its registers each), since each leaves a row of
@@ -752,7 +778,7 @@ void nr_kernel(const NrRoute& r, const NrArgs& a, Fn&& fn) {
   else if (r.nv == 1 && r.threads <= 512) more(integral_constant<int, 1>{}, integral_constant<int, 512>{}, false_type{});
   else if (r.nv == 1) more(integral_constant<int, 1>{}, integral_constant<int, 1024>{}, false_type{});
   else if (r.nv == 2) more(integral_constant<int, 2>{}, integral_constant<int, 1024>{}, false_type{});
-  else if constexpr (C == 4) more(integral_constant<int, 4>{}, integral_constant<int, 1024>{}, false_type{});
+  else if constexpr (C == 4) more(integral_constant<int, 3>{}, integral_constant<int, 1024>{}, false_type{});
 }
 
 }  // namespace
