@@ -25,21 +25,19 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_walk(GsArgs p) {
   for (int v = 0; v < V; ++v) h[v] = p.first && v < nl ? p.first[off[kGsState] + v] : 0.0f;
   for (uint64_t t = 0; t < p.T; t += kGsBatch) {
     const int steps = p.T - t < uint64_t(kGsBatch) ? int(p.T - t) : kGsBatch;
-    float b[kGsBatch][V], g[kGsBatch][V];
+    GsBatch<TX, V> b;
+    GsBatch<TG, V> g;
     bool cuts[kGsBatch];
+    b.load(x, p.ts[kGsX], p.ls[kGsX], nl, steps);
+    g.load(gate, p.ts[kGsGate], p.ls[kGsGate], nl, steps);
 #pragma unroll
-    for (int s = 0; s < kGsBatch; ++s) {
-      if (s >= steps) break;
-      gs_load<TX, V>(x + s * p.ts[kGsX], p.ls[kGsX], nl, b[s]);
-      gs_load<TG, V>(gate + s * p.ts[kGsGate], p.ls[kGsGate], nl, g[s]);
-      cuts[s] = reset && reset[s * p.ts[kGsReset]];
-    }
+    for (int s = 0; s < kGsBatch; ++s) cuts[s] = reset && s < steps && reset[s * p.ts[kGsReset]];
 #pragma unroll
     for (int s = 0; s < kGsBatch; ++s) {
       if (s >= steps) break;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        float a = g[s][v], in = b[s][v];
+        float a = g.get(s, v), in = b.get(s, v);
         if constexpr (BLEND) {
           float rest;
           gs_sigmoid(a, a, rest);

@@ -74,25 +74,6 @@ __device__ inline void gs_sigmoid(float g, float& s, float& rest) {
   rest = g >= 0.0f ? er : r;
 }
 
-// V consecutive lanes as f32: from a vector, from one shared element (lane stride 0), or element by
-// element (the last lanes of a row).
-template <class T, int V>
-__device__ inline void gs_load(const T* p, int64_t ls, int nl, float (&o)[V]) {
-  if constexpr (V == 1) {
-    o[0] = float(*p);
-  } else if (ls == 0) {
-    const float e = float(*p);
-#pragma unroll
-    for (int v = 0; v < V; ++v) o[v] = e;
-  } else if (nl == V) {
-    const Vec<T, V> w = vload_el<T, V, false>(p);
-#pragma unroll
-    for (int v = 0; v < V; ++v) o[v] = float(w.v[v]);
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) o[v] = v < nl ? float(p[v]) : 0.0f;
-  }
-}
 template <class T, int V>
 __device__ inline void gs_store(T* p, int nl, const float (&x)[V]) {
   if (nl == V) {
@@ -119,6 +100,25 @@ __device__ inline void gs_load_steps(Pack<T, V> (&w)[S], const T* p, int64_t ts,
     else w[s] = pack_load<NT, V>(at, FULL ? V : nl, none);
   }
 }
+
+// The steps that a walk loads at a time, zeros past the last.
+template <class T, int V>
+struct GsBatch {
+  Pack<T, V> w[kGsBatch];
+  __device__ void load(const T* p, int64_t ts, int64_t ls, int nl, int steps) {
+    gs_load_steps<false, false>(w, p, ts, ls, nl, steps, T(0.0f));
+  }
+  __device__ float get(int s, int v) const { return pack_get(w[s], v); }
+};
+template <class T>
+struct GsBatch<T, 1> {
+  T w[kGsBatch];
+  __device__ void load(const T* p, int64_t ts, int64_t, int, int steps) {
+#pragma unroll
+    for (int s = 0; s < kGsBatch; ++s) w[s] = s < steps ? p[s * ts] : T(0.0f);
+  }
+  __device__ float get(int s, int) const { return float(w[s]); }
+};
 
 // ---- tiles of steps -------------------------------------------------------------------------------
 // A run of steps maps the state c in front of it to A c + H behind it, and two runs compose to

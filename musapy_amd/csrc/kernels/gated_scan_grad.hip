@@ -23,39 +23,35 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
   for (int v = 0; v < V; ++v) c[v] = p.first && v < nl ? p.first[off[kGsState] + v] : 0.0f;
   for (uint64_t k0 = 0; k0 < p.T; k0 += kGsBatch) {
   const int steps = p.T - k0 < uint64_t(kGsBatch) ? int(p.T - k0) : kGsBatch;
-  float bd[kGsBatch][V], bg[kGsBatch][V], bh[kGsBatch][V], bx[kGsBatch][V];
+  const int64_t tl = int64_t(p.T - 1 - k0);
+  GsBatch<TX, V> bd, bh, bx;
+  GsBatch<TG, V> bg;
   bool cuts[kGsBatch];
+  const int some = on ? steps : 0;
+  bd.load(static_cast<const TX*>(p.dh) + off[kGsDh] + tl * p.ts[kGsDh], -p.ts[kGsDh], p.ls[kGsDh], nl, some);
+  bg.load(static_cast<const TG*>(p.gate) + off[kGsGate] + tl * p.ts[kGsGate], -p.ts[kGsGate], p.ls[kGsGate], nl, some);
+  if constexpr (BLEND) bx.load(static_cast<const TX*>(p.x) + off[kGsX] + tl * p.ts[kGsX], -p.ts[kGsX], p.ls[kGsX], nl, some);
+  // (step t = 0 has no h[t-1])
+  bh.load(static_cast<const TX*>(p.h) + off[kGsH] + (tl - 1) * p.ts[kGsH], -p.ts[kGsH], p.ls[kGsH], nl,
+          some > 0 && k0 + steps == p.T ? some - 1 : some);
 #pragma unroll
-  for (int s = 0; s < kGsBatch; ++s) {
-    const int64_t t = int64_t(p.T - 1 - k0) - s;
-#pragma unroll
-    for (int v = 0; v < V; ++v) bd[s][v] = bg[s][v] = bh[s][v] = bx[s][v] = 0.0f;
-    cuts[s] = false;
-    if (s < steps && on) {
-      gs_load<TX, V>(static_cast<const TX*>(p.dh) + off[kGsDh] + t * p.ts[kGsDh], p.ls[kGsDh], nl, bd[s]);
-      gs_load<TG, V>(static_cast<const TG*>(p.gate) + off[kGsGate] + t * p.ts[kGsGate], p.ls[kGsGate], nl, bg[s]);
-      if constexpr (BLEND)
-        gs_load<TX, V>(static_cast<const TX*>(p.x) + off[kGsX] + t * p.ts[kGsX], p.ls[kGsX], nl, bx[s]);
-      cuts[s] = p.reset && p.reset[off[kGsReset] + t * p.ts[kGsReset]];
-      if (t > 0)
-        gs_load<TX, V>(static_cast<const TX*>(p.h) + off[kGsH] + (t - 1) * p.ts[kGsH], p.ls[kGsH], nl, bh[s]);
-      else if (p.h_first)
-#pragma unroll
-        for (int v = 0; v < V; ++v) bh[s][v] = v < nl ? p.h_first[off[kGsState] + v] : 0.0f;
-    }
-  }
+  for (int s = 0; s < kGsBatch; ++s)
+    cuts[s] = p.reset && s < some && p.reset[off[kGsReset] + (tl - s) * p.ts[kGsReset]];
 #pragma unroll
   for (int s = 0; s < kGsBatch; ++s) {
     if (s >= steps) break;
-    const int64_t t = int64_t(p.T - 1 - k0) - s;
+    const int64_t t = tl - s;
     const bool cut = cuts[s];
-    float dg[V], dx[V];
-    const float(&dh)[V] = bd[s];
-    const float(&g)[V] = bg[s];
-    const float(&x)[V] = bx[s];
-    float hb[V];
+    float dg[V], dx[V], dh[V], g[V], x[V], hb[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) hb[v] = cut ? 0.0f : bh[s][v];
+    for (int v = 0; v < V; ++v) {
+      dh[v] = bd.get(s, v);
+      g[v] = bg.get(s, v);
+      if constexpr (BLEND) x[v] = bx.get(s, v);
+      hb[v] = bh.get(s, v);
+      if (t == 0) hb[v] = p.h_first && v < nl ? p.h_first[off[kGsState] + v] : 0.0f;
+      if (cut) hb[v] = 0.0f;
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const float G = dh[v] + c[v];

@@ -213,7 +213,8 @@ __global__ __launch_bounds__(kNrBlock) void k_nr_grad(NrArgs p) {
 // summed, and weights and the gradient's column sums stay in registers across rows; with more
 // there is no room for that, and the sums stay in LDS.  Forward C = 8, the columns of one call of the random generator; the
 // gradient, which holds five inputs, three weights and three sums of a column, C = 4: with 8 it took 180
-// registers, one workgroup of 512 a CU.  WAVE: rows that a wave holds, without barriers.  LAYER: one of
+// registers, one workgroup of 512 a CU.  GL: lanes of a row (16, 32 or a wave's 64, without
+// barriers), 0: a workgroup.  LAYER: one of
 // the norms is a layer norm.  FULL: the width is a multiple of C, so that every vector is a whole one.
 
 // Sum over a wave, the same in every lane: DPP moves within rows of 16 lanes and across them.
@@ -231,14 +232,29 @@ __device__ inline float nr_wave_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
-// Sums of N values over the threads of a row.  Every wave reads the (up to 16) waves' sums with one
-// load and adds them by rotations of 16 lanes.  The two halves of `sm` alternate, so that one barrier
-// a sum is enough.
-template <int N, bool WAVE>
+// Sums of N values over the GL lanes of a row, or (GL = 0) over a workgroup's: every wave reads the
+// (up to 16) waves' sums with one load and adds them by rotations of 16 lanes.  The two halves of
+// `sm` alternate, so that one barrier a sum is enough.
+__device__ inline float nr_sum16(float v) {
+  v += nr_dpp<0x128, 0xf>(v);  // row_ror:8
+  v += nr_dpp<0x124, 0xf>(v);  // row_ror:4
+  v += nr_dpp<0x122, 0xf>(v);  // row_ror:2
+  v += nr_dpp<0x121, 0xf>(v);  // row_ror:1
+  return v;
+}
+template <int N, int GL>
 __device__ inline void nr_sums_of(float (&v)[N], float (*sm)[4][16], int& half, int waves) {
+  if constexpr (GL == 16 || GL == 32) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = nr_sum16(v[i]);
+      if (GL == 32) v[i] += __shfl_xor(v[i], 16, kWave);
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = nr_wave_sum(v[i]);
-  if constexpr (!WAVE) {
+  if constexpr (GL == 0) {
     const int wv = threadIdx.x / kWave, l = threadIdx.x % 16;
     if (threadIdx.x % kWave == 0)
 #pragma unroll
@@ -247,13 +263,7 @@ __device__ inline void nr_sums_of(float (&v)[N], float (*sm)[4][16], int& half, 
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = sm[half][i][l];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      v[i] = l < waves ? v[i] : 0.0f;
-      v[i] += nr_dpp<0x128, 0xf>(v[i]);  // row_ror:8
-      v[i] += nr_dpp<0x124, 0xf>(v[i]);  // row_ror:4
-      v[i] += nr_dpp<0x122, 0xf>(v[i]);  // row_ror:2
-      v[i] += nr_dpp<0x121, 0xf>(v[i]);  // row_ror:1
-    }
+    for (int i = 0; i < N; ++i) v[i] = nr_sum16(l < waves ? v[i] : 0.0f);
     half ^= 1;
   }
 }
@@ -277,17 +287,19 @@ __device__ inline void nr_load_weight(const void* w, bool f32, uint64_t col, int
 }
 
 // Where a thread works: its row, the rows' step, and its vectors' widths.
-template <int C, int NV, bool WAVE, bool FULL>
+template <int C, int NV, int GL, bool FULL>
 struct NrPlace {
   uint32_t t, threads, row, step;
   int waves, n[NV];
   __device__ explicit NrPlace(uint32_t width) {
-    threads = WAVE ? kWave : blockDim.x;
-    waves = int(threads / kWave);
-    t = WAVE ? threadIdx.x % kWave : threadIdx.x;
-    const uint32_t per = WAVE ? blockDim.x / kWave : 1;
-    // the same for the whole wave, which keeps it and the rows' addresses in scalar registers
-    row = WAVE ? blockIdx.x * per + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) : blockIdx.x;
+    threads = GL ? GL : blockDim.x;
+    waves = int(blockDim.x / kWave);
+    t = GL ? threadIdx.x % GL : threadIdx.x;
+    const uint32_t per = GL ? blockDim.x / GL : 1;
+    // where it is the same for the whole wave, it and the rows' addresses stay in scalar registers
+    row = GL == kWave ? blockIdx.x * per + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)
+          : GL        ? blockIdx.x * per + threadIdx.x / GL
+                      : blockIdx.x;
     step = gridDim.x * per;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -301,10 +313,10 @@ struct NrPlace {
   __device__ uint32_t col(int i) const { return vec(i) * C; }  // (widths in registers are small: 32-bit offsets)
 };
 
-template <class T, class TS, int NV, int BS, bool WAVE, bool LAYER, bool FULL, bool NT>
+template <class T, class TS, int NV, int BS, int GL, bool LAYER, bool FULL, bool NT>
 __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
   __shared__ float sm[2][4][16];
-  const NrPlace<8, NV, WAVE, FULL> at(p.width);
+  const NrPlace<8, NV, GL, FULL> at(p.width);
   int half = 0;
   constexpr bool kAhead = NV == 1;
   const int kind = p.gate ? p.gate_kind : MUSAPY_GATE_SIGMOID;
@@ -360,7 +372,7 @@ __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
         for (int i = 0; i < NV; ++i)
 #pragma unroll
           for (int e = 0; e < 8; ++e) s[0] += v[i][e];
-        nr_sums_of<1, WAVE>(s, sm, half, at.waves);
+        nr_sums_of<1, GL>(s, sm, half, at.waves);
         const float mean = s[0] * over;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -372,7 +384,7 @@ __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < 8; ++e) q[0] = __builtin_fmaf(v[i][e], v[i][e], q[0]);
-      nr_sums_of<1, WAVE>(q, sm, half, at.waves);
+      nr_sums_of<1, GL>(q, sm, half, at.waves);
       return nr_rsqrt(q[0] * over + p.eps);
     };
     const float inv1 = p.post != MUSAPY_NORM_NONE ? stats(p.post, u) : 1.0f;
@@ -407,11 +419,11 @@ __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
 // The gradient.  With m the mean (0 for rms norms) the sums that depend on the row's inputs alone,
 // (x - m)^2, (r - m)^2, dy w2 (r - m) and dy w2, are formed in one round; those of the post norm's input
 // gradient, which need D, in a second.
-template <class T, class TS, int NV, int BS, bool WAVE, bool LAYER, bool FULL, bool NT>
+template <class T, class TS, int NV, int BS, int GL, bool LAYER, bool FULL, bool NT>
 __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
   __shared__ float sm[2][4][16];
   constexpr int C = 4;
-  const NrPlace<C, NV, WAVE, FULL> at(p.width);
+  const NrPlace<C, NV, GL, FULL> at(p.width);
   int half = 0;
   constexpr bool kAhead = NV == 1;
   const int kind = p.gate ? p.gate_kind : MUSAPY_GATE_SIGMOID;
@@ -504,7 +516,7 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
           s[0] += pack_get(x[i], e);
           s[1] += pack_get(r[i], e);
         }
-      nr_sums_of<2, WAVE>(s, sm, half, at.waves);
+      nr_sums_of<2, GL>(s, sm, half, at.waves);
       if (p.post == MUSAPY_NORM_LAYER) m1 = s[0] * over;
       if (p.pre == MUSAPY_NORM_LAYER) m2 = s[1] * over;
     }
@@ -536,7 +548,7 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
         pack_opaque(r[i]);
         pack_opaque(y[i]);
       }
-      nr_sums_of<LAYER ? 4 : 3, WAVE>(s, sm, half, at.waves);
+      nr_sums_of<LAYER ? 4 : 3, GL>(s, sm, half, at.waves);
       if (p.post != MUSAPY_NORM_NONE) inv1 = nr_rsqrt(s[0] * over + p.eps);
       if (pre) {
         inv2 = nr_rsqrt(s[1] * over + p.eps);
@@ -597,7 +609,7 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
       pack_opaque(x[i]);
     }
     if (p.post != MUSAPY_NORM_NONE) {
-      nr_sums_of<LAYER ? 2 : 1, WAVE>(s2, sm, half, at.waves);
+      nr_sums_of<LAYER ? 2 : 1, GL>(s2, sm, half, at.waves);
       const float along1 = s2[0] * over * inv1;
       float flat1 = 0.0f;
       if constexpr (LAYER)
@@ -612,20 +624,36 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
       for (int i = 0; i < NV; ++i)
         if (at.has(i)) pack_store<NT>(static_cast<T*>(p.dx) + base + at.col(i), at.count(i), q1[i]);
   }
-  if (p.part) {
-    const uint32_t worker = WAVE ? blockIdx.x * (blockDim.x / kWave) + threadIdx.x / kWave : blockIdx.x;
-    if (worker >= p.workers) return;
-    float* const part = p.part + uint64_t(worker) * 3 * p.width;
+  if (p.part == nullptr) return;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      sums(i, false);
+  for (int i = 0; i < NV; ++i) {
+    sums(i, false);
+    if constexpr (GL != 0) {  // the rows of a workgroup, in order
+      __shared__ float s_rows[3 * C][BS];
 #pragma unroll
-      for (int e = 0; e < C; ++e) as[e] *= p.scale_value * p.keep_scale;
-      if (!at.has(i)) continue;
-      pack_store<false>(part + at.col(i), at.count(i), a1);
-      pack_store<false>(part + p.width + at.col(i), at.count(i), as);
-      pack_store<false>(part + 2 * uint64_t(p.width) + at.col(i), at.count(i), a2);
+      for (int e = 0; e < C; ++e) {
+        s_rows[e][threadIdx.x] = a1[e];
+        s_rows[C + e][threadIdx.x] = as[e];
+        s_rows[2 * C + e][threadIdx.x] = a2[e];
+        a1[e] = as[e] = a2[e] = 0.0f;
+      }
+      __syncthreads();
+      if (threadIdx.x >= GL) return;
+      for (int r = 0; r < BS / GL; ++r)
+#pragma unroll
+        for (int e = 0; e < C; ++e) {
+          a1[e] += s_rows[e][r * GL + threadIdx.x];
+          as[e] += s_rows[C + e][r * GL + threadIdx.x];
+          a2[e] += s_rows[2 * C + e][r * GL + threadIdx.x];
+        }
     }
+#pragma unroll
+    for (int e = 0; e < C; ++e) as[e] *= p.scale_value * p.keep_scale;
+    if (!at.has(i)) continue;
+    float* const part = p.part + uint64_t(blockIdx.x) * 3 * p.width;
+    pack_store<false>(part + at.col(i), at.count(i), a1);
+    pack_store<false>(part + p.width + at.col(i), at.count(i), as);
+    pack_store<false>(part + 2 * uint64_t(p.width) + at.col(i), at.count(i), a2);
   }
 }
 
@@ -667,7 +695,7 @@ namespace {
 // How the rows of a call are spread: `threads` to a workgroup, `blocks` of them.
 struct NrRoute {
   int nv = 0;  // vectors to a thread; 0: the kernels for any width
-  bool wave = false;
+  int lanes = 0;  // of a row; 0: a workgroup
   unsigned threads = kNrBlock, blocks = 0;
   uint32_t workers = 0;
 };
@@ -681,10 +709,9 @@ NrRoute nr_route(const musapy_norm_residual_args* p, bool grad) {
   }
   if (vecs <= kWave) {
     r.nv = 1;
-    r.wave = true;
-    const uint64_t most = grad ? 512 : 2048, want = (rows + 3) / 4;
-    r.blocks = unsigned(want < most ? want : most);
-    r.workers = uint32_t(rows < r.blocks * uint64_t(4) ? rows : r.blocks * uint64_t(4));
+    r.lanes = vecs <= 16 ? 16 : vecs <= 32 ? 32 : kWave;
+    const uint64_t most = grad ? 512 : 2048, want = (rows * r.lanes + kNrBlock - 1) / kNrBlock;
+    r.blocks = r.workers = unsigned(want < most ? want : most);
     return r;
   }
   r.nv = int((vecs + 1023) / 1024);
@@ -759,7 +786,7 @@ void nr_types(int dtype, int stream_dtype, Fn&& fn) {
 
 bool nr_sums(const musapy_norm_residual_args* p) { return p->dpost_weight || p->dscale || p->dpre_weight; }
 
-// Calls fn with (NV, BS, WAVE, LAYER, FULL, NT) of the kernel for a call.
+// Calls fn with (NV, BS, GL, LAYER, FULL, NT) of the kernel for a call.
 template <int C, class Fn>
 void nr_kernel(const NrRoute& r, const NrArgs& a, Fn&& fn) {
   using std::false_type;
@@ -767,18 +794,22 @@ void nr_kernel(const NrRoute& r, const NrArgs& a, Fn&& fn) {
   using std::true_type;
   const bool layer = a.post == MUSAPY_NORM_LAYER || a.pre == MUSAPY_NORM_LAYER;
   const bool nt = uint64_t(a.rows) * a.width * 8 >= kStreamLoadBytes;
-  auto more = [&](auto nv, auto bs, auto wave) {
+  auto more = [&](auto nv, auto bs, auto gl) {
     with_store_policy(layer, [&](auto LAYER) {
-      if (a.width % C) fn(nv, bs, wave, LAYER, false_type{}, false_type{});
-      else if (nt) fn(nv, bs, wave, LAYER, true_type{}, true_type{});
-      else fn(nv, bs, wave, LAYER, true_type{}, false_type{});
+      if (a.width % C) fn(nv, bs, gl, LAYER, false_type{}, false_type{});
+      else if (nt) fn(nv, bs, gl, LAYER, true_type{}, true_type{});
+      else fn(nv, bs, gl, LAYER, true_type{}, false_type{});
     });
   };
-  if (r.wave) more(integral_constant<int, 1>{}, integral_constant<int, 256>{}, true_type{});
-  else if (r.nv == 1 && r.threads <= 512) more(integral_constant<int, 1>{}, integral_constant<int, 512>{}, false_type{});
-  else if (r.nv == 1) more(integral_constant<int, 1>{}, integral_constant<int, 1024>{}, false_type{});
-  else if (r.nv == 2) more(integral_constant<int, 2>{}, integral_constant<int, 1024>{}, false_type{});
-  else if constexpr (C == 4) more(integral_constant<int, 3>{}, integral_constant<int, 1024>{}, false_type{});
+  using One = integral_constant<int, 1>;
+  using Block = integral_constant<int, 0>;
+  if (r.lanes == 16) more(One{}, integral_constant<int, kNrBlock>{}, integral_constant<int, 16>{});
+  else if (r.lanes == 32) more(One{}, integral_constant<int, kNrBlock>{}, integral_constant<int, 32>{});
+  else if (r.lanes == kWave) more(One{}, integral_constant<int, kNrBlock>{}, integral_constant<int, kWave>{});
+  else if (r.nv == 1 && r.threads <= 512) more(One{}, integral_constant<int, 512>{}, Block{});
+  else if (r.nv == 1) more(One{}, integral_constant<int, 1024>{}, Block{});
+  else if (r.nv == 2) more(integral_constant<int, 2>{}, integral_constant<int, 1024>{}, Block{});
+  else if constexpr (C == 4) more(integral_constant<int, 3>{}, integral_constant<int, 1024>{}, Block{});
 }
 
 }  // namespace
@@ -805,8 +836,8 @@ int musapy_norm_residual_v1(const musapy_norm_residual_args* p, hipStream_t st) 
     using TS = decltype(ts);
     if (r.nv == 0) k_nr<T, TS><<<r.blocks, r.threads, 0, st>>>(a);
     else
-      nr_kernel<8>(r, a, [&](auto NV, auto BS, auto WAVE, auto LAYER, auto FULL, auto NT) {
-        k_nr_rows<T, TS, NV.value, BS.value, WAVE.value, LAYER.value, FULL.value, NT.value><<<r.blocks, r.threads, 0, st>>>(a);
+      nr_kernel<8>(r, a, [&](auto NV, auto BS, auto GL, auto LAYER, auto FULL, auto NT) {
+        k_nr_rows<T, TS, NV.value, BS.value, GL.value, LAYER.value, FULL.value, NT.value><<<r.blocks, r.threads, 0, st>>>(a);
       });
   });
   return 0;
@@ -832,8 +863,8 @@ int musapy_norm_residual_grad_v1(const musapy_norm_residual_args* p, void* scrat
     using TS = decltype(ts);
     if (r.blocks > 0 && r.nv == 0) k_nr_grad<T, TS><<<r.blocks, r.threads, 0, st>>>(a);
     else if (r.blocks > 0)
-      nr_kernel<4>(r, a, [&](auto NV, auto BS, auto WAVE, auto LAYER, auto FULL, auto NT) {
-        k_nr_grad_rows<T, TS, NV.value, BS.value, WAVE.value, LAYER.value, FULL.value, NT.value>
+      nr_kernel<4>(r, a, [&](auto NV, auto BS, auto GL, auto LAYER, auto FULL, auto NT) {
+        k_nr_grad_rows<T, TS, NV.value, BS.value, GL.value, LAYER.value, FULL.value, NT.value>
             <<<r.blocks, r.threads, 0, st>>>(a);
       });
     if (nr_sums(p))
