@@ -270,14 +270,16 @@ __device__ inline void nr_sums_of(float (&v)[N], float (*sm)[4][16], int& half, 
 // (the hardware's reciprocal square root is within 1 ulp)
 __device__ inline float nr_rsqrt(float v) { return __builtin_amdgcn_rsqf(v); }
 
-template <class T, int C>
-__device__ inline void nr_load_weight(const void* w, bool f32, uint64_t col, int n, float (&o)[C]) {
-  Pack<float, C> p = pack_all<float, C>(n ? 1.0f : 0.0f);
-  if (w != nullptr && n > 0) {
+template <class T, int C, class Place>
+__device__ inline void nr_load_weight(const void* w, bool f32, const Place& at, int i, float (&o)[C]) {
+  Pack<float, C> p = pack_all<float, C>(at.has(i) ? 1.0f : 0.0f);
+  if (w != nullptr && at.has(i)) {
     if (f32) {
-      p = pack_load<false, C>(static_cast<const float*>(w) + col, n, 0.0f);
+      p = pack_load<false, C>(static_cast<const float*>(w) + at.from(i), at.span(i), 0.0f);
+      at.put(p, i);
     } else {
-      const Pack<T, C> q = pack_load<false, C>(static_cast<const T*>(w) + col, n, T(0.0f));
+      Pack<T, C> q = pack_load<false, C>(static_cast<const T*>(w) + at.from(i), at.span(i), T(0.0f));
+      at.put(q, i);
 #pragma unroll
       for (int e = 0; e < C; ++e) p.w[e] = __builtin_bit_cast(uint32_t, pack_get(q, e));
     }
@@ -290,7 +292,7 @@ __device__ inline void nr_load_weight(const void* w, bool f32, uint64_t col, int
 template <int C, int NV, int GL, bool FULL>
 struct NrPlace {
   uint32_t t, threads, row, step;
-  int waves, n[NV];
+  int waves, n[NV], back[NV];
   __device__ explicit NrPlace(uint32_t width) {
     threads = GL ? GL : blockDim.x;
     waves = int(blockDim.x / kWave);
@@ -305,12 +307,20 @@ struct NrPlace {
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = col(i);
       n[i] = c >= width ? 0 : !FULL && width - c < uint32_t(C) ? int(width - c) : C;
+      back[i] = !FULL && n[i] && width >= uint32_t(C) ? C - n[i] : 0;
     }
   }
   __device__ uint32_t vec(int i) const { return t + uint32_t(i) * threads; }
   __device__ bool has(int i) const { return n[i] != 0; }
   __device__ int count(int i) const { return FULL ? C : n[i]; }  // where it has one
   __device__ uint32_t col(int i) const { return vec(i) * C; }  // (widths in registers are small: 32-bit offsets)
+  // what is loaded for it: a row's last columns in one piece that ends with the row
+  __device__ uint32_t from(int i) const { return FULL ? col(i) : col(i) - back[i]; }
+  __device__ int span(int i) const { return FULL ? C : n[i] + back[i]; }
+  template <class T>
+  __device__ void put(Pack<T, C>& p, int i) const {
+    if constexpr (!FULL) pack_shift(p, back[i]);
+  }
 };
 
 template <class T, class TS, int NV, int BS, int GL, bool LAYER, bool FULL, bool NT>
@@ -322,12 +332,12 @@ __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
   const int kind = p.gate ? p.gate_kind : MUSAPY_GATE_SIGMOID;
   float w1[8], sc[8], w2[8];
   auto weights = [&](int i) {
-    nr_load_weight<T>(p.w1, p.weight_f32, at.col(i), at.n[i], w1);
-    nr_load_weight<T>(p.scale, p.weight_f32, at.col(i), at.n[i], sc);
+    nr_load_weight<T>(p.w1, p.weight_f32, at, i, w1);
+    nr_load_weight<T>(p.scale, p.weight_f32, at, i, sc);
 #pragma unroll
     for (int e = 0; e < 8; ++e) sc[e] *= p.scale_value;
   };
-  auto pre_weights = [&](int i) { nr_load_weight<T>(p.w2, p.weight_f32, at.col(i), at.n[i], w2); };
+  auto pre_weights = [&](int i) { nr_load_weight<T>(p.w2, p.weight_f32, at, i, w2); };
   if (kAhead) {
     weights(0);
     pre_weights(0);
@@ -338,9 +348,9 @@ __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (!at.has(i)) continue;
-      nx[i] = pack_load<NT, 8>(static_cast<const T*>(p.x) + int64_t(row) * p.xp + at.col(i), at.count(i), T(0.0f));
-      if (p.gate) ng[i] = pack_load<NT, 8>(static_cast<const T*>(p.gate) + int64_t(row) * p.gatep + at.col(i), at.count(i), T(0.0f));
-      if (p.res) nres[i] = pack_load<NT, 8>(static_cast<const TS*>(p.res) + int64_t(row) * p.resp + at.col(i), at.count(i), TS(0.0f));
+      nx[i] = pack_load<NT, 8>(static_cast<const T*>(p.x) + int64_t(row) * p.xp + at.from(i), at.span(i), T(0.0f));
+      if (p.gate) ng[i] = pack_load<NT, 8>(static_cast<const T*>(p.gate) + int64_t(row) * p.gatep + at.from(i), at.span(i), T(0.0f));
+      if (p.res) nres[i] = pack_load<NT, 8>(static_cast<const TS*>(p.res) + int64_t(row) * p.resp + at.from(i), at.span(i), TS(0.0f));
     }
   };
 #pragma unroll
@@ -358,10 +368,14 @@ __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
     float u[NV][8];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      Pack<T, 8> x = nx[i];
       g[i] = ng[i];
       res[i] = nres[i];
+      at.put(x, i);
+      if (p.gate) at.put(g[i], i);
+      at.put(res[i], i);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) u[i][e] = pack_get(nx[i], e);
+      for (int e = 0; e < 8; ++e) u[i][e] = pack_get(x, e);
     }
     if (kAhead && row + at.step < p.rows) load(row + at.step);
     // mean and 1 / deviation of `v`, which is left centred
@@ -450,12 +464,12 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
     }
   };
   auto weights = [&](int i) {
-    nr_load_weight<T>(p.w1, p.weight_f32, at.col(i), at.n[i], w1);
-    nr_load_weight<T>(p.scale, p.weight_f32, at.col(i), at.n[i], sc);
+    nr_load_weight<T>(p.w1, p.weight_f32, at, i, w1);
+    nr_load_weight<T>(p.scale, p.weight_f32, at, i, sc);
 #pragma unroll
     for (int e = 0; e < C; ++e) sc[e] *= p.scale_value * p.keep_scale;
   };
-  auto pre_weights = [&](int i) { nr_load_weight<T>(p.w2, p.weight_f32, at.col(i), at.n[i], w2); };
+  auto pre_weights = [&](int i) { nr_load_weight<T>(p.w2, p.weight_f32, at, i, w2); };
   if (kAhead) {
     weights(0);
     pre_weights(0);
@@ -473,11 +487,11 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (!at.has(i)) continue;
-      nx[i] = pack_load<NT, C>(static_cast<const T*>(p.x) + int64_t(row) * p.xp + at.col(i), at.count(i), T(0.0f));
-      if (p.gate) ng[i] = pack_load<NT, C>(static_cast<const T*>(p.gate) + int64_t(row) * p.gatep + at.col(i), at.count(i), T(0.0f));
-      if (pre) nr[i] = pack_load<NT, C>(static_cast<const TS*>(p.res) + int64_t(row) * p.resp + at.col(i), at.count(i), TS(0.0f));
-      if (p.dr) nd[i] = pack_load<NT, C>(static_cast<const TS*>(p.dr) + int64_t(row) * p.drp + at.col(i), at.count(i), TS(0.0f));
-      if (p.dy) ny[i] = pack_load<NT, C>(static_cast<const T*>(p.dy) + int64_t(row) * p.dyp + at.col(i), at.count(i), T(0.0f));
+      nx[i] = pack_load<NT, C>(static_cast<const T*>(p.x) + int64_t(row) * p.xp + at.from(i), at.span(i), T(0.0f));
+      if (p.gate) ng[i] = pack_load<NT, C>(static_cast<const T*>(p.gate) + int64_t(row) * p.gatep + at.from(i), at.span(i), T(0.0f));
+      if (pre) nr[i] = pack_load<NT, C>(static_cast<const TS*>(p.res) + int64_t(row) * p.resp + at.from(i), at.span(i), TS(0.0f));
+      if (p.dr) nd[i] = pack_load<NT, C>(static_cast<const TS*>(p.dr) + int64_t(row) * p.drp + at.from(i), at.span(i), TS(0.0f));
+      if (p.dy) ny[i] = pack_load<NT, C>(static_cast<const T*>(p.dy) + int64_t(row) * p.dyp + at.from(i), at.span(i), T(0.0f));
     }
   };
 #pragma unroll
@@ -504,6 +518,11 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
       y[i] = ny[i];
       r[i] = nr[i];
       d[i] = nd[i];
+      at.put(x[i], i);
+      if (p.gate) at.put(g[i], i);
+      at.put(y[i], i);
+      at.put(r[i], i);
+      at.put(d[i], i);
     }
     if (kAhead && row + at.step < p.rows) load(row + at.step);
     float m1 = 0.0f, m2 = 0.0f;

@@ -64,6 +64,29 @@ __device__ inline Pack<T, N> pack_load(const T* at, int n, T none) {
   return p;
 }
 
+// Of elements that were loaded from `by` elements in front of their place: those from there on, then
+// zeros.  The last elements of a row are loaded so, as N in one piece that ends with the row: one by
+// one, under a branch, each operand's loads were waited for before the next one's were issued.
+template <class T, int N>
+__device__ inline void pack_shift(Pack<T, N>& p, int by) {
+  if (by == 0) return;
+  auto words = [&](int k) {
+#pragma unroll
+    for (int i = 0; i < p.kWords; ++i) p.w[i] = i + k < p.kWords ? p.w[i + k < p.kWords ? i + k : 0] : 0;
+  };
+  if constexpr (sizeof(T) == 2) {
+    if (by & 1)
+#pragma unroll
+      for (int i = 0; i < p.kWords; ++i)
+        p.w[i] = p.w[i] >> 16 | (i + 1 < p.kWords ? p.w[i + 1 < p.kWords ? i + 1 : 0] << 16 : 0);
+    by /= 2;
+  }
+  if (by & 1) words(1);
+  if (by & 2) words(2);
+  if constexpr (Pack<T, N>::kWords > 4)
+    if (by & 4) words(4);
+}
+
 // The first n of N elements, rounded to T, to any element address.
 template <bool NT, class T, int N>
 __device__ inline void pack_store(T* at, int n, const float (&x)[N]) {
