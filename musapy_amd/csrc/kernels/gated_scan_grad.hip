@@ -22,65 +22,65 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
 #pragma unroll
   for (int v = 0; v < V; ++v) c[v] = p.first && v < nl ? p.first[off[kGsState] + v] : 0.0f;
   for (uint64_t k0 = 0; k0 < p.T; k0 += kGsBatch) {
-  const int steps = p.T - k0 < uint64_t(kGsBatch) ? int(p.T - k0) : kGsBatch;
-  const int64_t tl = int64_t(p.T - 1 - k0);
-  GsBatch<TX, V> bd, bh, bx;
-  GsBatch<TG, V> bg;
-  bool cuts[kGsBatch];
-  const int some = on ? steps : 0;
-  bd.load(static_cast<const TX*>(p.dh) + off[kGsDh] + tl * p.ts[kGsDh], -p.ts[kGsDh], p.ls[kGsDh], nl, some);
-  bg.load(static_cast<const TG*>(p.gate) + off[kGsGate] + tl * p.ts[kGsGate], -p.ts[kGsGate], p.ls[kGsGate], nl, some);
-  if constexpr (BLEND) bx.load(static_cast<const TX*>(p.x) + off[kGsX] + tl * p.ts[kGsX], -p.ts[kGsX], p.ls[kGsX], nl, some);
-  // (step t = 0 has no h[t-1])
-  bh.load(static_cast<const TX*>(p.h) + off[kGsH] + (tl - 1) * p.ts[kGsH], -p.ts[kGsH], p.ls[kGsH], nl,
-          some > 0 && k0 + steps == p.T ? some - 1 : some);
+    const int steps = p.T - k0 < uint64_t(kGsBatch) ? int(p.T - k0) : kGsBatch;
+    const int64_t tl = int64_t(p.T - 1 - k0);
+    GsBatch<TX, V> bd, bh, bx;
+    GsBatch<TG, V> bg;
+    bool cuts[kGsBatch];
+    const int some = on ? steps : 0;
+    bd.load(static_cast<const TX*>(p.dh) + off[kGsDh] + tl * p.ts[kGsDh], -p.ts[kGsDh], p.ls[kGsDh], nl, some);
+    bg.load(static_cast<const TG*>(p.gate) + off[kGsGate] + tl * p.ts[kGsGate], -p.ts[kGsGate], p.ls[kGsGate], nl, some);
+    if constexpr (BLEND) bx.load(static_cast<const TX*>(p.x) + off[kGsX] + tl * p.ts[kGsX], -p.ts[kGsX], p.ls[kGsX], nl, some);
+    // (step t = 0 has no h[t-1])
+    bh.load(static_cast<const TX*>(p.h) + off[kGsH] + (tl - 1) * p.ts[kGsH], -p.ts[kGsH], p.ls[kGsH], nl,
+            some > 0 && k0 + steps == p.T ? some - 1 : some);
 #pragma unroll
-  for (int s = 0; s < kGsBatch; ++s)
-    cuts[s] = p.reset && s < some && p.reset[off[kGsReset] + (tl - s) * p.ts[kGsReset]];
+    for (int s = 0; s < kGsBatch; ++s)
+      cuts[s] = p.reset && s < some && p.reset[off[kGsReset] + (tl - s) * p.ts[kGsReset]];
 #pragma unroll
-  for (int s = 0; s < kGsBatch; ++s) {
-    if (s >= steps) break;
-    const int64_t t = tl - s;
-    const bool cut = cuts[s];
-    float dg[V], dx[V], dh[V], g[V], x[V], hb[V];
+    for (int s = 0; s < kGsBatch; ++s) {
+      if (s >= steps) break;
+      const int64_t t = tl - s;
+      const bool cut = cuts[s];
+      float dg[V], dx[V], dh[V], g[V], x[V], hb[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      dh[v] = bd.get(s, v);
-      g[v] = bg.get(s, v);
-      if constexpr (BLEND) x[v] = bx.get(s, v);
-      hb[v] = bh.get(s, v);
-      if (t == 0) hb[v] = p.h_first && v < nl ? p.h_first[off[kGsState] + v] : 0.0f;
-      if (cut) hb[v] = 0.0f;
-    }
+      for (int v = 0; v < V; ++v) {
+        dh[v] = bd.get(s, v);
+        g[v] = bg.get(s, v);
+        if constexpr (BLEND) x[v] = bx.get(s, v);
+        hb[v] = bh.get(s, v);
+        if (t == 0) hb[v] = p.h_first && v < nl ? p.h_first[off[kGsState] + v] : 0.0f;
+        if (cut) hb[v] = 0.0f;
+      }
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float G = dh[v] + c[v];
-      if constexpr (BLEND) {
-        float s, rest;
-        gs_sigmoid(g[v], s, rest);
-        dx[v] = rest * G;
-        dg[v] = G * (hb[v] - x[v]) * (s * rest);
-        c[v] = cut ? 0.0f : s * G;
-      } else {
-        dx[v] = G;
-        dg[v] = cut ? 0.0f : G * hb[v];
-        c[v] = cut ? 0.0f : g[v] * G;
+      for (int v = 0; v < V; ++v) {
+        const float G = dh[v] + c[v];
+        if constexpr (BLEND) {
+          float s, rest;
+          gs_sigmoid(g[v], s, rest);
+          dx[v] = rest * G;
+          dg[v] = G * (hb[v] - x[v]) * (s * rest);
+          c[v] = cut ? 0.0f : s * G;
+        } else {
+          dx[v] = G;
+          dg[v] = cut ? 0.0f : G * hb[v];
+          c[v] = cut ? 0.0f : g[v] * G;
+        }
+      }
+      if (on) gs_store<TX, V>(static_cast<TX*>(p.out) + off[kGsOut] + t * p.ts[kGsOut], nl, dx);
+      if (p.part_lanes >= 0) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum += v < nl ? dg[v] : 0.0f;
+        for (int m = 1; m < (1 << p.part_lanes); m <<= 1) sum += __shfl_xor(sum, m, kWave);
+        if (on && (vec & ((1u << p.part_lanes) - 1)) == 0)
+          static_cast<float*>(p.dgate)[off[kGsDgate] + t * p.ts[kGsDgate] + (vec >> p.part_lanes)] = sum;
+      } else if (on) {
+        const int64_t at = off[kGsDgate] + t * p.ts[kGsDgate];
+        if (p.dgate_f32) gs_store<float, V>(static_cast<float*>(p.dgate) + at, nl, dg);
+        else gs_store<TG, V>(static_cast<TG*>(p.dgate) + at, nl, dg);
       }
     }
-    if (on) gs_store<TX, V>(static_cast<TX*>(p.out) + off[kGsOut] + t * p.ts[kGsOut], nl, dx);
-    if (p.part_lanes >= 0) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int v = 0; v < V; ++v) sum += v < nl ? dg[v] : 0.0f;
-      for (int m = 1; m < (1 << p.part_lanes); m <<= 1) sum += __shfl_xor(sum, m, kWave);
-      if (on && (vec & ((1u << p.part_lanes) - 1)) == 0)
-        static_cast<float*>(p.dgate)[off[kGsDgate] + t * p.ts[kGsDgate] + (vec >> p.part_lanes)] = sum;
-    } else if (on) {
-      const int64_t at = off[kGsDgate] + t * p.ts[kGsDgate];
-      if (p.dgate_f32) gs_store<float, V>(static_cast<float*>(p.dgate) + at, nl, dg);
-      else gs_store<TG, V>(static_cast<TG*>(p.dgate) + at, nl, dg);
-    }
-  }
   }
   if (p.last) {
 #pragma unroll
