@@ -48,16 +48,19 @@ __device__ inline float nr_weight(const void* w, bool f32, uint32_t c) {
   return f32 ? static_cast<const float*>(w)[c] : float(static_cast<const T*>(w)[c]);
 }
 
-// Sum over a block of 256, the same for every thread.
+constexpr int kNrBlock = 256;
+constexpr int kNrWide = 1024;  // of rows of any width
+
+// Sum over a block of kNrWide, the same for every thread.
 __device__ inline float nr_block_sum(float v, float* sm) {
   for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m, kWave);
   __syncthreads();
   if (threadIdx.x % kWave == 0) sm[threadIdx.x / kWave] = v;
   __syncthreads();
-  return (sm[0] + sm[1]) + (sm[2] + sm[3]);
+  v = sm[threadIdx.x % (kNrWide / kWave)];
+  for (int m = kNrWide / kWave / 2; m > 0; m >>= 1) v += __shfl_xor(v, m, kWave);
+  return v;
 }
-
-constexpr int kNrBlock = 256;
 
 // ---- rows of any width ----------------------------------------------------------------------------
 // Rows that do not fit a workgroup's registers are read again for every sum: one workgroup a row.
@@ -97,11 +100,11 @@ __device__ inline void nr_stats(int kind, uint32_t width, float eps, float* sm, 
   if (kind == MUSAPY_NORM_NONE) return;
   if (kind == MUSAPY_NORM_LAYER) {
     float s = 0.0f;
-    for (uint32_t c = threadIdx.x; c < width; c += kNrBlock) s += f(c);
+    for (uint32_t c = threadIdx.x; c < width; c += kNrWide) s += f(c);
     mean = nr_block_sum(s, sm) / float(width);
   }
   float q = 0.0f;
-  for (uint32_t c = threadIdx.x; c < width; c += kNrBlock) {
+  for (uint32_t c = threadIdx.x; c < width; c += kNrWide) {
     const float v = f(c) - mean;
     q = __builtin_fmaf(v, v, q);
   }
@@ -109,14 +112,14 @@ __device__ inline void nr_stats(int kind, uint32_t width, float eps, float* sm, 
 }
 
 template <class T, class TS>
-__global__ __launch_bounds__(kNrBlock) void k_nr(NrArgs p) {
-  __shared__ float sm[kNrBlock / kWave];
+__global__ __launch_bounds__(kNrWide) void k_nr(NrArgs p) {
+  __shared__ float sm[kNrWide / kWave];
   NrRow<T, TS> row{p, blockIdx.x};
   const uint64_t base = uint64_t(blockIdx.x) * p.width;
   nr_stats(p.post, p.width, p.eps, sm, row.mean1, row.inv1, [&](uint32_t c) { return row.x(c); });
   float mean2, inv2;
   nr_stats(p.pre, p.width, p.eps, sm, mean2, inv2, [&](uint32_t c) { return row.r(c); });
-  for (uint32_t c = threadIdx.x; c < p.width; c += kNrBlock) {
+  for (uint32_t c = threadIdx.x; c < p.width; c += kNrWide) {
     const float r = row.r(c);
     static_cast<TS*>(p.r)[base + c] = TS(r);
     if (p.y) static_cast<T*>(p.y)[base + c] = T((r - mean2) * inv2 * nr_weight<T>(p.w2, p.weight_f32, c));
@@ -124,8 +127,8 @@ __global__ __launch_bounds__(kNrBlock) void k_nr(NrArgs p) {
 }
 
 template <class T, class TS>
-__global__ __launch_bounds__(kNrBlock) void k_nr_grad(NrArgs p) {
-  __shared__ float sm[kNrBlock / kWave];
+__global__ __launch_bounds__(kNrWide) void k_nr_grad(NrArgs p) {
+  __shared__ float sm[kNrWide / kWave];
   float* const part = p.part ? p.part + uint64_t(blockIdx.x) * 3 * p.width : nullptr;
   const float over = 1.0f / float(p.width);
   for (uint32_t at = blockIdx.x; at < p.rows; at += gridDim.x) {
@@ -138,7 +141,7 @@ __global__ __launch_bounds__(kNrBlock) void k_nr_grad(NrArgs p) {
     if (p.pre != MUSAPY_NORM_NONE) {
       nr_stats(p.pre, p.width, p.eps, sm, mean2, inv2, r_of);
       float s = 0, q = 0;
-      for (uint32_t c = threadIdx.x; c < p.width; c += kNrBlock) {
+      for (uint32_t c = threadIdx.x; c < p.width; c += kNrWide) {
         const float g = dy_of(c) * nr_weight<T>(p.w2, p.weight_f32, c);
         s += g * (r_of(c) - mean2) * inv2;
         q += g;
@@ -173,7 +176,7 @@ __global__ __launch_bounds__(kNrBlock) void k_nr_grad(NrArgs p) {
     float along1 = 0, flat1 = 0;
     if (p.post != MUSAPY_NORM_NONE) {
       float s = 0, q = 0;
-      for (uint32_t c = threadIdx.x; c < p.width; c += kNrBlock) {
+      for (uint32_t c = threadIdx.x; c < p.width; c += kNrWide) {
         float du, dg;
         back(c, du, dg);
         const float g = du * nr_weight<T>(p.w1, p.weight_f32, c);
@@ -184,7 +187,7 @@ __global__ __launch_bounds__(kNrBlock) void k_nr_grad(NrArgs p) {
       q = nr_block_sum(q, sm) * over;
       flat1 = p.post == MUSAPY_NORM_LAYER ? q : 0.0f;
     }
-    for (uint32_t c = threadIdx.x; c < p.width; c += kNrBlock) {
+    for (uint32_t c = threadIdx.x; c < p.width; c += kNrWide) {
       float du, dg;
       back(c, du, dg);
       const float D = total(c), n1 = row.n1(c);
@@ -273,6 +276,7 @@ __device__ inline float nr_rsqrt(float v) { return __builtin_amdgcn_rsqf(v); }
 template <class T, int C, class Place>
 __device__ inline void nr_load_weight(const void* w, bool f32, const Place& at, int i, float (&o)[C]) {
   Pack<float, C> p = pack_all<float, C>(at.has(i) ? 1.0f : 0.0f);
+  if constexpr (Place::kVectors > 1) asm volatile("" : "+s"(w));  // loaded for each row: kept across rows, they were spilt
   if (w != nullptr && at.has(i)) {
     if (f32) {
       p = pack_load<false, C>(static_cast<const float*>(w) + at.from(i), at.span(i), 0.0f);
@@ -291,6 +295,7 @@ __device__ inline void nr_load_weight(const void* w, bool f32, const Place& at, 
 // Where a thread works: its row, the rows' step, and its vectors' widths.
 template <int C, int NV, int GL, bool FULL>
 struct NrPlace {
+  static constexpr int kVectors = NV;
   uint32_t t, threads, row, step;
   int waves, n[NV], back[NV];
   __device__ explicit NrPlace(uint32_t width) {
@@ -353,16 +358,22 @@ __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
       if (p.res) nres[i] = pack_load<NT, 8>(static_cast<const TS*>(p.res) + int64_t(row) * p.resp + at.from(i), at.span(i), TS(0.0f));
     }
   };
+  auto fill = [&]() {  // what is not there is zero; no gate: one whose sigmoid is 1
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {  // what is not there is zero; no gate: one whose sigmoid is 1
-    nx[i] = pack_all<T, 8>(T(0.0f));
-    ng[i] = pack_all<T, 8>(T(p.gate ? 0.0f : __builtin_inff()));
-    nres[i] = pack_all<TS, 8>(TS(0.0f));
-  }
+    for (int i = 0; i < NV; ++i) {
+      nx[i] = pack_all<T, 8>(T(0.0f));
+      ng[i] = pack_all<T, 8>(T(p.gate ? 0.0f : __builtin_inff()));
+      nres[i] = pack_all<TS, 8>(TS(0.0f));
+    }
+  };
+  fill();
   const float over = 1.0f / float(p.width);
   if (kAhead && at.row < p.rows) load(at.row);
   for (uint32_t row = at.row; row < p.rows; row += at.step) {
-    if (!kAhead) load(row);
+    if (!kAhead) {
+      fill();  // (kept across rows, it would take the registers that the row is then copied to)
+      load(row);
+    }
     Pack<T, 8> g[NV];
     Pack<TS, 8> res[NV];
     float u[NV][8];
@@ -494,12 +505,15 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
       if (p.dy) ny[i] = pack_load<NT, C>(static_cast<const T*>(p.dy) + int64_t(row) * p.dyp + at.from(i), at.span(i), T(0.0f));
     }
   };
+  auto fill = [&]() {  // what is not there is zero; no gate: one whose sigmoid is 1
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {  // what is not there is zero; no gate: one whose sigmoid is 1
-    nx[i] = ny[i] = pack_all<T, C>(T(0.0f));
-    ng[i] = pack_all<T, C>(T(p.gate ? 0.0f : __builtin_inff()));
-    nr[i] = nd[i] = pack_all<TS, C>(TS(0.0f));
-  }
+    for (int i = 0; i < NV; ++i) {
+      nx[i] = ny[i] = pack_all<T, C>(T(0.0f));
+      ng[i] = pack_all<T, C>(T(p.gate ? 0.0f : __builtin_inff()));
+      nr[i] = nd[i] = pack_all<TS, C>(TS(0.0f));
+    }
+  };
+  fill();
   const int shift = at.t % 2 * C;
   uint32_t keeps[NV], later[NV];
   bool spare = false;
@@ -508,7 +522,10 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
   const float over = 1.0f / float(p.width);
   if (kAhead && at.row < p.rows) load(at.row);
   for (uint32_t row = at.row; row < p.rows; row += at.step) {
-    if (!kAhead) load(row);
+    if (!kAhead) {
+      fill();  // (kept across rows, it would take the registers that the row is then copied to)
+      load(row);
+    }
     Pack<T, C> x[NV], g[NV], y[NV];
     Pack<TS, C> r[NV], d[NV];
 #pragma unroll
@@ -554,7 +571,10 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
       float s[LAYER ? 4 : 3] = {};
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (!kAhead) pre_weights(i);
+        if (!kAhead) {
+          __builtin_amdgcn_sched_barrier(0);  // else every vector's weights are loaded first, and spilt
+          pre_weights(i);
+        }
 #pragma unroll
         for (int e = 0; e < C; ++e) {
           const float a = xc(i, e), b = rc(i, e), q = dy(i, e) * w2[e];
@@ -599,6 +619,7 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
       const uint32_t keep = keeps[i] >> shift;
       float D[C], dg[C];
       if (!kAhead) {
+        __builtin_amdgcn_sched_barrier(0);
         weights(i);
         pre_weights(i);
       }
@@ -723,6 +744,7 @@ NrRoute nr_route(const musapy_norm_residual_args* p, bool grad) {
   const uint64_t vecs = grad ? (p->width + 3) / 4 : (p->width + 7) / 8;
   const uint64_t rows = p->rows;
   if (p->width > (grad ? 12288 : 16384)) {
+    r.threads = kNrWide;
     r.blocks = r.workers = unsigned(grad ? (rows < 512 ? rows : 512) : rows);
     return r;
   }
