@@ -200,7 +200,7 @@ __device__ inline float gs_look_back(const GsSplit& sp, uint32_t chain, uint32_t
   uint32_t spins = 0;
   bool done = false;
   // the tiles of the group in front of this one
-  uint64_t w[kGsGroup - 1];
+  uint64_t w[kGsGroup - 1] = {};
   for (; !done && spins < sp.spin_limit; ++spins) {
     bool ok = true;
 #pragma unroll
