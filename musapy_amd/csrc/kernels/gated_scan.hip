@@ -3,8 +3,9 @@
 
 namespace mpy {
 
-// One thread per V lanes, in batches of steps whose loads are all in flight before the first is used;
-// V = 1 takes any strides.
+// One thread per V lanes, in batches of steps: two lanes, so that short scans have threads enough
+// (16 steps of (64, 8192) lanes bf16 14.4 us, with eight lanes a thread 30.2); V = 1 takes any strides.  A
+// batch's loads are issued before the stores of the one in front, which they would else wait behind.
 template <class TX, class TG, bool BLEND, int V>
 __global__ __launch_bounds__(kGsBlock) void k_gs_walk(GsArgs p) {
   const uint64_t q = uint64_t(blockIdx.x) * kGsBlock + threadIdx.x;
@@ -23,15 +24,28 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_walk(GsArgs p) {
   float h[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) h[v] = p.first && v < nl ? p.first[off[kGsState] + v] : 0.0f;
+  GsBatch<TX, V> nb;
+  GsBatch<TG, V> ng;
+  bool ncuts[kGsBatch];
+  auto load = [&](uint64_t t) {
+    const int steps = p.T - t < uint64_t(kGsBatch) ? int(p.T - t) : kGsBatch;
+    nb.load(x, p.ts[kGsX], p.ls[kGsX], nl, steps);
+    ng.load(gate, p.ts[kGsGate], p.ls[kGsGate], nl, steps);
+#pragma unroll
+    for (int s = 0; s < kGsBatch; ++s) ncuts[s] = reset && s < steps && reset[s * p.ts[kGsReset]];
+    x += kGsBatch * p.ts[kGsX];
+    gate += kGsBatch * p.ts[kGsGate];
+    if (reset) reset += kGsBatch * p.ts[kGsReset];
+  };
+  if (p.T > 0) load(0);
   for (uint64_t t = 0; t < p.T; t += kGsBatch) {
     const int steps = p.T - t < uint64_t(kGsBatch) ? int(p.T - t) : kGsBatch;
-    GsBatch<TX, V> b;
-    GsBatch<TG, V> g;
+    const GsBatch<TX, V> b = nb;
+    const GsBatch<TG, V> g = ng;
     bool cuts[kGsBatch];
-    b.load(x, p.ts[kGsX], p.ls[kGsX], nl, steps);
-    g.load(gate, p.ts[kGsGate], p.ls[kGsGate], nl, steps);
 #pragma unroll
-    for (int s = 0; s < kGsBatch; ++s) cuts[s] = reset && s < steps && reset[s * p.ts[kGsReset]];
+    for (int s = 0; s < kGsBatch; ++s) cuts[s] = ncuts[s];
+    if (t + kGsBatch < p.T) load(t + kGsBatch);
 #pragma unroll
     for (int s = 0; s < kGsBatch; ++s) {
       if (s >= steps) break;
@@ -47,10 +61,7 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_walk(GsArgs p) {
       }
       gs_store<TX, V>(out + s * p.ts[kGsOut], nl, h);
     }
-    x += kGsBatch * p.ts[kGsX];
-    gate += kGsBatch * p.ts[kGsGate];
     out += kGsBatch * p.ts[kGsOut];
-    if (reset) reset += kGsBatch * p.ts[kGsReset];
   }
   if (p.last) {
 #pragma unroll
@@ -356,9 +367,23 @@ GsRoute gs_route(GsPlan& pl, int dtype) {
     if (grid_fits((r.chains + kGsShards) * (r.words ? r.tiles : 1), kGsBlock)) return r;
     r = GsRoute{};
   }
-  r.V = pl.lanes ? gs_vector(dtype) : 1;
+  const int V = gs_vector(dtype);
+  // A walk takes about 0.3 us a step (gradient: 0.8), however many lanes run beside each other; a tile's
+  // time hardly depends on how many of its 128 steps there are.  bf16, us, walk and tiles: 600 lanes x 4 rows,
+  // 8 steps 6.6 and 7.0, 32 steps 11.7 and 7.1; 131072 lanes, 32 steps 14.0 and 17.9, 64 steps 27.8 and 23.5;
+  // 262144 lanes, 64 steps 31.4 and 41.3, 128 steps 58.5 and 40.6; 524288 lanes, 512 steps 309 and 353.
+  const uint64_t lanes = pl.rows * pl.a.D;
+  if (!pl.lanes || T <= 8 + lanes / 4096 || lanes >= 524288) {
+    r.V = pl.lanes ? 2 : 1;
+    if (pl.a.part_lanes >= 0) {  // the lanes of a sum stay those of whole vectors
+      if (pl.a.D % V) r.V = V;
+      else pl.a.part_lanes += V == 8 ? 2 : 1;
+    }
+    gs_vectors(pl, r.V);
+    return r;
+  }
+  r.V = V;
   gs_vectors(pl, r.V);
-  if (!pl.lanes || T <= 16) return r;
   r.chains = (uint64_t(pl.a.nvec) + kGsLt - 1) / kGsLt;
   r.tiles = (T + kGsTileSteps - 1) / kGsTileSteps;
   if (!grid_fits((r.chains + kGsShards) * r.tiles, kGsBlock)) return r;
@@ -456,13 +481,12 @@ int musapy_gated_scan_v1(const musapy_gated_scan_args* p, void* scratch, size_t 
   gs_types(p->dtype, p->gate_dtype, [&](auto tx, auto tg) {
     using TX = decltype(tx);
     using TG = decltype(tg);
-    constexpr int kV = 16 / int(sizeof(TX));
     if (p->kind == MUSAPY_SCAN_BLEND) {
       if (V == 1) k_gs_walk<TX, TG, true, 1><<<grid, kGsBlock, 0, st>>>(pl.a);
-      else k_gs_walk<TX, TG, true, kV><<<grid, kGsBlock, 0, st>>>(pl.a);
+      else k_gs_walk<TX, TG, true, 2><<<grid, kGsBlock, 0, st>>>(pl.a);
     } else {
       if (V == 1) k_gs_walk<TX, TG, false, 1><<<grid, kGsBlock, 0, st>>>(pl.a);
-      else k_gs_walk<TX, TG, false, kV><<<grid, kGsBlock, 0, st>>>(pl.a);
+      else k_gs_walk<TX, TG, false, 2><<<grid, kGsBlock, 0, st>>>(pl.a);
     }
   });
   return 0;

@@ -3,8 +3,7 @@
 
 namespace mpy {
 
-// One thread per V lanes, from the last step to the first, in batches of steps whose loads are all in
-// flight before the first is used; V = 1 takes any strides.
+// One thread per V lanes, from the last step to the first, in batches as the forward's.
 template <class TX, class TG, bool BLEND, int V>
 __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
   const uint64_t q = uint64_t(blockIdx.x) * kGsBlock + threadIdx.x;
@@ -21,22 +20,33 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
   float c[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) c[v] = p.first && v < nl ? p.first[off[kGsState] + v] : 0.0f;
+  GsBatch<TX, V> nd, nh, nx;
+  GsBatch<TG, V> ng;
+  bool ncuts[kGsBatch];
+  auto load = [&](uint64_t k0) {
+    const int64_t t = int64_t(p.T - 1 - k0);
+    const int steps = !on ? 0 : p.T - k0 < uint64_t(kGsBatch) ? int(p.T - k0) : kGsBatch;
+    nd.load(static_cast<const TX*>(p.dh) + off[kGsDh] + t * p.ts[kGsDh], -p.ts[kGsDh], p.ls[kGsDh], nl, steps);
+    ng.load(static_cast<const TG*>(p.gate) + off[kGsGate] + t * p.ts[kGsGate], -p.ts[kGsGate], p.ls[kGsGate], nl, steps);
+    if constexpr (BLEND)
+      nx.load(static_cast<const TX*>(p.x) + off[kGsX] + t * p.ts[kGsX], -p.ts[kGsX], p.ls[kGsX], nl, steps);
+    // (step t = 0 has no h[t-1])
+    nh.load(static_cast<const TX*>(p.h) + off[kGsH] + (t - 1) * p.ts[kGsH], -p.ts[kGsH], p.ls[kGsH], nl,
+            steps > 0 && k0 + steps == p.T ? steps - 1 : steps);
+#pragma unroll
+    for (int s = 0; s < kGsBatch; ++s)
+      ncuts[s] = p.reset && s < steps && p.reset[off[kGsReset] + (t - s) * p.ts[kGsReset]];
+  };
+  if (p.T > 0) load(0);
   for (uint64_t k0 = 0; k0 < p.T; k0 += kGsBatch) {
     const int steps = p.T - k0 < uint64_t(kGsBatch) ? int(p.T - k0) : kGsBatch;
     const int64_t tl = int64_t(p.T - 1 - k0);
-    GsBatch<TX, V> bd, bh, bx;
-    GsBatch<TG, V> bg;
+    const GsBatch<TX, V> bd = nd, bh = nh, bx = nx;
+    const GsBatch<TG, V> bg = ng;
     bool cuts[kGsBatch];
-    const int some = on ? steps : 0;
-    bd.load(static_cast<const TX*>(p.dh) + off[kGsDh] + tl * p.ts[kGsDh], -p.ts[kGsDh], p.ls[kGsDh], nl, some);
-    bg.load(static_cast<const TG*>(p.gate) + off[kGsGate] + tl * p.ts[kGsGate], -p.ts[kGsGate], p.ls[kGsGate], nl, some);
-    if constexpr (BLEND) bx.load(static_cast<const TX*>(p.x) + off[kGsX] + tl * p.ts[kGsX], -p.ts[kGsX], p.ls[kGsX], nl, some);
-    // (step t = 0 has no h[t-1])
-    bh.load(static_cast<const TX*>(p.h) + off[kGsH] + (tl - 1) * p.ts[kGsH], -p.ts[kGsH], p.ls[kGsH], nl,
-            some > 0 && k0 + steps == p.T ? some - 1 : some);
 #pragma unroll
-    for (int s = 0; s < kGsBatch; ++s)
-      cuts[s] = p.reset && s < some && p.reset[off[kGsReset] + (tl - s) * p.ts[kGsReset]];
+    for (int s = 0; s < kGsBatch; ++s) cuts[s] = ncuts[s];
+    if (k0 + kGsBatch < p.T) load(k0 + kGsBatch);
 #pragma unroll
     for (int s = 0; s < kGsBatch; ++s) {
       if (s >= steps) break;
@@ -335,9 +345,11 @@ int musapy_gated_scan_grad_v1(const musapy_gated_scan_args* p, void* scratch, si
     constexpr int kV = 16 / int(sizeof(TX));
     if (p->kind == MUSAPY_SCAN_BLEND) {
       if (V == 1) k_gs_grad_walk<TX, TG, true, 1><<<grid, kGsBlock, 0, st>>>(pl.a);
+      else if (V == 2) k_gs_grad_walk<TX, TG, true, 2><<<grid, kGsBlock, 0, st>>>(pl.a);
       else k_gs_grad_walk<TX, TG, true, kV><<<grid, kGsBlock, 0, st>>>(pl.a);
     } else {
       if (V == 1) k_gs_grad_walk<TX, TG, false, 1><<<grid, kGsBlock, 0, st>>>(pl.a);
+      else if (V == 2) k_gs_grad_walk<TX, TG, false, 2><<<grid, kGsBlock, 0, st>>>(pl.a);
       else k_gs_grad_walk<TX, TG, false, kV><<<grid, kGsBlock, 0, st>>>(pl.a);
     }
   });
