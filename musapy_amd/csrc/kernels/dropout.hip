@@ -20,6 +20,8 @@ struct DropArgs {
 
 // A thread takes kDropGroups groups of eight columns, one call of the generator each, a workgroup's width
 // apart: their loads are all in flight before the first is used.  UNIT: the columns are unit-stride.
+// Bound by HBM: (16384, 4096) bf16 47.5 us, 5.6 TB/s (one group a thread 126 us); (2047, 999) f32 out of rows
+// of 2048 6.4 us, a launch's time.
 constexpr int kDropGroups = 4;
 
 template <class T, bool UNIT, bool NT>

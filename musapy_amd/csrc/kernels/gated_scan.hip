@@ -70,7 +70,10 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_walk(GsArgs p) {
   }
 }
 
-// One tile (gated_scan.hpp) a workgroup; SPLIT: several tiles to a chain.
+// One tile (gated_scan.hpp) a workgroup; SPLIT: several tiles to a chain.  Bound by HBM as rows in pieces of
+// 128 bytes use it: (8, 2048, 4096) bf16 blend 93 us with the clearing of its words, 4.3 TB/s, where a copy in
+// that order takes 88 us (of 512-byte pieces, for twice the registers or a quarter of the steps, 65 to
+// 69); (65536, 2048) bf16 with f32 gates 228 us, 4.7 TB/s.
 template <class TX, class TG, bool BLEND, bool RESET, bool SPLIT, bool NT>
 __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(4))) void k_gs_tiles(GsArgs p, GsSplit sp) {
   constexpr int V = 16 / int(sizeof(TX));
@@ -147,7 +150,8 @@ __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(4))) v
   if (tile + 1 == sp.tiles && p.last && at.state_on) p.last[at.state] = P;
 }
 
-// Rows of unit-stride steps (gated_scan_rows.hpp).
+// Rows of unit-stride steps (gated_scan_rows.hpp): (4, 1500, 5001) f32 76.9 us, 4.7 TB/s, on rows that start
+// off cache lines.
 template <class TX, class TG, bool BLEND, bool RESET, int GW, bool SPLIT, bool NT>
 __global__ __launch_bounds__(kGsBlock) void k_gs_rows(GsArgs p, GsSplit sp) {
   __shared__ GsRowTile sm;

@@ -3,7 +3,8 @@
 
 namespace mpy {
 
-// One thread per V lanes, from the last step to the first, in batches as the forward's.
+// One thread per V lanes, from the last step to the first, in batches as the forward's (16 steps of (64, 8192)
+// bf16 blend 32 us, 3.3 TB/s; with eight lanes a thread 63).
 template <class TX, class TG, bool BLEND, int V>
 __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
   const uint64_t q = uint64_t(blockIdx.x) * kGsBlock + threadIdx.x;
@@ -101,7 +102,9 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
 
 // One tile a workgroup, over reversed time: step k is t = T - 1 - k.  What was loaded stays as it was,
 // and the factors are formed twice, for the tile's map and for its results: registers are dearer here
-// than the second sigmoid.
+// than the second sigmoid.  Bound as the forward's tiles: (8, 2048, 4096) bf16 blend 177 us with the
+// clearing of its words, 4.6 TB/s; (2, 4099, 16, 128) f16 with decays shared by a head's channels 42 us, of which
+// clearing takes 4.7 and the sums over the rest of a head 4.6.
 template <class TX, class TG, bool BLEND, bool RESET, bool SPLIT, bool NT>
 __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(3))) void k_gs_grad_tiles(GsArgs p, GsSplit sp) {
   constexpr int V = 16 / int(sizeof(TX));

