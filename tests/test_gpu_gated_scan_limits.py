@@ -4,7 +4,7 @@ import pytest
 
 import musapy_amd as ms
 from tests import blocks_reference as R
-from tests.test_gpu_gated_scan import run_forward
+from tests.test_gpu_gated_scan import run_forward, run_grad
 from tests.test_gpu_wait_faults import _fresh_stream_case
 
 pytestmark = pytest.mark.gpu
@@ -54,3 +54,21 @@ def test_vectors_that_end_inside_rows_of_any_size():
         for steps in (3, 20, 300):
             run_forward(rng, (2, steps, width), 1, "blend", "bf16", "bf16", h0=True)
             run_forward(rng, (2, steps, width), 1, "decay", "f16", "f32", reset=(2, steps, 1))
+
+
+# few steps of many lanes go step by step, one step more in tiles
+@pytest.mark.parametrize("steps", [20, 21])
+@pytest.mark.parametrize("dt,gdt", [("bf16", "bf16"), ("f16", "f32"), ("f32", "f32")])
+def test_few_steps_of_many_lanes(dt, gdt, steps):
+    rng = np.random.default_rng(steps)
+    run_forward(rng, (5, steps, 9999), 1, "blend", dt, gdt, h0=True, reset=(5, steps, 1))
+    run_grad(rng, (5, steps, 9999), 1, "blend", dt, gdt, h0=True, reset=(5, steps, 1), dstate=True)
+
+
+@pytest.mark.parametrize("steps", [1, 6, 8, 9, 20])
+@pytest.mark.parametrize("width", [64, 125, 128, 200])
+def test_few_steps_of_gates_shared_by_a_heads_channels(width, steps):
+    rng = np.random.default_rng(width + steps)
+    for dt, gdt in (("f16", "f32"), ("bf16", "bf16"), ("f32", "f32")):
+        for heads in (3, 80):
+            run_grad(rng, (5, steps, heads, width), 1, "decay", dt, gdt, gshape=(5, steps, heads, 1), h0=True, dstate=True)
