@@ -501,6 +501,16 @@ typedef struct {
 } musapy_gated_scan_args;
 size_t musapy_gated_scan_scratch_v1(const musapy_gated_scan_args* args, int grad);
 size_t musapy_gated_scan_parts_v1(const musapy_gated_scan_args* args);
+/* How these arguments are launched (nothing is, here): `kind`; rows of `lanes` lanes each, as `vectors`
+ * vectors of `vector` lanes to a row (the last may be a part of one); WALK: a thread to a vector; TILES,
+ * ROWS: `chains` of neighbouring vectors, or rows, with `tiles` of steps each, a workgroup to a tile where
+ * `split`.  An empty call has rows 0. */
+enum { MUSAPY_SCAN_WALK = 0, MUSAPY_SCAN_TILES = 1, MUSAPY_SCAN_ROWS = 2 };
+typedef struct {
+  int kind, vector, split;
+  size_t rows, lanes, vectors, chains, tiles;
+} musapy_gated_scan_route;
+int musapy_gated_scan_route_v1(const musapy_gated_scan_args* args, int grad, musapy_gated_scan_route* route);
 int musapy_gated_scan_v1(const musapy_gated_scan_args* args, void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes, hipStream_t stream);
 int musapy_gated_scan_grad_v1(const musapy_gated_scan_args* args, void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes, hipStream_t stream);
 

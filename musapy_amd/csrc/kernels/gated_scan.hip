@@ -377,7 +377,9 @@ GsRoute gs_route(GsPlan& pl, int dtype) {
   // 8 steps 6.6 and 7.0, 32 steps 11.7 and 7.1; 131072 lanes, 32 steps 14.0 and 17.9, 64 steps 27.8 and 23.5;
   // 262144 lanes, 64 steps 31.4 and 41.3, 128 steps 58.5 and 40.6; 524288 lanes, 512 steps 309 and 353.
   const uint64_t lanes = pl.rows * pl.a.D;
-  if (!pl.lanes || T <= 8 + lanes / 4096 || lanes >= 524288) {
+  gs_vectors(pl, V);
+  const uint64_t chains = (uint64_t(pl.a.nvec) + kGsLt - 1) / kGsLt, tiles = (T + kGsTileSteps - 1) / kGsTileSteps;
+  if (!pl.lanes || T <= 8 + lanes / 4096 || lanes >= 524288 || !grid_fits((chains + kGsShards) * tiles, kGsBlock)) {
     r.V = pl.lanes ? 2 : 1;
     if (pl.a.part_lanes >= 0) {  // the lanes of a sum stay those of whole vectors
       if (pl.a.D % V) r.V = V;
@@ -386,12 +388,10 @@ GsRoute gs_route(GsPlan& pl, int dtype) {
     gs_vectors(pl, r.V);
     return r;
   }
-  r.V = V;
-  gs_vectors(pl, r.V);
-  r.chains = (uint64_t(pl.a.nvec) + kGsLt - 1) / kGsLt;
-  r.tiles = (T + kGsTileSteps - 1) / kGsTileSteps;
-  if (!grid_fits((r.chains + kGsShards) * r.tiles, kGsBlock)) return r;
   r.kind = GsRoute::kTiles;
+  r.V = V;
+  r.chains = chains;
+  r.tiles = tiles;
   if (r.tiles > 1) words(kGsLt * uint64_t(r.V));
   return r;
 }
@@ -438,6 +438,24 @@ size_t musapy_gated_scan_scratch_v1(const musapy_gated_scan_args* p, int grad) {
   return gs_route(pl, p->dtype).words * 8;
 }
 
+int musapy_gated_scan_route_v1(const musapy_gated_scan_args* p, int grad, musapy_gated_scan_route* route) {
+  GsPlan pl;
+  if (route == nullptr) return gs_bad() ? 0 : -1;
+  if (!gs_plan(p, grad != 0, pl)) return -1;
+  *route = musapy_gated_scan_route{};
+  if (pl.rows == 0 || pl.a.D == 0) return 0;
+  const GsRoute r = gs_route(pl, p->dtype);
+  route->kind = r.kind == GsRoute::kWalk ? MUSAPY_SCAN_WALK : r.kind == GsRoute::kTiles ? MUSAPY_SCAN_TILES : MUSAPY_SCAN_ROWS;
+  route->vector = r.V;
+  route->rows = pl.rows;
+  route->lanes = pl.a.D;
+  route->vectors = pl.a.nv;
+  route->chains = r.chains;
+  route->tiles = r.tiles;
+  route->split = r.words != 0;
+  return 0;
+}
+
 size_t musapy_gated_scan_parts_v1(const musapy_gated_scan_args* p) {
   if (p == nullptr || p->shape == nullptr || p->gate_strides == nullptr || p->ndim < 2 || p->ndim > kMaxDims ||
       p->axis == p->ndim - 1 || p->gate_strides[p->ndim - 1] != 0 || !gs_dtype(p->dtype))
@@ -481,7 +499,7 @@ int musapy_gated_scan_v1(const musapy_gated_scan_args* p, void* scratch, size_t 
     return 0;
   }
   const unsigned grid = unsigned((uint64_t(pl.a.nvec) + kGsBlock - 1) / kGsBlock);
-  if (!grid_fits(grid, kGsBlock)) return gs_bad() ? 0 : -1;
+  if (!grid_fits(grid, kGsBlock) || (V != 1 && V != 2)) return gs_bad() ? 0 : -1;  // (the walks that there are)
   gs_types(p->dtype, p->gate_dtype, [&](auto tx, auto tg) {
     using TX = decltype(tx);
     using TG = decltype(tg);
