@@ -41,7 +41,10 @@ void need_shape(const char* op, const char* what, const Array& a, const Shape& w
 }
 
 // One call's inputs and outputs: the device check, the outputs' checks and allocation, and the
-// ordering across streams before and after the launch.
+// ordering across streams before and after the launch.  The call runs on the stream of the first array given for
+// an output.  A buffer counts as written on its home stream only (where reads are not recorded, and where
+// its array is read back), so the call waits for the home streams of the other given outputs, and
+// those wait for the call.
 class Call {
  public:
   Call(const char* op, const Array& first, const Array* out) : op_(op), device_(first.device), s_(pick_stream(first, out)) {}
@@ -69,7 +72,6 @@ class Call {
         if (o.data.get() == given->data.get()) throw MemoryError("alias detected: two outputs share their buffer");
     }
     Array r = given ? *given : new_array(shape, dtype, device_, s_);
-    r.stream = s_;
     outputs_.push_back(r);
     return r;
   }
@@ -85,12 +87,18 @@ class Call {
     for (const Array& a : outputs_) {
       a.data->wait_last_write_on(s_);
       a.data->wait_reads_on(s_);
+      stream_wait_stream(s_, a.stream);
     }
   }
   void end() {
     check_launch(op_);
     for (const Array& a : inputs_) a.data->record_read(s_);
-    for (const Array& a : outputs_) a.data->record_write(s_);
+    for (const Array& a : outputs_) a.data->record_write(s_);  // (what stays where a wait below fails)
+    for (const Array& a : outputs_) {
+      if (a.stream.get() == s_.get()) continue;
+      stream_wait_stream(a.stream, s_);
+      a.data->record_write(a.stream);
+    }
   }
 
  private:
@@ -223,7 +231,7 @@ std::pair<Array, Array> gated_scan(const Array& x0, const Array& gate0, const Ar
   const Shape shape = x0.shape();
   Strides gs = spread(op, "gate", gate0, shape);
   Strides rs = reset ? spread(op, "reset", *reset, shape) : Strides{};
-  Call call(op, x0, out);
+  Call call(op, x0, out ? out : state_out);
   call.input(&x0, "x");
   call.input(&gate0, "gate");
   call.input(h0, "h0");
@@ -280,7 +288,7 @@ GatedScanGrad gated_scan_grad(const Array& dh0, const Array& x0, const Array& ga
   if (dh0_out && !h0) throw ShapeError("gated_scan_grad: an output for the gradient of h0, but no h0");
   Strides gs = spread(op, "gate", gate0, shape);
   Strides rs = reset ? spread(op, "reset", *reset, shape) : Strides{};
-  Call call(op, x0, dx_out);
+  Call call(op, x0, dx_out ? dx_out : dgate_out ? dgate_out : dh0_out);
   call.input(&dh0, "dh");
   call.input(&x0, "x");
   call.input(&gate0, "gate");
@@ -543,7 +551,10 @@ NormResidualGrad norm_residual_grad(const Array* dr, const Array* dy, const Arra
                                     const NormOptions& o, const NormResidualGrad& outs) {
   const char* op = "norm_residual_grad";
   auto given = [](const std::optional<Array>& a) { return a ? &*a : nullptr; };
-  NormCall c(op, x, o, given(outs.dx));
+  const Array* first = nullptr;
+  for (auto* a : {&outs.dx, &outs.dresidual, &outs.dgate, &outs.dpost_weight, &outs.dscale, &outs.dpre_weight})
+    if (!first) first = given(*a);
+  NormCall c(op, x, o, first);
   if (!dr && !dy) throw ShapeError("norm_residual_grad: neither dresidual nor dy is given");
   if (dy && o.pre == NormKind::None) throw ShapeError("norm_residual_grad: dy without a pre norm");
   if (!r && o.pre != NormKind::None) throw ShapeError("norm_residual_grad: the pre norm's gradient needs residual_out");

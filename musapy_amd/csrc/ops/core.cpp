@@ -414,8 +414,6 @@ void set_current_stream(StreamPtr s) { g_current_stream = std::move(s); }
 
 // ---------------------------------------------------------------------------------------------
 // buffers
-namespace {
-// make `waiter` wait for everything submitted so far on `target`
 void stream_wait_stream(const StreamPtr& waiter, const StreamPtr& target) {
   if (!waiter || !target || waiter.get() == target.get()) return;
   hipEvent_t ev = nullptr;
@@ -425,7 +423,6 @@ void stream_wait_stream(const StreamPtr& waiter, const StreamPtr& target) {
   mpy_rt_event_destroy(ev);  // also when the record or the wait failed
   check_rt(e, "stream wait event");
 }
-}  // namespace
 
 std::shared_ptr<Buffer> Buffer::alloc(size_t nbytes, int device, const StreamPtr& stream) {
   std::shared_ptr<Buffer> b(new Buffer());

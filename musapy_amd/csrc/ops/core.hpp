@@ -161,6 +161,9 @@ class Stream : public std::enable_shared_from_this<Stream> {
 };
 using StreamPtr = std::shared_ptr<Stream>;
 
+// makes `waiter` wait for everything submitted so far on `target` (an event; nothing for one stream)
+void stream_wait_stream(const StreamPtr& waiter, const StreamPtr& target);
+
 // per-device default stream of this backend (one non-blocking stream per device)
 StreamPtr default_stream(int device);
 // ms.synchronize(device): waits for the whole device, then synchronizes every live stream of
