@@ -456,9 +456,11 @@ uint32_t musapy_kernels_set_spin_limit(uint32_t polls);
  *   MUSAPY_SCAN_DECAY  h[t] = g[t] h[t-1] + x[t]
  *   MUSAPY_SCAN_BLEND  h[t] = s h[t-1] + (1 - s) x[t], s = sigmoid(g[t])
  * h[-1] is `first` (zeros when NULL), and counts as 0 at every t whose `reset` byte is not 0,
- * whatever it holds.  Gates are finite; a gate that is not may give NaN where a step-by-step
- * evaluation gives an infinity.  `last` receives h at the last step in f32 (`first` itself when the
- * axis is empty); it may be NULL.
+ * whatever it holds.  Wherever the recurrence's states, from `first` and from 0 at any step, stay in f32's
+ * range, its results are right to f32 rounding, however far products of decays go on the way.  A state beyond
+ * that range is infinite or NaN, and one behind it that would be back is that, infinite or NaN.  Gates are
+ * finite; a gate that is not may give NaN where a step-by-step evaluation gives an infinity.  `last`
+ * receives h at the last step in f32 (`first` itself when the axis is empty); it may be NULL.
  *
  * Its gradient, from dh, dlast (the gradient of `last`; zeros when NULL), x, gate, h and first:
  *   G[t] = dh[t] + c[t+1], c[t] = a[t] G[t] (0 at a reset), c[end] = dlast, with a = g or s

@@ -79,7 +79,8 @@ __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(4))) v
   constexpr int V = 16 / int(sizeof(TX));
   constexpr int S = kGsS;
   constexpr uint32_t kSteps = kGsTileSteps;
-  __shared__ GsTile<V> sm;
+  using F = GsFactor<BLEND>;
+  __shared__ GsTile<V, F> sm;
   uint32_t chain, tile;
   if (!gs_take<SPLIT>(sp, sm.ticket, chain, tile)) return;
   const GsPlace<V> at(p, chain);
@@ -110,38 +111,51 @@ __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(4))) v
 
   float P = 0.0f;
   if (p.first && at.state_on) P = p.first[at.state];
-  float a[S][V], b[S][V], A[V], H[V], c[V];
+  // blend: kept for the results, decay: formed again from the packed words
+  float a[BLEND ? S : 1][V], b[BLEND ? S : 1][V], H[V], c[V];
+  F A[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    A[v] = 1.0f;
+    A[v] = gs_one<F>();
     H[v] = 0.0f;
   }
+  auto step = [&](int s, int v, float h) {
+    const bool cut = RESET && ((cuts >> s) & 1);
+    const float as = BLEND ? a[BLEND ? s : 0][v] : pack_get(wg[s], v), bs = BLEND ? b[BLEND ? s : 0][v] : pack_get(wx[s], v);
+    return cut ? bs : __builtin_fmaf(as, h, bs);
+  };
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    const bool cut = RESET && ((cuts >> s) & 1);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      a[s][v] = pack_get(wg[s], v);
-      b[s][v] = pack_get(wx[s], v);
+      float as = pack_get(wg[s], v);
       if constexpr (BLEND) {
         float rest;
-        gs_sigmoid(a[s][v], a[s][v], rest);
-        b[s][v] *= rest;
+        gs_sigmoid(as, as, rest);
+        a[s][v] = as;
+        b[s][v] = pack_get(wx[s], v) * rest;
       }
-      H[v] = cut ? b[s][v] : __builtin_fmaf(a[s][v], H[v], b[s][v]);
-      A[v] = cut ? __builtin_nanf("") : A[v] * a[s][v];
+      H[v] = step(s, v, H[v]);
+      if constexpr (BLEND) A[v] = RESET && ((cuts >> s) & 1) ? gs_none<F>() : A[v] * as;
     }
   }
 
-  gs_tile_state<V, SPLIT>(sm, A, H, c, P, sp, chain, tile);
+  if constexpr (!BLEND) gs_run_lanes(A, wg, RESET && cuts);
+  gs_tile_state<V, SPLIT, F>(sm, A, H, c, P, sp, chain, tile);
 
+  if constexpr (!BLEND) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      pack_opaque(wx[s]);
+      pack_opaque(wg[s]);
+    }
+  }
   auto finish = [&](auto FULL) {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       if (!decltype(FULL)::value && s >= steps) continue;
-      const bool cut = RESET && ((cuts >> s) & 1);
 #pragma unroll
-      for (int v = 0; v < V; ++v) c[v] = cut ? b[s][v] : __builtin_fmaf(a[s][v], c[v], b[s][v]);
+      for (int v = 0; v < V; ++v) c[v] = step(s, v, c[v]);
       pack_store<NT>(out + s * p.ts[kGsOut], decltype(FULL)::value ? V : at.nl, c);
     }
   };
@@ -154,10 +168,11 @@ __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(4))) v
 // off cache lines.
 template <class TX, class TG, bool BLEND, bool RESET, int GW, bool SPLIT, bool NT>
 __global__ __launch_bounds__(kGsBlock) void k_gs_rows(GsArgs p, GsSplit sp) {
-  __shared__ GsRowTile sm;
+  using F = GsFactor<BLEND>;
+  __shared__ GsRowTile<F> sm;
   uint32_t chain, tile;
   int64_t off[kGsOps];
-  if (!gs_row_take<GW, SPLIT>(p, sp, sm, chain, tile, off)) return;
+  if (!gs_row_take<GW, SPLIT>(p, sp, sm.ticket, chain, tile, off)) return;
   constexpr uint32_t kSteps = GW * kGsRun;
   uint64_t t = uint64_t(tile) * kSteps + threadIdx.x % GW * kGsRun;  // the thread's first step
   auto left = [&](uint64_t at) { return at >= p.T ? 0 : p.T - at < uint64_t(kGsRun) ? int(p.T - at) : kGsRun; };
@@ -176,7 +191,8 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_rows(GsArgs p, GsSplit sp) {
   float P = p.first ? p.first[off[kGsState]] : 0.0f;
   int half = 0;
   for (;;) {
-    float a[kGsRun], b[kGsRun], A = 1.0f, H = 0.0f;
+    float a[kGsRun], b[kGsRun], H = 0.0f;
+    F A = gs_one<F>();
     const uint32_t cuts = ncuts;
 #pragma unroll
     for (int e = 0; e < kGsRun; ++e) {
@@ -189,10 +205,16 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_rows(GsArgs p, GsSplit sp) {
       }
       const bool cut = RESET && ((cuts >> e) & 1);
       H = cut ? b[e] : __builtin_fmaf(a[e], H, b[e]);
-      A = cut ? __builtin_nanf("") : A * a[e];
+      if constexpr (BLEND) A = cut ? gs_none<F>() : A * a[e];
+    }
+    if constexpr (!BLEND) {
+      bool plain = true;
+      A = gs_run(a, plain);
+      if (!plain) A = gs_run_stepwise(a);
+      if (RESET && cuts) A = gs_none<F>();
     }
     if (!SPLIT && tile + 1 < sp.tiles) load(t + kSteps);
-    float c = gs_row_state<GW, SPLIT>(sm, half, A, H, P, sp, chain, tile);
+    float c = gs_row_state<GW, SPLIT, F>(sm, half, A, H, P, sp, chain, tile);
     float h[kGsRun];
 #pragma unroll
     for (int e = 0; e < kGsRun; ++e) {

@@ -7,6 +7,7 @@
 #pragma once
 
 #include <tuple>
+#include <type_traits>
 
 #include "kcommon.hpp"
 #include "pack.hpp"
@@ -122,11 +123,96 @@ struct GsBatch<T, 1> {
 
 // ---- tiles of steps -------------------------------------------------------------------------------
 // A run of steps maps the state c in front of it to A c + H behind it, and two runs compose to
-// (A2 A1, A2 H1 + H2).  A = NaN says that the state in front does not matter (the run holds a
-// reset, or its H is NaN already); a state of 0 is not multiplied, so that a product of growing
-// gates that overflowed does not make it NaN.
+// (A2 A1, A2 H1 + H2).  A run that holds a reset has A = gs_none(), "the state in front does not matter";
+// a state of 0 is not multiplied, so that a product of growing gates that overflowed does not make it NaN.
+//
+// The type of A.  "blend": f32; its factors are at most 1, so that A is at most 1, and what it loses below 2^-126 is
+// lost to the rounding of the state in front.  "decay": a fraction and an exponent, as decays may grow: a product that
+// runs through 2^200 and back, on a state that stays in f32's range all the way, has to come back.  (While the states stay
+// there, products of any run of steps are between 2^-278 and 2^278.)  In f64 it cost 5% more of (65536, 2048) bf16 and
+// twice the registers.
+struct GsWide {
+  float m;  // 0, or from 0.5 to 1 in size; NaN: gs_none()
+  int e;
+};
+template <bool BLEND>
+using GsFactor = std::conditional_t<BLEND, float, GsWide>;
+
+template <class F>
+__device__ inline F gs_one();
+template <>
+__device__ inline float gs_one<float>() { return 1.0f; }
+template <>
+__device__ inline GsWide gs_one<GsWide>() { return {0.5f, 1}; }
+template <class F>  // (a NaN gate gives it too, and has made H NaN already)
+__device__ inline F gs_none();
+template <>
+__device__ inline float gs_none<float>() { return __builtin_nanf(""); }
+template <>
+__device__ inline GsWide gs_none<GsWide>() { return {__builtin_nanf(""), 0}; }
+
 __device__ inline float gs_apply(float A, float H, float c) {
   return c == 0.0f || A != A ? H : __builtin_fmaf(A, c, H);
+}
+__device__ inline float gs_apply(GsWide A, float H, float c) {
+  return c == 0.0f || A.m != A.m ? H : __builtin_amdgcn_ldexpf(A.m * c, A.e) + H;
+}
+// The factor of a run and of the one in front of it together.
+__device__ inline float gs_then(float A, float front) { return A * front; }
+__device__ inline GsWide gs_then(GsWide A, GsWide front) {
+  const float p = A.m * front.m;
+  return {__builtin_amdgcn_frexp_mantf(p), A.e + front.e + __builtin_amdgcn_frexp_expf(p)};
+}
+// The factor of N steps in a row, from their gates.  "decay": as one product where those of two neighbours are of a
+// size that no product of all of them can leave f32's range or its normal numbers; `plain` becomes false where they
+// are not, and the factor is to be formed step by step (which for eight steps takes twice the instructions).
+template <int N>
+__device__ inline GsWide gs_run(const float (&a)[N], bool& plain) {
+  float p[N / 2];
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) p[i] = a[2 * i] * a[2 * i + 1];
+  float all = p[0];
+#pragma unroll
+  for (int i = 1; i < N / 2; ++i) all *= p[i];
+  constexpr float kMost = N == 4 ? 0x1p60f : 0x1p30f;
+  float lo = __builtin_fabsf(p[0]), hi = lo;
+#pragma unroll
+  for (int i = 1; i < N / 2; ++i) {  // (where one is a NaN, so is the product: the factor is gs_none() either way)
+    lo = __builtin_fminf(lo, __builtin_fabsf(p[i]));
+    hi = __builtin_fmaxf(hi, __builtin_fabsf(p[i]));
+  }
+  plain = plain && lo >= 1.0f / kMost && hi <= kMost;
+  return {__builtin_amdgcn_frexp_mantf(all), __builtin_amdgcn_frexp_expf(all)};
+}
+template <int N>
+__device__ inline GsWide gs_run_stepwise(const float (&a)[N]) {
+  GsWide A = gs_one<GsWide>();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float p = a[i] * A.m;
+    A = {__builtin_amdgcn_frexp_mantf(p), A.e + __builtin_amdgcn_frexp_expf(p)};
+  }
+  return A;
+}
+// ... of the steps of each lane of a thread of the tiles
+template <class T, int V, int S>
+__device__ inline void gs_run_lanes(GsWide (&A)[V], const Pack<T, V> (&gates)[S], bool cut) {
+  auto lane = [&](int v, auto&& run) {
+    float a[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) a[s] = pack_get(gates[s], v);
+    A[v] = run(a);
+  };
+  bool plain = true;
+#pragma unroll
+  for (int v = 0; v < V; ++v) lane(v, [&](const float (&a)[S]) { return gs_run(a, plain); });
+  if (!plain) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) lane(v, [&](const float (&a)[S]) { return gs_run_stepwise(a); });
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (cut) A[v] = gs_none<GsWide>();
 }
 
 // Tiles of 32 segments of 4 steps by 8 vectors of lanes: 128 bytes of x a step, every cache line one
@@ -135,7 +221,7 @@ constexpr int kGsLt = 8;
 constexpr int kGsS = 4;                                  // steps of a segment
 constexpr int kGsTileSteps = kGsBlock / kGsLt * kGsS;    // 128
 
-template <int V>
+template <int V, class F>
 struct GsTile {
   static constexpr int BS = kGsBlock;
   static constexpr int kSegs = BS / kGsLt;
@@ -144,14 +230,16 @@ struct GsTile {
   static constexpr int kPer = kSegs / kParts;           // segments of each
   // element v of thread (segment, vector); the padding puts the v of a vector on banks of their own, so
   // that both the threads' accesses and those lane by lane touch every bank once
-  float a[V][BS + kGsLt], h[V][BS + kGsLt];
-  float pa[kParts][kLanes], ph[kParts][kLanes], c[kParts][kLanes];
+  F a[V][BS + kGsLt];
+  float h[V][BS + kGsLt];
+  F pa[kParts][kLanes];
+  float ph[kParts][kLanes], c[kParts][kLanes];
   uint32_t ticket;
 };
 
 // Steps split over workgroups.  For each tile of each chain (a group of vectors) and lane, one word
 // holds the tile's (A, H); every kGsGroup tiles form a group, whose last tile publishes the group's
-// (A, H) too, and later, in the same word, the state behind the group as (NaN, state), which is the
+// (A, H) too, and later, in the same word, the state behind the group as (none, state), which is the
 // map that gives that state whatever lies in front.  A word is 0 until it is published: (+0, +0)
 // goes as (-0, +0), which means the same.
 constexpr uint32_t kGsGroup = 4;
@@ -173,12 +261,41 @@ struct GsSplit {
 constexpr uint32_t kGsShards = 32;
 constexpr uint32_t kGsCounterWords = 16;
 
-__device__ inline uint64_t gs_pack(float A, float H) {
-  const uint64_t w = (uint64_t(__float_as_uint(A)) << 32) | __float_as_uint(H);
+// A word's upper half is A in 32 bits: an f32's own, or a sign, ten bits of exponent and 21 of fraction, rounded
+// to nearest (2^-22, as much as a few of the tile's roundings).  What is too small for the exponent is as small as it
+// can be and what is too large comes back as 2^1000000: the states behind them are 0 and infinite, and infinite behind both.
+__device__ inline uint32_t gs_code(float A) { return __float_as_uint(A); }
+constexpr uint32_t kGsHuge = 1023u << 21, kGsNone = kGsHuge | 1u, kGsTiny = 1u;
+__device__ inline uint32_t gs_code(GsWide A) {
+  const uint32_t b = __float_as_uint(A.m), sign = b & 0x80000000u, f = b & 0x7fffffu;
+  uint32_t c = (uint32_t(A.e + 511) << 21) + ((f + 1u + ((f >> 2) & 1u)) >> 2);
+  c = A.e < -510 ? kGsTiny : A.e > 511 || c > kGsHuge ? kGsHuge : c;
+  c = A.m == 0.0f ? 0u : c;
+  return A.m != A.m ? kGsNone : c | sign;
+}
+template <class F>
+__device__ inline F gs_decode(uint32_t c);
+template <>
+__device__ inline float gs_decode<float>(uint32_t c) { return __uint_as_float(c); }
+template <>
+__device__ inline GsWide gs_decode<GsWide>(uint32_t c) {
+  const uint32_t u = c & 0x7fffffffu, f = u >> 21;
+  const float m = __uint_as_float((c & 0x80000000u) | 0x3f000000u | (u & 0x1fffffu) << 2);
+  return {u == kGsNone ? __builtin_nanf("") : u == 0 ? 0.0f : m, f == 1023 ? 1000000 : int(f) - 511};
+}
+template <class F>
+__device__ inline uint64_t gs_pack(F A, float H) {
+  const uint64_t w = (uint64_t(gs_code(A)) << 32) | __float_as_uint(H);
   return w ? w : uint64_t(0x80000000u) << 32;
 }
-__device__ inline float gs_apply(uint64_t w, float c) {
-  return gs_apply(__uint_as_float(uint32_t(w >> 32)), __uint_as_float(uint32_t(w)), c);
+template <class F>
+__device__ inline F gs_word_factor(uint64_t w) { return gs_decode<F>(uint32_t(w >> 32)); }
+template <class F>
+__device__ inline float gs_apply_word(uint64_t w, float c) { return gs_apply(gs_word_factor<F>(w), __uint_as_float(uint32_t(w)), c); }
+template <class F>
+__device__ inline bool gs_word_is_state(uint64_t w) {
+  const uint32_t c = uint32_t(w >> 32);
+  return std::is_same_v<F, GsWide> ? c == kGsNone : c << 1 > 0xff000000u;
 }
 
 // The state in front of `tile` for one lane, from the group in front's and the tiles of its own
@@ -187,9 +304,8 @@ __device__ inline float gs_apply(uint64_t w, float c) {
 // look-back starts, so results are the same bits run to run.  (ta, th) is the tile's own map; the last
 // tile of a group publishes its group's.  A wait makes at most spin_limit polls, then records its
 // fault and goes on with 0, so every workgroup exits.
-template <int LANES>
-__device__ inline float gs_look_back(const GsSplit& sp, uint32_t chain, uint32_t tile, int lane, float first, float ta,
-                                     float th) {
+template <int LANES, class F>
+__device__ inline float gs_look_back(const GsSplit& sp, uint32_t chain, uint32_t tile, int lane, float first, F ta, float th) {
   const uint32_t group = tile / kGsGroup, in = tile % kGsGroup;
   const uint64_t ws = uint64_t(sp.chains) * LANES;
   uint64_t* const wt = sp.words + (uint64_t(tile) * sp.chains + chain) * LANES + lane;
@@ -205,7 +321,7 @@ __device__ inline float gs_look_back(const GsSplit& sp, uint32_t chain, uint32_t
     bool ok = true;
 #pragma unroll
     for (uint32_t i = 0; i < kGsGroup - 1; ++i) {
-      w[i] = i < in ? ld_relaxed(wt - uint64_t(in - i) * ws) : gs_pack(1.0f, 0.0f);
+      w[i] = i < in ? ld_relaxed(wt - uint64_t(in - i) * ws) : gs_pack(gs_one<F>(), 0.0f);
       ok = ok && w[i] != 0;
     }
     done = __all(ok);
@@ -213,13 +329,14 @@ __device__ inline float gs_look_back(const GsSplit& sp, uint32_t chain, uint32_t
   }
   uint64_t mine = 0;
   if (last) {
-    float ga = 1.0f, gh = 0.0f;
+    F ga = gs_one<F>();
+    float gh = 0.0f;
 #pragma unroll
     for (uint32_t i = 0; i < kGsGroup - 1; ++i) {
-      gh = gs_apply(w[i], gh);
-      ga = ga * __uint_as_float(uint32_t(w[i] >> 32));
+      gh = gs_apply_word<F>(w[i], gh);
+      ga = gs_then(gs_word_factor<F>(w[i]), ga);
     }
-    mine = gs_pack(ga * ta, gs_apply(ta, th, gh));
+    mine = gs_pack(gs_then(ta, ga), gs_apply(ta, th, gh));
     st_relaxed(wg, mine);
   }
   // the state behind the group in front
@@ -230,19 +347,22 @@ __device__ inline float gs_look_back(const GsSplit& sp, uint32_t chain, uint32_t
       uint64_t m[kGsWindow];
       m[0] = ld_relaxed(wg - ws);
       P = __uint_as_float(uint32_t(m[0]));
-      auto state = [](uint64_t x) { return uint32_t(x >> 32) << 1 > 0xff000000u; };  // A is NaN
-      done = __all(state(m[0]));
+      done = __all(gs_word_is_state<F>(m[0]));
       if (done) break;
 #pragma unroll
       for (int d = 1; d < kGsWindow; ++d) m[d] = uint32_t(d) < group ? ld_relaxed(wg - uint64_t(d + 1) * ws) : 0;
-      bool have = false;
+      // the nearest group whose state all lanes know, with the maps of all between
+      int from = 0;
+#pragma unroll
+      for (int d = 1; d < kGsWindow; ++d) {
+        if (from == 0 && !__all(m[d - 1] != 0)) from = kGsWindow;
+        if (from == 0 && __all(gs_word_is_state<F>(m[d]))) from = d;
+      }
+      done = from > 0 && from < kGsWindow;
       P = 0.0f;
 #pragma unroll
-      for (int d = kGsWindow - 1; d >= 0; --d) {
-        P = gs_apply(m[d], P);
-        have = (have || state(m[d])) && m[d] != 0;
-      }
-      done = __all(have);
+      for (int d = kGsWindow - 1; d >= 0; --d)
+        if (done && d <= from) P = gs_apply_word<F>(m[d], P);
       if (!done) __builtin_amdgcn_s_sleep(1);
     }
   }
@@ -250,19 +370,19 @@ __device__ inline float gs_look_back(const GsSplit& sp, uint32_t chain, uint32_t
     if (lane == 0) atomicOr(sp.fault, kFaultGatedScanWait);
     P = 0.0f;
   }
-  if (last) st_relaxed(wg, (uint64_t(0x7fc00000u) << 32) | __float_as_uint(gs_apply(mine, P)));
+  if (last) st_relaxed(wg, gs_pack(gs_none<F>(), gs_apply_word<F>(mine, P)));
 #pragma unroll
   for (uint32_t i = 0; i < kGsGroup - 1; ++i)
-    if (i < in) P = gs_apply(w[i], P);
+    if (i < in) P = gs_apply_word<F>(w[i], P);
   return P;
 }
 
 // From each thread's segment (A, H) to the state c in front of it.  `P` (thread l: the tile's lane l)
 // is the state in front of the first tile; it becomes the one behind this tile.
-template <int V, bool SPLIT>
-__device__ inline void gs_tile_state(GsTile<V>& sm, const float (&A)[V], const float (&H)[V], float (&c)[V], float& P,
+template <int V, bool SPLIT, class F>
+__device__ inline void gs_tile_state(GsTile<V, F>& sm, const F (&A)[V], const float (&H)[V], float (&c)[V], float& P,
                                      const GsSplit& sp, uint32_t chain, uint32_t tile) {
-  using G = GsTile<V>;
+  using G = GsTile<V, F>;
   const int tid = threadIdx.x, lt = tid % kGsLt, seg = tid / kGsLt;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -272,39 +392,43 @@ __device__ inline void gs_tile_state(GsTile<V>& sm, const float (&A)[V], const f
   lds_barrier();
   // lane l of the tile: element l / 8 of vector l % 8
   const int lane = tid % G::kLanes, part = tid / G::kLanes;
-  float* const la = &sm.a[lane / kGsLt][part * G::kPer * kGsLt + lane % kGsLt];
+  F* const la = &sm.a[lane / kGsLt][part * G::kPer * kGsLt + lane % kGsLt];
   float* const lh = &sm.h[lane / kGsLt][part * G::kPer * kGsLt + lane % kGsLt];
-  float a[G::kPer], h[G::kPer];
+  F a[G::kPer];
+  float h[G::kPer];
 #pragma unroll
   for (int i = 0; i < G::kPer; ++i) {
     a[i] = la[i * kGsLt];
     h[i] = lh[i * kGsLt];
   }
-  float pa = 1.0f, ph = 0.0f;
+  F pa = gs_one<F>();
+  float ph = 0.0f;
 #pragma unroll
   for (int i = 0; i < G::kPer; ++i) {
     la[i * kGsLt] = pa;
     lh[i * kGsLt] = ph;
     ph = gs_apply(a[i], h[i], ph);
-    pa = pa * a[i];
+    pa = gs_then(a[i], pa);
   }
   sm.pa[part][lane] = pa;
   sm.ph[part][lane] = ph;
   lds_barrier();
   if (tid < kWave) {  // (of 32 lanes, the wave's other half follows)
-    float xa[G::kParts], xh[G::kParts];
+    F xa[G::kParts];
+    float xh[G::kParts];
 #pragma unroll
     for (int i = 0; i < G::kParts; ++i) {
       xa[i] = sm.pa[i][lane];
       xh[i] = sm.ph[i][lane];
     }
-    float ta = xa[0], th = xh[0];
+    F ta = xa[0];
+    float th = xh[0];
 #pragma unroll
     for (int i = 1; i < G::kParts; ++i) {
       th = gs_apply(xa[i], xh[i], th);
-      ta = ta * xa[i];
+      ta = gs_then(xa[i], ta);
     }
-    if constexpr (SPLIT) P = gs_look_back<G::kLanes>(sp, chain, tile, lane, P, ta, th);
+    if constexpr (SPLIT) P = gs_look_back<G::kLanes, F>(sp, chain, tile, lane, P, ta, th);
     float q = P;
 #pragma unroll
     for (int i = 0; i < G::kParts; ++i) {

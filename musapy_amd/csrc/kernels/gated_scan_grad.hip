@@ -110,7 +110,8 @@ __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(3))) v
   constexpr int V = 16 / int(sizeof(TX));
   constexpr int S = kGsS;
   constexpr uint32_t kSteps = kGsTileSteps;
-  __shared__ GsTile<V> sm;
+  using F = GsFactor<BLEND>;
+  __shared__ GsTile<V, F> sm;
   uint32_t chain, tile;
   if (!gs_take<SPLIT>(sp, sm.ticket, chain, tile)) return;
   const GsPlace<V> at(p, chain);
@@ -144,10 +145,11 @@ __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(3))) v
   else load(std::false_type{});
   float P = 0.0f;
   if (p.first && at.state_on) P = p.first[at.state];
-  float A[V], H[V], c[V];
+  float H[V], c[V];
+  F A[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    A[v] = 1.0f;
+    A[v] = gs_one<F>();
     H[v] = 0.0f;
   }
 #pragma unroll
@@ -158,11 +160,12 @@ __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(3))) v
       float a = pack_get(wg[s], v), rest;
       if constexpr (BLEND) gs_sigmoid(a, a, rest);
       H[v] = cut ? 0.0f : a * (pack_get(wd[s], v) + H[v]);
-      A[v] = cut ? __builtin_nanf("") : A[v] * a;
+      if constexpr (BLEND) A[v] = cut ? gs_none<F>() : A[v] * a;
     }
   }
 
-  gs_tile_state<V, SPLIT>(sm, A, H, c, P, sp, chain, tile);
+  if constexpr (!BLEND) gs_run_lanes(A, wg, RESET && cuts);
+  gs_tile_state<V, SPLIT, F>(sm, A, H, c, P, sp, chain, tile);
 
 #pragma unroll
   for (int s = 0; s < S; ++s) {
@@ -222,10 +225,11 @@ __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(3))) v
 // Rows of unit-stride steps (gated_scan_rows.hpp), over reversed time: step k is t = T - 1 - k.
 template <class TX, class TG, bool BLEND, bool RESET, int GW, bool SPLIT, bool NT>
 __global__ __launch_bounds__(kGsBlock) void k_gs_grad_rows(GsArgs p, GsSplit sp) {
-  __shared__ GsRowTile sm;
+  using F = GsFactor<BLEND>;
+  __shared__ GsRowTile<F> sm;
   uint32_t chain, tile;
   int64_t off[kGsOps];
-  if (!gs_row_take<GW, SPLIT>(p, sp, sm, chain, tile, off)) return;
+  if (!gs_row_take<GW, SPLIT>(p, sp, sm.ticket, chain, tile, off)) return;
   constexpr uint32_t kSteps = GW * kGsRun;
   uint64_t k = uint64_t(tile) * kSteps + threadIdx.x % GW * kGsRun;
   auto left = [&](uint64_t at) { return at >= p.T ? 0 : p.T - at < uint64_t(kGsRun) ? int(p.T - at) : kGsRun; };
@@ -248,7 +252,8 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_rows(GsArgs p, GsSplit sp)
   int half = 0;
   for (;;) {
     const uint32_t cuts = ncuts;
-    float a[kGsRun], rest[kGsRun], dh[kGsRun], hb[kGsRun], x[kGsRun], A = 1.0f, H = 0.0f;
+    float a[kGsRun], rest[kGsRun], dh[kGsRun], hb[kGsRun], x[kGsRun], H = 0.0f;
+    F A = gs_one<F>();
     const int n = left(k);
 #pragma unroll
     for (int e = 0; e < kGsRun; ++e) {
@@ -263,7 +268,13 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_rows(GsArgs p, GsSplit sp)
       }
       const bool cut = RESET && ((cuts >> e) & 1);
       H = cut ? 0.0f : a[e] * (dh[e] + H);
-      A = cut ? __builtin_nanf("") : A * a[e];
+      if constexpr (BLEND) A = cut ? gs_none<F>() : A * a[e];
+    }
+    if constexpr (!BLEND) {
+      bool plain = true;
+      A = gs_run(a, plain);
+      if (!plain) A = gs_run_stepwise(a);
+      if (RESET && cuts) A = gs_none<F>();
     }
     if (k + n == p.T && n > 0) {
       const float first = p.h_first ? p.h_first[off[kGsState]] : 0.0f;
@@ -271,7 +282,7 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_rows(GsArgs p, GsSplit sp)
       for (int e = 0; e < kGsRun; ++e) hb[e] = e == n - 1 ? first : hb[e];
     }
     if (!SPLIT && tile + 1 < sp.tiles) load(k + kSteps);
-    float c = gs_row_state<GW, SPLIT>(sm, half, A, H, P, sp, chain, tile);
+    float c = gs_row_state<GW, SPLIT, F>(sm, half, A, H, P, sp, chain, tile);
     float ox[kGsRun], og[kGsRun];
 #pragma unroll
     for (int e = 0; e < kGsRun; ++e) {

@@ -18,19 +18,36 @@ __device__ inline float gs_dpp(float none, float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, MASK, 0xf, false));
 }
 
+template <int CTRL, int MASK>
+__device__ inline GsWide gs_dpp(GsWide none, GsWide v) {
+  return {gs_dpp<CTRL, MASK>(none.m, v.m), __builtin_amdgcn_update_dpp(none.e, v.e, CTRL, MASK, 0xf, false)};
+}
+// the value of the last lane of the thread's group of GW lanes
+template <int GW>
+__device__ inline float gs_lane(float v) {
+  if constexpr (GW == kWave) return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), kWave - 1));
+  else return __shfl(v, GW - 1, GW);
+}
+template <int GW>
+__device__ inline GsWide gs_lane(GsWide v) {
+  if constexpr (GW == kWave) return {gs_lane<GW>(v.m), __builtin_amdgcn_readlane(v.e, kWave - 1)};
+  else return {__shfl(v.m, GW - 1, GW), __shfl(v.e, GW - 1, GW)};
+}
+
 // From each thread's map (A, H) to the one of all threads in front of it in its group (of at most a
 // wave), and the whole group's (ta, th).
-template <int GW>
-__device__ inline void gs_join(float A, float H, float& ea, float& eh, float& ta, float& th) {
+template <int GW, class F>
+__device__ inline void gs_join(F A, float H, F& ea, float& eh, F& ta, float& th) {
   const int l = threadIdx.x % GW;
   auto step = [&](auto ctrl, auto mask, int d) {
-    float pa = gs_dpp<ctrl.value, mask.value>(1.0f, A), ph = gs_dpp<ctrl.value, mask.value>(0.0f, H);
+    F pa = gs_dpp<ctrl.value, mask.value>(gs_one<F>(), A);
+    float ph = gs_dpp<ctrl.value, mask.value>(0.0f, H);
     if (GW < 16 && l < d) {  // a neighbour group's
-      pa = 1.0f;
+      pa = gs_one<F>();
       ph = 0.0f;
     }
     H = gs_apply(A, H, ph);
-    A = A * pa;
+    A = gs_then(A, pa);
   };
   using std::integral_constant;
   step(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{}, 1);  // row_shr:1, 2, 4, 8
@@ -40,34 +57,37 @@ __device__ inline void gs_join(float A, float H, float& ea, float& eh, float& ta
     step(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{}, 8);
     step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{}, 0);  // row_bcast:15
     step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{}, 0);  // row_bcast:31
-    ta = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(A), kWave - 1));
-    th = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(H), kWave - 1));
-    ea = gs_dpp<0x138, 0xf>(1.0f, A);  // wave_shr:1
+    ta = gs_lane<GW>(A);
+    th = gs_lane<GW>(H);
+    ea = gs_dpp<0x138, 0xf>(gs_one<F>(), A);  // wave_shr:1
     eh = gs_dpp<0x138, 0xf>(0.0f, H);
   } else {
-    ta = __shfl(A, GW - 1, GW);
-    th = __shfl(H, GW - 1, GW);
-    ea = gs_dpp<0x111, 0xf>(1.0f, A);
+    ta = gs_lane<GW>(A);
+    th = gs_lane<GW>(H);
+    ea = gs_dpp<0x111, 0xf>(gs_one<F>(), A);
     eh = gs_dpp<0x111, 0xf>(0.0f, H);
     if (l == 0) {
-      ea = 1.0f;
+      ea = gs_one<F>();
       eh = 0.0f;
     }
   }
 }
 
+template <class F>
 struct GsRowTile {
-  float a[2][kGsBlock / kWave], h[2][kGsBlock / kWave];
+  F a[2][kGsBlock / kWave];
+  float h[2][kGsBlock / kWave];
   float state;
   uint32_t ticket;
 };
 
 // The state in front of each thread, from its steps' map; `P`, the state in front of the tile (of the
 // row with SPLIT), becomes the one behind it.  `half` alternates between tiles.
-template <int GW, bool SPLIT>
-__device__ inline float gs_row_state(GsRowTile& sm, int& half, float A, float H, float& P, const GsSplit& sp, uint32_t chain,
+template <int GW, bool SPLIT, class F>
+__device__ inline float gs_row_state(GsRowTile<F>& sm, int& half, F A, float H, float& P, const GsSplit& sp, uint32_t chain,
                                      uint32_t tile) {
-  float ea, eh, ta, th;
+  F ea, ta;
+  float eh, th;
   gs_join<GW < kWave ? GW : kWave>(A, H, ea, eh, ta, th);
   if constexpr (GW <= kWave) {
     const float c = gs_apply(ea, eh, P);
@@ -81,7 +101,8 @@ __device__ inline float gs_row_state(GsRowTile& sm, int& half, float A, float H,
       sm.h[half][wv] = th;
     }
     lds_barrier();
-    float wa[kWaves], wh[kWaves];
+    F wa[kWaves];
+    float wh[kWaves];
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
       wa[i] = sm.a[half][i];
@@ -90,13 +111,14 @@ __device__ inline float gs_row_state(GsRowTile& sm, int& half, float A, float H,
     half ^= 1;
     if constexpr (SPLIT) {
       if (threadIdx.x == 0) {
-        float A4 = wa[0], H4 = wh[0];
+        F A4 = wa[0];
+        float H4 = wh[0];
 #pragma unroll
         for (int i = 1; i < kWaves; ++i) {
           H4 = gs_apply(wa[i], wh[i], H4);
-          A4 = A4 * wa[i];
+          A4 = gs_then(wa[i], A4);
         }
-        sm.state = gs_look_back<1>(sp, chain, tile, 0, P, A4, H4);
+        sm.state = gs_look_back<1, F>(sp, chain, tile, 0, P, A4, H4);
       }
       lds_barrier();
       P = sm.state;
@@ -157,9 +179,9 @@ __device__ inline uint32_t gs_load_cuts(const uint8_t* at, int64_t ts, int n) {
 
 // The row and tile a thread's group starts with; false where there is none.
 template <int GW, bool SPLIT>
-__device__ inline bool gs_row_take(const GsArgs& p, const GsSplit& sp, GsRowTile& sm, uint32_t& chain, uint32_t& tile,
+__device__ inline bool gs_row_take(const GsArgs& p, const GsSplit& sp, uint32_t& ticket, uint32_t& chain, uint32_t& tile,
                                    int64_t (&off)[kGsOps]) {
-  if (!gs_take<SPLIT>(sp, sm.ticket, chain, tile)) return false;
+  if (!gs_take<SPLIT>(sp, ticket, chain, tile)) return false;
   if constexpr (GW < kGsBlock) {
     chain = blockIdx.x * (kGsBlock / GW) + threadIdx.x / GW;
     if (chain >= p.nvec) return false;  // a whole group: the others go on
