@@ -564,8 +564,8 @@ int musapy_norm_residual_grad_v1(const musapy_norm_residual_args* args, void* sc
  * The 16-bit number of column c (last axis) of row r (C-order index of the other axes) comes from
  * Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011)
  * with the key (seed low, seed high) and the counter (c / 8, r, offset low, offset high): column c
- * takes half c % 8 of its four words, low half of word 0 first.  Fewer than 2^32 rows, and fewer
- * than 2^35 columns. */
+ * takes half c % 8 of its four words, low half of word 0 first.  The rows, and the rows times the
+ * columns' groups of eight, are fewer than 2^32: a single row has up to 2^35 - 8 columns. */
 int musapy_dropout_v1(const void* a, void* out, int dtype, int ndim, const size_t* shape, const ssize_t* strides, uint32_t threshold, uint64_t seed, uint64_t offset, hipStream_t stream);
 
 /* ---- planning helper (new; no counterpart in kernels.rs) ----

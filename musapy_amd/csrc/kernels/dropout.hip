@@ -9,7 +9,7 @@ constexpr int kDropBlock = 256;
 struct DropArgs {
   RowIndexer<1> ix;   // all axes but the last
   int64_t ls;         // stride of the last axis
-  uint32_t width;
+  uint64_t width;
   uint32_t groups;    // groups of 8 columns in a row
   uint32_t total;     // groups in all
   FastDiv gdiv;       // divides a group's number by `groups`
@@ -71,12 +71,19 @@ template <class T>
 int launch_dropout(const void* a, void* out, int ndim, const size_t* shape, const ssize_t* strides, uint32_t threshold,
                    uint64_t seed, uint64_t offset, hipStream_t st) {
   DropArgs p{};
+  for (int i = 0; i < ndim; ++i)
+    if (shape[i] == 0) return 0;
+  constexpr uint64_t kLimit = uint64_t(1) << 32;  // rows, groups of columns and their product are numbered in 32 bits
   uint64_t rows = 1;
   int n = 0;
   uint64_t size[kMaxDims];
   int64_t stride[kMaxDims];
+  auto bad = [] {
+    g_wrapper_error = 6;
+    return -1;
+  };
   for (int i = ndim - 2; i >= 0; --i) {
-    rows *= shape[i];
+    if (shape[i] >= kLimit || (rows *= shape[i]) >= kLimit) return bad();
     if (shape[i] == 1) continue;
     if (n > 0 && int64_t(strides[i]) == stride[n - 1] * int64_t(size[n - 1])) {
       size[n - 1] *= shape[i];
@@ -86,30 +93,25 @@ int launch_dropout(const void* a, void* out, int ndim, const size_t* shape, cons
     stride[n++] = strides[i];
   }
   const uint64_t width = ndim ? shape[ndim - 1] : 1;
-  if (rows == 0 || width == 0) return 0;
-  const uint64_t groups = (width + 7) / 8;
-  // rows and groups are numbered in 32 bits
-  if (rows >= (uint64_t(1) << 32) || width >= (uint64_t(1) << 32) || groups * rows >= (uint64_t(1) << 32) ||
-      !grid_fits((groups * rows + kDropBlock - 1) / kDropBlock, kDropBlock)) {
-    g_wrapper_error = 6;
-    return -1;
-  }
+  const uint64_t groups = width / 8 + (width % 8 != 0);
+  if (groups >= kLimit || groups * rows >= kLimit) return bad();
+  const uint64_t grid = (groups * rows + kDropBlock * kDropGroups - 1) / (kDropBlock * kDropGroups);
+  if (!grid_fits(grid, kDropBlock)) return bad();
   p.ix.nd = n;
   for (int i = 0; i < n; ++i) {
     p.ix.div[i] = make_fastdiv(uint32_t(size[i]));
     p.ix.stride[0][i] = stride[i];
   }
   p.ls = ndim ? strides[ndim - 1] : 1;
-  p.width = uint32_t(width);
+  p.width = width;
   p.groups = uint32_t(groups);
   p.total = uint32_t(groups * rows);
   p.gdiv = make_fastdiv(p.groups);
   p.key = philox_key(seed, offset);
   p.threshold = threshold;
   p.scale = dropout_scale(threshold);
-  const unsigned grid = unsigned((uint64_t(p.total) + kDropBlock * kDropGroups - 1) / (kDropBlock * kDropGroups));
   auto go = [&](auto UNIT, auto NT) {
-    k_dropout<T, UNIT.value, NT.value><<<grid, kDropBlock, 0, st>>>(static_cast<const T*>(a), static_cast<T*>(out), p);
+    k_dropout<T, UNIT.value, NT.value><<<unsigned(grid), kDropBlock, 0, st>>>(static_cast<const T*>(a), static_cast<T*>(out), p);
   };
   if (p.ls != 1 && width > 1) go(std::false_type{}, std::false_type{});
   else if (rows * width * sizeof(T) >= kStreamLoadBytes) go(std::true_type{}, std::true_type{});
@@ -131,9 +133,9 @@ extern "C" int musapy_dropout_v1(const void* a, void* out, int dtype, int ndim, 
     g_wrapper_error = 6;
     return -1;
   }
-  uint64_t numel = 1;
-  for (int i = 0; i < ndim; ++i) numel *= shape[i];
-  if (numel > 0 && (a == nullptr || out == nullptr)) {
+  bool any = true;
+  for (int i = 0; i < ndim; ++i) any = any && shape[i] != 0;
+  if (any && (a == nullptr || out == nullptr)) {
     g_wrapper_error = 6;
     return -1;
   }
