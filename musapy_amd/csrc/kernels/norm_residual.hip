@@ -23,8 +23,7 @@ struct NrArgs {
   const void *x, *res, *gate, *dr, *dy, *w1, *scale, *w2;
   int64_t xp, resp, gatep, drp, dyp;
   void *r, *y, *dx, *dres, *dgate;
-  float* part;       // column sums of each worker: [worker][3][width] (dw1, ds, dw2)
-  uint32_t workers;  // workgroups, or waves, that go from row to row
+  float* part;  // column sums of each workgroup: [workgroup][3][width] (dw1, ds, dw2)
 };
 
 __device__ inline float nr_sigmoid(float g) {
@@ -116,15 +115,17 @@ __device__ inline void nr_stats(int kind, uint32_t width, float eps, float* sm, 
 template <class T, class TS>
 __global__ __launch_bounds__(kNrWide) void k_nr(NrArgs p) {
   __shared__ float sm[kNrWide / kWave];
-  NrRow<T, TS> row{p, blockIdx.x};
-  const uint64_t base = uint64_t(blockIdx.x) * p.width;
-  nr_stats(p.post, p.width, p.eps, sm, row.mean1, row.inv1, [&](uint32_t c) { return row.x(c); });
-  float mean2, inv2;
-  nr_stats(p.pre, p.width, p.eps, sm, mean2, inv2, [&](uint32_t c) { return row.r(c); });
-  for (uint32_t c = threadIdx.x; c < p.width; c += kNrWide) {
-    const float r = row.r(c);
-    static_cast<TS*>(p.r)[base + c] = TS(r);
-    if (p.y) static_cast<T*>(p.y)[base + c] = T((r - mean2) * inv2 * nr_weight<T>(p.w2, p.weight_f32, c));
+  for (uint32_t at = blockIdx.x; at < p.rows; at += gridDim.x) {
+    NrRow<T, TS> row{p, at};
+    const uint64_t base = uint64_t(at) * p.width;
+    nr_stats(p.post, p.width, p.eps, sm, row.mean1, row.inv1, [&](uint32_t c) { return row.x(c); });
+    float mean2, inv2;
+    nr_stats(p.pre, p.width, p.eps, sm, mean2, inv2, [&](uint32_t c) { return row.r(c); });
+    for (uint32_t c = threadIdx.x; c < p.width; c += kNrWide) {
+      const float r = row.r(c);
+      static_cast<TS*>(p.r)[base + c] = TS(r);
+      if (p.y) static_cast<T*>(p.y)[base + c] = T((r - mean2) * inv2 * nr_weight<T>(p.w2, p.weight_f32, c));
+    }
   }
 }
 
@@ -751,7 +752,9 @@ NrRoute nr_route(const musapy_norm_residual_args* p, bool grad) {
   const uint64_t rows = p->rows;
   if (p->width > (grad ? 12288 : 16384)) {
     r.threads = kNrWide;
-    r.blocks = r.workers = unsigned(grad ? (rows < 512 ? rows : 512) : rows);
+    // four times what the CUs hold at a time: a workgroup a row would pass a grid's 2^32 threads from 2^22 rows on
+    const uint64_t most = grad ? 512 : 2048;
+    r.blocks = r.workers = unsigned(rows < most ? rows : most);
     return r;
   }
   if (vecs <= kWave) {
@@ -878,6 +881,7 @@ int musapy_norm_residual_v1(const musapy_norm_residual_args* p, hipStream_t st) 
   if (a.rows == 0 || a.width == 0) return 0;
   if (a.x == nullptr || a.r == nullptr) return nr_bad();
   const NrRoute r = nr_route(p, false);
+  if (!grid_fits(r.blocks, r.threads)) return nr_bad();
   nr_types(p->dtype, p->stream_dtype, [&](auto t, auto ts) {
     using T = decltype(t);
     using TS = decltype(ts);
@@ -897,7 +901,6 @@ int musapy_norm_residual_grad_v1(const musapy_norm_residual_args* p, void* scrat
   if (a.rows > 0 && (a.x == nullptr || (a.pre != MUSAPY_NORM_NONE && a.res == nullptr))) return nr_bad();
   if (a.pre == MUSAPY_NORM_NONE) a.dy = nullptr;
   const NrRoute r = nr_route(p, true);
-  a.workers = r.workers;
   if (nr_sums(p) && r.workers > 0) {
     if (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 15) || scratch_bytes < musapy_norm_residual_scratch_v1(p)) {
       g_wrapper_error = 1;
