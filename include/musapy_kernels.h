@@ -469,7 +469,7 @@ uint32_t musapy_kernels_set_spin_limit(uint32_t polls);
  * NULL there.
  *
  * x, gate, reset, h (grad) and dh are strided views of `shape` (stride 0 where one is broadcast; up to
- * 8 dims, or as many as merge to that);
+ * 8 dims, or as many as merge to that; every extent, and the lanes in all, fewer than 2^32);
  * first, last and dlast are C-contiguous over the shape without `axis`; `out` (h, or dx) is
  * C-contiguous over `shape`.  dgate is C-contiguous over `shape` in `dgate_dtype` (gate_dtype or
  * F32) when `parts` is 0.  Where the gate is shared along the last axis (gate stride 0, last axis
@@ -527,8 +527,8 @@ int musapy_gated_scan_grad_v1(const musapy_gated_scan_args* args, void* scratch,
  *   D = dr + norm'(r)(dy pre_weight), dresidual = D, dv = dropout'(D scale), du = dv act(gate),
  *   dx = norm'(x)(du post_weight), dgate = dv u act'(gate), and the column sums over all rows
  *   dpost_weight = sum du n1, dscale = sum D d scale_value, dpre_weight = sum dy n2.
- * Every output may be NULL but the forward's r.  Arrays of `stream_dtype` (dtype or F32): residual, r, dr, dresidual; all others are of
- * `dtype`.  Inputs have unit-stride rows `*_pitch` elements apart; outputs are C-contiguous.
+ * Every output may be NULL but the forward's r; rows and width are fewer than 2^31.  Arrays of
+ * `stream_dtype` (dtype or F32): residual, r, dr, dresidual; all others are of `dtype`.  Inputs have unit-stride rows `*_pitch` elements apart; outputs are C-contiguous.
  * Dropout keeps column c of a row where its 16-bit random number (musapy_dropout_v1) is at least
  * `threshold`, times 65536 / (65536 - threshold); threshold 0 keeps all, 65536 drops all.
  * The column sums go through `scratch` (musapy_norm_residual_scratch_v1 bytes, 16-byte aligned). */

@@ -262,16 +262,21 @@ bool gs_plan(const musapy_gated_scan_args* p, bool grad, GsPlan& out) {
   if (grad && (p->h_strides == nullptr || p->dh_strides == nullptr ||
                (p->dgate_dtype != p->gate_dtype && p->dgate_dtype != MUSAPY_DT_F32)))
     return gs_bad();
-  uint64_t numel = 1;
+  bool empty = false;
   for (int i = 0; i < p->ndim; ++i) {
     if (p->shape[i] >= (uint64_t(1) << 32)) return gs_bad();
-    numel *= p->shape[i];
+    empty = empty || (i != p->axis && p->shape[i] == 0);
   }
-  if (numel > 0 && (p->gate == nullptr || p->out == nullptr || (reads_x && p->x == nullptr) ||
+  out = GsPlan{};
+  if (empty) return true;  // no lanes
+  uint64_t lanes = 1;
+  for (int i = 0; i < p->ndim; ++i)  // lanes are numbered in 32 bits
+    if (i != p->axis && (lanes *= p->shape[i]) >= (uint64_t(1) << 32)) return gs_bad();
+  if (p->shape[p->axis] > (uint64_t(1) << 60) / lanes) return gs_bad();
+  if (p->shape[p->axis] > 0 && (p->gate == nullptr || p->out == nullptr || (reads_x && p->x == nullptr) ||
                     (grad && (p->h == nullptr || p->dh == nullptr || p->dgate == nullptr))))
     return gs_bad();
 
-  out = GsPlan{};
   GsArgs& a = out.a;
   const int nd = p->ndim, axis = p->axis;
   const bool parts = grad && p->parts != 0;
@@ -336,7 +341,6 @@ bool gs_plan(const musapy_gated_scan_args* p, bool grad, GsPlan& out) {
     a.ls[o] = cst[o][0];
     a.ts[o] = st[o][axis];
   }
-  if (uint64_t(lane) >= (uint64_t(1) << 32)) return gs_bad();  // lanes are numbered in 32 bits
   auto unit = [&](int o) { return a.ls[o] == 1 || a.D == 1; };
   out.lanes = (!reads_x || unit(kGsX)) && unit(kGsOut) && unit(kGsState) && (unit(kGsGate) || a.ls[kGsGate] == 0) &&
               (p->reset == nullptr || a.ls[kGsReset] == 0 || a.D == 1) && (!grad || (unit(kGsH) && unit(kGsDh)));

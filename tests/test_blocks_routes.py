@@ -70,3 +70,18 @@ def test_which_calls_go_step_by_step():
     assert route((2, 0, 5), 1, F32, 0).rows == 2 and route((2, 4, 0), 1, F32, 0).rows == 0
     L = lib()
     assert L.musapy_gated_scan_route_v1(None, 0, ctypes.byref(Route())) == -1 and L.musapy_kernels_take_error() == 6
+
+
+def test_extents_whose_products_wrap_round():
+    """Lanes, and elements, that 64 bits do not hold are refused, not numbered by what is left of them."""
+    L = lib()
+    L.musapy_gated_scan_route_v1.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
+    for shape, axis in (((1 << 31, 1, 1 << 31, 4), 1), ((1 << 31, 9, 1 << 31, 1 << 2), 1), ((1 << 16, 5, 1 << 16, 1 << 32), 1),
+                        ((1 << 31, (1 << 32) - 1, 2), 1), (((1 << 32) - 1, (1 << 32) - 1), 0)):
+        n = len(shape)
+        st = (ctypes.c_ssize_t * n)(*[0] * n)
+        for grad in (0, 1):
+            a = ScanArgs(kind=0, dtype=F32, gate_dtype=F32, dgate_dtype=F32, ndim=n, axis=axis, shape=(S * n)(*shape), x=64,
+                         x_strides=st, gate=64, gate_strides=st, h=64, h_strides=st, dh=64, dh_strides=st, out=64, dgate=64)
+            assert L.musapy_gated_scan_route_v1(ctypes.byref(a), grad, ctypes.byref(Route())) == -1, shape
+            assert L.musapy_kernels_take_error() == 6
