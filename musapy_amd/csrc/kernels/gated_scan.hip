@@ -54,12 +54,12 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_walk(GsArgs p) {
         float a = g.get(s, v), in = b.get(s, v);
         if constexpr (BLEND) {
           float rest;
-          gs_sigmoid(a, a, rest);
+          sigmoid_pair(a, a, rest);
           in = rest * in;
         }
         h[v] = cuts[s] ? in : __builtin_fmaf(a, h[v], in);
       }
-      gs_store<TX, V>(out + s * p.ts[kGsOut], nl, h);
+      pack_store<false>(out + s * p.ts[kGsOut], nl, h);
     }
     out += kGsBatch * p.ts[kGsOut];
   }
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(4))) v
       float as = pack_get(wg[s], v);
       if constexpr (BLEND) {
         float rest;
-        gs_sigmoid(as, as, rest);
+        sigmoid_pair(as, as, rest);
         a[s][v] = as;
         b[s][v] = pack_get(wx[s], v) * rest;
       }
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_rows(GsArgs p, GsSplit sp) {
       b[e] = pack_get(nx, e);
       if constexpr (BLEND) {
         float rest;
-        gs_sigmoid(a[e], a[e], rest);
+        sigmoid_pair(a[e], a[e], rest);
         b[e] *= rest;
       }
       const bool cut = RESET && ((cuts >> e) & 1);

@@ -65,30 +65,6 @@ struct GsArgs {
   int part_lanes;            // lanes that share one dgate partial sum: log2 of the vectors; < 0: no sums
 };
 
-// s = sigmoid(g) and 1 - s, each with a small relative error: both from exp(-|g|) <= 1, so neither
-// is a difference of near numbers.  The hardware's exp2 and reciprocal are within 1 ulp.
-__device__ inline void gs_sigmoid(float g, float& s, float& rest) {
-  const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(g));
-  const float r = __builtin_amdgcn_rcpf(1.0f + e);
-  const float er = e * r;
-  s = g >= 0.0f ? r : er;      // a NaN gate: both are NaN
-  rest = g >= 0.0f ? er : r;
-}
-
-template <class T, int V>
-__device__ inline void gs_store(T* p, int nl, const float (&x)[V]) {
-  if (nl == V) {
-    Vec<T, V> w;
-#pragma unroll
-    for (int v = 0; v < V; ++v) w.v[v] = T(x[v]);
-    vstore_el<false, T, V>(p, w);
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v < nl) p[v] = T(x[v]);
-  }
-}
-
 // The S steps of a thread as they lie in memory, `p` at the first one.  FULL: all steps and lanes are
 // there; else `steps` and `nl` of them, and `none` in the others' place.
 template <bool FULL, bool NT, class T, int V, int S>

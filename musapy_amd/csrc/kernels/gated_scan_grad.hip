@@ -68,7 +68,7 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
         const float G = dh[v] + c[v];
         if constexpr (BLEND) {
           float s, rest;
-          gs_sigmoid(g[v], s, rest);
+          sigmoid_pair(g[v], s, rest);
           dx[v] = rest * G;
           dg[v] = G * (hb[v] - x[v]) * (s * rest);
           c[v] = cut ? 0.0f : s * G;
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
           c[v] = cut ? 0.0f : g[v] * G;
         }
       }
-      if (on) gs_store<TX, V>(static_cast<TX*>(p.out) + off[kGsOut] + t * p.ts[kGsOut], nl, dx);
+      if (on) pack_store<false>(static_cast<TX*>(p.out) + off[kGsOut] + t * p.ts[kGsOut], nl, dx);
       if (p.part_lanes >= 0) {
         float sum = 0.0f;
 #pragma unroll
@@ -88,8 +88,8 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
           static_cast<float*>(p.dgate)[off[kGsDgate] + t * p.ts[kGsDgate] + (vec >> p.part_lanes)] = sum;
       } else if (on) {
         const int64_t at = off[kGsDgate] + t * p.ts[kGsDgate];
-        if (p.dgate_f32) gs_store<float, V>(static_cast<float*>(p.dgate) + at, nl, dg);
-        else gs_store<TG, V>(static_cast<TG*>(p.dgate) + at, nl, dg);
+        if (p.dgate_f32) pack_store<false>(static_cast<float*>(p.dgate) + at, nl, dg);
+        else pack_store<false>(static_cast<TG*>(p.dgate) + at, nl, dg);
       }
     }
   }
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(3))) v
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float a = pack_get(wg[s], v), rest;
-      if constexpr (BLEND) gs_sigmoid(a, a, rest);
+      if constexpr (BLEND) sigmoid_pair(a, a, rest);
       H[v] = cut ? 0.0f : a * (pack_get(wd[s], v) + H[v]);
       if constexpr (BLEND) A[v] = cut ? gs_none<F>() : A[v] * a;
     }
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(3))) v
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         float a = pack_get(wg[s], v), rest = 1.0f;
-        if constexpr (BLEND) gs_sigmoid(a, a, rest);
+        if constexpr (BLEND) sigmoid_pair(a, a, rest);
         float hb = pack_get(wh[s], v);
         if (!F && k0 + s + 1 == p.T && p.h_first && v < at.nl) hb = p.h_first[at.off[kGsState] + v];
         if (cut) hb = 0.0f;
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_rows(GsArgs p, GsSplit sp)
       dh[e] = pack_get(nd, j);
       hb[e] = pack_get(nh, j);
       if constexpr (BLEND) {
-        gs_sigmoid(a[e], a[e], rest[e]);
+        sigmoid_pair(a[e], a[e], rest[e]);
         x[e] = pack_get(nx, j);
       }
       const bool cut = RESET && ((cuts >> e) & 1);

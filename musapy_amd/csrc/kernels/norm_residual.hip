@@ -26,16 +26,10 @@ struct NrArgs {
   float* part;  // column sums of each workgroup: [workgroup][3][width] (dw1, ds, dw2)
 };
 
-__device__ inline float nr_sigmoid(float g) {
-  const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(g));
-  const float r = __builtin_amdgcn_rcpf(1.0f + e);
-  return g >= 0.0f ? r : e * r;
-}
 // act(g) and its derivative: with m = g (silu) or 1, act = s m and act' = s (1 - s) m [+ s for silu]
 __device__ inline void nr_act(int kind, float g, float& a, float& slope) {
-  const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(g));
-  const float r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
-  const float s = g >= 0.0f ? r : er, rest = g >= 0.0f ? er : r;
+  float s, rest;
+  sigmoid_pair(g, s, rest);
   const bool silu = kind == MUSAPY_GATE_SILU;
   a = s * (silu ? g : 1.0f);
   slope = __builtin_fmaf(a, rest, silu ? s : 0.0f);
@@ -427,7 +421,9 @@ __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
       for (int e = 0; e < 8; ++e) {
         float v = u[i][e] * inv1 * w1[e];
         const float gv = pack_get(g[i], e);
-        v *= nr_sigmoid(gv) * (kind == MUSAPY_GATE_SILU ? gv : 1.0f);
+        float sg, rest;
+        sigmoid_pair(gv, sg, rest);
+        v *= sg * (kind == MUSAPY_GATE_SILU ? gv : 1.0f);
         v = (keep >> e) & 1 ? v * p.keep_scale : 0.0f;
         u[i][e] = __builtin_fmaf(sc[e], v, pack_get(res[i], e));
       }

@@ -110,4 +110,14 @@ __device__ inline void pack_opaque(Pack<T, N>& p) {
   for (int i = 0; i < p.kWords; ++i) asm volatile("" : "+v"(p.w[i]));
 }
 
+// s = sigmoid(g) and 1 - s, each with a small relative error: both from exp(-|g|) <= 1, so neither
+// is a difference of near numbers.  The hardware's exp2 and reciprocal are within 1 ulp.
+__device__ inline void sigmoid_pair(float g, float& s, float& rest) {
+  const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(g));
+  const float r = __builtin_amdgcn_rcpf(1.0f + e);
+  const float er = e * r;
+  s = g >= 0.0f ? r : er;      // a NaN gate: both are NaN
+  rest = g >= 0.0f ? er : r;
+}
+
 }  // namespace mpy
