@@ -71,9 +71,9 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_walk(GsArgs p) {
 }
 
 // One tile (gated_scan.hpp) a workgroup; SPLIT: several tiles to a chain.  Bound by HBM as rows in pieces of
-// 128 bytes use it: (8, 2048, 4096) bf16 blend 93 us with the clearing of its words, 4.3 TB/s, where a copy in
-// that order takes 88 us (of 512-byte pieces, for twice the registers or a quarter of the steps, 65 to
-// 69); (65536, 2048) bf16 with f32 gates 228 us, 4.7 TB/s.
+// 128 bytes use it: (8, 2048, 4096) bf16 blend 93 us with the clearing of its words, 4.3 TB/s, where a plain copy in
+// that order takes 88 us (of 512-byte pieces 65 to 69: tiles of wider pieces were not tried); (65536, 2048) bf16
+// decay with f32 gates 233 us, 4.6 TB/s.
 template <class TX, class TG, bool BLEND, bool RESET, bool SPLIT, bool NT>
 __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(4))) void k_gs_tiles(GsArgs p, GsSplit sp) {
   constexpr int V = 16 / int(sizeof(TX));
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(4))) v
   if (tile + 1 == sp.tiles && p.last && at.state_on) p.last[at.state] = P;
 }
 
-// Rows of unit-stride steps (gated_scan_rows.hpp): (4, 1500, 5001) f32 76.9 us, 4.7 TB/s, on rows that start
+// Rows of unit-stride steps (gated_scan_rows.hpp): (4, 1500, 5001) f32 77.0 us, 4.7 TB/s, on rows that start
 // off cache lines.
 template <class TX, class TG, bool BLEND, bool RESET, int GW, bool SPLIT, bool NT>
 __global__ __launch_bounds__(kGsBlock) void k_gs_rows(GsArgs p, GsSplit sp) {
@@ -402,6 +402,11 @@ GsRoute gs_route(GsPlan& pl, int dtype) {
   // time hardly depends on how many of its 128 steps there are.  bf16, us, walk and tiles: 600 lanes x 4 rows,
   // 8 steps 6.6 and 7.0, 32 steps 11.7 and 7.1; 131072 lanes, 32 steps 14.0 and 17.9, 64 steps 27.8 and 23.5;
   // 262144 lanes, 64 steps 31.4 and 41.3, 128 steps 58.5 and 40.6; 524288 lanes, 512 steps 309 and 353.
+  // The gradient's tiles are slower by as much: 2400 lanes, 8 steps 10.2 and 11.2, 16 steps 16.3 and 11.0; 65536
+  // lanes, 16 steps 17.1 and 21.2, 32 steps 29.9 and 21.5; 262144 lanes, 64 steps 72 and 97, 128 steps 140 and 111;
+  // 524288 lanes, 512 steps 729 and 780.  f32 decay: 16384 lanes, 8 steps 5.7 and 5.7; 65536 lanes, 16 steps 8.0 and
+  // 9.1, 32 steps 12.3 and 10.3; 262144 lanes, 64 steps 41.3 and 40.3; 524288 lanes, 512 steps 602 and 780 (gradient
+  // 8.6 and 7.2; 13.8 and 13.9, 23.2 and 14.9; 71.1 and 71.3; 1052 and 1022).
   const uint64_t lanes = pl.rows * pl.a.D;
   gs_vectors(pl, V);
   const uint64_t chains = (uint64_t(pl.a.nvec) + kGsLt - 1) / kGsLt, tiles = (T + kGsTileSteps - 1) / kGsTileSteps;

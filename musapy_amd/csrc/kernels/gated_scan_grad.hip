@@ -102,9 +102,10 @@ __global__ __launch_bounds__(kGsBlock) void k_gs_grad_walk(GsArgs p) {
 
 // One tile a workgroup, over reversed time: step k is t = T - 1 - k.  What was loaded stays as it was,
 // and the factors are formed twice, for the tile's map and for its results: registers are dearer here
-// than the second sigmoid.  Bound as the forward's tiles: (8, 2048, 4096) bf16 blend 177 us with the
-// clearing of its words, 4.6 TB/s; (2, 4099, 16, 128) f16 with decays shared by a head's channels 42 us, of which
-// clearing takes 4.7 and the sums over the rest of a head 4.6.
+// than the second sigmoid.  Bound as the forward's tiles: (8, 2048, 4096) bf16 blend, with the clearing of its
+// words, 172 to 203 us, 4.0 to 4.7 TB/s, by where its five arrays lie (the same build, calls and process); (2, 4099, 16, 128)
+// f16 with decays shared by a head's channels 45 to 50 us, of which clearing takes 4.9 and the sums over the rest of a
+// head 4.6.
 template <class TX, class TG, bool BLEND, bool RESET, bool SPLIT, bool NT>
 __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(3))) void k_gs_grad_tiles(GsArgs p, GsSplit sp) {
   constexpr int V = 16 / int(sizeof(TX));
@@ -222,7 +223,8 @@ __global__ __launch_bounds__(kGsBlock) __attribute__((amdgpu_waves_per_eu(3))) v
   if (tile + 1 == sp.tiles && p.last && at.state_on) p.last[at.state] = P;
 }
 
-// Rows of unit-stride steps (gated_scan_rows.hpp), over reversed time: step k is t = T - 1 - k.
+// Rows of unit-stride steps (gated_scan_rows.hpp), over reversed time: step k is t = T - 1 - k.  (4, 1500, 5001) f32
+// 130 us, 4.6 TB/s.
 template <class TX, class TG, bool BLEND, bool RESET, int GW, bool SPLIT, bool NT>
 __global__ __launch_bounds__(kGsBlock) void k_gs_grad_rows(GsArgs p, GsSplit sp) {
   using F = GsFactor<BLEND>;

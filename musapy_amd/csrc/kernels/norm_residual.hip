@@ -56,9 +56,10 @@ __device__ inline float nr_block_sum(float v, float* sm) {
 }
 
 // ---- rows of any width ----------------------------------------------------------------------------
-// Rows that do not fit a workgroup's registers are read again for every sum: one workgroup a row.  Bound by
-// those reads, out of L2, element by element: (2000, 16392) bf16 rms 405 us, its gradient at (693, 13056)
-// with dropout 361 us.
+// Rows that do not fit a workgroup's registers are read again for every sum, element by element.  Bound by waits for
+// those loads, out of L2, and at the barriers of the sums, three quarters of the waves' time: (2000, 16392) bf16 rms
+// 400 us, the gradient at (693, 13056) 336 us, with dropout 361, although that forms eight columns' bits for each one
+// and nearly doubles the vector instructions (busy 38% of the time, without it 22%).
 template <class T, class TS>
 struct NrRow {  // one row of a call, evaluated element by element
   const NrArgs& p;
@@ -446,7 +447,7 @@ __global__ __launch_bounds__(BS) void k_nr_rows(NrArgs p) {
 // (x - m)^2, (r - m)^2, dy w2 (r - m) and dy w2, are formed in one round; those of the post norm's input
 // gradient, which need D, in a second.  Bound by HBM and by the 16 waves a CU that its registers leave:
 // (8192, 4096) bf16 with dropout 109 us with the column sums, 4.9 TB/s; (5003, 1111) f32 layer norms 58 us,
-// 3.1 TB/s, on rows off lines; (4096, 8192) bf16 144 us, 3.7 TB/s.
+// 3.1 TB/s, on rows off lines; (4096, 8192) bf16 with dropout 153 us, 3.5 TB/s.
 template <class T, class TS, int NV, int BS, int GL, bool LAYER, bool FULL, bool NT>
 __global__ __launch_bounds__(BS) void k_nr_grad_rows(NrArgs p) {
   __shared__ float sm[2][4][16];
