@@ -9,7 +9,7 @@ becomes a loss in training or the next token in serving.  The operators here are
                          q = softmax(z / T), s = softmax(z);
                          loss = weight T^2 sum_k p_k (log p_k - log q[i_k]) - (1 - weight) log s[label].
                          The first term is 0 without entries, the second where the label is no column.  It also gives the
-                         logarithms of the two softmaxes' sums, 0 where a row has no use for one.
+                         highest logit m, log sum exp((z - m) / T) and log sum exp(z - m), 0 where a row has no use for one.
 * ``distill_loss_grad``  dz = dloss (weight T (q - p) + (1 - weight) (s - one-hot(label))).
 * ``adjust_logits``      for each sequence, with c the number of times a token is in its history:
                          z = (z > 0 ? z / repetition : z repetition) - (frequency c + presence) where c > 0; z += bias;
@@ -149,7 +149,7 @@ def _tensors(c, seed):
             t["labels"] = torch.where(uniform((rows,)) < _UNLABELLED, -100, index[:, 0]).to(ids)
         if op == "distill_grad":
             t["dloss"] = uniform((rows,), 0.5, 1.5) / rows
-            t["lse"] = _log_sums(c, t)
+            t["sums"] = _log_sums(c, t)
     else:
         rows = c["rows"]
         t["logits"] = normal((rows, v), dt, 0.0, 3.0)
@@ -186,17 +186,19 @@ def _uses(c, t):
 
 
 def _log_sums(c, t):
-    """What the loss keeps for its gradient: (rows, 2), in 64 bits, rounded."""
-    out = torch.zeros(c["rows"], 2, device="cuda")
+    """What the loss keeps for its gradient: (rows, 3), in 64 bits, rounded."""
+    out = torch.zeros(c["rows"], 3, device="cuda")
     first, second = _uses(c, t)
     step = max(1, (1 << 28) // c["vocab"])
     for i in range(0, c["rows"], step):
         z = t["logits"][i:i + step].double()
         top = z.max(1, keepdim=True).values
-        for j, (used, temp) in enumerate(((first, c["temperature"]), (second, 1.0))):
+        for j, (used, temp) in enumerate(((first, c["temperature"]), (second, 1.0)), 1):
             if used is not None:
-                s = torch.log(torch.exp((z - top) / temp).sum(1, keepdim=True)) + top / temp
-                out[i:i + step, j:j + 1] = torch.where(used[i:i + step], s, 0.0).float()
+                u = used[i:i + step]
+                s = torch.log(torch.exp((z - top) / temp).sum(1, keepdim=True))
+                out[i:i + step, j:j + 1] = torch.where(u, s, 0.0).float()
+                out[i:i + step, :1] = torch.where(u, top.float(), out[i:i + step, :1])
     return out
 
 
@@ -213,7 +215,7 @@ def prepare(case, seed):
         elif op == "embed_grad":
             outs = [((c["vocab"], c["width"]), _DT[c["to"]])]
         elif op == "distill":
-            outs = [((c["rows"],), f32), ((c["rows"], 2), f32)]
+            outs = [((c["rows"],), f32), ((c["rows"], 3), f32)]
         elif op == "distill_grad":
             outs = [(t["logits"].shape, _DT[c["dtype"]])]
         else:
@@ -244,7 +246,7 @@ def _run_own(c, state):
         ms.distill_loss(a["logits"], a["index"], a["teacher"], a.get("labels"), temperature=c["temperature"],
                         weight=c["weight"], out=tuple(o))
     elif op == "distill_grad":
-        ms.distill_loss_grad(a["dloss"], a["logits"], a["lse"], a["index"], a["teacher"], a.get("labels"),
+        ms.distill_loss_grad(a["dloss"], a["logits"], a["sums"], a["index"], a["teacher"], a.get("labels"),
                              temperature=c["temperature"], weight=c["weight"], out=o[0])
     else:
         penalties = {k: a[k] for k in ("repetition", "presence", "frequency") if k in a}
@@ -285,25 +287,24 @@ def _run_plain(c, state):
         first, second = _uses(c, t)
         if op == "distill":
             top = z.max(1, keepdim=True).values
-            lse = [torch.log(torch.exp((z - top) / temp).sum(1, keepdim=True)) + top / temp]
-            log_q = z.gather(1, index) / temp - lse[0]
-            terms = torch.where(p > 0.0, p * (log_p - log_q), 0.0)
-            loss = weight * temp * temp * terms.sum(1)
+            soft = torch.log(torch.exp((z - top) / temp).sum(1, keepdim=True))
+            log_q = (z.gather(1, index) - top) / temp - soft
+            loss = weight * temp * temp * torch.where(p > 0.0, p * (log_p - log_q), 0.0).sum(1)
+            hard = torch.zeros_like(soft)
+            used = first
             if second is not None:
-                lse.append(torch.log(torch.exp(z - top).sum(1, keepdim=True)) + top)
+                hard = torch.where(second, torch.log(torch.exp(z - top).sum(1, keepdim=True)), 0.0)
                 at = z.gather(1, torch.where(second, t["labels"].long()[:, None], 0))
-                loss = loss + (1.0 - weight) * torch.where(second, lse[1] - at, 0.0)[:, 0]
-            else:
-                second = torch.zeros_like(first)
-                lse.append(lse[0])
-            return [loss, torch.where(torch.cat([first, second], 1), torch.cat(lse, 1), 0.0)]
-        dl = t["dloss"][:, None]
+                loss = loss + (1.0 - weight) * torch.where(second, top - at + hard, 0.0)[:, 0]
+                used = first | second
+            return [loss, torch.cat([torch.where(used, top, 0.0), torch.where(first, soft, 0.0), hard], 1)]
+        dl, m = t["dloss"][:, None], t["sums"][:, :1]
         scale = dl * (weight * temp)
-        grad = torch.where(first, scale * torch.exp(z / temp - t["lse"][:, :1]), 0.0)
+        grad = torch.where(first, scale * torch.exp((z - m) / temp - t["sums"][:, 1:2]), 0.0)
         grad.scatter_add_(1, index, -scale * p)
         if second is not None:
             scale = dl * (1.0 - weight)
-            grad += torch.where(second, scale * torch.exp(z - t["lse"][:, 1:]), 0.0)
+            grad += torch.where(second, scale * torch.exp(z - m - t["sums"][:, 2:]), 0.0)
             grad.scatter_add_(1, torch.where(second, t["labels"].long()[:, None], 0), torch.where(second, -scale, 0.0))
         return [grad.to(_DT[c["dtype"]])]
     z = t["logits"].float()
@@ -348,8 +349,8 @@ def work(case):
         r, k, both = c["rows"], c["entries"], c["weight"] < 1.0
         b = r * v * es + r * k * (ids + _SIZE[c["teacher"]]) + (r * ids if both else 0)
         if op == "distill":
-            return {"bytes": b + 12 * r, "flops": r * v * (8 if both else 5)}
-        return {"bytes": b + r * v * es + r * (12 if both else 8), "flops": r * v * (10 if both else 5)}
+            return {"bytes": b + 16 * r, "flops": r * v * (8 if both else 5)}
+        return {"bytes": b + r * v * es + r * (16 if both else 12), "flops": r * v * (10 if both else 5)}
     r = c["rows"]
     b = r * v * (es + _SIZE[c["to"]]) + int(0.75 * r * c["history"]) * ids + (r * (12 + ids) if c["history"] else 0)
     b += {"none": 0, "dense": 4 * v, "sparse": r * c["entries"] * (4 + ids)}[c["bias"]]
@@ -379,22 +380,23 @@ def _exact_distill(c, t):
             labelled = (label >= 0) & (label < v)
             label = label.masked_fill(~labelled, 0)
         if not grad:
-            lse = torch.logsumexp(z / temp, 1)
-            got = z[rows[:, None], index] / temp - lse[:, None]
+            m = z.amax(1)
+            lse, one = torch.logsumexp((z - m[:, None]) / temp, 1), torch.logsumexp(z - m[:, None], 1)
+            got = (z[rows[:, None], index] - m[:, None]) / temp - lse[:, None]
             loss = weight * temp ** 2 * (torch.xlogy(p, p) - p * got).sum(1)
-            one = torch.logsumexp(z, 1)
             if "labels" in t:
-                loss = loss + (1.0 - weight) * (one - z[rows, label]).masked_fill(~labelled, 0.0)
-            parts.append((loss, torch.stack([lse.masked_fill(~some, 0.0), one.masked_fill(~labelled, 0.0)], 1)))
+                loss = loss + (1.0 - weight) * (one + m - z[rows, label]).masked_fill(~labelled, 0.0)
+            parts.append((loss, torch.stack([m.masked_fill(~(some | labelled), 0.0), lse.masked_fill(~some, 0.0),
+                                             one.masked_fill(~labelled, 0.0)], 1)))
             continue
-        lse = t["lse"][i:i + step].double()
-        d = torch.exp(z / temp - lse[:, :1])
+        sums = t["sums"][i:i + step].double()
+        d = torch.exp((z - sums[:, :1]) / temp - sums[:, 1:2])
         d[~some] = 0.0
         for k in range(index.shape[1]):
             d[rows, index[:, k]] -= p[:, k]
         d *= weight * temp
         if "labels" in t:
-            s = torch.exp(z - lse[:, 1:])
+            s = torch.exp(z - sums[:, :1] - sums[:, 2:])
             s[rows, label] -= 1.0
             s[~labelled] = 0.0
             d += (1.0 - weight) * s
