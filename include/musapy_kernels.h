@@ -415,7 +415,7 @@ int musapy_reduce_fused_noalloc_v1(int op, int dtype, const void* a, void* c, in
  * per-tile length reaches 2^31 elements (pass more tiles), 3 ndim outside [0, 32] or an axis
  * outside [0, ndim) (32 is the reference's MUSAPY_MAX_NDIM), 4 a cumsum with 2^32 or more rows
  * (or a dimension outside the scanned axis of 2^32 or more), 5 a no-alloc reduction whose slots
- * need more than the library's static scratch, 6 an argument of a gated recurrent block's operator that is
+ * need more than the library's static scratch, 6 an argument of an operator of a gated recurrent block or over a vocabulary that is
  * out of range.  A wrapper that reports an error launches
  * nothing. */
 int musapy_kernels_take_error(void);
@@ -567,6 +567,106 @@ int musapy_norm_residual_grad_v1(const musapy_norm_residual_args* args, void* sc
  * takes half c % 8 of its four words, low half of word 0 first.  The rows, and the rows times the
  * columns' groups of eight, are fewer than 2^32: a single row has up to 2^35 - 8 columns. */
 int musapy_dropout_v1(const void* a, void* out, int dtype, int ndim, const size_t* shape, const ssize_t* strides, uint32_t threshold, uint64_t seed, uint64_t offset, hipStream_t stream);
+
+/* ---- operators over a vocabulary (new; no counterpart in kernels.rs) ----
+ * Element types are MUSAPY_DT_F32, _F16 or _BF16, all arithmetic is f32 and a result is rounded once.  Token numbers, labels,
+ * indices and lengths (`*_dtype` of theirs) are MUSAPY_DT_I32 or _I64.  Rows, columns and tokens are each fewer
+ * than 2^31.  Every entry point returns 0 when its work was launched (or there was none), -1 when an argument is out
+ * of range (wrapper error 6) or scratch is missing (wrapper error 1); nothing is launched then.
+ *
+ * Embedding: out[n] = scale * table[ids[n]]; a number outside [0, rows) is padding: its row is zeros.  `ids` has `tokens`
+ * numbers, `out` (tokens, width) is C-contiguous; the table's strides are in elements (groups of 4 or 8 columns of all
+ * tokens together fewer than 2^32).
+ *
+ * Its gradient: out[v] = scale * sum of dy[n] over the n with ids[n] = v, for every row v of the table, zeros where no
+ * token is v; with `accumulate` 1 the sums are added to `out` instead, and rows without a token stay as they are.  A row's
+ * terms are added in one order that the tokens alone decide: results are the same from call to call.  dy's rows are
+ * unit-stride, dy_pitch elements apart.  `scratch` (musapy_embedding_grad_scratch_v1 bytes, 16-byte aligned) is the call's own,
+ * of any contents. */
+typedef struct {
+  int table_dtype, out_dtype, id_dtype;
+  float scale;
+  size_t tokens, rows, width;
+  const void* table;
+  ssize_t row_stride, column_stride;
+  const void* ids;
+  void* out;
+} musapy_embedding_args;
+int musapy_embedding_v1(const musapy_embedding_args* args, hipStream_t stream);
+typedef struct {
+  int dy_dtype, out_dtype, id_dtype, accumulate;
+  float scale;
+  size_t tokens, rows, width;
+  const void* dy;
+  size_t dy_pitch;
+  const void* ids;
+  void* out;
+} musapy_embedding_grad_args;
+size_t musapy_embedding_grad_scratch_v1(const musapy_embedding_grad_args* args);
+int musapy_embedding_grad_v1(const musapy_embedding_grad_args* args, void* scratch, size_t scratch_bytes, hipStream_t stream);
+
+/* Distillation from a teacher's top entries, with labels beside it.  For each row of logits z, with T the temperature:
+ *   p = softmax(teacher / T) over the row's entries, q = softmax(z / T), s = softmax(z)
+ *   loss = weight T^2 sum_k p_k (log p_k - log q[index_k]) - (1 - weight) log s[label]
+ *   dlogits = dloss (weight T (q - p) + (1 - weight) (s - one-hot(label)))
+ * An entry whose index is no column, or whose value is -inf, does not count; the same index may stand in several
+ * entries.  The first term is 0 in a row without entries that count, the second where the label is no column (and
+ * both where their factor is 0); the logits of a row without either are not read.  sums (rows, 3) receives the highest
+ * logit m, log(sum exp((z - m) / T)) and log(sum exp(z - m)), 0 where a row has no use for one, and the gradient reads it.  A
+ * column of -inf has probability 0; a row of nothing else, and one with +inf or NaN, gives NaN.
+ * At most 1024 entries; T from 2^-20 to 2^20, weight from 0 to 1.  Rows of logits, indices and values are unit-stride, `*_pitch`
+ * elements apart; labels (NULL: none) and the outputs are C-contiguous; dloss is `dloss_stride` elements apart. */
+typedef struct {
+  int dtype, index_dtype, teacher_dtype, label_dtype;
+  float temperature, weight;
+  size_t rows, width, entries;
+  const void* logits;
+  size_t pitch;
+  const void* index;
+  size_t index_pitch;
+  const void* teacher;
+  size_t teacher_pitch;
+  const void* labels;
+  float* loss;        /* forward */
+  float* sums;        /* forward: written; grad: read */
+  const float* dloss; /* grad */
+  ssize_t dloss_stride;
+  void* dlogits; /* grad */
+} musapy_distill_args;
+int musapy_distill_loss_v1(const musapy_distill_args* args, hipStream_t stream);
+int musapy_distill_loss_grad_v1(const musapy_distill_args* args, hipStream_t stream);
+
+/* Logits of the next token, made ready for its choice.  For each row, with c the number of times that a column is among the
+ * first `lengths[row]` (NULL: `length`; cut to 0 .. length) numbers of its history:
+ *   z = (z > 0 ? z / repetition : z * repetition) - (frequency * c + presence) where c > 0
+ *   z = z + bias
+ *   z = -inf where `allowed` is 0
+ * Numbers of the history that are no column do not count.  Each of the penalties is an array of a number for each row, or
+ * (NULL) its `_value`.  The bias is a row of `width` values, bias_pitch apart (0: one row for all), or, with `entries`
+ * (at most 1024), values for the columns bias_index of each row: an index that is no column has no effect, and
+ * biases of one column add up.  `allowed` is bytes, or 32-bit words whose lowest bits come first, in rows
+ * allowed_pitch bytes or words apart (0: one row for all). */
+enum { MUSAPY_ALLOWED_BYTES = 0, MUSAPY_ALLOWED_BITS = 1 };
+typedef struct {
+  int dtype, out_dtype; /* out_dtype: dtype or F32 */
+  int history_dtype, lengths_dtype, bias_dtype, index_dtype, allowed_kind;
+  size_t rows, width, length, entries;
+  const void* logits;
+  size_t pitch;
+  const void* history; /* NULL: no penalties */
+  size_t history_pitch;
+  const void* lengths;
+  const float *repetition, *presence, *frequency;
+  float repetition_value, presence_value, frequency_value;
+  const void* bias; /* NULL: none */
+  size_t bias_pitch;
+  const void* bias_index;
+  size_t index_pitch;
+  const void* allowed; /* NULL: all */
+  size_t allowed_pitch;
+  void* out;
+} musapy_adjust_logits_args;
+int musapy_adjust_logits_v1(const musapy_adjust_logits_args* args, hipStream_t stream);
 
 /* ---- planning helper (new; no counterpart in kernels.rs) ----
  * Tiles per output that the partial entry points should be given for this reduction on this

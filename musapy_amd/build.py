@@ -43,9 +43,12 @@ HIP_SOURCES = [
     "kernels/gated_scan_grad.hip",
     "kernels/norm_residual.hip",
     "kernels/dropout.hip",
+    "kernels/embedding.hip",
+    "kernels/distill.hip",
+    "kernels/adjust_logits.hip",
     "runtime/hip_runtime.cpp",
 ]
-CXX_SOURCES = ["ops/core.cpp", "ops/ops.cpp", "ops/blocks.cpp", "ops/interop.cpp", "python/module.cpp"]
+CXX_SOURCES = ["ops/core.cpp", "ops/ops.cpp", "ops/blocks.cpp", "ops/vocabulary.cpp", "ops/interop.cpp", "python/module.cpp"]
 
 
 def _run(cmd: list[str]) -> None:

@@ -1,0 +1,352 @@
+// distill.hip -- a student's loss against a teacher's top entries and labels, and its gradient, for gfx950.
+#include "vocab.hpp"
+
+namespace mpy {
+
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
+constexpr int kEntriesMost = 1024;
+
+struct DistillArgs {
+  const void* logits;
+  uint64_t pitch;
+  Ids index;
+  uint64_t index_pitch;
+  const void* teacher;
+  int teacher_dtype;
+  uint64_t teacher_pitch;
+  Ids labels;              // at: NULL for none
+  uint32_t rows, width, entries;
+  float inv_t;             // 1 / T
+  float c;                 // log2(e) / T
+  float soft;              // weight T^2; of the gradient, weight T
+  float hard;              // 1 - weight
+  int use_soft;            // weight is not 0
+  float* loss;
+  float* sums;             // (rows, 3): m, log sum exp((z - m) / T), log sum exp(z - m); of the gradient, read
+  const float* dloss;
+  int64_t dloss_stride;
+  void* grad;
+  uint32_t segment, segments;  // of the gradient: columns of a workgroup, workgroups of a row
+};
+
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Sum (or, of each wave's, the maximum) over a workgroup's waves; every thread has the result.
+template <int WAVES, class F>
+__device__ inline float block_fold(float v, float* part, F&& f) {
+  const int wave = threadIdx.x / 64;
+  if (threadIdx.x % 64 == 0) part[wave] = v;
+  __syncthreads();
+  float r = part[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) r = f(r, part[w]);
+  __syncthreads();
+  return r;
+}
+
+// The teacher's entries of a row, lane by lane: their maximum (-inf where none counts), and whether any
+// counts.  An entry counts where its index is a column and its value is not -inf.
+__device__ inline float teacher_max(const DistillArgs& p, uint32_t row, int lane, bool& any) {
+  float top = -__builtin_inff();
+  bool some = false;
+  for (uint32_t k = lane; k < p.entries; k += 64) {
+    const bool in = id_at(p.index, row * p.index_pitch + k, p.width) < p.width;
+    const float v = float_at(p.teacher, p.teacher_dtype, row * p.teacher_pitch + k);
+    if (in && v != -__builtin_inff()) {
+      some = true;
+      top = fmaxf(top, v);
+    }
+  }
+  any = __ballot(some) != 0;
+  return wave_max(top);
+}
+
+// A workgroup takes a row: every thread keeps the maximum m of its logits and the sums of exp((z - m) / T) and,
+// with labels at a T other than 1, exp(z - m), rescaled when m rises; they are joined at the end.  The first
+// wave forms the teacher's part, which needs K logits and the sum only:
+//   sum_k p_k (log p_k - log q_k) = B / A - log A + (m - r) / T + log sum exp((z - m) / T),
+//   e_k = exp((v_k - max v) / T),  A = sum e_k,  B = sum e_k ((v_k - max v) - (z_k - r)) / T
+// with r the highest of the entries' logits: all differences are of near numbers, so that logits far from 0 lose nothing.
+template <class T, int BLOCK, bool TWO>
+__global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
+  constexpr int N = 16 / int(sizeof(T)), U = 4, kWaves = BLOCK / 64;
+  __shared__ float part[kWaves];
+  const uint32_t row = blockIdx.x;
+  const int lane = threadIdx.x % 64;
+  const uint32_t wave = wave_uniform(threadIdx.x / 64);
+  const T* z = static_cast<const T*>(p.logits) + uint64_t(row) * p.pitch;
+  bool soft = false;
+  const float top = p.use_soft ? teacher_max(p, row, lane, soft) : 0.0f;
+  const uint32_t label = p.labels.at ? id_at(p.labels, row, p.width) : p.width;
+  const bool hard = label < p.width;
+  if (!soft && !hard) {
+    if (threadIdx.x == 0) {
+      p.loss[row] = 0.0f;
+      for (int i = 0; i < 3; ++i) p.sums[uint64_t(row) * 3 + i] = 0.0f;
+    }
+    return;
+  }
+  float a = 0.0f, b = 0.0f, r = -__builtin_inff();
+  if (soft && wave == 0) {
+    auto each = [&](auto fn) {
+      for (uint32_t k = lane; k < p.entries; k += 64) {
+        const uint32_t i = id_at(p.index, row * p.index_pitch + k, p.width);
+        const float v = float_at(p.teacher, p.teacher_dtype, row * p.teacher_pitch + k);
+        if (i < p.width && v != -__builtin_inff()) fn(v - top, float(z[i]));
+      }
+    };
+    each([&](float, float x) { r = fmaxf(r, x); });
+    r = wave_max(r);
+    if (r == -__builtin_inff()) r = 0.0f;
+    each([&](float d, float x) {
+      const float e = exp2_fast(d * p.c);
+      a += e;
+      if (!(e == 0.0f)) b += e * ((d - (x - r)) * p.inv_t);
+    });
+  }
+
+  float m = -__FLT_MAX__, s = 0.0f, s1 = 0.0f;
+  auto add = [&](const float (&x)[N * U]) {
+    float high = m;
+#pragma unroll
+    for (int e = 0; e < N * U; ++e) high = fmaxf(high, x[e]);
+    s *= exp2_fast((m - high) * p.c);
+    if (TWO) s1 *= exp2_fast((m - high) * kLog2e);
+    m = high;
+#pragma unroll
+    for (int e = 0; e < N * U; ++e) {
+      const float d = x[e] - m;
+      s += exp2_fast(d * p.c);
+      if (TWO) s1 += exp2_fast(d * kLog2e);
+    }
+  };
+  const uint32_t vectors = p.width / N;
+  for (uint32_t base = 0; base < vectors; base += BLOCK * U) {
+    Vec<T, N> v[U];
+    float x[N * U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t at = base + u * BLOCK + threadIdx.x;
+      v[u] = vload_el<T, N, true>(z + uint64_t(at < vectors ? at : vectors - 1) * N);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        x[u * N + e] = base + u * BLOCK + threadIdx.x < vectors ? float(v[u].v[e]) : -__builtin_inff();
+    add(x);
+  }
+  if (threadIdx.x < p.width - vectors * N) {
+    float x[N * U];
+#pragma unroll
+    for (int e = 0; e < N * U; ++e) x[e] = -__builtin_inff();
+    x[0] = float(z[vectors * N + threadIdx.x]);
+    add(x);
+  }
+  const float most = block_fold<kWaves>(wave_max(m), part, [](float u, float w) { return fmaxf(u, w); });
+  auto plus = [](float u, float w) { return u + w; };
+  s = block_fold<kWaves>(wave_sum(s * exp2_fast((m - most) * p.c)), part, plus);
+  if (TWO) s1 = block_fold<kWaves>(wave_sum(s1 * exp2_fast((m - most) * kLog2e)), part, plus);
+  if (wave != 0) return;
+  a = wave_sum(a);
+  b = wave_sum(b);
+  if (lane != 0) return;
+  const float ls = kLn2 * __builtin_amdgcn_logf(s);
+  const float ls1 = TWO ? kLn2 * __builtin_amdgcn_logf(s1) : ls;
+  float loss = 0.0f;
+  if (soft) loss = p.soft * (b / a - kLn2 * __builtin_amdgcn_logf(a) + (most - r) * p.inv_t + ls);
+  if (hard) loss += p.hard * ((most - float(z[label])) + ls1);
+  p.loss[row] = loss;
+  float* sums = p.sums + uint64_t(row) * 3;
+  sums[0] = most;
+  sums[1] = soft ? ls : 0.0f;
+  sums[2] = hard ? ls1 : 0.0f;
+}
+
+// A workgroup takes a segment of a row: dloss (weight T softmax(z / T) + (1 - weight) softmax(z)) of every
+// column, from the maximum and the logarithms of the sums that the loss left.  Then the columns of the teacher's entries and the label, at
+// most K + 1, are formed again with what is taken off there, and stored over the first values behind a
+// barrier; a column that several entries name is formed by the first of them.
+template <class T, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void k_distill_grad(DistillArgs p) {
+  constexpr int N = 16 / int(sizeof(T)), U = 4, kWaves = BLOCK / 64;
+  __shared__ float part[kWaves];
+  __shared__ uint32_t index[kEntriesMost];
+  __shared__ float prob[kEntriesMost];
+  const uint32_t row = blockIdx.x / p.segments, seg = blockIdx.x - row * p.segments;
+  const uint32_t first = seg * p.segment;
+  const uint32_t last = p.width - first < p.segment ? p.width : first + p.segment;
+  const T* z = static_cast<const T*>(p.logits) + uint64_t(row) * p.pitch;
+  T* out = static_cast<T*>(p.grad) + uint64_t(row) * p.width;
+  const float dl = p.dloss[int64_t(row) * p.dloss_stride];
+
+  // the entries, and their probabilities
+  bool some = false;
+  float top = -__builtin_inff();
+  for (uint32_t k = threadIdx.x; k < p.entries; k += BLOCK) {
+    uint32_t i = p.use_soft ? id_at(p.index, row * p.index_pitch + k, p.width) : p.width;
+    const float v = float_at(p.teacher, p.teacher_dtype, row * p.teacher_pitch + k);
+    if (v == -__builtin_inff()) i = p.width;
+    index[k] = i;
+    prob[k] = v;
+    if (i < p.width) {
+      some = true;
+      top = fmaxf(top, v);
+    }
+  }
+  const bool soft = __syncthreads_or(some);
+  if (soft) {
+    top = block_fold<kWaves>(wave_max(top), part, [](float u, float w) { return fmaxf(u, w); });
+    float a = 0.0f;
+    for (uint32_t k = threadIdx.x; k < p.entries; k += BLOCK) {
+      const float e = index[k] < p.width ? exp2_fast((prob[k] - top) * p.c) : 0.0f;
+      prob[k] = e;
+      a += e;
+    }
+    a = block_fold<kWaves>(wave_sum(a), part, [](float u, float w) { return u + w; });
+    for (uint32_t k = threadIdx.x; k < p.entries; k += BLOCK) prob[k] /= a;
+  }
+  const uint32_t label = p.labels.at ? id_at(p.labels, row, p.width) : p.width;
+  const bool hard = label < p.width;
+  const float ka = dl * p.soft, kb = dl * p.hard;
+  const float m = p.sums[uint64_t(row) * 3];
+  const float la = p.sums[uint64_t(row) * 3 + 1] * kLog2e, lb = p.sums[uint64_t(row) * 3 + 2] * kLog2e;
+
+  auto stream = [&](auto fn) {
+    const uint32_t vectors = (last - first) / N;
+    for (uint32_t base = 0; base < vectors; base += BLOCK * U) {
+      Vec<T, N> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t at = base + u * BLOCK + threadIdx.x;
+        v[u] = vload_el<T, N, true>(z + first + uint64_t(at < vectors ? at : vectors - 1) * N);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t at = base + u * BLOCK + threadIdx.x;
+        if (at >= vectors) continue;
+        Vec<T, N> o;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o.v[e] = T(fn(float(v[u].v[e])));
+        vstore_el<true, T, N>(out + first + uint64_t(at) * N, o);
+      }
+    }
+    const uint32_t rest = first + vectors * N + threadIdx.x;
+    if (rest < last) out[rest] = T(fn(float(z[rest])));
+  };
+  auto q = [&](float x) { return exp2_fast(__builtin_fmaf(x - m, p.c, -la)); };
+  auto s = [&](float x) { return exp2_fast(__builtin_fmaf(x - m, kLog2e, -lb)); };
+  if (soft && hard) stream([&](float x) { return ka * q(x) + kb * s(x); });
+  else if (soft) stream([&](float x) { return ka * q(x); });
+  else if (hard) stream([&](float x) { return kb * s(x); });
+  else {
+    const T zero = T(0.0f);
+    Vec<T, N> o;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o.v[e] = zero;
+    const uint32_t vectors = (last - first) / N;
+    for (uint32_t at = threadIdx.x; at < vectors; at += BLOCK) vstore_el<true, T, N>(out + first + uint64_t(at) * N, o);
+    const uint32_t rest = first + vectors * N + threadIdx.x;
+    if (rest < last) out[rest] = zero;
+    return;
+  }
+  __syncthreads();
+  auto column = [&](uint32_t i, float taken) {
+    const float x = float(z[i]);
+    float g = 0.0f;
+    if (soft) g = ka * (q(x) - taken);
+    if (hard) g += kb * (s(x) - (i == label ? 1.0f : 0.0f));
+    out[i] = T(g);
+  };
+  bool labelled = false;  // whether an entry's column is the label's
+  for (uint32_t k = threadIdx.x; soft && k < p.entries; k += BLOCK) {
+    const uint32_t i = index[k];
+    if (i == label && hard) labelled = true;
+    if (i < first || i >= last) continue;
+    float taken = 0.0f;
+    bool leads = true;
+    for (uint32_t j = 0; j < p.entries; ++j) {
+      if (index[j] != i) continue;
+      if (j < k) leads = false;
+      taken += prob[j];
+    }
+    if (leads) column(i, taken);
+  }
+  labelled = __syncthreads_or(labelled);
+  if (hard && !labelled && threadIdx.x == 0 && label >= first && label < last) column(label, 0.0f);
+}
+
+static bool distill_args(const musapy_distill_args* a, bool grad, DistillArgs& p) {
+  if (a == nullptr || !vocab_float(a->dtype) || a->rows >= kVocabLimit || a->width >= kVocabLimit) return false;
+  if (a->entries > size_t(kEntriesMost) || !(a->temperature >= 0x1p-20f && a->temperature <= 0x1p20f)) return false;
+  if (!(a->weight >= 0.0f && a->weight <= 1.0f)) return false;
+  if (a->entries > 0 && (!vocab_id(a->index_dtype) || !vocab_float(a->teacher_dtype))) return false;
+  if (a->labels != nullptr && !vocab_id(a->label_dtype)) return false;
+  p.logits = a->logits;
+  p.pitch = a->pitch;
+  p.index = vocab_ids(a->index, a->index_dtype);
+  p.index_pitch = a->index_pitch;
+  p.teacher = a->teacher;
+  p.teacher_dtype = a->teacher_dtype;
+  p.teacher_pitch = a->teacher_pitch;
+  p.use_soft = a->weight > 0.0f && a->entries > 0;
+  p.labels = vocab_ids(a->weight < 1.0f ? a->labels : nullptr, a->label_dtype);
+  p.rows = uint32_t(a->rows);
+  p.width = uint32_t(a->width);
+  p.entries = uint32_t(a->entries);
+  p.inv_t = 1.0f / a->temperature;
+  p.c = kLog2e / a->temperature;
+  p.soft = a->weight * a->temperature * (grad ? 1.0f : a->temperature);
+  p.hard = 1.0f - a->weight;
+  p.loss = a->loss;
+  p.sums = a->sums;
+  p.dloss = a->dloss;
+  p.dloss_stride = a->dloss_stride;
+  p.grad = a->dlogits;
+  return true;
+}
+
+}  // namespace mpy
+
+using namespace mpy;
+
+extern "C" {
+
+int musapy_distill_loss_v1(const musapy_distill_args* a, hipStream_t st) {
+  DistillArgs p{};
+  if (!distill_args(a, false, p)) return vocab_bad();
+  if (p.rows == 0) return 0;
+  if (p.loss == nullptr || p.sums == nullptr || (p.width > 0 && p.logits == nullptr) ||
+      (p.entries > 0 && (p.index.at == nullptr || p.teacher == nullptr)) || !grid_fits(p.rows, 512))
+    return vocab_bad();
+  const bool two = p.labels.at != nullptr && a->temperature != 1.0f;
+  vocab_type(a->dtype, [&](auto t) {
+    using T = decltype(t);
+    if (two) k_distill_loss<T, 512, true><<<p.rows, 512, 0, st>>>(p);
+    else k_distill_loss<T, 512, false><<<p.rows, 512, 0, st>>>(p);
+  });
+  return 0;
+}
+
+int musapy_distill_loss_grad_v1(const musapy_distill_args* a, hipStream_t st) {
+  DistillArgs p{};
+  if (!distill_args(a, true, p)) return vocab_bad();
+  if (p.rows == 0 || p.width == 0) return 0;
+  if (p.logits == nullptr || p.sums == nullptr || p.dloss == nullptr || p.grad == nullptr ||
+      (p.entries > 0 && (p.index.at == nullptr || p.teacher == nullptr)))
+    return vocab_bad();
+  // whole rows where they fill the chip, and segments of a multiple of 4096 columns
+  p.segments = 1;
+  p.segment = p.width;
+  while (uint64_t(p.rows) * p.segments < 2048 && p.segment > 8192) {
+    p.segment = ((p.segment + 1) / 2 + 4095) / 4096 * 4096;
+    p.segments = (p.width + p.segment - 1) / p.segment;
+  }
+  if (!grid_fits(uint64_t(p.rows) * p.segments, 256)) return vocab_bad();
+  vocab_type(a->dtype, [&](auto t) {
+    k_distill_grad<decltype(t), 256><<<p.rows * p.segments, 256, 0, st>>>(p);
+  });
+  return 0;
+}
+
+}  // extern "C"

@@ -249,7 +249,8 @@ __device__ inline T shfl_xor(T v, int m) {
 // 1 = cumsum scratch missing or too small, 2 = a reduction tile longer than 2^31 elements,
 // 3 = ndim outside [0, 32] or axis outside [0, ndim), 4 = a scan with 2^32 or more rows (or a
 // non-axis extent of 2^32 or more), 5 = a no-alloc reduction that needs more than the static
-// scratch holds, 6 = an argument of a gated recurrent block's operator that is out of range.
+// scratch holds, 6 = an argument of an operator of a gated recurrent block or
+// over a vocabulary that is out of range.
 inline thread_local int g_wrapper_error = 0;
 
 // ---------------------------------------------------------------------------------------------

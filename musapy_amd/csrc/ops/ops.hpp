@@ -78,6 +78,29 @@ NormResidualGrad norm_residual_grad(const Array* dr, const Array* dy, const Arra
                                     const NormOptions& o, const NormResidualGrad& outs);
 Array dropout(const Array& x, double p, uint64_t seed, uint64_t offset, const Array* out);
 
+// Operators over a vocabulary (vocabulary.cpp); the formulas stand in musapy_kernels.h.  Results are of `dtype`, else
+// of the dtype of `out`, else of the first argument's.
+Array embedding(const Array& table, const Array& tokens, double scale, std::optional<Dtype> dtype, const Array* out);
+// with `accumulate`, added to `out`
+Array embedding_grad(const Array& dout, const Array& tokens, size_t rows, double scale, std::optional<Dtype> dtype,
+                     bool accumulate, const Array* out);
+// (loss, sums): one number for each row of logits, and the three that the gradient takes
+std::pair<Array, Array> distill_loss(const Array& logits, const Array& indices, const Array& teacher, const Array* labels,
+                                     double temperature, double weight, const Array* out, const Array* sums_out);
+Array distill_loss_grad(const Array& dloss, const Array& logits, const Array& sums, const Array& indices, const Array& teacher,
+                        const Array* labels, double temperature, double weight, const Array* out);
+struct LogitPenalty {
+  const Array* each = nullptr;  // one for each row of logits
+  double value = 0.0;           // or one for all
+};
+struct LogitOptions {
+  const Array *history = nullptr, *lengths = nullptr;
+  LogitPenalty repetition{nullptr, 1.0}, presence, frequency;
+  const Array *bias = nullptr, *bias_index = nullptr;
+  const Array* allowed = nullptr;
+};
+Array adjust_logits(const Array& logits, const LogitOptions& o, std::optional<Dtype> dtype, const Array* out);
+
 // indexing.rs views + materialisation
 Array transpose(const Array& a, const std::vector<size_t>* axes);
 Array flip(const Array& a, size_t axis);

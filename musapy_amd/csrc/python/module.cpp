@@ -213,6 +213,15 @@ NormOptions norm_options(const py::object& post, const py::object& pre, const st
 const Array* scale_array(const py::object& scale) { return py::isinstance<Array>(scale) ? opt_array(scale) : nullptr; }
 std::optional<Array> opt_copy(const Array* a) { return a ? std::optional<Array>(*a) : std::nullopt; }
 
+std::optional<Dtype> opt_dtype(const py::object& o) {
+  return o.is_none() ? std::nullopt : std::optional<Dtype>(dtype_arg(o));
+}
+// a number for all rows, or an array of one for each
+LogitPenalty logit_penalty(const py::object& o) {
+  if (py::isinstance<Array>(o)) return {opt_array(o), 0.0};
+  return {nullptr, o.cast<double>()};
+}
+
 // Runs a block operator and, in debug mode, records its OpContext on the stream of `first(result)`.
 template <class F, class G>
 auto traced_block(const char* name, std::initializer_list<const Array*> inputs, F&& f, G&& first) {
@@ -651,6 +660,90 @@ PYBIND11_MODULE(_core, m) {
       "x / (1 - p) where kept, 0 where dropped.  Which elements are kept follows from seed, offset and an\n"
       "element's place in the array alone (Philox4x32-10), so the gradient is dropout(dy, p, seed, offset) and no mask is\n"
       "stored.  p is rounded to a multiple of 2^-16.");
+
+  // operators over a vocabulary
+  m.def(
+      "embedding",
+      [](const Array& table, const Array& tokens, double scale, const py::object& dtype, const Array* out) {
+        const auto d = opt_dtype(dtype);
+        return traced("embedding", {&table, &tokens}, [&] { return embedding(table, tokens, scale, d, out); });
+      },
+      py::arg("table"), py::arg("tokens"), py::arg("scale") = 1.0, py::kw_only(), py::arg("dtype") = py::none(),
+      py::arg("out") = nullptr,
+      "scale * table[tokens]: rows of a (rows, width) table (f32, f16 or bf16, any strides) by token number (i32 or i64).\n"
+      "A number outside [0, rows) is padding and gives a row of zeros.  dtype: the result's, the table's when None.");
+  m.def(
+      "embedding_grad",
+      [](const Array& dout, const Array& tokens, size_t rows, double scale, const py::object& dtype, bool accumulate,
+         const Array* out) {
+        const auto d = opt_dtype(dtype);
+        return traced("embedding_grad", {&dout, &tokens},
+                      [&] { return embedding_grad(dout, tokens, rows, scale, d, accumulate, out); });
+      },
+      py::arg("dout"), py::arg("tokens"), py::arg("rows"), py::arg("scale") = 1.0, py::kw_only(), py::arg("dtype") = py::none(),
+      py::arg("accumulate") = false, py::arg("out") = nullptr,
+      "Gradient of embedding's table, (rows, width): to each token's row, scale times the sum of its rows of dout, in f32 and\n"
+      "in an order that the tokens alone decide; zeros to the others.  accumulate: add to out= instead, rows of\n"
+      "tokens that do not occur stay as they are.  dtype: the result's, out's or dout's when None.");
+  m.def(
+      "distill_loss",
+      [](const Array& logits, const Array& indices, const Array& teacher, const py::object& labels, double temperature,
+         double weight, const py::object& out) {
+        auto o = out_arrays(out, 2);
+        auto r = traced_block(
+            "distill_loss", {&logits, &indices, &teacher},
+            [&] { return distill_loss(logits, indices, teacher, opt_array(labels), temperature, weight, o[0], o[1]); },
+            [](const std::pair<Array, Array>& v) -> const Array& { return v.first; });
+        return py::make_tuple(r.first, r.second);
+      },
+      py::arg("logits"), py::arg("indices"), py::arg("teacher"), py::arg("labels") = py::none(), py::kw_only(),
+      py::arg("temperature") = 1.0, py::arg("weight") = 1.0, py::arg("out") = py::none(),
+      "A student's loss against a teacher's top entries, and labels: for each row of logits (..., columns), with\n"
+      "p = softmax(teacher / T) over the row's entries (at most 1024) and q = softmax(logits / T),\n"
+      "  weight T^2 sum_k p_k (log p_k - log q[indices_k]) - (1 - weight) log softmax(logits)[label].\n"
+      "indices (i32 or i64) and teacher (f32, f16 or bf16): (..., entries); an index that is no column and a value of\n"
+      "-inf do not count.  labels (...): a label that is no column does not count.  Returns (loss (...), sums (..., 3)), f32;\n"
+      "sums holds each row's highest logit m, log sum exp((z - m) / T) and log sum exp(z - m) for distill_loss_grad.\n"
+      "out: a tuple of two arrays or Nones.");
+  m.def(
+      "distill_loss_grad",
+      [](const Array& dloss, const Array& logits, const Array& sums, const Array& indices, const Array& teacher,
+         const py::object& labels, double temperature, double weight, const Array* out) {
+        return traced("distill_loss_grad", {&dloss, &logits, &sums, &indices, &teacher}, [&] {
+          return distill_loss_grad(dloss, logits, sums, indices, teacher, opt_array(labels), temperature, weight, out);
+        });
+      },
+      py::arg("dloss"), py::arg("logits"), py::arg("sums"), py::arg("indices"), py::arg("teacher"), py::arg("labels") = py::none(),
+      py::kw_only(), py::arg("temperature") = 1.0, py::arg("weight") = 1.0, py::arg("out") = nullptr,
+      "Gradient of distill_loss for its logits, in their shape and dtype, from dloss (f32: one for each row, or a 0-d array),\n"
+      "the forward's sums and the same other arguments.");
+  m.def(
+      "adjust_logits",
+      [](const Array& logits, const py::object& history, const py::object& lengths, const py::object& repetition,
+         const py::object& presence, const py::object& frequency, const py::object& bias, const py::object& bias_index,
+         const py::object& allowed, const py::object& dtype, const Array* out) {
+        const auto d = opt_dtype(dtype);
+        LogitOptions o;
+        o.history = opt_array(history);
+        o.lengths = opt_array(lengths);
+        o.repetition = logit_penalty(repetition);
+        o.presence = logit_penalty(presence);
+        o.frequency = logit_penalty(frequency);
+        o.bias = opt_array(bias);
+        o.bias_index = opt_array(bias_index);
+        o.allowed = opt_array(allowed);
+        return traced("adjust_logits", {&logits}, [&] { return adjust_logits(logits, o, d, out); });
+      },
+      py::arg("logits"), py::arg("history") = py::none(), py::arg("lengths") = py::none(), py::kw_only(),
+      py::arg("repetition") = 1.0, py::arg("presence") = 0.0, py::arg("frequency") = 0.0, py::arg("bias") = py::none(),
+      py::arg("bias_index") = py::none(), py::arg("allowed") = py::none(), py::arg("dtype") = py::none(),
+      py::arg("out") = nullptr,
+      "Logits (..., columns) made ready for the choice of the next token.  With c the number of times that a column is among\n"
+      "the first `lengths` (...) numbers of its row of history (..., n), where c > 0:\n"
+      "  z = (z / repetition if z > 0 else z * repetition) - (frequency * c + presence);\n"
+      "then z + bias; then -inf where not allowed.  Penalties: numbers, or f32 arrays (...).  bias: (columns,) or (..., columns),\n"
+      "or with bias_index (..., m), m at most 1024, one value for each named column.  allowed: bool, or 32-bit words with\n"
+      "the lowest bit first, in one row or (...) rows.  Numbers that are no column have no effect.  dtype: logits' or f32.");
 
   // views
   m.def(

@@ -455,7 +455,7 @@ const char* mpy_rt_error_string(int code) {
   if (code == -3) return "kernel wrapper error: ndim outside [0, 32] or axis outside [0, ndim)";
   if (code == -4) return "kernel wrapper error: a cumsum with 2^32 or more rows (or a non-axis extent of 2^32 or more)";
   if (code == -5) return "kernel wrapper error: the reduction needs more scratch than the no-alloc entry point holds";
-  if (code == -6) return "kernel wrapper error: an argument of a gated recurrent block operator is out of range";
+  if (code == -6) return "kernel wrapper error: an argument of an operator of a gated recurrent block or over a vocabulary is out of range";
   if (code < 0) return "kernel wrapper error";
   return hipGetErrorString(hipError_t(code));
 }

@@ -1,0 +1,202 @@
+"""Adjusted logits against a 64-bit form, row by row."""
+import numpy as np
+import pytest
+
+import musapy_amd as ms
+from tests import vocab_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+def check(z, dt, to=None, history=None, lengths=None, id_dt="i64", repetition=1.0, presence=0.0, frequency=0.0, bias=None,
+          bias_index=None, allowed=None, packed=False, logits=None, bias_dt="f32"):
+    rows, width = z.shape
+    to = to or dt
+    kw, each = {}, lambda v, r: v if np.ndim(v) == 0 else float(v[r])
+    for k, v in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+        kw[k] = v if np.ndim(v) == 0 else ms.from_numpy(v)
+    if bias is not None:
+        kw["bias"] = R.to_device(bias, bias_dt)
+    if bias_index is not None:
+        kw["bias_index"] = R.ids(bias_index, id_dt)
+    if allowed is not None:
+        kw["allowed"] = ms.from_numpy(R.pack(allowed)) if packed else ms.array(allowed, dtype="bool")
+    got = ms.adjust_logits(R.to_device(z, dt) if logits is None else logits, None if history is None else R.ids(history, id_dt),
+                           None if lengths is None else R.ids(lengths, id_dt), dtype=to, **kw)
+    assert got.shape == z.shape and got.dtype == to
+    want, bound = np.empty(z.shape), np.empty(z.shape)
+    for r in range(rows):
+        past = None
+        if history is not None:
+            n = history.shape[1] if lengths is None else min(max(int(lengths[r]), 0), history.shape[1])
+            past = history[r, :n]
+        own = lambda a: None if a is None else a if a.ndim == 1 else a[r]
+        want[r], bound[r] = R.adjust(z[r], past, each(repetition, r), each(presence, r), each(frequency, r), own(bias),
+                                     None if bias_index is None else bias_index[r], own(allowed))
+    R.within(got, want, bound, to)
+    return got
+
+
+def some(rng, rows, width, length):
+    h = (width ** rng.random((rows, length))).astype(np.int64) - 1
+    h[rng.random(h.shape) < 0.05] = -1
+    f = lambda lo, hi: rng.uniform(lo, hi, rows).astype(np.float32)
+    return dict(history=h, lengths=rng.integers(0, length + 1, rows), repetition=f(0.8, 1.5), presence=f(-0.5, 1.5),
+                frequency=f(-0.2, 0.5))
+
+
+@pytest.mark.parametrize("dt,to", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f16", "f32")])
+@pytest.mark.parametrize("width", [1, 7, 8, 9, 31, 32, 33, 2047, 2048, 2049, 8200, 50001])
+def test_everything_at_once(dt, to, width):
+    rng = np.random.default_rng(width)
+    z = R.draw(rng, (5, width), dt, 3.0)
+    m = min(width, 9)
+    index = np.stack([rng.permutation(width)[:m] for _ in range(5)])
+    for packed in (False, True):
+        check(z, dt, to, bias=R.draw(rng, (5, m), "f32"), bias_index=index, allowed=rng.random((5, width)) < 0.6, packed=packed,
+              id_dt="i32" if packed else "i64", **some(rng, 5, width, 70))
+    check(z, dt, to, bias=R.draw(rng, (width,), dt), bias_dt=dt, allowed=rng.random(width) < 0.6, packed=True,
+          **some(rng, 5, width, 33))
+
+
+@pytest.mark.parametrize("length", [0, 1, 511, 512, 513, 5000, 70000])
+def test_lengths_of_history(length):
+    rng = np.random.default_rng(length)
+    z = R.draw(rng, (3, 3000), "f32", 3.0)
+    check(z, "f32", **some(rng, 3, 3000, length), id_dt="i32")
+    kw = some(rng, 3, 3000, length)
+    del kw["lengths"]
+    check(z, "f32", **kw)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 200, 1100])
+def test_numbers_of_rows(rows):
+    rng = np.random.default_rng(rows)
+    z = R.draw(rng, (rows, 4500), "bf16", 3.0)
+    check(z, "bf16", "f32", allowed=rng.random((rows, 4500)) < 0.5, packed=True, **some(rng, rows, 4500, 20))
+
+
+def test_each_alone():
+    rng = np.random.default_rng(1)
+    z = R.draw(rng, (4, 999), "f32", 3.0)
+    h = rng.integers(0, 999, (4, 300))
+    check(z, "f32")
+    check(R.rounded(z, "bf16"), "bf16", "f32")
+    check(z, "f32", history=h)
+    check(z, "f32", history=h, repetition=1.3)
+    check(z, "f32", history=h, presence=0.7)
+    check(z, "f32", history=h, frequency=-0.3)
+    check(z, "f32", repetition=1.3, presence=1.0)  # no history: nothing occurred
+    check(z, "f32", bias=R.draw(rng, (999,), "f32"))
+    check(z, "f32", bias=R.draw(rng, (4, 999), "f32"))
+    check(z, "f32", allowed=rng.random((4, 999)) < 0.5)
+    check(z, "f32", allowed=rng.random(999) < 0.5)
+
+
+def test_one_token_many_times():
+    """Counts past 16 bits, and numbers that are no column, near and far."""
+    rng = np.random.default_rng(2)
+    z = R.draw(rng, (2, 100), "f32")
+    h = np.full((2, 70001), 42)
+    h[1, :1000] = np.array([-1, 100, 1 << 32, (1 << 32) + 42, -(1 << 63), (1 << 63) - 1, 99, 0, -43, 101] * 100)
+    check(z, "f32", history=h, repetition=2.0, presence=0.25, frequency=2.0 ** -10)
+
+
+def test_lengths_outside():
+    rng = np.random.default_rng(3)
+    z, h = R.draw(rng, (6, 64), "f32"), rng.integers(0, 64, (6, 10))
+    check(z, "f32", history=h, lengths=np.array([-5, 0, 1, 10, 11, 1 << 40]), presence=1.0)
+    check(z, "f32", history=h, lengths=np.array([-(1 << 31), 0, 9, 10, 11, (1 << 31) - 1]), presence=1.0, id_dt="i32")
+
+
+def test_infinities_and_nan():
+    """-inf stays; a NaN that is not allowed is -inf; a row may have nothing left; lowest values stay finite."""
+    z = np.array([[-np.inf, np.inf, np.nan, 1.0, np.nan, 0.0, -0.0, -2.0] * 5] * 3)
+    z[2] = -np.finfo(np.float32).max
+    h = np.tile(np.arange(0, 40, 2), (3, 1))
+    allowed = np.ones((3, 40), dtype=bool)
+    allowed[0, 4::8], allowed[1] = False, False
+    for packed in (False, True):
+        got = check(z, "f32", history=h, repetition=0.5, presence=1.0, frequency=0.5, allowed=allowed, packed=packed).numpy()
+        assert (got[1] == -np.inf).all() and np.isneginf(got[0, 0]) and np.isfinite(got[2]).all()
+    check(z, "f32", bias=np.array([np.inf, -np.inf] * 20), allowed=allowed)
+
+
+def test_biases_of_one_column():
+    """The same column several times, columns outside, none at all."""
+    rng = np.random.default_rng(4)
+    z = R.draw(rng, (3, 5000), "f32")
+    index = rng.integers(-2, 12, (3, 40))
+    index[1] = 4999
+    index[2] = -1
+    check(z, "f32", bias=R.draw(rng, (3, 40), "f32"), bias_index=index, **some(rng, 3, 5000, 40))
+    check(z, "f32", bias=np.zeros((3, 0)), bias_index=np.zeros((3, 0), np.int64))
+    many = np.stack([rng.permutation(5000)[:1024] for _ in range(3)])
+    check(z, "f32", bias=R.draw(rng, (3, 1024), "bf16"), bias_index=many, bias_dt="f32", id_dt="i32")
+
+
+def test_views_and_shapes():
+    rng = np.random.default_rng(5)
+    z = R.draw(rng, (6, 300), "f32", 3.0)
+    Z = R.to_device(z, "f32")
+    kw = some(rng, 6, 200, 30)
+    check(z[:, 3:203], "f32", logits=Z[:, 3:203], **kw)
+    check(z[:, ::2], "f32", logits=Z[:, ::2], **some(rng, 6, 150, 30))
+    check(z[::-1], "f32", logits=ms.flip(Z, 0), **some(rng, 6, 300, 30))
+    # (2, 3, columns) and one row without an axis give what (6, columns) gives
+    kw = some(rng, 6, 300, 30)
+    ok = rng.random((6, 300)) < 0.5
+    flat = check(z, "f32", allowed=ok, **kw).numpy()
+    cube = {k: ms.from_numpy(np.ascontiguousarray(v).reshape((2, 3) + v.shape[1:])) for k, v in kw.items()}
+    got = ms.adjust_logits(ms.from_numpy(z.astype(np.float32).reshape(2, 3, 300)), allowed=ms.array(ok.reshape(2, 3, 300), dtype="bool"), **cube)
+    assert got.shape == (2, 3, 300) and np.array_equal(got.numpy().reshape(6, 300), flat)
+    one = {k: ms.from_numpy(v)[4] for k, v in kw.items()}
+    got = ms.adjust_logits(Z[4], allowed=ms.array(ok[4], dtype="bool"), **one)
+    assert got.shape == (300,) and np.array_equal(got.numpy(), flat[4])
+    # views of the other operands
+    h2 = ms.from_numpy(np.ascontiguousarray(kw["history"].T))
+    ok2 = ms.array(np.ascontiguousarray(ok.T), dtype="bool")
+    wide = ms.from_numpy(np.repeat(kw["presence"], 2))
+    same = {k: ms.from_numpy(v) for k, v in kw.items()} | {"history": ms.transpose(h2), "presence": wide[::2]}
+    assert np.array_equal(ms.adjust_logits(Z, allowed=ms.transpose(ok2), **same).numpy(), flat)
+
+
+def test_no_rows_or_columns():
+    assert ms.adjust_logits(ms.from_numpy(np.zeros((0, 5), np.float32))).shape == (0, 5)
+    assert ms.adjust_logits(ms.from_numpy(np.zeros((5, 0), np.float32))).shape == (5, 0)
+
+
+def test_refusals():
+    z = ms.from_numpy(np.zeros((4, 40), np.float32))
+    h, n = R.ids(np.zeros((4, 6), np.int64)), R.ids(np.zeros(4, np.int64))
+    f = ms.from_numpy(np.ones(4, np.float32))
+    row = ms.from_numpy(np.ones(40, np.float32))
+    few = ms.from_numpy(np.ones((4, 2), np.float32))
+    for err, call in [
+        (ms.DtypeError, lambda: ms.adjust_logits(ms.from_numpy(np.zeros((4, 40))))),
+        (ms.DtypeError, lambda: ms.adjust_logits(z, dtype="bf16")),
+        (ms.DtypeError, lambda: ms.adjust_logits(z, few)),
+        (ms.ShapeError, lambda: ms.adjust_logits(z, h[:3])),
+        (ms.ShapeError, lambda: ms.adjust_logits(z, h, n[:3])),
+        (ms.ShapeError, lambda: ms.adjust_logits(z, lengths=n)),
+        (ms.DtypeError, lambda: ms.adjust_logits(z, h, f)),
+        (ValueError, lambda: ms.adjust_logits(z, h, repetition=0.0)),
+        (ValueError, lambda: ms.adjust_logits(z, h, repetition=float("inf"))),
+        (ValueError, lambda: ms.adjust_logits(z, h, presence=float("nan"))),
+        (ms.ShapeError, lambda: ms.adjust_logits(z, h, frequency=row)),
+        (ms.DtypeError, lambda: ms.adjust_logits(z, h, frequency=n)),
+        (ms.ShapeError, lambda: ms.adjust_logits(z, bias=row[:39])),
+        (ms.DtypeError, lambda: ms.adjust_logits(z, bias=ms.from_numpy(np.ones(40)))),
+        (ms.ShapeError, lambda: ms.adjust_logits(z, bias_index=h)),
+        (ms.ShapeError, lambda: ms.adjust_logits(z, bias=few, bias_index=h)),
+        (ms.DtypeError, lambda: ms.adjust_logits(z, bias=few, bias_index=few)),
+        (ms.ShapeError, lambda: ms.adjust_logits(z, bias=ms.from_numpy(np.zeros((4, 1025), np.float32)),
+                                                 bias_index=ms.from_numpy(np.zeros((4, 1025), np.int32)))),
+        (ms.DtypeError, lambda: ms.adjust_logits(z, allowed=row)),
+        (ms.ShapeError, lambda: ms.adjust_logits(z, allowed=ms.from_numpy(np.zeros((4, 3), np.int32)))),
+        (ms.ShapeError, lambda: ms.adjust_logits(z, allowed=ms.array(np.ones((3, 40), bool), dtype="bool"))),
+        (ms.MemoryError, lambda: ms.adjust_logits(z, out=z)),
+        (ms.ShapeError, lambda: ms.adjust_logits(z, out=row)),
+    ]:
+        with pytest.raises(err):
+            call()
