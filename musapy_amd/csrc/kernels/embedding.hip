@@ -62,7 +62,7 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embedding(EmbedArgs p) {
 
 template <class T, class O>
 int launch_embedding(const musapy_embedding_args* a, hipStream_t st) {
-  constexpr int kN = sizeof(T) == 2 && sizeof(O) == 2 ? 8 : 4;
+  constexpr int kN = sizeof(T) == 2 || sizeof(O) == 2 ? 8 : 4;
   const bool narrow = a->width < uint64_t(kN);
   const uint64_t groups = narrow ? a->width : (a->width + kN - 1) / kN;
   const uint64_t total = groups * a->tokens;
@@ -108,48 +108,100 @@ struct OrderArgs {
   uint32_t* hist;                    // [tile][bin]
   uint32_t tile, tiles;              // tokens of a workgroup, and workgroups
   int shift, bits;
+  char* zero;                        // part of the table's gradient, which the launch clears
+  uint64_t zero_bytes;
+  uint32_t order_blocks;             // workgroups in front of those that clear
+  uint32_t zero_pieces;              // of a vector for every thread, of a workgroup that clears
 };
 
-// Up to 16 * 1024 tokens: the place of a token in the order is the number of tokens in front of it, counted against
-// all others, 64 comparisons an instruction.  A workgroup ranks 64 tokens, its 16 waves hold G groups of 64
-// others each.  One launch without a wait; n^2 / 64 comparisons of four cycles on 1024 SIMDs.
-constexpr int kRankWaves = 16;
+// Every row is cleared while the order begins, though those of tokens are written again: 4 KB a workgroup, one vector a
+// thread, in the order of addresses, run at 6.7 TB/s (8 to 128 KB a workgroup 5.5 to 6.1).  Clearing only the other
+// rows beside the sums, with the sorted tokens or bits of the rows to look up, took the (131072, 2048) f32 gradient of 16384
+// tokens 225 to 240 us, against 157 for this and some 30 for the sums.  The order's later launches, whose few workgroups
+// take some 8 us whatever is cleared beside them, take 40 MB of it each.
+constexpr uint64_t kClearBeside = uint64_t(40) << 20;
 
-template <int G>
-__global__ __launch_bounds__(kRankWaves * 64) void k_embed_rank(OrderArgs p) {
-  __shared__ uint32_t part[kRankWaves][64];
+template <int BLOCK>
+__device__ inline void order_clear(const OrderArgs& p, uint32_t block) {
+  typedef uint32_t W __attribute__((ext_vector_type(4)));
+  const uint64_t past = reinterpret_cast<uintptr_t>(p.zero) % 16;
+  const uint64_t head = past == 0 ? 0 : 16 - past < p.zero_bytes ? 16 - past : p.zero_bytes;
+  const uint64_t vectors = (p.zero_bytes - head) / 16;
+  W* out = reinterpret_cast<W*>(p.zero + head);
+  for (uint32_t k = 0; k < p.zero_pieces; ++k) {
+    const uint64_t at = (uint64_t(block) * p.zero_pieces + k) * BLOCK + threadIdx.x;
+    if (at < vectors) out[at] = W{0, 0, 0, 0};
+  }
+  if (block != 0 || threadIdx.x >= 32) return;
+  const uint64_t edge = threadIdx.x < 16 ? threadIdx.x : head + vectors * 16 + threadIdx.x - 16;  // single bytes at both ends
+  if (threadIdx.x < 16 ? edge < head : edge < p.zero_bytes) p.zero[edge] = 0;
+}
+
+// Up to 16384 tokens, in two launches.  First, blocks of 256 tokens: a token's place in its block is the number of tokens
+// in front of it, counted against all others of the block.
+constexpr int kBlockTokens = 256, kOrderBlock = 1024, kOrderWaves = kOrderBlock / 64;
+constexpr int kOrderMost = 16384;
+
+__global__ __launch_bounds__(kBlockTokens) void k_embed_blocks(OrderArgs p) {
+  if (blockIdx.x >= p.order_blocks) return order_clear<kBlockTokens>(p, blockIdx.x - p.order_blocks);
+  __shared__ uint32_t all[kBlockTokens];
+  const uint32_t item = threadIdx.x, wave = wave_uniform(threadIdx.x / 64);
+  const uint32_t first = blockIdx.x * kBlockTokens;
+  const uint32_t key = first + item < p.n ? id_at(p.ids, first + item, p.rows) : ~0u;
+  all[item] = key;
+  __syncthreads();
+  uint32_t count = 0;
+#pragma unroll 1
+  for (uint32_t w = 0; w < kBlockTokens / 64; ++w) {
+    const uint32_t limit = w < wave ? key + 1 : key;  // equals count in front of the token (a missing one's limit is not used)
+#pragma unroll 16
+    for (uint32_t j = 0; j < 64; ++j) count += all[w * 64 + j] < limit ? 1 : 0;
+  }
+#pragma unroll 16
+  for (uint32_t j = 0; j < 64; ++j) count += all[wave * 64 + j] == key && j < item % 64 ? 1 : 0;
+  if (first + item >= p.n) return;
+  p.keys[first + count] = key;
+  p.pos[first + count] = first + item;
+}
+
+// Then a token's place among all is its place in its block and, of every other block, the number of keys below
+// its own (or not above it, of the blocks in front), each found by halving.  All keys lie in LDS; a workgroup places 64
+// tokens, and each of its 16 waves searches every sixteenth block, four at a time.
+__global__ __launch_bounds__(kOrderBlock) void k_embed_merge(OrderArgs p) {
+  if (blockIdx.x >= p.order_blocks) return order_clear<kOrderBlock>(p, blockIdx.x - p.order_blocks);
+  extern __shared__ uint32_t all[];
+  __shared__ uint32_t part[kOrderWaves][64];
+  const uint32_t blocks = (p.n + kBlockTokens - 1) / kBlockTokens;
+  for (uint32_t i = threadIdx.x; i < blocks * kBlockTokens; i += kOrderBlock) all[i] = i < p.n ? p.keys_in[i] : ~0u;
+  __syncthreads();
   const int lane = threadIdx.x % 64;
   const uint32_t wave = wave_uniform(threadIdx.x / 64);
-  uint32_t other[G];
-  uint32_t before[G];  // 1 where the group stands in front of this workgroup's: equals count there
-#pragma unroll
-  for (int i = 0; i < G; ++i) {
-    const uint32_t g = uint32_t(i) * kRankWaves + wave;
-    const uint32_t at = g * 64 + lane;
-    other[i] = at < p.n ? id_at(p.ids, at, p.rows) : ~0u;
-    before[i] = g < blockIdx.x ? 1u : 0u;
-  }
-  const uint32_t own = blockIdx.x * 64 + lane;
-  const uint32_t mine = own < p.n ? id_at(p.ids, own, p.rows) : ~0u;
+  const uint32_t at = blockIdx.x * 64 + lane, own = blockIdx.x * 64 / kBlockTokens;
+  const uint32_t key = all[at];
   uint32_t count = 0;
-#pragma unroll 4
-  for (int e = 0; e < 64; ++e) {
-    const uint32_t key = uint32_t(__builtin_amdgcn_readlane(int(mine), e));
-    uint32_t c = 0;
+  for (uint32_t b0 = wave; b0 < blocks; b0 += 4 * kOrderWaves) {
+    uint32_t base[4], limit[4], c[4] = {};
 #pragma unroll
-    for (int i = 0; i < G; ++i) c += uint32_t(__popcll(__ballot(other[i] < key + before[i])));
-    if (wave == 0) c += uint32_t(__popcll(__ballot(mine == key) & ((uint64_t(1) << e) - 1)));
-    if (lane == e) count = c;
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t b = b0 + i * kOrderWaves;
+      base[i] = b < blocks ? b * kBlockTokens : 0;
+      limit[i] = b < blocks && b != own ? key + (b < own ? 1 : 0) : 0;  // nothing is below 0
+    }
+#pragma unroll
+    for (uint32_t step = kBlockTokens / 2; step > 0; step /= 2)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] += all[base[i] + c[i] + step - 1] < limit[i] ? step : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) count += c[i] + (all[base[i] + c[i]] < limit[i] ? 1 : 0);
   }
   part[wave][lane] = count;
   __syncthreads();
-  if (wave == 0 && own < p.n) {
-    uint32_t rank = 0;
+  if (wave != 0 || at >= p.n) return;
+  uint32_t to = at - own * kBlockTokens;
 #pragma unroll
-    for (int w = 0; w < kRankWaves; ++w) rank += part[w][lane];
-    p.keys[rank] = mine;
-    p.pos[rank] = own;
-  }
+  for (int w = 0; w < kOrderWaves; ++w) to += part[w][lane];
+  p.keys[to] = key;
+  p.pos[to] = p.pos_in[at];
 }
 
 // More tokens: passes over up to nine bits each, lowest first; a pass counts its digits in every tile of
@@ -165,21 +217,23 @@ __device__ inline uint32_t order_key(const OrderArgs& p, uint32_t i) {
 }
 
 template <bool FIRST>
-__global__ __launch_bounds__(kSortBlock) void k_embed_digits(OrderArgs p) {
+__global__ __launch_bounds__(kBlockTokens) void k_embed_digits(OrderArgs p) {
+  if (blockIdx.x >= p.order_blocks) return order_clear<kBlockTokens>(p, blockIdx.x - p.order_blocks);
   __shared__ uint32_t count[kDigits];
-  static_assert(kSortBlock == kDigits, "a thread to a digit");
-  count[threadIdx.x] = 0;
+  for (int d = threadIdx.x; d < kDigits; d += kBlockTokens) count[d] = 0;
   __syncthreads();
   const uint32_t first = blockIdx.x * p.tile;
   const uint32_t last = p.n - first < p.tile ? p.n : first + p.tile;
-  for (uint32_t i = first + threadIdx.x; i < last; i += kSortBlock)
+  for (uint32_t i = first + threadIdx.x; i < last; i += kBlockTokens)
     atomicAdd(&count[(order_key<FIRST>(p, i) >> p.shift) & ((1u << p.bits) - 1)], 1u);
   __syncthreads();
-  p.hist[blockIdx.x * kDigits + threadIdx.x] = count[threadIdx.x];
+  for (int d = threadIdx.x; d < kDigits; d += kBlockTokens) p.hist[blockIdx.x * kDigits + d] = count[d];
 }
 
 template <bool FIRST>
 __global__ __launch_bounds__(kSortBlock) void k_embed_place(OrderArgs p) {
+  if (blockIdx.x >= p.order_blocks) return order_clear<kSortBlock>(p, blockIdx.x - p.order_blocks);
+  static_assert(kSortBlock == kDigits, "a thread to a digit");
   __shared__ uint32_t base[kDigits];
   __shared__ uint32_t at[kSortWaves][kDigits];
   const int lane = threadIdx.x % 64;
@@ -271,63 +325,8 @@ struct EmbedGradArgs {
   uint32_t padded;             // the width, rounded up to 4
   uint32_t chunk, chunks;      // tokens of a chunk, and chunks
   uint32_t tiles;              // of 64 * N columns
-  uint32_t sum_blocks;         // workgroups that sum; those behind them fill
-  uint32_t fill_rows;          // rows of a workgroup that fills
-  uint32_t fill_groups;        // groups of a row there
-  FastDiv fill_div;
   float scale;
 };
-
-// How many of the sorted keys are below `key`; all lanes of a wave take part, 64 probes a step.
-__device__ inline uint32_t wave_lower_bound(const uint32_t* keys, uint32_t lo, uint32_t hi, uint32_t key, int lane) {
-  while (hi - lo > 64) {
-    const uint32_t step = (hi - lo + 63) / 64;
-    const uint64_t at = uint64_t(lo) + uint64_t(lane) * step;
-    const uint32_t below = uint32_t(__popcll(__ballot(at < hi && keys[at < hi ? at : lo] < key)));
-    if (below == 0) return lo;
-    const uint64_t end = uint64_t(lo) + uint64_t(below) * step;  // (the first probe that is not below, or behind all)
-    lo += (below - 1) * step + 1;
-    hi = end < hi ? uint32_t(end) : hi;
-  }
-  return lo + uint32_t(__popcll(__ballot(lo + lane < hi && keys[lo + lane < hi ? lo + lane : lo] < key)));
-}
-
-// Rows of zeros for the tokens that do not occur.
-template <class O, int N>
-__device__ inline void embed_fill(const EmbedGradArgs& p, uint32_t block) {
-  __shared__ uint32_t present[2];
-  const uint32_t first = block * p.fill_rows;
-  const uint32_t count = p.rows - first < p.fill_rows ? p.rows - first : p.fill_rows;
-  if (threadIdx.x < 64) {
-    const uint32_t lane = threadIdx.x;
-    uint32_t lo = wave_lower_bound(p.keys, 0, p.n, first, int(lane));
-    uint32_t hi = wave_lower_bound(p.keys, lo, p.n, first + count, int(lane));
-    const uint32_t end = hi, key = first + lane;
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      if (p.keys[mid] < key) lo = mid + 1;
-      else hi = mid;
-    }
-    const uint64_t m = __ballot(lane < count && lo < end && p.keys[lo < end ? lo : 0] == key);
-    if (lane == 0) {
-      present[0] = uint32_t(m);
-      present[1] = uint32_t(m >> 32);
-    }
-  }
-  __syncthreads();
-  const uint64_t mask = present[0] | uint64_t(present[1]) << 32;
-  Vec<O, N> zero;
-#pragma unroll
-  for (int e = 0; e < N; ++e) zero.v[e] = O(0.0f);
-  const uint32_t total = count * p.fill_groups;
-  O* out = static_cast<O*>(p.out) + uint64_t(first) * p.width;
-  for (uint32_t q = threadIdx.x; q < total; q += kEmbedBlock) {
-    const uint32_t row = fd_div(p.fill_div, q);
-    const uint32_t c = (q - row * p.fill_groups) * N;
-    if ((mask >> row) & 1) continue;
-    vstore_el<true, O, N>(out + uint64_t(row) * p.width + (c + N <= p.width ? c : p.width - N), zero);
-  }
-}
 
 template <class O, int N, bool ADD>
 __device__ inline void embed_store(O* at, int skip, const float (&sum)[N], float scale) {
@@ -351,10 +350,6 @@ constexpr int kEmbedRows = 8;
 
 template <class T, class O, int N, bool ADD>
 __global__ __launch_bounds__(kEmbedBlock) void k_embed_sum(EmbedGradArgs p) {
-  if (blockIdx.x >= p.sum_blocks) {
-    if constexpr (!ADD) embed_fill<O, N == 1 ? 1 : 16 / int(sizeof(O))>(p, blockIdx.x - p.sum_blocks);
-    return;
-  }
   const int lane = threadIdx.x % 64;
   const uint32_t unit = blockIdx.x * (kEmbedBlock / 64) + wave_uniform(threadIdx.x / 64);
   const uint32_t chunk = unit / p.tiles;
@@ -466,19 +461,17 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embed_join(EmbedGradArgs p) {
 
 // ---- launches -------------------------------------------------------------------------------------------
 struct EmbedGradPlan {
-  int passes, bits;         // 0 passes: by rank
+  int passes, bits;         // 0 passes: by blocks
   uint32_t tile, tiles;     // of a pass
   uint32_t chunk, chunks;
   uint32_t padded;
   size_t keys, pos, keys2, pos2, hist, slots, bytes;  // offsets into the scratch
 };
 
-constexpr uint64_t kRankMost = uint64_t(kRankWaves) * 64 * 16;
-
 inline EmbedGradPlan embed_grad_plan(const musapy_embedding_grad_args* a) {
   EmbedGradPlan pl{};
   const uint64_t n = a->tokens;
-  if (n > kRankMost) {
+  if (n > uint64_t(kOrderMost)) {
     int bits = 1;
     while (bits < 32 && (uint64_t(a->rows) >> bits) != 0) ++bits;
     pl.passes = (bits + kDigitBits - 1) / kDigitBits;
@@ -498,9 +491,11 @@ inline EmbedGradPlan embed_grad_plan(const musapy_embedding_grad_args* a) {
   };
   pl.keys = take(n * 4);
   pl.pos = take(n * 4);
-  if (pl.passes > 0) {
+  if (n > uint64_t(kBlockTokens)) {
     pl.keys2 = take(n * 4);
     pl.pos2 = take(n * 4);
+  }
+  if (pl.passes > 0) {
     pl.hist = take(size_t(pl.tiles) * kDigits * 4);
   }
   pl.slots = take(size_t(pl.chunks) * 2 * pl.padded * 4);
@@ -514,16 +509,38 @@ inline void launch_order(const musapy_embedding_grad_args* a, const EmbedGradPla
   o.rows = uint32_t(a->rows);
   uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(ws + pl.keys), reinterpret_cast<uint32_t*>(ws + pl.keys2)};
   uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(ws + pl.pos), reinterpret_cast<uint32_t*>(ws + pl.pos2)};
+  const uint32_t blocks = pl.passes ? pl.tiles : (o.n + kBlockTokens - 1) / kBlockTokens;
+  const int launches = pl.passes ? 2 * pl.passes : blocks > 1 ? 2 : 1;
+  uint64_t bytes = a->accumulate ? 0 : a->rows * a->width * (a->out_dtype == MUSAPY_DT_F32 ? 4 : 2);
+  char* out = static_cast<char*>(a->out);
+  uint64_t beside = bytes / uint64_t(launches) < kClearBeside ? bytes / uint64_t(launches) : kClearBeside;
+  beside = beside / 4096 * 4096;
+  // the workgroups of a launch: those that order, and those that clear the next `part` bytes
+  auto grid = [&](uint32_t order, uint64_t threads, uint64_t part) {
+    o.order_blocks = order;
+    o.zero = out;
+    o.zero_bytes = part;
+    out += part;
+    bytes -= part;
+    const uint64_t pieces = part ? part / (16 * threads) + 1 : 0;
+    o.zero_pieces = 1;
+    while (!grid_fits(order + (pieces + o.zero_pieces - 1) / o.zero_pieces, threads)) o.zero_pieces *= 2;
+    return unsigned(order + (pieces + o.zero_pieces - 1) / o.zero_pieces);
+  };
+  const uint64_t most = bytes - beside * uint64_t(launches - 1);  // of the first launch
   if (pl.passes == 0) {
+    const bool one = blocks <= 1;
+    o.keys = keys[one ? 0 : 1];
+    o.pos = pos[one ? 0 : 1];
+    const unsigned first = grid(blocks, kBlockTokens, most);
+    if (first > 0) k_embed_blocks<<<first, kBlockTokens, 0, st>>>(o);
+    if (one) return;
+    o.keys_in = o.keys;
+    o.pos_in = o.pos;
     o.keys = keys[0];
     o.pos = pos[0];
-    const unsigned grid = unsigned((o.n + 63) / 64);
-    const int most = kRankWaves * 64;
-    if (o.n <= 1 * most) k_embed_rank<1><<<grid, most, 0, st>>>(o);
-    else if (o.n <= 2 * most) k_embed_rank<2><<<grid, most, 0, st>>>(o);
-    else if (o.n <= 4 * most) k_embed_rank<4><<<grid, most, 0, st>>>(o);
-    else if (o.n <= 8 * most) k_embed_rank<8><<<grid, most, 0, st>>>(o);
-    else k_embed_rank<16><<<grid, most, 0, st>>>(o);
+    const unsigned second = grid((o.n + 63) / 64, kOrderBlock, beside);
+    k_embed_merge<<<second, kOrderBlock, blocks * kBlockTokens * 4, st>>>(o);
     return;
   }
   o.hist = reinterpret_cast<uint32_t*>(ws + pl.hist);
@@ -537,13 +554,12 @@ inline void launch_order(const musapy_embedding_grad_args* a, const EmbedGradPla
     o.pos = pos[to];
     o.keys_in = keys[1 - to];
     o.pos_in = pos[1 - to];
-    if (i == 0) {
-      k_embed_digits<true><<<pl.tiles, kSortBlock, 0, st>>>(o);
-      k_embed_place<true><<<pl.tiles, kSortBlock, 0, st>>>(o);
-    } else {
-      k_embed_digits<false><<<pl.tiles, kSortBlock, 0, st>>>(o);
-      k_embed_place<false><<<pl.tiles, kSortBlock, 0, st>>>(o);
-    }
+    const unsigned count = grid(blocks, kBlockTokens, i == 0 ? most : beside);
+    if (i == 0) k_embed_digits<true><<<count, kBlockTokens, 0, st>>>(o);
+    else k_embed_digits<false><<<count, kBlockTokens, 0, st>>>(o);
+    const unsigned place = grid(blocks, kSortBlock, beside);
+    if (i == 0) k_embed_place<true><<<place, kSortBlock, 0, st>>>(o);
+    else k_embed_place<false><<<place, kSortBlock, 0, st>>>(o);
   }
 }
 
@@ -551,9 +567,8 @@ template <class T, class O>
 int launch_embedding_grad(const musapy_embedding_grad_args* a, char* ws, hipStream_t st) {
   const EmbedGradPlan pl = embed_grad_plan(a);
   constexpr int kN = sizeof(T) == 2 ? 8 : 4;
-  constexpr int kFill = 16 / int(sizeof(O));
-  const bool narrow = a->width < uint64_t(kN) || a->width < uint64_t(kFill);
-  const int n = narrow ? 1 : kN, fill = narrow ? 1 : kFill;
+  const bool narrow = a->width < uint64_t(kN);
+  const int n = narrow ? 1 : kN;
   EmbedGradArgs p{};
   p.keys = reinterpret_cast<uint32_t*>(ws + pl.keys);
   p.pos = reinterpret_cast<uint32_t*>(ws + pl.pos);
@@ -569,21 +584,13 @@ int launch_embedding_grad(const musapy_embedding_grad_args* a, char* ws, hipStre
   p.chunks = pl.chunks;
   p.tiles = uint32_t((a->width + 64 * n - 1) / (64 * n));
   p.scale = a->scale;
-  const uint64_t units = uint64_t(p.chunks) * p.tiles;
-  p.sum_blocks = uint32_t((units + 3) / 4);
-  p.fill_groups = uint32_t((a->width + fill - 1) / fill);
-  p.fill_div = make_fastdiv(p.fill_groups);
-  p.fill_rows = 64;  // rows of some 128 KB a workgroup, 8 at least
-  while (p.fill_rows > 8 && uint64_t(p.fill_rows) * a->width * sizeof(O) > (128u << 10)) p.fill_rows /= 2;
-  const uint64_t fills = a->accumulate ? 0 : (a->rows + p.fill_rows - 1) / p.fill_rows;
-  if (units >= kVocabLimit || !grid_fits(p.sum_blocks + fills, kEmbedBlock)) return vocab_bad();
+  const uint64_t units = uint64_t(p.chunks) * p.tiles, grid = (units + 3) / 4;
   const uint64_t joins = (pl.padded + 255) / 256;
-  if (joins > 65535) return vocab_bad();
-  if (p.n > 0) launch_order(a, pl, ws, st);
-  const unsigned grid = unsigned(p.sum_blocks + fills);
+  if (units >= kVocabLimit || !grid_fits(grid, kEmbedBlock) || joins > 65535) return vocab_bad();
+  launch_order(a, pl, ws, st);
   const dim3 join(pl.chunks, unsigned(joins));
   auto go = [&](auto N, auto ADD) {
-    if (grid > 0) k_embed_sum<T, O, N.value, ADD.value><<<grid, kEmbedBlock, 0, st>>>(p);
+    if (grid > 0) k_embed_sum<T, O, N.value, ADD.value><<<unsigned(grid), kEmbedBlock, 0, st>>>(p);
     if (pl.chunks > 1) k_embed_join<O, ADD.value><<<join, kEmbedBlock, 0, st>>>(p);
   };
   using Full = std::integral_constant<int, kN>;
