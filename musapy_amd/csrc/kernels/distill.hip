@@ -26,7 +26,7 @@ struct DistillArgs {
   const float* dloss;
   int64_t dloss_stride;
   void* grad;
-  uint32_t segment, segments;  // of the gradient: columns of a workgroup, workgroups of a row
+  uint32_t segments;       // of the gradient: workgroups of a row
 };
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -61,15 +61,26 @@ __device__ inline float teacher_max(const DistillArgs& p, uint32_t row, int lane
   return wave_max(top);
 }
 
+// The columns of a row in front of its first address that is a multiple of 16 bytes.
+template <class T>
+__device__ inline uint32_t row_head(const T* row, uint32_t width) {
+  constexpr uint32_t N = 16 / sizeof(T);
+  const uint32_t head = (N - uint32_t(reinterpret_cast<uintptr_t>(row) / sizeof(T)) % N) % N;
+  return head < width ? head : width;
+}
+
 // A workgroup takes a row: every thread keeps the maximum m of its logits and the sums of exp((z - m) / T) and,
 // with labels at a T other than 1, exp(z - m), rescaled when m rises; they are joined at the end.  The first
 // wave forms the teacher's part, which needs K logits and the sum only:
 //   sum_k p_k (log p_k - log q_k) = B / A - log A + (m - r) / T + log sum exp((z - m) / T),
 //   e_k = exp((v_k - max v) / T),  A = sum e_k,  B = sum e_k ((v_k - max v) - (z_k - r)) / T
 // with r the highest of the entries' logits: all differences are of near numbers, so that logits far from 0 lose nothing.
-template <class T, int BLOCK, bool TWO>
+enum { kOne = 0, kTwo = 1, kSquare = 2 };  // one sum; two; two at T = 2, where exp(z - m) is the square of exp((z - m) / 2)
+
+template <class T, int BLOCK, int SUMS>
 __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
   constexpr int N = 16 / int(sizeof(T)), U = 4, kWaves = BLOCK / 64;
+  constexpr bool TWO = SUMS != kOne;
   __shared__ float part[kWaves];
   const uint32_t row = blockIdx.x;
   const int lane = threadIdx.x % 64;
@@ -115,19 +126,32 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
     m = high;
 #pragma unroll
     for (int e = 0; e < N * U; ++e) {
-      const float d = x[e] - m;
-      s += exp2_fast(d * p.c);
-      if (TWO) s1 += exp2_fast(d * kLog2e);
+      const float d = x[e] - m, w = exp2_fast(d * p.c);
+      s += w;
+      if (SUMS == kTwo) s1 += exp2_fast(d * kLog2e);
+      if (SUMS == kSquare) s1 = __builtin_fmaf(w, w, s1);
     }
   };
-  const uint32_t vectors = p.width / N;
-  for (uint32_t base = 0; base < vectors; base += BLOCK * U) {
+  const uint32_t head = row_head<T>(z, p.width), vectors = (p.width - head) / N;
+  uint32_t base = 0;
+  for (; base + BLOCK * U <= vectors; base += BLOCK * U) {
+    Vec<T, N> v[U];
+    float x[N * U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = vload_el<T, N, true>(z + head + uint64_t(base + u * BLOCK + threadIdx.x) * N);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[u * N + e] = float(v[u].v[e]);
+    add(x);
+  }
+  if (base < vectors) {
     Vec<T, N> v[U];
     float x[N * U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t at = base + u * BLOCK + threadIdx.x;
-      v[u] = vload_el<T, N, true>(z + uint64_t(at < vectors ? at : vectors - 1) * N);
+      v[u] = vload_el<T, N, true>(z + head + uint64_t(at < vectors ? at : vectors - 1) * N);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -136,11 +160,11 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
         x[u * N + e] = base + u * BLOCK + threadIdx.x < vectors ? float(v[u].v[e]) : -__builtin_inff();
     add(x);
   }
-  if (threadIdx.x < p.width - vectors * N) {
+  if (threadIdx.x < p.width - vectors * N) {  // the columns in front of and behind the vectors
     float x[N * U];
 #pragma unroll
     for (int e = 0; e < N * U; ++e) x[e] = -__builtin_inff();
-    x[0] = float(z[vectors * N + threadIdx.x]);
+    x[0] = float(z[threadIdx.x < head ? threadIdx.x : threadIdx.x + vectors * N]);
     add(x);
   }
   const float most = block_fold<kWaves>(wave_max(m), part, [](float u, float w) { return fmaxf(u, w); });
@@ -163,94 +187,113 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
   sums[2] = hard ? ls1 : 0.0f;
 }
 
-// A workgroup takes a segment of a row: dloss (weight T softmax(z / T) + (1 - weight) softmax(z)) of every
-// column, from the maximum and the logarithms of the sums that the loss left.  Then the columns of the teacher's entries and the label, at
-// most K + 1, are formed again with what is taken off there, and stored over the first values behind a
-// barrier; a column that several entries name is formed by the first of them.
-template <class T, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void k_distill_grad(DistillArgs p) {
-  constexpr int N = 16 / int(sizeof(T)), U = 4, kWaves = BLOCK / 64;
-  __shared__ float part[kWaves];
+// A workgroup takes a segment of a row, four vectors of 16 bytes to a thread: dloss (weight T softmax(z / T) +
+// (1 - weight) softmax(z)) of every column, from the maximum and the logarithms of the sums that the loss left.  Then the
+// columns of the teacher's entries and the label, at most K + 1 a row, are formed again with what is taken off there, and
+// stored over the first values behind a barrier.  The first wave does that, and what the entries need before it, from the
+// entries that lie in the segment; a column that several of them name is formed by the first.
+// 16 KB a workgroup: 6.1 TB/s of logits and results in bf16; whole rows of 256 KB 5.0.
+constexpr int kGradBlock = 256, kGradVectors = 4;
+template <class T>
+constexpr uint32_t kGradSegment = kGradBlock * kGradVectors * 16 / sizeof(T);
+
+template <class T, bool SQUARE>
+__global__ __launch_bounds__(kGradBlock) void k_distill_grad(DistillArgs p) {
+  constexpr int N = 16 / int(sizeof(T)), U = kGradVectors;
   __shared__ uint32_t index[kEntriesMost];
   __shared__ float prob[kEntriesMost];
   const uint32_t row = blockIdx.x / p.segments, seg = blockIdx.x - row * p.segments;
-  const uint32_t first = seg * p.segment;
-  const uint32_t last = p.width - first < p.segment ? p.width : first + p.segment;
+  const int lane = threadIdx.x % 64;
+  const uint32_t wave = wave_uniform(threadIdx.x / 64);
   const T* z = static_cast<const T*>(p.logits) + uint64_t(row) * p.pitch;
   T* out = static_cast<T*>(p.grad) + uint64_t(row) * p.width;
-  const float dl = p.dloss[int64_t(row) * p.dloss_stride];
 
-  // the entries, and their probabilities
-  bool some = false;
-  float top = -__builtin_inff();
-  for (uint32_t k = threadIdx.x; k < p.entries; k += BLOCK) {
-    uint32_t i = p.use_soft ? id_at(p.index, row * p.index_pitch + k, p.width) : p.width;
-    const float v = float_at(p.teacher, p.teacher_dtype, row * p.teacher_pitch + k);
-    if (v == -__builtin_inff()) i = p.width;
-    index[k] = i;
-    prob[k] = v;
-    if (i < p.width) {
-      some = true;
-      top = fmaxf(top, v);
-    }
+  // Vectors lie where the results' addresses are multiples of 16 bytes (and the logits' too, where both rows begin
+  // alike); the first segment has the columns in front of them, the last one those behind.
+  const uint32_t head = row_head<T>(out, p.width), vectors = (p.width - head) / N;
+  const uint32_t start = seg * (kGradBlock * U), from = start < vectors ? start : vectors;
+  const uint32_t to = vectors - from < kGradBlock * U ? vectors : from + kGradBlock * U;
+  const bool ends = seg == p.segments - 1;
+  const uint32_t first = seg == 0 ? 0 : head + from * N, last = ends ? p.width : head + to * N;
+  const uint32_t before = seg == 0 ? head : 0;
+  uint32_t lone = threadIdx.x < before ? threadIdx.x : head + vectors * N + (threadIdx.x - before);
+  if (threadIdx.x >= before && !ends) lone = p.width;
+  Vec<T, N> v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t at = from + u * kGradBlock + threadIdx.x;
+    if (at < to) v[u] = vload_el<T, N, true>(z + head + uint64_t(at) * N);
   }
-  const bool soft = __syncthreads_or(some);
-  if (soft) {
-    top = block_fold<kWaves>(wave_max(top), part, [](float u, float w) { return fmaxf(u, w); });
-    float a = 0.0f;
-    for (uint32_t k = threadIdx.x; k < p.entries; k += BLOCK) {
-      const float e = index[k] < p.width ? exp2_fast((prob[k] - top) * p.c) : 0.0f;
-      prob[k] = e;
-      a += e;
-    }
-    a = block_fold<kWaves>(wave_sum(a), part, [](float u, float w) { return u + w; });
-    for (uint32_t k = threadIdx.x; k < p.entries; k += BLOCK) prob[k] /= a;
-  }
+
+  bool soft = false;
+  const float top = p.use_soft ? teacher_max(p, row, lane, soft) : 0.0f;
   const uint32_t label = p.labels.at ? id_at(p.labels, row, p.width) : p.width;
   const bool hard = label < p.width;
+  const float dl = p.dloss[int64_t(row) * p.dloss_stride];
   const float ka = dl * p.soft, kb = dl * p.hard;
   const float m = p.sums[uint64_t(row) * 3];
   const float la = p.sums[uint64_t(row) * 3 + 1] * kLog2e, lb = p.sums[uint64_t(row) * 3 + 2] * kLog2e;
+  uint32_t listed = 0;  // entries of the segment, in order (of the first wave)
+  if (soft && wave == 0) {
+    float a = 0.0f;
+    for (uint32_t k0 = 0; k0 < p.entries; k0 += 64) {
+      const uint32_t k = k0 + lane;
+      uint32_t i = p.width;
+      float e = 0.0f;
+      if (k < p.entries) {
+        i = id_at(p.index, row * p.index_pitch + k, p.width);
+        const float x = float_at(p.teacher, p.teacher_dtype, row * p.teacher_pitch + k);
+        if (x == -__builtin_inff()) i = p.width;
+        if (i < p.width) e = exp2_fast((x - top) * p.c);
+      }
+      a += e;
+      const bool here = i >= first && i < last;
+      const uint64_t those = __ballot(here);
+      if (here) {
+        const uint32_t at = listed + uint32_t(__popcll(those & ((uint64_t(1) << lane) - 1)));
+        index[at] = i;
+        prob[at] = e;
+      }
+      listed += uint32_t(__popcll(those));
+    }
+    a = wave_sum(a);
+    for (uint32_t k = lane; k < listed; k += 64) prob[k] /= a;
+  }
 
   auto stream = [&](auto fn) {
-    const uint32_t vectors = (last - first) / N;
-    for (uint32_t base = 0; base < vectors; base += BLOCK * U) {
-      Vec<T, N> v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t at = base + u * BLOCK + threadIdx.x;
-        v[u] = vload_el<T, N, true>(z + first + uint64_t(at < vectors ? at : vectors - 1) * N);
-      }
+    for (int u = 0; u < U; ++u) {
+      const uint32_t at = from + u * kGradBlock + threadIdx.x;
+      if (at >= to) continue;
+      Vec<T, N> o;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t at = base + u * BLOCK + threadIdx.x;
-        if (at >= vectors) continue;
-        Vec<T, N> o;
-#pragma unroll
-        for (int e = 0; e < N; ++e) o.v[e] = T(fn(float(v[u].v[e])));
-        vstore_el<true, T, N>(out + first + uint64_t(at) * N, o);
-      }
+      for (int e = 0; e < N; ++e) o.v[e] = T(fn(float(v[u].v[e])));
+      vstore_el<true, T, N>(out + head + uint64_t(at) * N, o);
     }
-    const uint32_t rest = first + vectors * N + threadIdx.x;
-    if (rest < last) out[rest] = T(fn(float(z[rest])));
+    if (lone < p.width) out[lone] = T(fn(float(z[lone])));
   };
   auto q = [&](float x) { return exp2_fast(__builtin_fmaf(x - m, p.c, -la)); };
   auto s = [&](float x) { return exp2_fast(__builtin_fmaf(x - m, kLog2e, -lb)); };
-  if (soft && hard) stream([&](float x) { return ka * q(x) + kb * s(x); });
-  else if (soft) stream([&](float x) { return ka * q(x); });
-  else if (hard) stream([&](float x) { return kb * s(x); });
-  else {
-    const T zero = T(0.0f);
-    Vec<T, N> o;
-#pragma unroll
-    for (int e = 0; e < N; ++e) o.v[e] = zero;
-    const uint32_t vectors = (last - first) / N;
-    for (uint32_t at = threadIdx.x; at < vectors; at += BLOCK) vstore_el<true, T, N>(out + first + uint64_t(at) * N, o);
-    const uint32_t rest = first + vectors * N + threadIdx.x;
-    if (rest < last) out[rest] = zero;
+  if (soft && hard && SQUARE) {  // exp(z - m) is the square of exp((z - m) / 2)
+    const float kc = kb * exp2_fast(2.0f * la - lb);
+    stream([&](float x) {
+      const float w = q(x);
+      return w * __builtin_fmaf(kc, w, ka);
+    });
+  } else if (soft && hard && p.c == kLog2e) {  // T = 1: one softmax
+    stream([&](float x) { return (ka + kb) * q(x); });
+  } else if (soft && hard) {
+    stream([&](float x) { return ka * q(x) + kb * s(x); });
+  } else if (soft) {
+    stream([&](float x) { return ka * q(x); });
+  } else if (hard) {
+    stream([&](float x) { return kb * s(x); });
+  } else {
+    stream([&](float) { return 0.0f; });
     return;
   }
   __syncthreads();
+  if (wave != 0) return;
   auto column = [&](uint32_t i, float taken) {
     const float x = float(z[i]);
     float g = 0.0f;
@@ -259,21 +302,19 @@ __global__ __launch_bounds__(BLOCK) void k_distill_grad(DistillArgs p) {
     out[i] = T(g);
   };
   bool labelled = false;  // whether an entry's column is the label's
-  for (uint32_t k = threadIdx.x; soft && k < p.entries; k += BLOCK) {
+  for (uint32_t k = lane; k < listed; k += 64) {
     const uint32_t i = index[k];
     if (i == label && hard) labelled = true;
-    if (i < first || i >= last) continue;
     float taken = 0.0f;
     bool leads = true;
-    for (uint32_t j = 0; j < p.entries; ++j) {
+    for (uint32_t j = 0; j < listed; ++j) {
       if (index[j] != i) continue;
       if (j < k) leads = false;
       taken += prob[j];
     }
     if (leads) column(i, taken);
   }
-  labelled = __syncthreads_or(labelled);
-  if (hard && !labelled && threadIdx.x == 0 && label >= first && label < last) column(label, 0.0f);
+  if (hard && __ballot(labelled) == 0 && lane == 0 && label >= first && label < last) column(label, 0.0f);
 }
 
 static bool distill_args(const musapy_distill_args* a, bool grad, DistillArgs& p) {
@@ -322,8 +363,9 @@ int musapy_distill_loss_v1(const musapy_distill_args* a, hipStream_t st) {
   const bool two = p.labels.at != nullptr && a->temperature != 1.0f;
   vocab_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    if (two) k_distill_loss<T, 512, true><<<p.rows, 512, 0, st>>>(p);
-    else k_distill_loss<T, 512, false><<<p.rows, 512, 0, st>>>(p);
+    if (two && a->temperature == 2.0f) k_distill_loss<T, 512, kSquare><<<p.rows, 512, 0, st>>>(p);
+    else if (two) k_distill_loss<T, 512, kTwo><<<p.rows, 512, 0, st>>>(p);
+    else k_distill_loss<T, 512, kOne><<<p.rows, 512, 0, st>>>(p);
   });
   return 0;
 }
@@ -335,17 +377,18 @@ int musapy_distill_loss_grad_v1(const musapy_distill_args* a, hipStream_t st) {
   if (p.logits == nullptr || p.sums == nullptr || p.dloss == nullptr || p.grad == nullptr ||
       (p.entries > 0 && (p.index.at == nullptr || p.teacher == nullptr)))
     return vocab_bad();
-  // whole rows where they fill the chip, and segments of a multiple of 4096 columns
-  p.segments = 1;
-  p.segment = p.width;
-  while (uint64_t(p.rows) * p.segments < 2048 && p.segment > 8192) {
-    p.segment = ((p.segment + 1) / 2 + 4095) / 4096 * 4096;
-    p.segments = (p.width + p.segment - 1) / p.segment;
-  }
-  if (!grid_fits(uint64_t(p.rows) * p.segments, 256)) return vocab_bad();
   vocab_type(a->dtype, [&](auto t) {
-    k_distill_grad<decltype(t), 256><<<p.rows * p.segments, 256, 0, st>>>(p);
+    using T = decltype(t);
+    p.segments = (p.width + kGradSegment<T> - 1) / kGradSegment<T>;
+    const uint64_t grid = uint64_t(p.rows) * p.segments;
+    if (!grid_fits(grid, kGradBlock)) {
+      p.segments = 0;
+      return;
+    }
+    if (a->temperature == 2.0f) k_distill_grad<T, true><<<unsigned(grid), kGradBlock, 0, st>>>(p);
+    else k_distill_grad<T, false><<<unsigned(grid), kGradBlock, 0, st>>>(p);
   });
+  if (p.segments == 0) return vocab_bad();
   return 0;
 }
 

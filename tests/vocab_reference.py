@@ -167,7 +167,8 @@ def distill_grad_bound(dl, z, sums, index, teacher, label, temp, weight):
         np.add.at(g, i, weight * temp * p * (2 * _teacher_bound(kept, temp, len(index)) + 8 * U))
     if hard:
         s = np.exp(-d - sums[2]) * np.isfinite(z)
-        g += (1 - weight) * (s * U * (4 * d + 4 * sums[2] + 10) + 2.0 ** -125)
+        # (or, at T = 2, the square of exp((x - m) / 2 - l): twice its relative error, and the constant's own)
+        g += (1 - weight) * (s * U * (4 * d + 4 * sums[2] + 10 + (8 * sums[1] + 20 if temp == 2 else 0)) + 2.0 ** -125)
         g[label] += 4 * U * (1 - weight)
     return abs(dl) * g
 
