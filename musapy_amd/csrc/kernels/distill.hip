@@ -86,6 +86,7 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
   const int lane = threadIdx.x % 64;
   const uint32_t wave = wave_uniform(threadIdx.x / 64);
   const T* z = static_cast<const T*>(p.logits) + uint64_t(row) * p.pitch;
+  const uint32_t head = row_head<T>(z, p.width), vectors = (p.width - head) / N;
   bool soft = false;
   const float top = p.use_soft ? teacher_max(p, row, lane, soft) : 0.0f;
   const uint32_t label = p.labels.at ? id_at(p.labels, row, p.width) : p.width;
@@ -132,7 +133,6 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
       if (SUMS == kSquare) s1 = __builtin_fmaf(w, w, s1);
     }
   };
-  const uint32_t head = row_head<T>(z, p.width), vectors = (p.width - head) / N;
   uint32_t base = 0;
   for (; base + BLOCK * U <= vectors; base += BLOCK * U) {
     Vec<T, N> v[U];
@@ -187,90 +187,158 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
   sums[2] = hard ? ls1 : 0.0f;
 }
 
-// A workgroup takes a segment of a row, four vectors of 16 bytes to a thread: dloss (weight T softmax(z / T) +
-// (1 - weight) softmax(z)) of every column, from the maximum and the logarithms of the sums that the loss left.  Then the
-// columns of the teacher's entries and the label, at most K + 1 a row, are formed again with what is taken off there, and
-// stored over the first values behind a barrier.  The first wave does that, and what the entries need before it, from the
-// entries that lie in the segment; a column that several of them name is formed by the first.
-// 16 KB a workgroup: 6.1 TB/s of logits and results in bf16; whole rows of 256 KB 5.0.
-constexpr int kGradBlock = 256, kGradVectors = 4;
-template <class T>
-constexpr uint32_t kGradSegment = kGradBlock * kGradVectors * 16 / sizeof(T);
+// A workgroup of one wave takes a segment of a row, four vectors of 16 bytes to a lane: dloss (weight T softmax(z / T) +
+// (1 - weight) softmax(z)) of every column, from the maximum and the logarithms of the sums that the loss left, less what
+// the teacher's entries and the label take off.  While the logits are on their way the wave lists the segment's
+// entries in LDS, and under every column the place of what is taken off there; a column that several entries name has
+// one place, with their sum.  So every value is stored once, and no wave waits for another.
+constexpr int kGradVectors = 4;
+constexpr unsigned grad_lds(uint32_t entries) { return (entries + 1) * 12; }
 
 template <class T, bool SQUARE>
-__global__ __launch_bounds__(kGradBlock) void k_distill_grad(DistillArgs p) {
-  constexpr int N = 16 / int(sizeof(T)), U = kGradVectors;
-  __shared__ uint32_t index[kEntriesMost];
-  __shared__ float prob[kEntriesMost];
-  const uint32_t row = blockIdx.x / p.segments, seg = blockIdx.x - row * p.segments;
-  const int lane = threadIdx.x % 64;
-  const uint32_t wave = wave_uniform(threadIdx.x / 64);
+__global__ __launch_bounds__(64) void k_distill_grad(DistillArgs p) {
+  constexpr int N = 16 / int(sizeof(T)), U = kGradVectors, kColumns = 64 * U * N;
+  __shared__ Vec<uint16_t, N> map[64 * U];  // of the vectors' columns: 0, or 1 + the place in the list
+  extern __shared__ uint32_t column[];      // [entries + 1] the list: columns, the entries' exponentials, what is taken off
+  float* part = reinterpret_cast<float*>(column + p.entries + 1);
+  float* taken = part + p.entries + 1;
+  const uint32_t row = blockIdx.x / p.segments, seg = blockIdx.x - row * p.segments, lane = threadIdx.x;
   const T* z = static_cast<const T*>(p.logits) + uint64_t(row) * p.pitch;
   T* out = static_cast<T*>(p.grad) + uint64_t(row) * p.width;
 
   // Vectors lie where the results' addresses are multiples of 16 bytes (and the logits' too, where both rows begin
   // alike); the first segment has the columns in front of them, the last one those behind.
   const uint32_t head = row_head<T>(out, p.width), vectors = (p.width - head) / N;
-  const uint32_t start = seg * (kGradBlock * U), from = start < vectors ? start : vectors;
-  const uint32_t to = vectors - from < kGradBlock * U ? vectors : from + kGradBlock * U;
+  const uint32_t start = seg * (64 * U), from = start < vectors ? start : vectors;
+  const uint32_t to = vectors - from < 64 * U ? vectors : from + 64 * U;
   const bool ends = seg == p.segments - 1;
-  const uint32_t first = seg == 0 ? 0 : head + from * N, last = ends ? p.width : head + to * N;
+  const uint32_t base = head + from * N;  // the vectors' first column
+  const uint32_t first = seg == 0 ? 0 : base, last = ends ? p.width : head + to * N;
   const uint32_t before = seg == 0 ? head : 0;
-  uint32_t lone = threadIdx.x < before ? threadIdx.x : head + vectors * N + (threadIdx.x - before);
-  if (threadIdx.x >= before && !ends) lone = p.width;
+  uint32_t lone = lane < before ? lane : head + vectors * N + (lane - before);
+  if (lane >= before && !ends) lone = p.width;
+  // the first 64 entries, then the logits: all on their way at once
+  auto entry = [&](uint32_t k, uint32_t& i, float& x) {
+    i = p.width;
+    x = -__builtin_inff();
+    if (!p.use_soft || k >= p.entries) return;
+    i = id_at(p.index, row * p.index_pitch + k, p.width);
+    x = float_at(p.teacher, p.teacher_dtype, row * p.teacher_pitch + k);
+  };
+  uint32_t i0;
+  float x0;
+  entry(lane, i0, x0);
+  const uint32_t label = p.labels.at ? id_at(p.labels, row, p.width) : p.width;
+  const float dl = p.dloss[int64_t(row) * p.dloss_stride];
+  const float m = p.sums[uint64_t(row) * 3];
+  const float la = p.sums[uint64_t(row) * 3 + 1] * kLog2e, lb = p.sums[uint64_t(row) * 3 + 2] * kLog2e;
   Vec<T, N> v[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const uint32_t at = from + u * kGradBlock + threadIdx.x;
+    const uint32_t at = from + u * 64 + lane;
     if (at < to) v[u] = vload_el<T, N, true>(z + head + uint64_t(at) * N);
+    map[u * 64 + lane] = Vec<uint16_t, N>{};
   }
 
-  bool soft = false;
-  const float top = p.use_soft ? teacher_max(p, row, lane, soft) : 0.0f;
-  const uint32_t label = p.labels.at ? id_at(p.labels, row, p.width) : p.width;
   const bool hard = label < p.width;
-  const float dl = p.dloss[int64_t(row) * p.dloss_stride];
   const float ka = dl * p.soft, kb = dl * p.hard;
-  const float m = p.sums[uint64_t(row) * 3];
-  const float la = p.sums[uint64_t(row) * 3 + 1] * kLog2e, lb = p.sums[uint64_t(row) * 3 + 2] * kLog2e;
-  uint32_t listed = 0;  // entries of the segment, in order (of the first wave)
-  if (soft && wave == 0) {
-    float a = 0.0f;
+  auto each = [&](auto fn) {  // an entry that counts to a lane, or the width in its place
     for (uint32_t k0 = 0; k0 < p.entries; k0 += 64) {
-      const uint32_t k = k0 + lane;
-      uint32_t i = p.width;
-      float e = 0.0f;
-      if (k < p.entries) {
-        i = id_at(p.index, row * p.index_pitch + k, p.width);
-        const float x = float_at(p.teacher, p.teacher_dtype, row * p.teacher_pitch + k);
-        if (x == -__builtin_inff()) i = p.width;
-        if (i < p.width) e = exp2_fast((x - top) * p.c);
-      }
+      uint32_t i = i0;
+      float x = x0;
+      if (k0 > 0) entry(k0 + lane, i, x);
+      fn(x == -__builtin_inff() ? p.width : i, x);
+    }
+  };
+  float top = -__builtin_inff(), a = 0.0f;
+  bool some = false;
+  each([&](uint32_t i, float x) {
+    if (i >= p.width) return;
+    some = true;
+    top = fmaxf(top, x);
+  });
+  const bool soft = __ballot(some) != 0;
+  uint32_t listed = 0;
+  if (soft) {
+    top = wave_max(top);
+    each([&](uint32_t i, float x) {
+      const float e = i < p.width ? exp2_fast((x - top) * p.c) : 0.0f;
       a += e;
       const bool here = i >= first && i < last;
       const uint64_t those = __ballot(here);
       if (here) {
         const uint32_t at = listed + uint32_t(__popcll(those & ((uint64_t(1) << lane) - 1)));
-        index[at] = i;
-        prob[at] = e;
+        column[at] = i;
+        part[at] = e;
       }
       listed += uint32_t(__popcll(those));
-    }
+    });
     a = wave_sum(a);
-    for (uint32_t k = lane; k < listed; k += 64) prob[k] /= a;
+  }
+  {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    uint16_t* place = reinterpret_cast<uint16_t*>(map);
+    bool labelled = false;  // whether an entry's column is the label's
+    for (uint32_t k = lane; k < listed; k += 64) {
+      const uint32_t i = column[k];
+      float sum = 0.0f;
+      bool leads = true;
+      for (uint32_t j = 0; j < listed; ++j) {
+        if (column[j] != i) continue;
+        if (j < k) leads = false;
+        sum += part[j];
+      }
+      sum = ka * (sum / a);
+      if (hard && i == label) {
+        labelled = true;
+        sum += kb;
+      }
+      taken[k] = sum;
+      if (leads && i - base < uint32_t(kColumns)) place[i - base] = uint16_t(k + 1);
+    }
+    if (__ballot(labelled) == 0 && hard && label >= first && label < last) {
+      if (lane == 0) {
+        column[listed] = label;
+        taken[listed] = kb;
+        if (label - base < uint32_t(kColumns)) place[label - base] = uint16_t(listed + 1);
+      }
+      ++listed;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
   }
 
   auto stream = [&](auto fn) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t at = from + u * kGradBlock + threadIdx.x;
+      const uint32_t at = from + u * 64 + lane;
       if (at >= to) continue;
+      const Vec<uint16_t, N> where = map[u * 64 + lane];
+      float g[N];
+      uint32_t any = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        g[e] = fn(float(v[u].v[e]));
+        any |= where.v[e];
+      }
+      if (any) {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (where.v[e]) g[e] -= taken[where.v[e] - 1];
+      }
       Vec<T, N> o;
 #pragma unroll
-      for (int e = 0; e < N; ++e) o.v[e] = T(fn(float(v[u].v[e])));
+      for (int e = 0; e < N; ++e) o.v[e] = T(g[e]);
       vstore_el<true, T, N>(out + head + uint64_t(at) * N, o);
     }
-    if (lone < p.width) out[lone] = T(fn(float(z[lone])));
+    if (lone < p.width) {
+      float g = fn(float(z[lone]));
+      for (uint32_t j = 0; j < listed; ++j)
+        if (column[j] == lone) {  // the first of those that name it
+          g -= taken[j];
+          break;
+        }
+      out[lone] = T(g);
+    }
   };
   auto q = [&](float x) { return exp2_fast(__builtin_fmaf(x - m, p.c, -la)); };
   auto s = [&](float x) { return exp2_fast(__builtin_fmaf(x - m, kLog2e, -lb)); };
@@ -290,31 +358,7 @@ __global__ __launch_bounds__(kGradBlock) void k_distill_grad(DistillArgs p) {
     stream([&](float x) { return kb * s(x); });
   } else {
     stream([&](float) { return 0.0f; });
-    return;
   }
-  __syncthreads();
-  if (wave != 0) return;
-  auto column = [&](uint32_t i, float taken) {
-    const float x = float(z[i]);
-    float g = 0.0f;
-    if (soft) g = ka * (q(x) - taken);
-    if (hard) g += kb * (s(x) - (i == label ? 1.0f : 0.0f));
-    out[i] = T(g);
-  };
-  bool labelled = false;  // whether an entry's column is the label's
-  for (uint32_t k = lane; k < listed; k += 64) {
-    const uint32_t i = index[k];
-    if (i == label && hard) labelled = true;
-    float taken = 0.0f;
-    bool leads = true;
-    for (uint32_t j = 0; j < listed; ++j) {
-      if (index[j] != i) continue;
-      if (j < k) leads = false;
-      taken += prob[j];
-    }
-    if (leads) column(i, taken);
-  }
-  if (hard && __ballot(labelled) == 0 && lane == 0 && label >= first && label < last) column(label, 0.0f);
 }
 
 static bool distill_args(const musapy_distill_args* a, bool grad, DistillArgs& p) {
@@ -363,9 +407,18 @@ int musapy_distill_loss_v1(const musapy_distill_args* a, hipStream_t st) {
   const bool two = p.labels.at != nullptr && a->temperature != 1.0f;
   vocab_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    if (two && a->temperature == 2.0f) k_distill_loss<T, 512, kSquare><<<p.rows, 512, 0, st>>>(p);
-    else if (two) k_distill_loss<T, 512, kTwo><<<p.rows, 512, 0, st>>>(p);
-    else k_distill_loss<T, 512, kOne><<<p.rows, 512, 0, st>>>(p);
+    auto go = [&](auto BLOCK) {
+      constexpr int kB = BLOCK.value;
+      if (two && a->temperature == 2.0f) k_distill_loss<T, kB, kSquare><<<p.rows, kB, 0, st>>>(p);
+      else if (two) k_distill_loss<T, kB, kTwo><<<p.rows, kB, 0, st>>>(p);
+      else k_distill_loss<T, kB, kOne><<<p.rows, kB, 0, st>>>(p);
+    };
+    // The fewest waves a row that fill the chip's 8192: a row takes some 7 us however short it is.  But with more than 32
+    // vectors a thread the larger workgroups are level or better.
+    const uint64_t vectors = p.width * sizeof(T) / 16;
+    if (p.rows >= 8192 && vectors <= 32 * 64) go(std::integral_constant<int, 64>{});
+    else if (p.rows >= 2048 && vectors <= 32 * 256) go(std::integral_constant<int, 256>{});
+    else go(std::integral_constant<int, 512>{});
   });
   return 0;
 }
@@ -379,14 +432,15 @@ int musapy_distill_loss_grad_v1(const musapy_distill_args* a, hipStream_t st) {
     return vocab_bad();
   vocab_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    p.segments = (p.width + kGradSegment<T> - 1) / kGradSegment<T>;
+    constexpr uint32_t kSegment = 64 * kGradVectors * 16 / sizeof(T);
+    p.segments = (p.width + kSegment - 1) / kSegment;
     const uint64_t grid = uint64_t(p.rows) * p.segments;
-    if (!grid_fits(grid, kGradBlock)) {
+    if (!grid_fits(grid, 64)) {
       p.segments = 0;
       return;
     }
-    if (a->temperature == 2.0f) k_distill_grad<T, true><<<unsigned(grid), kGradBlock, 0, st>>>(p);
-    else k_distill_grad<T, false><<<unsigned(grid), kGradBlock, 0, st>>>(p);
+    if (a->temperature == 2.0f) k_distill_grad<T, true><<<unsigned(grid), 64, grad_lds(p.entries), st>>>(p);
+    else k_distill_grad<T, false><<<unsigned(grid), 64, grad_lds(p.entries), st>>>(p);
   });
   if (p.segments == 0) return vocab_bad();
   return 0;
