@@ -31,34 +31,15 @@ struct DistillArgs {
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Sum (or, of each wave's, the maximum) over a workgroup's waves; every thread has the result.
-template <int WAVES, class F>
-__device__ inline float block_fold(float v, float* part, F&& f) {
-  const int wave = threadIdx.x / 64;
-  if (threadIdx.x % 64 == 0) part[wave] = v;
-  __syncthreads();
-  float r = part[0];
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w) r = f(r, part[w]);
-  __syncthreads();
-  return r;
-}
-
-// The teacher's entries of a row, lane by lane: their maximum (-inf where none counts), and whether any
-// counts.  An entry counts where its index is a column and its value is not -inf.
-__device__ inline float teacher_max(const DistillArgs& p, uint32_t row, int lane, bool& any) {
-  float top = -__builtin_inff();
-  bool some = false;
-  for (uint32_t k = lane; k < p.entries; k += 64) {
-    const bool in = id_at(p.index, row * p.index_pitch + k, p.width) < p.width;
-    const float v = float_at(p.teacher, p.teacher_dtype, row * p.teacher_pitch + k);
-    if (in && v != -__builtin_inff()) {
-      some = true;
-      top = fmaxf(top, v);
-    }
-  }
-  any = __ballot(some) != 0;
-  return wave_max(top);
+// A teacher's entry: its column and value, or the width where it does not count (there is none, its index is no
+// column, or its value is -inf).
+__device__ inline void teacher_entry(const DistillArgs& p, uint32_t row, uint32_t k, uint32_t& i, float& x) {
+  i = p.width;
+  x = -__builtin_inff();
+  if (!p.use_soft || k >= p.entries) return;
+  i = id_at(p.index, row * p.index_pitch + k, p.width);
+  x = float_at(p.teacher, p.teacher_dtype, row * p.teacher_pitch + k);
+  if (x == -__builtin_inff()) i = p.width;
 }
 
 // The columns of a row in front of its first address that is a multiple of 16 bytes.
@@ -71,7 +52,7 @@ __device__ inline uint32_t row_head(const T* row, uint32_t width) {
 
 // A workgroup takes a row: every thread keeps the maximum m of its logits and the sums of exp((z - m) / T) and,
 // with labels at a T other than 1, exp(z - m), rescaled when m rises; they are joined at the end.  The first
-// wave forms the teacher's part, which needs K logits and the sum only:
+// wave then forms the teacher's part, which needs K logits and the sum only:
 //   sum_k p_k (log p_k - log q_k) = B / A - log A + (m - r) / T + log sum exp((z - m) / T),
 //   e_k = exp((v_k - max v) / T),  A = sum e_k,  B = sum e_k ((v_k - max v) - (z_k - r)) / T
 // with r the highest of the entries' logits: all differences are of near numbers, so that logits far from 0 lose nothing.
@@ -81,16 +62,39 @@ template <class T, int BLOCK, int SUMS>
 __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
   constexpr int N = 16 / int(sizeof(T)), U = 4, kWaves = BLOCK / 64;
   constexpr bool TWO = SUMS != kOne;
-  __shared__ float part[kWaves];
+  __shared__ float part[kWaves][3];
   const uint32_t row = blockIdx.x;
   const int lane = threadIdx.x % 64;
   const uint32_t wave = wave_uniform(threadIdx.x / 64);
   const T* z = static_cast<const T*>(p.logits) + uint64_t(row) * p.pitch;
   const uint32_t head = row_head<T>(z, p.width), vectors = (p.width - head) / N;
-  bool soft = false;
-  const float top = p.use_soft ? teacher_max(p, row, lane, soft) : 0.0f;
+  Vec<T, N> v[U];
+  const uint32_t whole = vectors / (BLOCK * U) * (BLOCK * U);  // vectors in rounds of U for every thread
+  auto fetch = [&](uint32_t base) {
+    const T* at = z + head + (uint64_t(base) + threadIdx.x) * N;
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = vload_el<T, N, true>(at + u * BLOCK * N);
+  };
+  auto fetch_rest = [&] {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t at = whole + u * BLOCK + threadIdx.x;
+      v[u] = vload_el<T, N, true>(z + head + uint64_t(at < vectors ? at : vectors - 1) * N);
+    }
+  };
+  // the first 64 entries and the first logits, all on their way at once
+  uint32_t i0;
+  float x0;
+  teacher_entry(p, row, lane, i0, x0);
   const uint32_t label = p.labels.at ? id_at(p.labels, row, p.width) : p.width;
   const bool hard = label < p.width;
+  bool soft = __ballot(i0 < p.width) != 0;
+  for (uint32_t k0 = 64; k0 < p.entries && !soft; k0 += 64) {
+    uint32_t i;
+    float x;
+    teacher_entry(p, row, k0 + lane, i, x);
+    soft = __ballot(i < p.width) != 0;
+  }
   if (!soft && !hard) {
     if (threadIdx.x == 0) {
       p.loss[row] = 0.0f;
@@ -98,85 +102,118 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
     }
     return;
   }
-  float a = 0.0f, b = 0.0f, r = -__builtin_inff();
-  if (soft && wave == 0) {
-    auto each = [&](auto fn) {
-      for (uint32_t k = lane; k < p.entries; k += 64) {
-        const uint32_t i = id_at(p.index, row * p.index_pitch + k, p.width);
-        const float v = float_at(p.teacher, p.teacher_dtype, row * p.teacher_pitch + k);
-        if (i < p.width && v != -__builtin_inff()) fn(v - top, float(z[i]));
-      }
-    };
-    each([&](float, float x) { r = fmaxf(r, x); });
-    r = wave_max(r);
-    if (r == -__builtin_inff()) r = 0.0f;
-    each([&](float d, float x) {
-      const float e = exp2_fast(d * p.c);
-      a += e;
-      if (!(e == 0.0f)) b += e * ((d - (x - r)) * p.inv_t);
-    });
-  }
+  if (whole > 0) fetch(0);
+  else if (vectors > 0) fetch_rest();
+  float z0 = 0.0f;
+  if (wave == 0 && i0 < p.width) z0 = float(z[i0]);
 
+  // Below kNear, exponents are one multiply-add, x c - round(m c): the sums are then relative to 2^round(m c), and the rounding
+  // itself, the same for all terms, is taken off at the end.  Beyond it, where m c or x c may leave f32's range (rows and
+  // threads with nothing but -inf or the types' lowest values among them), (x - m) c.
+  constexpr float kNear = 1e30f;
   float m = -__FLT_MAX__, s = 0.0f, s1 = 0.0f;
-  auto add = [&](const float (&x)[N * U]) {
-    float high = m;
-#pragma unroll
-    for (int e = 0; e < N * U; ++e) high = fmaxf(high, x[e]);
-    s *= exp2_fast((m - high) * p.c);
-    if (TWO) s1 *= exp2_fast((m - high) * kLog2e);
+  auto change = [&](float from, float to, float c) {
+    return exp2_fast(__builtin_fabsf(to) < kNear ? from * c - to * c : (from - to) * c);
+  };
+  auto raise = [&](float high) {
+    s *= change(m, high, p.c);
+    if (TWO) s1 *= change(m, high, kLog2e);
     m = high;
+  };
+  auto one = [&](float w, float w1) {
+    s += w;
+    if (SUMS == kTwo) s1 += w1;
+    if (SUMS == kSquare) s1 = __builtin_fmaf(w, w, s1);
+  };
+  auto sum = [&](const auto& x, auto COUNT) {
+    if (__builtin_fabsf(m) < kNear) {
+      const float mc = -(m * p.c), mc1 = -(m * kLog2e);
 #pragma unroll
-    for (int e = 0; e < N * U; ++e) {
-      const float d = x[e] - m, w = exp2_fast(d * p.c);
-      s += w;
-      if (SUMS == kTwo) s1 += exp2_fast(d * kLog2e);
-      if (SUMS == kSquare) s1 = __builtin_fmaf(w, w, s1);
+      for (int e = 0; e < COUNT.value; ++e)
+        one(exp2_fast(__builtin_fmaf(x[e], p.c, mc)), SUMS == kTwo ? exp2_fast(__builtin_fmaf(x[e], kLog2e, mc1)) : 0.0f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < COUNT.value; ++e)
+        one(exp2_fast((x[e] - m) * p.c), SUMS == kTwo ? exp2_fast((x[e] - m) * kLog2e) : 0.0f);
     }
   };
-  uint32_t base = 0;
-  for (; base + BLOCK * U <= vectors; base += BLOCK * U) {
-    Vec<T, N> v[U];
+  auto add = [&](auto REST) {
     float x[N * U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = vload_el<T, N, true>(z + head + uint64_t(base + u * BLOCK + threadIdx.x) * N);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < N; ++e) x[u * N + e] = float(v[u].v[e]);
-    add(x);
-  }
-  if (base < vectors) {
-    Vec<T, N> v[U];
-    float x[N * U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t at = base + u * BLOCK + threadIdx.x;
-      v[u] = vload_el<T, N, true>(z + head + uint64_t(at < vectors ? at : vectors - 1) * N);
-    }
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        x[u * N + e] = base + u * BLOCK + threadIdx.x < vectors ? float(v[u].v[e]) : -__builtin_inff();
-    add(x);
+        x[u * N + e] = !REST.value || whole + u * BLOCK + threadIdx.x < vectors ? float(v[u].v[e]) : -__builtin_inff();
+    float high = m;
+#pragma unroll
+    for (int e = 0; e < N * U; ++e) high = fmaxf(high, x[e]);
+    raise(high);
+    sum(x, std::integral_constant<int, N * U>{});
+  };
+  for (uint32_t base = 0; base < whole; base += BLOCK * U) {
+    if (base > 0) fetch(base);
+    add(std::false_type{});
+  }
+  if (whole < vectors) {
+    if (whole > 0) fetch_rest();
+    add(std::true_type{});
   }
   if (threadIdx.x < p.width - vectors * N) {  // the columns in front of and behind the vectors
-    float x[N * U];
-#pragma unroll
-    for (int e = 0; e < N * U; ++e) x[e] = -__builtin_inff();
-    x[0] = float(z[threadIdx.x < head ? threadIdx.x : threadIdx.x + vectors * N]);
-    add(x);
+    const float x[1] = {float(z[threadIdx.x < head ? threadIdx.x : threadIdx.x + vectors * N])};
+    raise(fmaxf(m, x[0]));
+    sum(x, std::integral_constant<int, 1>{});
   }
-  const float most = block_fold<kWaves>(wave_max(m), part, [](float u, float w) { return fmaxf(u, w); });
-  auto plus = [](float u, float w) { return u + w; };
-  s = block_fold<kWaves>(wave_sum(s * exp2_fast((m - most) * p.c)), part, plus);
-  if (TWO) s1 = block_fold<kWaves>(wave_sum(s1 * exp2_fast((m - most) * kLog2e)), part, plus);
-  if (wave != 0) return;
-  a = wave_sum(a);
-  b = wave_sum(b);
+  float most = wave_max(m);
+  s = wave_sum(s * change(m, most, p.c));
+  if (TWO) s1 = wave_sum(s1 * change(m, most, kLog2e));
+  if constexpr (kWaves > 1) {
+    if (lane == 0) {
+      part[wave][0] = most;
+      part[wave][1] = s;
+      part[wave][2] = s1;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    m = lane < kWaves ? part[lane][0] : -__FLT_MAX__;
+    most = wave_max(m);
+    s = wave_sum(lane < kWaves ? part[lane][1] * change(m, most, p.c) : 0.0f);
+    if (TWO) s1 = wave_sum(lane < kWaves ? part[lane][2] * change(m, most, kLog2e) : 0.0f);
+  }
+  float a = 0.0f, b = 0.0f, r = -__builtin_inff();
+  if (soft) {
+    auto each = [&](auto fn) {
+      for (uint32_t k0 = 0; k0 < p.entries; k0 += 64) {
+        uint32_t i = i0;
+        float x = x0, y = z0;
+        if (k0 > 0) {
+          teacher_entry(p, row, k0 + lane, i, x);
+          if (i < p.width) y = float(z[i]);
+        }
+        if (i < p.width) fn(x, y);
+      }
+    };
+    float top = -__builtin_inff();
+    each([&](float x, float y) {
+      top = fmaxf(top, x);
+      r = fmaxf(r, y);
+    });
+    top = wave_max(top);
+    r = wave_max(r);
+    if (r == -__builtin_inff()) r = 0.0f;
+    each([&](float x, float y) {
+      const float d = x - top, e = exp2_fast(d * p.c);
+      a += e;
+      if (!(e == 0.0f)) b += e * ((d - (y - r)) * p.inv_t);
+    });
+    a = wave_sum(a);
+    b = wave_sum(b);
+  }
   if (lane != 0) return;
-  const float ls = kLn2 * __builtin_amdgcn_logf(s);
-  const float ls1 = TWO ? kLn2 * __builtin_amdgcn_logf(s1) : ls;
+  auto log_sum = [&](float sum, float c) {
+    const float off = __builtin_fabsf(most) < kNear ? __builtin_fmaf(most, c, -(most * c)) : 0.0f;
+    return kLn2 * (__builtin_amdgcn_logf(sum) - off);
+  };
+  const float ls = log_sum(s, p.c), ls1 = TWO ? log_sum(s1, kLog2e) : ls;
   float loss = 0.0f;
   if (soft) loss = p.soft * (b / a - kLn2 * __builtin_amdgcn_logf(a) + (most - r) * p.inv_t + ls);
   if (hard) loss += p.hard * ((most - float(z[label])) + ls1);
@@ -218,16 +255,9 @@ __global__ __launch_bounds__(64) void k_distill_grad(DistillArgs p) {
   uint32_t lone = lane < before ? lane : head + vectors * N + (lane - before);
   if (lane >= before && !ends) lone = p.width;
   // the first 64 entries, then the logits: all on their way at once
-  auto entry = [&](uint32_t k, uint32_t& i, float& x) {
-    i = p.width;
-    x = -__builtin_inff();
-    if (!p.use_soft || k >= p.entries) return;
-    i = id_at(p.index, row * p.index_pitch + k, p.width);
-    x = float_at(p.teacher, p.teacher_dtype, row * p.teacher_pitch + k);
-  };
   uint32_t i0;
   float x0;
-  entry(lane, i0, x0);
+  teacher_entry(p, row, lane, i0, x0);
   const uint32_t label = p.labels.at ? id_at(p.labels, row, p.width) : p.width;
   const float dl = p.dloss[int64_t(row) * p.dloss_stride];
   const float m = p.sums[uint64_t(row) * 3];
@@ -246,8 +276,8 @@ __global__ __launch_bounds__(64) void k_distill_grad(DistillArgs p) {
     for (uint32_t k0 = 0; k0 < p.entries; k0 += 64) {
       uint32_t i = i0;
       float x = x0;
-      if (k0 > 0) entry(k0 + lane, i, x);
-      fn(x == -__builtin_inff() ? p.width : i, x);
+      if (k0 > 0) teacher_entry(p, row, k0 + lane, i, x);
+      fn(i, x);
     }
   };
   float top = -__builtin_inff(), a = 0.0f;
