@@ -3,7 +3,6 @@
 
 namespace mpy {
 
-constexpr int kAdjustBlock = 512;
 constexpr int kBiasMost = 1024;
 
 // A number for all sequences, or one for each.
@@ -32,129 +31,229 @@ struct AdjustArgs {
   const void* allowed;     // bits: 32-bit words; else bytes
   uint64_t allowed_pitch;
   int bits;
-  uint32_t tile, tiles;    // columns of a workgroup, workgroups of a row
+  uint32_t tiles;          // workgroups of a row
 };
 
-// A workgroup takes a tile of a row's columns.  It counts the tokens of the row's history that fall into the tile, in
-// LDS, then reads the tile once and writes it once.  Biased tokens, few, are formed again and stored over the
-// first values behind a barrier; a token that several entries name gets the sum of their biases from the first.
-template <class T, class O, bool HISTORY>
-__global__ __launch_bounds__(kAdjustBlock) void k_adjust(AdjustArgs p) {
-  constexpr int N = 8;
-  extern __shared__ uint32_t count[];
+// Counts of a history's tokens that fall into a tile, in LDS: 16 bits each where no count can pass them.
+template <class C>
+__device__ inline void count_one(uint32_t* count, uint32_t at) {
+  if constexpr (sizeof(C) == 2) atomicAdd(&count[at / 2], at % 2 ? 0x10000u : 1u);
+  else atomicAdd(&count[at], 1u);
+}
+
+// A workgroup takes a tile of a row's columns, U vectors of 16 bytes of the result to a thread.  The tile, its mask, the first biased
+// columns and the first kPast vectors a thread of the row's history are on their way at once, whatever the history's
+// length turns out to be; the tokens that fall into the tile are counted in LDS, and the tile is read once and written
+// once.
+constexpr int kPast = 4;
+
+template <class T, class O, class C, bool HISTORY, int BLOCK, int TILE>
+__global__ __launch_bounds__(BLOCK) void k_adjust(AdjustArgs p) {
+  constexpr int N = 16 / int(sizeof(O)), U = TILE / BLOCK / N;
+  static_assert(U > 0 && U * BLOCK * N == TILE, "whole vectors");
+  typedef uint32_t Words __attribute__((ext_vector_type(4)));
+  typedef Words AnyWords __attribute__((aligned(4)));
+  __shared__ Vec<C, N> count[HISTORY ? TILE / N : 1];
   const uint32_t row = blockIdx.x / p.tiles;
-  const uint32_t first = (blockIdx.x - row * p.tiles) * p.tile;
-  const uint32_t last = p.width - first < p.tile ? p.width : first + p.tile;
-  const T* z = static_cast<const T*>(p.logits) + uint64_t(row) * p.pitch;
-  O* out = static_cast<O*>(p.out) + uint64_t(row) * p.width;
+  // Rows begin with different tiles: the common tokens' tile, which counts most, would else fall to one XCD of the eight
+  // wherever the tiles of a row are a multiple of them.
+  const uint32_t turn = blockIdx.x - row * p.tiles + row % p.tiles;
+  const uint32_t first = (turn < p.tiles ? turn : turn - p.tiles) * TILE;
+  const uint32_t columns = p.width - first < TILE ? p.width - first : TILE;
+  const T* z = static_cast<const T*>(p.logits) + uint64_t(row) * p.pitch + first;
+  O* out = static_cast<O*>(p.out) + uint64_t(row) * p.width + first;
+  const uint32_t vectors = columns / N;
+
+  // the history as 16-byte vectors of 4 or 2 tokens, and the tokens behind the last of them
+  const uint32_t per = p.history.wide ? 2 : 4;
+  const uint32_t past = HISTORY ? p.length / per : 0;
+  const char* ids = static_cast<const char*>(p.history.at) + row * p.history_pitch * (p.history.wide ? 8 : 4);
+  Words h[HISTORY ? kPast : 1];
+  auto fetch = [&](uint32_t base) {
+#pragma unroll
+    for (int u = 0; u < kPast; ++u) {
+      const uint32_t q = base + u * BLOCK + threadIdx.x;
+      h[u] = *reinterpret_cast<const AnyWords*>(ids + uint64_t(q < past ? q : past - 1) * 16);
+    }
+  };
   float rep = 1.0f, pres = 0.0f, freq = 0.0f;
+  RawId raw_length{};
   if constexpr (HISTORY) {
-    for (uint32_t i = threadIdx.x * 4; i < p.tile; i += kAdjustBlock * 4)
-      *reinterpret_cast<uint4*>(count + i) = uint4{0, 0, 0, 0};
+    if (past > 0) fetch(0);
+    if (p.lengths.at) raw_length = id_load(p.lengths, row);
     rep = per_row(p.repetition, row);
     pres = per_row(p.presence, row);
     freq = per_row(p.frequency, row);
-    uint32_t length = p.length;
-    if (p.lengths.at) {  // below 0: none; past the row's end: all of it
-      const int64_t n = p.lengths.wide ? static_cast<const int64_t*>(p.lengths.at)[row]
-                                       : static_cast<const int32_t*>(p.lengths.at)[row];
-      length = n < 0 ? 0 : n < int64_t(p.length) ? uint32_t(n) : p.length;
-    }
-    __syncthreads();
-    const uint64_t start = row * p.history_pitch;
-#pragma unroll 4
-    for (uint32_t i = threadIdx.x; i < length; i += kAdjustBlock) {
-      const uint32_t at = id_at(p.history, start + i, p.width) - first;
-      if (at < last - first) atomicAdd(&count[at], 1u);
-    }
-    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u) count[u * BLOCK + threadIdx.x] = Vec<C, N>{};
   }
   const uint8_t* bytes = nullptr;
   const uint32_t* words = nullptr;
   if (p.allowed) {
     if (p.bits) words = static_cast<const uint32_t*>(p.allowed) + uint64_t(row) * p.allowed_pitch;
-    else bytes = static_cast<const uint8_t*>(p.allowed) + uint64_t(row) * p.allowed_pitch;
+    else bytes = static_cast<const uint8_t*>(p.allowed) + uint64_t(row) * p.allowed_pitch + first;
+  }
+  Vec<T, N> v[U];
+  uint32_t mask[U][N / 4];  // bytes, or in the first word bits
+  typedef uint32_t AnyWord __attribute__((aligned(1)));
+  const auto clamped = [&](int u) {
+    const uint32_t q = u * BLOCK + threadIdx.x;
+    return q < vectors ? q : vectors - 1;
+  };
+  if (vectors > 0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = vload_el<T, N, true>(z + uint64_t(clamped(u)) * N);
+    if (words) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) mask[u][0] = words[(first + clamped(u) * N) / 32];
+    } else if (bytes) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int w = 0; w < N / 4; ++w) mask[u][w] = reinterpret_cast<const AnyWord*>(bytes + clamped(u) * N)[w];
+    }
   }
   const uint64_t bias_row = uint64_t(row) * p.bias_pitch;
-  const bool dense = p.bias && p.entries == 0;
-
-  auto seen = [&](float x, uint32_t c) {
-    const float y = x > 0.0f ? x / rep : x * rep;
-    return c ? y - (freq * float(c) + pres) : x;
+  // the first 64 biased columns, a lane each; one that is no column of the tile is past it
+  const uint32_t lane = threadIdx.x % 64;
+  RawId raw_index{};
+  uint32_t raw_bias = 0;
+  auto entry = [&](uint32_t k) {
+    const uint32_t at = k < p.entries ? k : p.entries - 1;
+    raw_index = id_load(p.bias_index, row * p.index_pitch + at);
+    raw_bias = float_load(p.bias, p.bias_dtype, bias_row + at);
   };
-  auto one = [&](uint32_t i, float bias) {
-    float x = float(z[i]);
-    if constexpr (HISTORY) x = seen(x, count[i - first]);
-    x += bias;
-    const bool ok = words ? (words[i / 32] >> (i % 32)) & 1 : bytes ? bytes[i] != 0 : true;
-    out[i] = O(ok ? x : -__builtin_inff());
-  };
-  const uint32_t vectors = (last - first) / N;
-  for (uint32_t q = threadIdx.x; q < vectors; q += kAdjustBlock) {
-    const uint32_t i = first + q * N;
-    const Vec<T, N> v = vload_el<T, N, true>(z + i);
-    uint32_t ok = 0xff;
-    if (words) {
-      ok = words[i / 32] >> (i % 32);
-    } else if (bytes) {
-      const Vec<uint8_t, N> m = vload_el<uint8_t, N, true>(bytes + i);
-      ok = 0;
-#pragma unroll
-      for (int e = 0; e < N; ++e) ok |= (m.v[e] != 0 ? 1u : 0u) << e;
+  if (p.entries > 0) entry(lane);
+  if constexpr (HISTORY) {
+    uint32_t length = p.length;
+    if (p.lengths.at) {  // below 0: none; past the row's end: all of it
+      const bool below = (p.lengths.wide ? raw_length.high : raw_length.low) >> 31;
+      length = below ? 0 : id_of(raw_length, p.length);
     }
-    float x[N];
+    lds_barrier();
+    uint32_t* counts = reinterpret_cast<uint32_t*>(count);
+    auto one = [&](uint32_t low, uint32_t high, uint32_t at) {  // a token that is no column of the tile, by all its bits, does not count
+      const uint32_t i = low - first;
+      if (i < columns && high == 0 && at < length) count_one<C>(counts, i);
+    };
+    for (uint32_t base = 0; base < past && base * per < length; base += BLOCK * kPast) {
+      if (base > 0) fetch(base);
 #pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = float(v.v[e]);
-    if constexpr (HISTORY) {
-      const Vec<uint32_t, N> c = *reinterpret_cast<const Vec<uint32_t, N>*>(count + q * N);
-      uint32_t any = 0;
+      for (int u = 0; u < kPast; ++u) {
+        const uint32_t q = base + u * BLOCK + threadIdx.x;
+        if (q >= past) continue;
+        if (p.history.wide) {
+          one(h[u].x, h[u].y, q * 2);
+          one(h[u].z, h[u].w, q * 2 + 1);
+        } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e) any |= c.v[e];
-      if (any) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) x[e] = seen(x[e], c.v[e]);
+          for (int e = 0; e < 4; ++e) one(h[u][e], 0, q * 4 + e);
+        }
       }
     }
-    if (dense) {
+    const uint32_t rest = past * per + threadIdx.x;
+    if (threadIdx.x < per && rest < length) {
+      const uint32_t i = id_at(p.history, row * p.history_pitch + rest, p.width) - first;
+      if (i < columns) count_one<C>(counts, i);
+    }
+  }
+  if constexpr (HISTORY) lds_barrier();
+  const bool dense = p.bias && p.entries == 0;
+  auto seen = [&](float x, uint32_t c) { return (x > 0.0f ? x / rep : x * rep) - (freq * float(c) + pres); };
+  float x[U][N];
 #pragma unroll
-      for (int e = 0; e < N; ++e) x[e] += float_at(p.bias, p.bias_dtype, bias_row + i + e);
+  for (int u = 0; u < U; ++u) {
+    const uint32_t q = u * BLOCK + threadIdx.x, i = q * N;
+    if (q >= vectors) continue;
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[u][e] = float(v[u].v[e]);
+    if constexpr (HISTORY) {
+      const Vec<C, N> c = count[q];
+#pragma unroll
+      for (int e = 0; e < N; ++e)  // (a branch each: few columns of a wave were seen, and the division is long)
+        if (c.v[e]) x[u][e] = seen(x[u][e], c.v[e]);
+    }
+    if (dense) {
+      if (p.bias_dtype == MUSAPY_DT_F32) {
+        const Vec<float, N> b = vload_el<float, N, false>(static_cast<const float*>(p.bias) + bias_row + first + i);
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[u][e] += b.v[e];
+      } else {
+        const Vec<T, N> b = vload_el<T, N, false>(static_cast<const T*>(p.bias) + bias_row + first + i);
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[u][e] += float(b.v[e]);
+      }
+    }
+  }
+  const uint32_t behind = vectors * N + threadIdx.x;  // a column behind the vectors
+  float y = behind < columns ? float(z[behind]) : 0.0f;
+  if constexpr (HISTORY) {
+    const uint32_t c = behind < columns ? reinterpret_cast<const C*>(count)[behind] : 0;
+    if (c) y = seen(y, c);
+  }
+  if (dense && behind < columns) y += float_at(p.bias, p.bias_dtype, bias_row + first + behind);
+  // Each wave adds the biases of its own columns, in the entries' order.
+  for (uint32_t k0 = 0; k0 < p.entries; k0 += 64) {
+    if (k0 > 0) entry(k0 + lane);
+    const uint32_t bi = id_of(raw_index, p.width) - first, q = bi / N;
+    const float bv = float_of(raw_bias, p.bias_dtype);
+    const bool mine = k0 + lane < p.entries && bi < columns && (q >= vectors || q % BLOCK / 64 == threadIdx.x / 64);
+    for (uint64_t those = __ballot(mine); those; those &= those - 1) {
+      const int from = __builtin_ctzll(those);
+      const uint32_t i = uint32_t(__builtin_amdgcn_readlane(int(bi), from));
+      const float b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, bv), from));
+      if (i == behind) y += b;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (i == (u * BLOCK + threadIdx.x) * N + e) x[u][e] += b;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t q = u * BLOCK + threadIdx.x, i = q * N;
+    if (q >= vectors) continue;
+    uint32_t ok = 0xff;
+    if (words) {
+      ok = mask[u][0] >> (i % 32);
+    } else if (bytes) {
+      ok = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e) ok |= ((mask[u][e / 4] >> (8 * (e % 4))) & 0xff ? 1u : 0u) << e;
     }
     Vec<O, N> o;
 #pragma unroll
-    for (int e = 0; e < N; ++e) o.v[e] = O((ok >> e) & 1 ? x[e] : -__builtin_inff());
-    vstore_el<false, O, N>(out + i, o);
+    for (int e = 0; e < N; ++e) o.v[e] = O((ok >> e) & 1 ? x[u][e] : -__builtin_inff());
+    vstore_el<true, O, N>(out + i, o);
   }
-  {
-    const uint32_t i = first + vectors * N + threadIdx.x;
-    if (i < last) one(i, dense ? float_at(p.bias, p.bias_dtype, bias_row + i) : 0.0f);
-  }
-  if (p.entries == 0) return;
-  __shared__ uint32_t index[kBiasMost];
-  __shared__ float value[kBiasMost];
-  for (uint32_t k = threadIdx.x; k < p.entries; k += kAdjustBlock) {
-    index[k] = id_at(p.bias_index, row * p.index_pitch + k, p.width);
-    value[k] = float_at(p.bias, p.bias_dtype, bias_row + k);
-  }
-  __syncthreads();
-  for (uint32_t k = threadIdx.x; k < p.entries; k += kAdjustBlock) {
-    const uint32_t i = index[k];
-    if (i < first || i >= last) continue;
-    float sum = 0.0f;
-    bool leads = true;
-    for (uint32_t j = 0; j < p.entries; ++j) {
-      if (index[j] != i) continue;
-      if (j < k) leads = false;
-      sum += value[j];
-    }
-    if (leads) one(i, sum);
-  }
+  if (behind >= columns) return;
+  const bool ok = words ? (words[(first + behind) / 32] >> ((first + behind) % 32)) & 1 : bytes ? bytes[behind] != 0 : true;
+  out[behind] = O(ok ? y : -__builtin_inff());
 }
 
+// The tile: 2048 columns without a history ((256, 131072) bf16 with packed masks and biases into f32 34.6 us, 35.1 with 8192); with one, which
+// every tile reads, 8192 (42.4, with 2048 54.6, for 4096 tokens each), and 4096 where that leaves the chip's 256 CUs few
+// ((4, 32768) f32 4.2 us, with 8192 4.9; (32, 50001) with 30000 tokens 13.8, with 2048 18.1).
 template <class T, class O>
-void launch_adjust(const AdjustArgs& p, bool history, hipStream_t st) {
-  const unsigned grid = p.rows * p.tiles;
-  if (history) k_adjust<T, O, true><<<grid, kAdjustBlock, p.tile * 4, st>>>(p);
-  else k_adjust<T, O, false><<<grid, kAdjustBlock, 0, st>>>(p);
+int launch_adjust(AdjustArgs& p, bool history, hipStream_t st) {
+  auto go = [&](auto HISTORY, auto BLOCK, auto TILE) {
+    constexpr uint32_t kTile = TILE.value;
+    p.tiles = (p.width + kTile - 1) / kTile;
+    const uint64_t grid = uint64_t(p.rows) * p.tiles;
+    if (!grid_fits(grid, BLOCK.value)) return vocab_bad();
+    if (p.length < 65536) k_adjust<T, O, uint16_t, HISTORY.value, BLOCK.value, kTile><<<unsigned(grid), BLOCK.value, 0, st>>>(p);
+    else if constexpr (HISTORY.value) k_adjust<T, O, uint32_t, true, BLOCK.value, kTile><<<unsigned(grid), BLOCK.value, 0, st>>>(p);
+    return 0;
+  };
+  using Few = std::integral_constant<int, 256>;
+  using Many = std::integral_constant<int, 512>;
+  if (!history) {
+    p.length = 0;
+    return go(std::false_type{}, Few{}, std::integral_constant<int, 2048>{});
+  }
+  if (p.rows * ((uint64_t(p.width) + 8191) / 8192) >= 512) return go(std::true_type{}, Many{}, std::integral_constant<int, 8192>{});
+  return go(std::true_type{}, Many{}, std::integral_constant<int, 4096>{});
 }
 
 }  // namespace mpy
@@ -194,15 +293,11 @@ extern "C" int musapy_adjust_logits_v1(const musapy_adjust_logits_args* a, hipSt
   p.allowed = a->allowed;
   p.allowed_pitch = a->allowed_pitch;
   p.bits = a->allowed_kind == MUSAPY_ALLOWED_BITS;
-  // the widest tile of up to 8192 columns that leaves the chip full: every tile reads the whole history
-  p.tile = 8192;
-  while (p.tile > 2048 && uint64_t(p.rows) * ((p.width + p.tile - 1) / p.tile) < 1024) p.tile /= 2;
-  p.tiles = (p.width + p.tile - 1) / p.tile;
-  if (!grid_fits(uint64_t(p.rows) * p.tiles, kAdjustBlock)) return vocab_bad();
+  int rc = 0;
   vocab_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    if (a->out_dtype == a->dtype) launch_adjust<T, T>(p, history, st);
-    else launch_adjust<T, float>(p, history, st);
+    if (a->out_dtype == a->dtype) rc = launch_adjust<T, T>(p, history, st);
+    else rc = launch_adjust<T, float>(p, history, st);
   });
-  return 0;
+  return rc;
 }

@@ -31,15 +31,23 @@ struct DistillArgs {
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// A teacher's entry: its column and value, or the width where it does not count (there is none, its index is no
-// column, or its value is -inf).
+// A teacher's entry as it is loaded (any one where there is none of that number), and its column and value: the width where
+// it does not count (there is none, its index is no column, or its value is -inf).
+struct RawEntry {
+  RawId index;
+  uint32_t value;
+};
+__device__ inline RawEntry entry_load(const DistillArgs& p, uint32_t row, uint32_t k) {
+  if (!p.use_soft) return RawEntry{RawId{0, 1}, 0};
+  const uint32_t at = k < p.entries ? k : p.entries - 1;
+  return RawEntry{id_load(p.index, row * p.index_pitch + at), float_load(p.teacher, p.teacher_dtype, row * p.teacher_pitch + at)};
+}
+__device__ inline void entry_of(const DistillArgs& p, const RawEntry& r, uint32_t k, uint32_t& i, float& x) {
+  x = float_of(r.value, p.teacher_dtype);
+  i = k < p.entries && x != -__builtin_inff() ? id_of(r.index, p.width) : p.width;
+}
 __device__ inline void teacher_entry(const DistillArgs& p, uint32_t row, uint32_t k, uint32_t& i, float& x) {
-  i = p.width;
-  x = -__builtin_inff();
-  if (!p.use_soft || k >= p.entries) return;
-  i = id_at(p.index, row * p.index_pitch + k, p.width);
-  x = float_at(p.teacher, p.teacher_dtype, row * p.teacher_pitch + k);
-  if (x == -__builtin_inff()) i = p.width;
+  entry_of(p, entry_load(p, row, k), k, i, x);
 }
 
 // The columns of a row in front of its first address that is a multiple of 16 bytes.
@@ -83,10 +91,14 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
     }
   };
   // the first 64 entries and the first logits, all on their way at once
+  const RawEntry e0 = entry_load(p, row, lane);
+  const RawId raw_label = p.labels.at ? id_load(p.labels, row) : RawId{0, 1};
+  if (whole > 0) fetch(0);
+  else if (vectors > 0) fetch_rest();
   uint32_t i0;
   float x0;
-  teacher_entry(p, row, lane, i0, x0);
-  const uint32_t label = p.labels.at ? id_at(p.labels, row, p.width) : p.width;
+  entry_of(p, e0, lane, i0, x0);
+  const uint32_t label = id_of(raw_label, p.width);
   const bool hard = label < p.width;
   bool soft = __ballot(i0 < p.width) != 0;
   for (uint32_t k0 = 64; k0 < p.entries && !soft; k0 += 64) {
@@ -102,8 +114,6 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
     }
     return;
   }
-  if (whole > 0) fetch(0);
-  else if (vectors > 0) fetch_rest();
   float z0 = 0.0f;
   if (wave == 0 && i0 < p.width) z0 = float(z[i0]);
 
@@ -255,13 +265,11 @@ __global__ __launch_bounds__(64) void k_distill_grad(DistillArgs p) {
   uint32_t lone = lane < before ? lane : head + vectors * N + (lane - before);
   if (lane >= before && !ends) lone = p.width;
   // the first 64 entries, then the logits: all on their way at once
-  uint32_t i0;
-  float x0;
-  teacher_entry(p, row, lane, i0, x0);
-  const uint32_t label = p.labels.at ? id_at(p.labels, row, p.width) : p.width;
+  const RawEntry e0 = entry_load(p, row, lane);
+  const RawId raw_label = p.labels.at ? id_load(p.labels, row) : RawId{0, 1};
   const float dl = p.dloss[int64_t(row) * p.dloss_stride];
   const float m = p.sums[uint64_t(row) * 3];
-  const float la = p.sums[uint64_t(row) * 3 + 1] * kLog2e, lb = p.sums[uint64_t(row) * 3 + 2] * kLog2e;
+  const float ls = p.sums[uint64_t(row) * 3 + 1], ls1 = p.sums[uint64_t(row) * 3 + 2];
   Vec<T, N> v[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -270,8 +278,12 @@ __global__ __launch_bounds__(64) void k_distill_grad(DistillArgs p) {
     map[u * 64 + lane] = Vec<uint16_t, N>{};
   }
 
+  uint32_t i0;
+  float x0;
+  entry_of(p, e0, lane, i0, x0);
+  const uint32_t label = id_of(raw_label, p.width);
   const bool hard = label < p.width;
-  const float ka = dl * p.soft, kb = dl * p.hard;
+  const float ka = dl * p.soft, kb = dl * p.hard, la = ls * kLog2e, lb = ls1 * kLog2e;
   auto each = [&](auto fn) {  // an entry that counts to a lane, or the width in its place
     for (uint32_t k0 = 0; k0 < p.entries; k0 += 64) {
       uint32_t i = i0;

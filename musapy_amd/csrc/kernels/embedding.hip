@@ -28,6 +28,7 @@ constexpr int kEmbedGroups = 4;
 template <class T, class O, int N, bool UNIT, bool NT>
 __global__ __launch_bounds__(kEmbedBlock) void k_embedding(EmbedArgs p) {
   const uint64_t first = uint64_t(blockIdx.x) * (kEmbedBlock * kEmbedGroups) + threadIdx.x;
+  RawId raw[kEmbedGroups];
   uint32_t token[kEmbedGroups], row[kEmbedGroups], col[kEmbedGroups];
 #pragma unroll
   for (int i = 0; i < kEmbedGroups; ++i) {
@@ -36,11 +37,12 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embedding(EmbedArgs p) {
     row[i] = fd_div(p.gdiv, at);
     const uint32_t c = (at - row[i] * p.groups) * N;
     col[i] = c + N <= p.width ? c : p.width - N;
-    token[i] = id_at(p.ids, row[i], p.rows);
+    raw[i] = id_load(p.ids, row[i]);
   }
   Vec<T, N> v[kEmbedGroups];
 #pragma unroll
   for (int i = 0; i < kEmbedGroups; ++i) {
+    token[i] = id_of(raw[i], p.rows);
     const uint32_t t = token[i] < p.rows ? token[i] : 0;  // the first row in the place of none
     const T* at = static_cast<const T*>(p.table) + int64_t(t) * p.rs + int64_t(col[i]) * p.cs;
     if constexpr (UNIT) {
@@ -212,8 +214,13 @@ constexpr int kSortWaves = 8, kSortBlock = kSortWaves * 64, kSortRounds = 4, kSo
 constexpr uint32_t kSortTiles = 256;
 
 template <bool FIRST>
-__device__ inline uint32_t order_key(const OrderArgs& p, uint32_t i) {
-  return FIRST ? id_at(p.ids, i, p.rows) : p.keys_in[i];
+__device__ inline RawId order_load(const OrderArgs& p, uint32_t i) {
+  if constexpr (FIRST) return id_load(p.ids, i);
+  else return RawId{p.keys_in[i], 0};
+}
+template <bool FIRST>
+__device__ inline uint32_t order_key(const OrderArgs& p, const RawId& r) {
+  return FIRST ? id_of(r, p.rows) : r.low;
 }
 
 template <bool FIRST>
@@ -225,7 +232,7 @@ __global__ __launch_bounds__(kBlockTokens) void k_embed_digits(OrderArgs p) {
   const uint32_t first = blockIdx.x * p.tile;
   const uint32_t last = p.n - first < p.tile ? p.n : first + p.tile;
   for (uint32_t i = first + threadIdx.x; i < last; i += kBlockTokens)
-    atomicAdd(&count[(order_key<FIRST>(p, i) >> p.shift) & ((1u << p.bits) - 1)], 1u);
+    atomicAdd(&count[(order_key<FIRST>(p, order_load<FIRST>(p, i)) >> p.shift) & ((1u << p.bits) - 1)], 1u);
   __syncthreads();
   for (int d = threadIdx.x; d < kDigits; d += kBlockTokens) p.hist[blockIdx.x * kDigits + d] = count[d];
 }
@@ -267,13 +274,16 @@ __global__ __launch_bounds__(kSortBlock) void k_embed_place(OrderArgs p) {
 #pragma unroll
     for (int w = 0; w < kSortWaves; ++w) at[w][threadIdx.x] = 0;
     __syncthreads();
+    RawId raw[kSortRounds];
     uint32_t key[kSortRounds], place[kSortRounds], rank[kSortRounds];
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
-      const uint32_t i = s + wave * (kSortRounds * 64) + uint32_t(r) * 64 + lane;
-      key[r] = i < last ? order_key<FIRST>(p, i) : ~0u;
-      place[r] = FIRST || i >= last ? i : p.pos_in[i];
+      const uint32_t i = s + wave * (kSortRounds * 64) + uint32_t(r) * 64 + lane, at = i < last ? i : last - 1;
+      raw[r] = order_load<FIRST>(p, at);
+      place[r] = FIRST ? at : p.pos_in[at];
     }
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) key[r] = order_key<FIRST>(p, raw[r]);
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
       const bool there = s + wave * (kSortRounds * 64) + uint32_t(r) * 64 + lane < last;

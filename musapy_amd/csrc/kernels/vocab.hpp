@@ -13,15 +13,25 @@ struct Ids {
   int wide;
 };
 
-// The number, or `none` where it is outside [0, none).
-__device__ inline uint32_t id_at(const Ids& ids, uint64_t i, uint32_t none) {
+// A number as it was loaded, and the number: `none` where it is outside [0, none).  What is loaded under a branch and used
+// there is waited for there, with every load in front of it; so loads that are to be under way together come first, their uses after.
+struct RawId {
+  uint32_t low, high;
+};
+__device__ inline RawId id_load(const Ids& ids, uint64_t i) {
+  RawId r;
   if (ids.wide) {
-    const uint64_t v = static_cast<const uint64_t*>(ids.at)[i];
-    return v < none ? uint32_t(v) : none;
+    const uint2 v = static_cast<const uint2*>(ids.at)[i];
+    r.low = v.x;
+    r.high = v.y;
+  } else {
+    r.low = static_cast<const uint32_t*>(ids.at)[i];
+    r.high = 0;
   }
-  const uint32_t v = static_cast<const uint32_t*>(ids.at)[i];
-  return v < none ? v : none;
+  return r;
 }
+__device__ inline uint32_t id_of(const RawId& r, uint32_t none) { return r.high == 0 && r.low < none ? r.low : none; }
+__device__ inline uint32_t id_at(const Ids& ids, uint64_t i, uint32_t none) { return id_of(id_load(ids, i), none); }
 
 inline bool vocab_float(int dtype) {
   return dtype == MUSAPY_DT_F32 || dtype == MUSAPY_DT_BF16 || dtype == MUSAPY_DT_F16;
@@ -45,11 +55,19 @@ inline void vocab_type(int dtype, F&& fn) {
   else fn(f16(0));
 }
 
-__device__ inline float float_at(const void* at, int dtype, uint64_t i) {
-  if (dtype == MUSAPY_DT_F32) return static_cast<const float*>(at)[i];
-  if (dtype == MUSAPY_DT_BF16) return float(static_cast<const bf16*>(at)[i]);
-  return float(static_cast<const f16*>(at)[i]);
+// The same for elements of a runtime dtype.
+__device__ inline uint32_t float_load(const void* at, int dtype, uint64_t i) {
+  uint32_t bits;
+  if (dtype == MUSAPY_DT_F32) bits = static_cast<const uint32_t*>(at)[i];
+  else bits = static_cast<const uint16_t*>(at)[i];
+  return bits;
 }
+__device__ inline float float_of(uint32_t bits, int dtype) {
+  if (dtype == MUSAPY_DT_F32) return __builtin_bit_cast(float, bits);
+  if (dtype == MUSAPY_DT_BF16) return __builtin_bit_cast(float, bits << 16);
+  return float(__builtin_bit_cast(f16, uint16_t(bits)));
+}
+__device__ inline float float_at(const void* at, int dtype, uint64_t i) { return float_of(float_load(at, dtype, i), dtype); }
 
 __device__ inline uint32_t wave_uniform(uint32_t v) { return uint32_t(__builtin_amdgcn_readfirstlane(int(v))); }
 
