@@ -243,7 +243,7 @@ constexpr int kGradVectors = 4;
 constexpr unsigned grad_lds(uint32_t entries) { return (entries + 1) * 12; }
 
 template <class T, bool SQUARE>
-__global__ __launch_bounds__(64) void k_distill_grad(DistillArgs p) {
+__global__ __launch_bounds__(64, 8) void k_distill_grad(DistillArgs p) {
   constexpr int N = 16 / int(sizeof(T)), U = kGradVectors, kColumns = 64 * U * N;
   __shared__ Vec<uint16_t, N> map[64 * U];  // of the vectors' columns: 0, or 1 + the place in the list
   extern __shared__ uint32_t column[];      // [entries + 1] the list: columns, the entries' exponentials, what is taken off
@@ -253,34 +253,38 @@ __global__ __launch_bounds__(64) void k_distill_grad(DistillArgs p) {
   const T* z = static_cast<const T*>(p.logits) + uint64_t(row) * p.pitch;
   T* out = static_cast<T*>(p.grad) + uint64_t(row) * p.width;
 
-  // Vectors lie where the results' addresses are multiples of 16 bytes (and the logits' too, where both rows begin
-  // alike); the first segment has the columns in front of them, the last one those behind.
+  // Vectors lie where the results' addresses are multiples of 16 bytes, segments where they are multiples of 4 KB (and the
+  // logits' too, where both rows begin alike): no line is shared with another wave, but at a row's ends.  The first segment has
+  // the columns in front of the vectors, the last one those behind.
   const uint32_t head = row_head<T>(out, p.width), vectors = (p.width - head) / N;
-  const uint32_t start = seg * (64 * U), from = start < vectors ? start : vectors;
-  const uint32_t to = vectors - from < 64 * U ? vectors : from + 64 * U;
-  const bool ends = seg == p.segments - 1;
-  const uint32_t base = head + from * N;  // the vectors' first column
-  const uint32_t first = seg == 0 ? 0 : base, last = ends ? p.width : head + to * N;
+  const int32_t start = int32_t(seg * (64 * U)) - int32_t(reinterpret_cast<uintptr_t>(out + head) / 16 % (64 * U));
+  if (seg > 0 && start >= int32_t(vectors)) return;
+  const uint32_t from = start < 0 ? 0 : uint32_t(start);
+  const uint32_t to = start + 64 * U < int32_t(vectors) ? uint32_t(start + 64 * U) : vectors;
+  const uint32_t base = head + uint32_t(start) * N;  // the first vector's column (below 0: past all columns)
+  const uint32_t first = seg == 0 ? 0 : base, last = to == vectors ? p.width : head + to * N;
   const uint32_t before = seg == 0 ? head : 0;
   uint32_t lone = lane < before ? lane : head + vectors * N + (lane - before);
-  if (lane >= before && !ends) lone = p.width;
-  // the first 64 entries, then the logits: all on their way at once
+  if (lane >= before && to < vectors) lone = p.width;
+  auto vector = [&](int u) { return uint32_t(start + u * 64) + lane; };
+  // The first 64 entries, which are waited for before the logits are asked for: with all loads under way at once (4096, 131072) bf16
+  // took 350 us, so 342.
   const RawEntry e0 = entry_load(p, row, lane);
   const RawId raw_label = p.labels.at ? id_load(p.labels, row) : RawId{0, 1};
+  uint32_t i0;
+  float x0;
+  entry_of(p, e0, lane, i0, x0);
   const float dl = p.dloss[int64_t(row) * p.dloss_stride];
   const float m = p.sums[uint64_t(row) * 3];
   const float ls = p.sums[uint64_t(row) * 3 + 1], ls1 = p.sums[uint64_t(row) * 3 + 2];
   Vec<T, N> v[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const uint32_t at = from + u * 64 + lane;
-    if (at < to) v[u] = vload_el<T, N, true>(z + head + uint64_t(at) * N);
+    const uint32_t at = vector(u);
+    if (at >= from && at < to) v[u] = vload_el<T, N, true>(z + head + uint64_t(at) * N);
     map[u * 64 + lane] = Vec<uint16_t, N>{};
   }
 
-  uint32_t i0;
-  float x0;
-  entry_of(p, e0, lane, i0, x0);
   const uint32_t label = id_of(raw_label, p.width);
   const bool hard = label < p.width;
   const float ka = dl * p.soft, kb = dl * p.hard, la = ls * kLog2e, lb = ls1 * kLog2e;
@@ -352,8 +356,8 @@ __global__ __launch_bounds__(64) void k_distill_grad(DistillArgs p) {
   auto stream = [&](auto fn) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t at = from + u * 64 + lane;
-      if (at >= to) continue;
+      const uint32_t at = vector(u);
+      if (at < from || at >= to) continue;
       const Vec<uint16_t, N> where = map[u * 64 + lane];
       float g[N];
       uint32_t any = 0;
@@ -474,8 +478,11 @@ int musapy_distill_loss_grad_v1(const musapy_distill_args* a, hipStream_t st) {
     return vocab_bad();
   vocab_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    constexpr uint32_t kSegment = 64 * kGradVectors * 16 / sizeof(T);
-    p.segments = (p.width + kSegment - 1) / kSegment;
+    // of 4 KB; one more where rows begin between them
+    constexpr uint64_t kSegment = 64 * kGradVectors * 16;
+    const uint64_t bytes = p.width * sizeof(T);
+    const bool even = reinterpret_cast<uintptr_t>(p.grad) % kSegment == 0 && bytes % kSegment == 0;
+    p.segments = uint32_t((bytes + kSegment - 1) / kSegment + (even ? 0 : 1));
     const uint64_t grid = uint64_t(p.rows) * p.segments;
     if (!grid_fits(grid, 64)) {
       p.segments = 0;

@@ -64,7 +64,9 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embedding(EmbedArgs p) {
 
 template <class T, class O>
 int launch_embedding(const musapy_embedding_args* a, hipStream_t st) {
-  constexpr int kN = sizeof(T) == 2 || sizeof(O) == 2 ? 8 : 4;
+  // 16 bytes of the result to a lane: with 32, each store leaves every other 16 bytes of a line to the next one (16384 rows of 4096 bf16
+  // into f32 104 us, so 51), and with 8, (f32 into bf16) 68 against 50.
+  constexpr int kN = 16 / int(sizeof(O));
   const bool narrow = a->width < uint64_t(kN);
   const uint64_t groups = narrow ? a->width : (a->width + kN - 1) / kN;
   const uint64_t total = groups * a->tokens;
@@ -119,8 +121,8 @@ struct OrderArgs {
 // Every row is cleared while the order begins, though those of tokens are written again: 4 KB a workgroup, one vector a
 // thread, in the order of addresses, run at 6.7 TB/s (8 to 128 KB a workgroup 5.5 to 6.1).  Clearing only the other
 // rows beside the sums, with the sorted tokens or bits of the rows to look up, took the (131072, 2048) f32 gradient of 16384
-// tokens 225 to 240 us, against 157 for this and some 30 for the sums.  The order's later launches, whose few workgroups
-// take some 8 us whatever is cleared beside them, take 40 MB of it each.
+// tokens 225 to 240 us, against 157 for this and some 30 for the sums.  The later launches of an order by digits, whose few
+// workgroups take 5 to 10 us whatever is cleared beside them, take 40 MB of it each.
 constexpr uint64_t kClearBeside = uint64_t(40) << 20;
 
 template <int BLOCK>
@@ -170,7 +172,6 @@ __global__ __launch_bounds__(kBlockTokens) void k_embed_blocks(OrderArgs p) {
 // its own (or not above it, of the blocks in front), each found by halving.  All keys lie in LDS; a workgroup places 64
 // tokens, and each of its 16 waves searches every sixteenth block, four at a time.
 __global__ __launch_bounds__(kOrderBlock) void k_embed_merge(OrderArgs p) {
-  if (blockIdx.x >= p.order_blocks) return order_clear<kOrderBlock>(p, blockIdx.x - p.order_blocks);
   extern __shared__ uint32_t all[];
   __shared__ uint32_t part[kOrderWaves][64];
   const uint32_t blocks = (p.n + kBlockTokens - 1) / kBlockTokens;
@@ -520,7 +521,7 @@ inline void launch_order(const musapy_embedding_grad_args* a, const EmbedGradPla
   uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(ws + pl.keys), reinterpret_cast<uint32_t*>(ws + pl.keys2)};
   uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(ws + pl.pos), reinterpret_cast<uint32_t*>(ws + pl.pos2)};
   const uint32_t blocks = pl.passes ? pl.tiles : (o.n + kBlockTokens - 1) / kBlockTokens;
-  const int launches = pl.passes ? 2 * pl.passes : blocks > 1 ? 2 : 1;
+  const int launches = pl.passes ? 2 * pl.passes : 1;
   uint64_t bytes = a->accumulate ? 0 : a->rows * a->width * (a->out_dtype == MUSAPY_DT_F32 ? 4 : 2);
   char* out = static_cast<char*>(a->out);
   uint64_t beside = bytes / uint64_t(launches) < kClearBeside ? bytes / uint64_t(launches) : kClearBeside;
@@ -549,8 +550,7 @@ inline void launch_order(const musapy_embedding_grad_args* a, const EmbedGradPla
     o.pos_in = o.pos;
     o.keys = keys[0];
     o.pos = pos[0];
-    const unsigned second = grid((o.n + 63) / 64, kOrderBlock, beside);
-    k_embed_merge<<<second, kOrderBlock, blocks * kBlockTokens * 4, st>>>(o);
+    k_embed_merge<<<(o.n + 63) / 64, kOrderBlock, blocks * kBlockTokens * 4, st>>>(o);
     return;
   }
   o.hist = reinterpret_cast<uint32_t*>(ws + pl.hist);
@@ -576,7 +576,7 @@ inline void launch_order(const musapy_embedding_grad_args* a, const EmbedGradPla
 template <class T, class O>
 int launch_embedding_grad(const musapy_embedding_grad_args* a, char* ws, hipStream_t st) {
   const EmbedGradPlan pl = embed_grad_plan(a);
-  constexpr int kN = sizeof(T) == 2 ? 8 : 4;
+  constexpr int kN = 16 / int(sizeof(O));  // 16 bytes of the result to a lane, as in the lookup
   const bool narrow = a->width < uint64_t(kN);
   const int n = narrow ? 1 : kN;
   EmbedGradArgs p{};

@@ -46,7 +46,7 @@ class Call {
     if (a->device != device_)
       throw DeviceError(std::string(op_) + ": " + what + " device hip:" + std::to_string(a->device) + " != hip:" +
                         std::to_string(device_));
-    inputs_.push_back(*a);
+    inputs_.push_back(a->data);
   }
   // `given` (checked), or a new array
   Array output(const Array* given, const char* what, const Shape& shape, Dtype dtype) {
@@ -57,8 +57,8 @@ class Call {
         throw DeviceError(std::string(op_) + ": " + what + " device hip:" + std::to_string(given->device) + " != hip:" +
                           std::to_string(device_));
       if (!given->layout.has_contiguous_strides()) throw ShapeError("out= must have C-contiguous strides");
-      for (const Array& in : inputs_)
-        if (in.data.get() == given->data.get()) throw MemoryError("alias detected: out= shares its buffer with an input");
+      for (const BufferRef& in : inputs_)
+        if (in.get() == given->data.get()) throw MemoryError("alias detected: out= shares its buffer with an input");
       for (const Array& o : outputs_)
         if (o.data.get() == given->data.get()) throw MemoryError("alias detected: two outputs share their buffer");
     }
@@ -74,7 +74,7 @@ class Call {
   }
   // before the launch; `copies` are the arrays the kernels read in the place of inputs
   void begin() {
-    for (const Array& a : inputs_) a.data->wait_last_write_on(s_);
+    for (const BufferRef& a : inputs_) a->wait_last_write_on(s_);
     for (const Array& a : outputs_) {
       a.data->wait_last_write_on(s_);
       a.data->wait_reads_on(s_);
@@ -83,7 +83,7 @@ class Call {
   }
   void end() {
     check_launch(op_);
-    for (const Array& a : inputs_) a.data->record_read(s_);
+    for (const BufferRef& a : inputs_) a->record_read(s_);
     for (const Array& a : outputs_) a.data->record_write(s_);  // (what stays where a wait below fails)
     for (const Array& a : outputs_) {
       if (a.stream.get() == s_.get()) continue;
@@ -96,12 +96,12 @@ class Call {
   const char* op_;
   int device_;
   StreamPtr s_;
-  std::vector<Array> inputs_, outputs_;
+  std::vector<BufferRef> inputs_;
+  std::vector<Array> outputs_;
 };
 
-// `a` with its leading dims as rows one pitch apart and unit-stride columns, copied when its strides do not
-// allow it.
-inline Array as_rows(const Array& a, size_t& pitch) {
+// Whether the leading dims of `a` are rows one pitch apart, and its columns unit-stride.
+inline bool rows_pitch(const Array& a, size_t& pitch) {
   const size_t nd = a.ndim();
   const size_t width = a.shape()[nd - 1];
   ssize_t st = ssize_t(width);
@@ -113,14 +113,15 @@ inline Array as_rows(const Array& a, size_t& pitch) {
     else ok = ok && a.layout.strides[i] == st * ssize_t(n);
     n *= a.shape()[i];
   }
-  ok = ok && st >= 0;
-  if (!ok && a.size() > 0) {
-    Array c = contiguous(a);
-    pitch = width;
-    return c;
-  }
   pitch = size_t(st);
-  return a;
+  return (ok && st >= 0) || a.size() == 0;
+}
+
+// `a` itself where it is such rows, a C-contiguous copy otherwise.
+inline Array as_rows(const Array& a, size_t& pitch) {
+  if (rows_pitch(a, pitch)) return a;
+  pitch = a.shape().back();
+  return contiguous(a);
 }
 
 }  // namespace ops

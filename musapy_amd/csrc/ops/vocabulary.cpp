@@ -30,20 +30,18 @@ size_t lead_rows(const Shape& shape) { return shape_numel(Shape(shape.begin(), s
 // One call's inputs as the kernels read them: C-contiguous, or rows one pitch apart.
 class Inputs {
  public:
-  explicit Inputs(Call& call) : call_(call) { held_.reserve(16); }
+  explicit Inputs(Call& call) : call_(call) {}
   const void* plain(const Array* a, const char* what) {
     if (!a) return nullptr;
     call_.input(a, what);
-    held_.push_back(a->layout.has_contiguous_strides() ? *a : contiguous(*a));
-    call_.input(&held_.back(), what);
-    return held_.back().data_ptr();
+    return a->layout.has_contiguous_strides() ? a->data_ptr() : copied(*a, what);
   }
   const void* rows(const Array* a, const char* what, size_t& pitch) {
     if (!a) return nullptr;
     call_.input(a, what);
-    held_.push_back(as_rows(*a, pitch));
-    call_.input(&held_.back(), what);
-    return held_.back().data_ptr();
+    if (rows_pitch(*a, pitch)) return a->data_ptr();
+    pitch = a->shape().back();
+    return copied(*a, what);
   }
   // rows of `n` for every row of `lead`, or one for all of them (pitch 0)
   const void* rows_or_one(const char* op, const Array* a, const char* what, const Shape& lead, size_t n, size_t& pitch) {
@@ -56,6 +54,11 @@ class Inputs {
   }
 
  private:
+  const void* copied(const Array& a, const char* what) {
+    held_.push_back(contiguous(a));
+    call_.input(&held_.back(), what);
+    return held_.back().data_ptr();
+  }
   Call& call_;
   std::vector<Array> held_;
 };
