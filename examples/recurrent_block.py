@@ -1,4 +1,4 @@
-"""A small gated recurrent language model: training on packed documents, then decoding token by token.
+"""A small gated recurrent language model: training on packed documents, decoding token by token, and a student of it.
 
 PyTorch holds the parameters, the matrix products and the optimizer; between the products run this library's
 operators, on the same memory (DLPack, no copies):
@@ -6,7 +6,11 @@ operators, on the same memory (DLPack, no copies):
     embedding -> dropout -> per block: products of y give the recurrence's input, its gates and the output gate
                  h = gated_scan(input, gates, reset=document starts, kind="blend")
                  r, y = norm_residual(h, r, gate=output gate, ...)      # norm, gate, dropout, residual scale, next norm
-              -> product with the embedding
+              -> product with the embedding -> a loss, or the choice of the next token
+
+The embedding's rows are looked up by ms.embedding and its gradient is ms.embedding_grad, beside the product's.  A student
+learns from a teacher's top logits and the labels (ms.distill_loss); ms.adjust_logits keeps what is generated from repeating
+itself and to the tokens that are allowed.
 
 The task needs the recurrence: every token of a document is to be answered with the document's first token.
 
@@ -78,6 +82,33 @@ class Dropout(torch.autograd.Function):
         return ten(ms.dropout(arr(dy), *ctx.args)), None, None, None
 
 
+class Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, tokens):
+        ctx.save_for_backward(tokens)
+        ctx.rows = table.shape[0]
+        return ten(ms.embedding(arr(table), arr(tokens)))
+
+    @staticmethod
+    def backward(ctx, dy):
+        return ten(ms.embedding_grad(arr(dy), arr(ctx.saved_tensors[0]), ctx.rows)), None
+
+
+class DistillLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, index, top, labels, temperature, weight):
+        ctx.args = dict(temperature=temperature, weight=weight)
+        loss, sums = ms.distill_loss(arr(logits), arr(index), arr(top), arr(labels), **ctx.args)
+        ctx.save_for_backward(logits, ten(sums), index, top, labels)
+        return ten(loss)
+
+    @staticmethod
+    def backward(ctx, dloss):
+        logits, sums, index, top, labels = ctx.saved_tensors
+        return ten(ms.distill_loss_grad(arr(dloss), arr(logits), arr(sums), arr(index), arr(top), arr(labels), **ctx.args)), \
+            None, None, None, None, None
+
+
 class Model:
     def __init__(self, width, blocks, seed=0, dtype=torch.bfloat16):
         g = torch.Generator(device="cuda").manual_seed(seed)
@@ -105,7 +136,7 @@ class Model:
         return (y.flatten(0, -2) @ self.embedding.to(self.dtype).t()).float().view(*y.shape[:-1], VOCABULARY) * self.width ** -0.5
 
     def forward(self, tokens, reset, p=0.0, seed=0, step=0):
-        r = self.embedding[tokens]  # the residual stream stays in 32 bits
+        r = Embedding.apply(self.embedding, tokens)  # the residual stream stays in 32 bits
         y = r.to(self.dtype)
         if p > 0:
             y = Dropout.apply(y, p, seed, step * 64)
@@ -118,7 +149,7 @@ class Model:
     @torch.no_grad()
     def step(self, token, states):
         """Logits behind one more token of each sequence; the states are carried on in place of the sequence."""
-        r = self.embedding[token][:, None]
+        r = ten(ms.embedding(arr(self.embedding), arr(token)))[:, None]
         y = r.to(self.dtype)
         for i, b in enumerate(self.blocks):
             x, g, o = self.products(b, y)
@@ -161,6 +192,41 @@ def train(model, steps, length, batch=8, report=None):
     return losses
 
 
+def distill(student, teacher, steps, length, batch=8, entries=4, temperature=2.0, weight=0.5, report=None):
+    """The student learns from the teacher's top logits and from the answers."""
+    generator = torch.Generator(device="cuda").manual_seed(3)
+    optimizer = torch.optim.AdamW(student.parameters(), lr=5e-3, weight_decay=0.0)
+    losses = []
+    for step in range(steps):
+        tokens, answers, starts = documents(batch, length, generator)
+        with torch.no_grad():
+            top, index = teacher.forward(tokens, starts).flatten(0, 1).topk(entries)
+        logits = student.forward(tokens, starts).flatten(0, 1)
+        loss = DistillLoss.apply(logits, index, top, answers.flatten(), temperature, weight).mean()
+        optimizer.zero_grad()
+        loss.backward()
+        optimizer.step()
+        losses.append(float(loss.detach()))
+        if report and (step + 1) % report == 0:
+            print(f"step {step + 1}: distillation loss {losses[-1]:.4f}", flush=True)
+    return losses
+
+
+@torch.no_grad()
+def generate(model, tokens, count, allowed=None, repetition=1.0, presence=0.0, frequency=0.0):
+    """`count` more tokens behind each prompt of `tokens` (batch, length): at every step the likeliest of the allowed ones (truth values,
+    one for each token of the vocabulary), less the penalties for those that occurred."""
+    states = [torch.zeros(tokens.shape[0], model.width, device="cuda") for _ in model.blocks]
+    logits = [model.step(tokens[:, t], states) for t in range(tokens.shape[1])][-1]
+    for _ in range(count):
+        best = ms.adjust_logits(arr(logits), arr(tokens), repetition=repetition, presence=presence, frequency=frequency,
+                                allowed=arr(allowed))
+        token = ten(ms.argmax(best, axis=1))
+        tokens = torch.cat([tokens, token[:, None]], 1)
+        logits = model.step(token, states)
+    return tokens
+
+
 @torch.no_grad()
 def decode(model, tokens):
     """Logits of every position, one token at a time."""
@@ -182,6 +248,12 @@ def main():
     tokens[:, 0] = torch.arange(16, device="cuda") % CLASSES
     answers = decode(model, tokens).argmax(-1)
     print(f"decoded token by token: {float((answers == tokens[:, :1]).float().mean()):.1%} of the answers right")
+    student = Model(a.width // 2, 1, seed=1)
+    distill(student, model, a.steps, a.length, report=max(1, a.steps // 10))
+    answers = decode(student, tokens).argmax(-1)
+    print(f"its student of half the width: {float((answers == tokens[:, :1]).float().mean()):.1%}")
+    longer = generate(student, tokens[:4, :6], 8, frequency=2.0)
+    print("generated with a penalty for repeated tokens:", longer[:, 6:].tolist())
 
 
 if __name__ == "__main__":
