@@ -615,7 +615,8 @@ int musapy_embedding_grad_v1(const musapy_embedding_grad_args* args, void* scrat
  * logit m, log(sum exp((z - m) / T)) and log(sum exp(z - m)), 0 where a row has no use for one, and the gradient reads it.  A
  * column of -inf has probability 0; a row of nothing else, and one with +inf or NaN, gives NaN.
  * At most 1024 entries; T from 2^-20 to 2^20, weight from 0 to 1.  Rows of logits, indices and values are unit-stride, `*_pitch`
- * elements apart; labels (NULL: none) and the outputs are C-contiguous; dloss is `dloss_stride` elements apart. */
+ * elements apart; labels (NULL: none) and the outputs are C-contiguous; dloss is `dloss_stride` elements apart.
+ * The loss of few long rows goes through `scratch` (musapy_distill_loss_scratch_v1 bytes, 4-byte aligned, any contents). */
 typedef struct {
   int dtype, index_dtype, teacher_dtype, label_dtype;
   float temperature, weight;
@@ -633,7 +634,8 @@ typedef struct {
   ssize_t dloss_stride;
   void* dlogits; /* grad */
 } musapy_distill_args;
-int musapy_distill_loss_v1(const musapy_distill_args* args, hipStream_t stream);
+size_t musapy_distill_loss_scratch_v1(const musapy_distill_args* args);
+int musapy_distill_loss_v1(const musapy_distill_args* args, void* scratch, size_t scratch_bytes, hipStream_t stream);
 int musapy_distill_loss_grad_v1(const musapy_distill_args* args, hipStream_t stream);
 
 /* Logits of the next token, made ready for its choice.  For each row, with c the number of times that a column is among the

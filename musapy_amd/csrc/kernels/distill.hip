@@ -26,7 +26,9 @@ struct DistillArgs {
   const float* dloss;
   int64_t dloss_stride;
   void* grad;
-  uint32_t segments;       // of the gradient: workgroups of a row
+  uint32_t segments;       // workgroups of a row
+  uint32_t segment;        // of the loss: columns of each
+  float* parts;            // of the loss, with more than one: (rows, segments, 3), a segment's maximum and sums
 };
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -58,28 +60,114 @@ __device__ inline uint32_t row_head(const T* row, uint32_t width) {
   return head < width ? head : width;
 }
 
-// A workgroup takes a row: every thread keeps the maximum m of its logits and the sums of exp((z - m) / T) and,
-// with labels at a T other than 1, exp(z - m), rescaled when m rises; they are joined at the end.  The first
-// wave then forms the teacher's part, which needs K logits and the sum only:
+// A workgroup takes a row, or a segment of one where there are few: every thread keeps the maximum m of its logits and the sums of
+// exp((z - m) / T) and, with labels at a T other than 1, exp(z - m), rescaled when m rises; they are joined at the
+// end.  A wave then forms the teacher's part, which needs K logits and the sum only:
 //   sum_k p_k (log p_k - log q_k) = B / A - log A + (m - r) / T + log sum exp((z - m) / T),
 //   e_k = exp((v_k - max v) / T),  A = sum e_k,  B = sum e_k ((v_k - max v) - (z_k - r)) / T
 // with r the highest of the entries' logits: all differences are of near numbers, so that logits far from 0 lose nothing.
+//
+// Below kNear, exponents are one multiply-add, x c - round(m c): the sums are then relative to 2^round(m c), and the rounding
+// itself, the same for all terms, is taken off at the end.  Beyond it, where m c or x c may leave f32's range (rows and
+// threads with nothing but -inf or the types' lowest values among them), (x - m) c.
 enum { kOne = 0, kTwo = 1, kSquare = 2 };  // one sum; two; two at T = 2, where exp(z - m) is the square of exp((z - m) / 2)
 
-template <class T, int BLOCK, int SUMS>
+constexpr float kNear = 1e30f;
+// what sums relative to the maximum `from` are multiplied with to be relative to `to`
+__device__ inline float sum_change(float from, float to, float c) {
+  return exp2_fast(__builtin_fabsf(to) < kNear ? from * c - to * c : (from - to) * c);
+}
+
+// What a wave knows of a row before its logits: the first 64 entries and the label, and which terms the row has.
+struct RowTerms {
+  uint32_t i0, label;  // an entry's column to a lane
+  float x0;
+  bool soft, hard;
+};
+__device__ inline RowTerms row_terms(const DistillArgs& p, uint32_t row, int lane, const RawEntry& e0, const RawId& raw_label) {
+  RowTerms r;
+  entry_of(p, e0, lane, r.i0, r.x0);
+  r.label = id_of(raw_label, p.width);
+  r.hard = r.label < p.width;
+  r.soft = __ballot(r.i0 < p.width) != 0;
+  for (uint32_t k0 = 64; k0 < p.entries && !r.soft; k0 += 64) {
+    uint32_t i;
+    float x;
+    teacher_entry(p, row, k0 + lane, i, x);
+    r.soft = __ballot(i < p.width) != 0;
+  }
+  return r;
+}
+__device__ inline void row_unused(const DistillArgs& p, uint32_t row) {
+  p.loss[row] = 0.0f;
+  for (int i = 0; i < 3; ++i) p.sums[uint64_t(row) * 3 + i] = 0.0f;
+}
+
+// The row's results, by one wave, from its maximum and sums; z0: the logits of the first 64 entries.
+template <class T, int SUMS>
+__device__ inline void row_finish(const DistillArgs& p, uint32_t row, int lane, const T* z, const RowTerms& t, float z0, float most, float s, float s1) {
+  float a = 0.0f, b = 0.0f, r = -__builtin_inff();
+  if (t.soft) {
+    auto each = [&](auto fn) {
+      for (uint32_t k0 = 0; k0 < p.entries; k0 += 64) {
+        uint32_t i = t.i0;
+        float x = t.x0, y = z0;
+        if (k0 > 0) {
+          teacher_entry(p, row, k0 + lane, i, x);
+          if (i < p.width) y = float(z[i]);
+        }
+        if (i < p.width) fn(x, y);
+      }
+    };
+    float top = -__builtin_inff();
+    each([&](float x, float y) {
+      top = fmaxf(top, x);
+      r = fmaxf(r, y);
+    });
+    top = wave_max(top);
+    r = wave_max(r);
+    if (r == -__builtin_inff()) r = 0.0f;
+    each([&](float x, float y) {
+      const float d = x - top, e = exp2_fast(d * p.c);
+      a += e;
+      if (!(e == 0.0f)) b += e * ((d - (y - r)) * p.inv_t);
+    });
+    a = wave_sum(a);
+    b = wave_sum(b);
+  }
+  if (lane != 0) return;
+  auto log_sum = [&](float sum, float c) {
+    const float off = __builtin_fabsf(most) < kNear ? __builtin_fmaf(most, c, -(most * c)) : 0.0f;
+    return kLn2 * (__builtin_amdgcn_logf(sum) - off);
+  };
+  const float ls = log_sum(s, p.c), ls1 = SUMS != kOne ? log_sum(s1, kLog2e) : ls;
+  float loss = 0.0f;
+  if (t.soft) loss = p.soft * (b / a - kLn2 * __builtin_amdgcn_logf(a) + (most - r) * p.inv_t + ls);
+  if (t.hard) loss += p.hard * ((most - float(z[t.label])) + ls1);
+  p.loss[row] = loss;
+  float* sums = p.sums + uint64_t(row) * 3;
+  sums[0] = most;
+  sums[1] = t.soft ? ls : 0.0f;
+  sums[2] = t.hard ? ls1 : 0.0f;
+}
+
+template <class T, int BLOCK, int SUMS, bool PART>
 __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
   constexpr int N = 16 / int(sizeof(T)), U = 4, kWaves = BLOCK / 64;
   constexpr bool TWO = SUMS != kOne;
   __shared__ float part[kWaves][3];
-  const uint32_t row = blockIdx.x;
+  const uint32_t row = PART ? blockIdx.x / p.segments : blockIdx.x, seg = PART ? blockIdx.x - row * p.segments : 0;
   const int lane = threadIdx.x % 64;
   const uint32_t wave = wave_uniform(threadIdx.x / 64);
+  const uint32_t first = PART ? seg * p.segment : 0;
+  const uint32_t width = PART && p.width - first > p.segment ? p.segment : p.width - first;
   const T* z = static_cast<const T*>(p.logits) + uint64_t(row) * p.pitch;
-  const uint32_t head = row_head<T>(z, p.width), vectors = (p.width - head) / N;
+  const T* zs = z + first;
+  const uint32_t head = row_head<T>(zs, width), vectors = (width - head) / N;
   Vec<T, N> v[U];
   const uint32_t whole = vectors / (BLOCK * U) * (BLOCK * U);  // vectors in rounds of U for every thread
   auto fetch = [&](uint32_t base) {
-    const T* at = z + head + (uint64_t(base) + threadIdx.x) * N;
+    const T* at = zs + head + (uint64_t(base) + threadIdx.x) * N;
 #pragma unroll
     for (int u = 0; u < U; ++u) v[u] = vload_el<T, N, true>(at + u * BLOCK * N);
   };
@@ -87,7 +175,7 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t at = whole + u * BLOCK + threadIdx.x;
-      v[u] = vload_el<T, N, true>(z + head + uint64_t(at < vectors ? at : vectors - 1) * N);
+      v[u] = vload_el<T, N, true>(zs + head + uint64_t(at < vectors ? at : vectors - 1) * N);
     }
   };
   // the first 64 entries and the first logits, all on their way at once
@@ -95,39 +183,18 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
   const RawId raw_label = p.labels.at ? id_load(p.labels, row) : RawId{0, 1};
   if (whole > 0) fetch(0);
   else if (vectors > 0) fetch_rest();
-  uint32_t i0;
-  float x0;
-  entry_of(p, e0, lane, i0, x0);
-  const uint32_t label = id_of(raw_label, p.width);
-  const bool hard = label < p.width;
-  bool soft = __ballot(i0 < p.width) != 0;
-  for (uint32_t k0 = 64; k0 < p.entries && !soft; k0 += 64) {
-    uint32_t i;
-    float x;
-    teacher_entry(p, row, k0 + lane, i, x);
-    soft = __ballot(i < p.width) != 0;
-  }
-  if (!soft && !hard) {
-    if (threadIdx.x == 0) {
-      p.loss[row] = 0.0f;
-      for (int i = 0; i < 3; ++i) p.sums[uint64_t(row) * 3 + i] = 0.0f;
-    }
+  const RowTerms terms = row_terms(p, row, lane, e0, raw_label);
+  if (!terms.soft && !terms.hard) {
+    if (!PART && threadIdx.x == 0) row_unused(p, row);
     return;
   }
   float z0 = 0.0f;
-  if (wave == 0 && i0 < p.width) z0 = float(z[i0]);
+  if (!PART && wave == 0 && terms.i0 < p.width) z0 = float(z[terms.i0]);
 
-  // Below kNear, exponents are one multiply-add, x c - round(m c): the sums are then relative to 2^round(m c), and the rounding
-  // itself, the same for all terms, is taken off at the end.  Beyond it, where m c or x c may leave f32's range (rows and
-  // threads with nothing but -inf or the types' lowest values among them), (x - m) c.
-  constexpr float kNear = 1e30f;
   float m = -__FLT_MAX__, s = 0.0f, s1 = 0.0f;
-  auto change = [&](float from, float to, float c) {
-    return exp2_fast(__builtin_fabsf(to) < kNear ? from * c - to * c : (from - to) * c);
-  };
   auto raise = [&](float high) {
-    s *= change(m, high, p.c);
-    if (TWO) s1 *= change(m, high, kLog2e);
+    s *= sum_change(m, high, p.c);
+    if (TWO) s1 *= sum_change(m, high, kLog2e);
     m = high;
   };
   auto one = [&](float w, float w1) {
@@ -168,14 +235,14 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
     if (whole > 0) fetch_rest();
     add(std::true_type{});
   }
-  if (threadIdx.x < p.width - vectors * N) {  // the columns in front of and behind the vectors
-    const float x[1] = {float(z[threadIdx.x < head ? threadIdx.x : threadIdx.x + vectors * N])};
+  if (threadIdx.x < width - vectors * N) {  // the columns in front of and behind the vectors
+    const float x[1] = {float(zs[threadIdx.x < head ? threadIdx.x : threadIdx.x + vectors * N])};
     raise(fmaxf(m, x[0]));
     sum(x, std::integral_constant<int, 1>{});
   }
   float most = wave_max(m);
-  s = wave_sum(s * change(m, most, p.c));
-  if (TWO) s1 = wave_sum(s1 * change(m, most, kLog2e));
+  s = wave_sum(s * sum_change(m, most, p.c));
+  if (TWO) s1 = wave_sum(s1 * sum_change(m, most, kLog2e));
   if constexpr (kWaves > 1) {
     if (lane == 0) {
       part[wave][0] = most;
@@ -186,52 +253,41 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
     if (wave != 0) return;
     m = lane < kWaves ? part[lane][0] : -__FLT_MAX__;
     most = wave_max(m);
-    s = wave_sum(lane < kWaves ? part[lane][1] * change(m, most, p.c) : 0.0f);
-    if (TWO) s1 = wave_sum(lane < kWaves ? part[lane][2] * change(m, most, kLog2e) : 0.0f);
+    s = wave_sum(lane < kWaves ? part[lane][1] * sum_change(m, most, p.c) : 0.0f);
+    if (TWO) s1 = wave_sum(lane < kWaves ? part[lane][2] * sum_change(m, most, kLog2e) : 0.0f);
   }
-  float a = 0.0f, b = 0.0f, r = -__builtin_inff();
-  if (soft) {
-    auto each = [&](auto fn) {
-      for (uint32_t k0 = 0; k0 < p.entries; k0 += 64) {
-        uint32_t i = i0;
-        float x = x0, y = z0;
-        if (k0 > 0) {
-          teacher_entry(p, row, k0 + lane, i, x);
-          if (i < p.width) y = float(z[i]);
-        }
-        if (i < p.width) fn(x, y);
-      }
-    };
-    float top = -__builtin_inff();
-    each([&](float x, float y) {
-      top = fmaxf(top, x);
-      r = fmaxf(r, y);
-    });
-    top = wave_max(top);
-    r = wave_max(r);
-    if (r == -__builtin_inff()) r = 0.0f;
-    each([&](float x, float y) {
-      const float d = x - top, e = exp2_fast(d * p.c);
-      a += e;
-      if (!(e == 0.0f)) b += e * ((d - (y - r)) * p.inv_t);
-    });
-    a = wave_sum(a);
-    b = wave_sum(b);
+  if constexpr (PART) {
+    if (lane != 0) return;
+    float* to = p.parts + (uint64_t(row) * p.segments + seg) * 3;
+    to[0] = most;
+    to[1] = s;
+    to[2] = s1;
+  } else {
+    row_finish<T, SUMS>(p, row, lane, z, terms, z0, most, s, s1);
   }
-  if (lane != 0) return;
-  auto log_sum = [&](float sum, float c) {
-    const float off = __builtin_fabsf(most) < kNear ? __builtin_fmaf(most, c, -(most * c)) : 0.0f;
-    return kLn2 * (__builtin_amdgcn_logf(sum) - off);
-  };
-  const float ls = log_sum(s, p.c), ls1 = TWO ? log_sum(s1, kLog2e) : ls;
-  float loss = 0.0f;
-  if (soft) loss = p.soft * (b / a - kLn2 * __builtin_amdgcn_logf(a) + (most - r) * p.inv_t + ls);
-  if (hard) loss += p.hard * ((most - float(z[label])) + ls1);
-  p.loss[row] = loss;
-  float* sums = p.sums + uint64_t(row) * 3;
-  sums[0] = most;
-  sums[1] = soft ? ls : 0.0f;
-  sums[2] = hard ? ls1 : 0.0f;
+}
+
+// The segments of a row, at most 64, to a wave.
+template <class T, int SUMS>
+__global__ __launch_bounds__(64) void k_distill_join(DistillArgs p) {
+  const uint32_t row = blockIdx.x;
+  const int lane = threadIdx.x;
+  const T* z = static_cast<const T*>(p.logits) + uint64_t(row) * p.pitch;
+  const RawEntry e0 = entry_load(p, row, lane);
+  const RawId raw_label = p.labels.at ? id_load(p.labels, row) : RawId{0, 1};
+  const float* from = p.parts + (uint64_t(row) * p.segments + (uint32_t(lane) < p.segments ? lane : 0)) * 3;
+  const float m0 = from[0], s0 = from[1], s10 = from[2];
+  const RowTerms terms = row_terms(p, row, lane, e0, raw_label);
+  if (!terms.soft && !terms.hard) {
+    if (lane == 0) row_unused(p, row);
+    return;
+  }
+  const float z0 = terms.i0 < p.width ? float(z[terms.i0]) : 0.0f;
+  const bool there = uint32_t(lane) < p.segments;
+  const float m = there ? m0 : -__FLT_MAX__, most = wave_max(m);
+  const float s = wave_sum(there ? s0 * sum_change(m, most, p.c) : 0.0f);
+  const float s1 = SUMS != kOne ? wave_sum(there ? s10 * sum_change(m, most, kLog2e) : 0.0f) : 0.0f;
+  row_finish<T, SUMS>(p, row, lane, z, terms, z0, most, s, s1);
 }
 
 // A workgroup of one wave takes a segment of a row, four vectors of 16 bytes to a lane: dloss (weight T softmax(z / T) +
@@ -407,6 +463,15 @@ __global__ __launch_bounds__(64, 8) void k_distill_grad(DistillArgs p) {
   }
 }
 
+// Segments of a row in the loss: few rows are split into what fills the chip, if they are long enough to be worth a second launch (one
+// row of 262144 bf16 8 us, whole 16; 64 of 131072 11.3 and 14.6; but 256 of them 20 and 17, 64 of 32768 9 and 6).
+static uint32_t distill_segments(uint64_t rows, uint64_t width, uint64_t size) {
+  if (rows == 0 || rows > 128 || width * size < 192 * 1024) return 1;
+  const uint64_t wanted = (1024 + rows - 1) / rows, most = width * size / 8192;
+  const uint64_t n = wanted < most ? wanted : most;
+  return uint32_t(n < 64 ? n : 64);
+}
+
 static bool distill_args(const musapy_distill_args* a, bool grad, DistillArgs& p) {
   if (a == nullptr || !vocab_float(a->dtype) || a->rows >= kVocabLimit || a->width >= kVocabLimit) return false;
   if (a->entries > size_t(kEntriesMost) || !(a->temperature >= 0x1p-20f && a->temperature <= 0x1p20f)) return false;
@@ -443,28 +508,46 @@ using namespace mpy;
 
 extern "C" {
 
-int musapy_distill_loss_v1(const musapy_distill_args* a, hipStream_t st) {
+size_t musapy_distill_loss_scratch_v1(const musapy_distill_args* a) {
+  DistillArgs p{};
+  if (!distill_args(a, false, p)) return 0;
+  const uint32_t n = distill_segments(p.rows, p.width, a->dtype == MUSAPY_DT_F32 ? 4 : 2);
+  return n > 1 ? size_t(p.rows) * n * 3 * sizeof(float) : 0;
+}
+
+int musapy_distill_loss_v1(const musapy_distill_args* a, void* scratch, size_t scratch_bytes, hipStream_t st) {
   DistillArgs p{};
   if (!distill_args(a, false, p)) return vocab_bad();
   if (p.rows == 0) return 0;
   if (p.loss == nullptr || p.sums == nullptr || (p.width > 0 && p.logits == nullptr) ||
       (p.entries > 0 && (p.index.at == nullptr || p.teacher == nullptr)) || !grid_fits(p.rows, 512))
     return vocab_bad();
+  const size_t need = musapy_distill_loss_scratch_v1(a);
+  if (need > 0 && (scratch == nullptr || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 3))) return vocab_bad(1);
   const bool two = p.labels.at != nullptr && a->temperature != 1.0f;
   vocab_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    auto go = [&](auto BLOCK) {
-      constexpr int kB = BLOCK.value;
-      if (two && a->temperature == 2.0f) k_distill_loss<T, kB, kSquare><<<p.rows, kB, 0, st>>>(p);
-      else if (two) k_distill_loss<T, kB, kTwo><<<p.rows, kB, 0, st>>>(p);
-      else k_distill_loss<T, kB, kOne><<<p.rows, kB, 0, st>>>(p);
+    auto go = [&](auto SUMS) {
+      constexpr int kS = SUMS.value;
+      p.segments = distill_segments(p.rows, p.width, sizeof(T));
+      if (p.segments > 1) {
+        p.parts = static_cast<float*>(scratch);
+        p.segment = (p.width / p.segments + 64) / 64 * 64;  // at least width / segments: no more segments than asked for
+        p.segments = (p.width + p.segment - 1) / p.segment;
+        k_distill_loss<T, 512, kS, true><<<p.rows * p.segments, 512, 0, st>>>(p);
+        k_distill_join<T, kS><<<p.rows, 64, 0, st>>>(p);
+        return;
+      }
+      // The fewest waves a row that fill the chip's 8192, since a row takes some 6 us however short it is ((16384, 4000) bf16 29 us, with
+      // 256 threads a row 45, with 512 91).  But with more than 32 vectors a thread the larger workgroups are level or better.
+      const uint64_t vectors = p.width * sizeof(T) / 16;
+      if (p.rows >= 8192 && vectors <= 32 * 64) k_distill_loss<T, 64, kS, false><<<p.rows, 64, 0, st>>>(p);
+      else if (p.rows >= 2048 && vectors <= 32 * 256) k_distill_loss<T, 256, kS, false><<<p.rows, 256, 0, st>>>(p);
+      else k_distill_loss<T, 512, kS, false><<<p.rows, 512, 0, st>>>(p);
     };
-    // The fewest waves a row that fill the chip's 8192: a row takes some 7 us however short it is.  But with more than 32
-    // vectors a thread the larger workgroups are level or better.
-    const uint64_t vectors = p.width * sizeof(T) / 16;
-    if (p.rows >= 8192 && vectors <= 32 * 64) go(std::integral_constant<int, 64>{});
-    else if (p.rows >= 2048 && vectors <= 32 * 256) go(std::integral_constant<int, 256>{});
-    else go(std::integral_constant<int, 512>{});
+    if (two && a->temperature == 2.0f) go(std::integral_constant<int, kSquare>{});
+    else if (two) go(std::integral_constant<int, kTwo>{});
+    else go(std::integral_constant<int, kOne>{});
   });
   return 0;
 }

@@ -200,7 +200,10 @@ std::pair<Array, Array> distill_loss(const Array& logits, const Array& indices, 
   c.p.loss = static_cast<float*>(loss.data_ptr());
   c.p.sums = static_cast<float*>(sums.data_ptr());
   c.call.begin();
-  (void)musapy_distill_loss_v1(&c.p, c.call.stream()->raw());
+  const size_t bytes = musapy_distill_loss_scratch_v1(&c.p);
+  BufferRef scratch;
+  if (bytes > 0) scratch = Buffer::alloc(bytes, logits.device, c.call.stream());
+  (void)musapy_distill_loss_v1(&c.p, scratch ? scratch->ptr() : nullptr, bytes, c.call.stream()->raw());
   c.call.end();
   return {loss, sums};
 }

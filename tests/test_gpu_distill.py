@@ -256,3 +256,21 @@ def test_refusals():
     ]:
         with pytest.raises(err):
             call()
+
+
+@pytest.mark.parametrize("rows,width", [(1, 65536), (1, 131072), (2, 65600), (9, 70001), (9, 131072), (128, 65600), (129, 65600)])
+def test_few_long_rows(rows, width):
+    """Rows that are split into segments, among them ones without a use and segments of nothing but masked columns."""
+    rng = np.random.default_rng(rows)
+    few = min(rows, 9)
+    for dt in ("bf16", "f32"):
+        z, index, teacher, label = inputs(rng, few, width, 70, dt, "f32")
+        z[few - 1, 1000:60000] = -np.inf
+        if few > 1:
+            index[0], label[0] = -1, -100
+            z[1, :] = R.rounded(np.full(1, -3e38), dt)
+            z[1, width - 1], index[1, :2], label[1] = 1.0, [width - 1, -1], width - 1
+            index[1, 2:] = -1
+        rep = np.arange(rows) % few
+        check(z[rep], index[rep], teacher[rep], label[rep], dt, "f32", 2.0, 0.5)
+        check(z[rep], index[rep], teacher[rep], None, dt, "f32", 1.0, 1.0)

@@ -81,10 +81,11 @@ class AdjustArgs(ctypes.Structure):
 
 def lib():
     L = ctypes.CDLL(LIB)
-    for n, args in {"musapy_embedding_v1": [P, P], "musapy_embedding_grad_v1": [P, P, S, P], "musapy_distill_loss_v1": [P, P],
+    for n, args in {"musapy_embedding_v1": [P, P], "musapy_embedding_grad_v1": [P, P, S, P], "musapy_distill_loss_v1": [P, P, S, P],
                     "musapy_distill_loss_grad_v1": [P, P], "musapy_adjust_logits_v1": [P, P]}.items():
         getattr(L, n).argtypes, getattr(L, n).restype = args, I
-    L.musapy_embedding_grad_scratch_v1.argtypes, L.musapy_embedding_grad_scratch_v1.restype = [P], S
+    for n in ("musapy_embedding_grad_scratch_v1", "musapy_distill_loss_scratch_v1"):
+        getattr(L, n).argtypes, getattr(L, n).restype = [P], S
     L.musapy_kernels_take_error()
     return L
 
@@ -143,15 +144,23 @@ def test_distill_refusals():
                 entries=8, logits=64, pitch=100, index=64, index_pitch=8, teacher=64, teacher_pitch=8, labels=64, loss=64, sums=64,
                 dloss=64, dloss_stride=1, dlogits=64)
     nan = float("nan")
-    for fn in (L.musapy_distill_loss_v1, L.musapy_distill_loss_grad_v1):
+    for fn, *scratch in ((L.musapy_distill_loss_v1, None, 0), (L.musapy_distill_loss_grad_v1,)):
         for kw in (dict(dtype=F64), dict(index_dtype=F32), dict(teacher_dtype=I32), dict(label_dtype=F32), dict(temperature=0),
                    dict(temperature=-1), dict(temperature=nan), dict(temperature=2e6), dict(weight=-0.1), dict(weight=1.1),
                    dict(weight=nan), dict(rows=1 << 31), dict(width=1 << 31), dict(entries=1025), dict(logits=None),
                    dict(index=None), dict(teacher=None), dict(sums=None)):
-            refused(fn, L, made(DistillArgs, base, kw))
-        refused(fn, L, None)
-        assert fn(ctypes.byref(made(DistillArgs, base, dict(rows=0, logits=None))), None) == 0
-    refused(L.musapy_distill_loss_v1, L, made(DistillArgs, base, dict(loss=None)))
+            refused(fn, L, made(DistillArgs, base, kw), *scratch)
+        refused(fn, L, None, *scratch)
+        assert fn(ctypes.byref(made(DistillArgs, base, dict(rows=0, logits=None))), *scratch, None) == 0
+    refused(L.musapy_distill_loss_v1, L, made(DistillArgs, base, dict(loss=None)), None, 0)
+    # few long rows go through scratch
+    assert L.musapy_distill_loss_scratch_v1(ctypes.byref(made(DistillArgs, base, {}))) == 0
+    long = made(DistillArgs, base, dict(width=1 << 20, pitch=1 << 20))
+    need = L.musapy_distill_loss_scratch_v1(ctypes.byref(long))
+    assert need > 0 and L.musapy_distill_loss_scratch_v1(None) == 0
+    refused(L.musapy_distill_loss_v1, L, long, None, 0, error=1)
+    refused(L.musapy_distill_loss_v1, L, long, 64, need - 1, error=1)
+    refused(L.musapy_distill_loss_v1, L, long, 66, need, error=1)
     for kw in (dict(dloss=None), dict(dlogits=None)):
         refused(L.musapy_distill_loss_grad_v1, L, made(DistillArgs, base, kw))
 

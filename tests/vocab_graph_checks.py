@@ -49,7 +49,7 @@ class Step:
         b, L = ctypes.byref, self.L
         rc = [L.musapy_embedding_v1(b(self.embed), s),
               L.musapy_embedding_grad_v1(b(self.grad), self.scratch.data_ptr(), self.scratch.numel() * 4, s),
-              L.musapy_distill_loss_v1(b(self.distill), s), L.musapy_distill_loss_grad_v1(b(self.distill), s),
+              L.musapy_distill_loss_v1(b(self.distill), None, 0, s), L.musapy_distill_loss_grad_v1(b(self.distill), s),
               L.musapy_adjust_logits_v1(b(self.adjust), s)]
         assert rc == [0] * 5, (rc, L.musapy_kernels_take_error())
 
