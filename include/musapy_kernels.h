@@ -571,8 +571,8 @@ int musapy_dropout_v1(const void* a, void* out, int dtype, int ndim, const size_
 /* ---- operators over a vocabulary (new; no counterpart in kernels.rs) ----
  * Element types are MUSAPY_DT_F32, _F16 or _BF16, all arithmetic is f32 and a result is rounded once.  Token numbers, labels,
  * indices and lengths (`*_dtype` of theirs) are MUSAPY_DT_I32 or _I64.  Rows, columns and tokens are each fewer
- * than 2^31.  Every entry point returns 0 when its work was launched (or there was none), -1 when an argument is out
- * of range (wrapper error 6) or scratch is missing (wrapper error 1); nothing is launched then.
+ * than 2^31, with what else is said below.  Every entry point returns 0 when its work was launched (or there was none), -1
+ * when an argument is out of range (wrapper error 6) or scratch is missing (wrapper error 1); nothing is launched then.
  *
  * Embedding: out[n] = scale * table[ids[n]]; a number outside [0, rows) is padding: its row is zeros.  `ids` has `tokens`
  * numbers, `out` (tokens, width) is C-contiguous; the table's strides are in elements (groups of 4 or 8 columns of all
@@ -581,8 +581,8 @@ int musapy_dropout_v1(const void* a, void* out, int dtype, int ndim, const size_
  * Its gradient: out[v] = scale * sum of dy[n] over the n with ids[n] = v, for every row v of the table, zeros where no
  * token is v; with `accumulate` 1 the sums are added to `out` instead, and rows without a token stay as they are.  A row's
  * terms are added in one order that the tokens alone decide: results are the same from call to call.  dy's rows are
- * unit-stride, dy_pitch elements apart.  `scratch` (musapy_embedding_grad_scratch_v1 bytes, 16-byte aligned) is the call's own,
- * of any contents. */
+ * unit-stride, dy_pitch elements apart, of at most 2^22 columns.  `scratch` (musapy_embedding_grad_scratch_v1 bytes, 16-byte
+ * aligned) is the call's own, of any contents. */
 typedef struct {
   int table_dtype, out_dtype, id_dtype;
   float scale;
@@ -616,6 +616,8 @@ int musapy_embedding_grad_v1(const musapy_embedding_grad_args* args, void* scrat
  * column of -inf has probability 0; a row of nothing else, and one with +inf or NaN, gives NaN.
  * At most 1024 entries; T from 2^-20 to 2^20, weight from 0 to 1.  Rows of logits, indices and values are unit-stride, `*_pitch`
  * elements apart; labels (NULL: none) and the outputs are C-contiguous; dloss is `dloss_stride` elements apart.
+ * The loss takes fewer than 2^26 rows of up to 32 KB (2^23 longer ones), the gradient rows of 2^26 pieces of 4 KB together, one
+ * more a row than it has.
  * The loss of few long rows goes through `scratch` (musapy_distill_loss_scratch_v1 bytes, 4-byte aligned, any contents). */
 typedef struct {
   int dtype, index_dtype, teacher_dtype, label_dtype;
@@ -638,7 +640,7 @@ size_t musapy_distill_loss_scratch_v1(const musapy_distill_args* args);
 int musapy_distill_loss_v1(const musapy_distill_args* args, void* scratch, size_t scratch_bytes, hipStream_t stream);
 int musapy_distill_loss_grad_v1(const musapy_distill_args* args, hipStream_t stream);
 
-/* Logits of the next token, made ready for its choice.  For each row, with c the number of times that a column is among the
+/* Logits of the next token, made ready for its choice (fewer than 2^23 tiles of 2048 columns in all rows).  For each row, with c the number of times that a column is among the
  * first `lengths[row]` (NULL: `length`; cut to 0 .. length) numbers of its history:
  *   z = (z > 0 ? z / repetition : z * repetition) - (frequency * c + presence) where c > 0
  *   z = z + bias
@@ -646,7 +648,7 @@ int musapy_distill_loss_grad_v1(const musapy_distill_args* args, hipStream_t str
  * Numbers of the history that are no column do not count.  Each of the penalties is an array of a number for each row, or
  * (NULL) its `_value`.  The bias is a row of `width` values, bias_pitch apart (0: one row for all), or, with `entries`
  * (at most 1024), values for the columns bias_index of each row: an index that is no column has no effect, and
- * biases of one column add up.  `allowed` is bytes, or 32-bit words whose lowest bits come first, in rows
+ * biases of one column add up; bias_dtype is `dtype` or F32.  `allowed` is bytes, or 32-bit words whose lowest bits come first, in rows
  * allowed_pitch bytes or words apart (0: one row for all). */
 enum { MUSAPY_ALLOWED_BYTES = 0, MUSAPY_ALLOWED_BITS = 1 };
 typedef struct {

@@ -267,7 +267,7 @@ extern "C" int musapy_adjust_logits_v1(const musapy_adjust_logits_args* a, hipSt
   if (a->rows == 0 || a->width == 0) return 0;
   const bool history = a->history != nullptr && a->length > 0;
   if (a->logits == nullptr || a->out == nullptr || (history && !vocab_id(a->history_dtype)) ||
-      (a->lengths != nullptr && !vocab_id(a->lengths_dtype)) || (a->bias != nullptr && !vocab_float(a->bias_dtype)) ||
+      (a->lengths != nullptr && !vocab_id(a->lengths_dtype)) || (a->bias != nullptr && a->bias_dtype != a->dtype && a->bias_dtype != MUSAPY_DT_F32) ||
       (a->entries > 0 && (a->bias == nullptr || a->bias_index == nullptr || !vocab_id(a->index_dtype))) ||
       (a->allowed != nullptr && a->allowed_kind != MUSAPY_ALLOWED_BYTES && a->allowed_kind != MUSAPY_ALLOWED_BITS))
     return vocab_bad();

@@ -519,8 +519,12 @@ int musapy_distill_loss_v1(const musapy_distill_args* a, void* scratch, size_t s
   DistillArgs p{};
   if (!distill_args(a, false, p)) return vocab_bad();
   if (p.rows == 0) return 0;
+  // The fewest waves a row that fill the chip's 8192, since a row takes some 6 us however short it is ((16384, 4000) bf16 29 us, with
+  // 256 threads a row 45, with 512 91).  But with more than 32 vectors a thread the larger workgroups are level or better.
+  const uint64_t vectors = uint64_t(p.width) * (a->dtype == MUSAPY_DT_F32 ? 4 : 2) / 16;
+  const unsigned block = p.rows >= 8192 && vectors <= 32 * 64 ? 64 : p.rows >= 2048 && vectors <= 32 * 256 ? 256 : 512;
   if (p.loss == nullptr || p.sums == nullptr || (p.width > 0 && p.logits == nullptr) ||
-      (p.entries > 0 && (p.index.at == nullptr || p.teacher == nullptr)) || !grid_fits(p.rows, 512))
+      (p.entries > 0 && (p.index.at == nullptr || p.teacher == nullptr)) || !grid_fits(p.rows, block))
     return vocab_bad();
   const size_t need = musapy_distill_loss_scratch_v1(a);
   if (need > 0 && (scratch == nullptr || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 3))) return vocab_bad(1);
@@ -538,11 +542,8 @@ int musapy_distill_loss_v1(const musapy_distill_args* a, void* scratch, size_t s
         k_distill_join<T, kS><<<p.rows, 64, 0, st>>>(p);
         return;
       }
-      // The fewest waves a row that fill the chip's 8192, since a row takes some 6 us however short it is ((16384, 4000) bf16 29 us, with
-      // 256 threads a row 45, with 512 91).  But with more than 32 vectors a thread the larger workgroups are level or better.
-      const uint64_t vectors = p.width * sizeof(T) / 16;
-      if (p.rows >= 8192 && vectors <= 32 * 64) k_distill_loss<T, 64, kS, false><<<p.rows, 64, 0, st>>>(p);
-      else if (p.rows >= 2048 && vectors <= 32 * 256) k_distill_loss<T, 256, kS, false><<<p.rows, 256, 0, st>>>(p);
+      if (block == 64) k_distill_loss<T, 64, kS, false><<<p.rows, 64, 0, st>>>(p);
+      else if (block == 256) k_distill_loss<T, 256, kS, false><<<p.rows, 256, 0, st>>>(p);
       else k_distill_loss<T, 512, kS, false><<<p.rows, 512, 0, st>>>(p);
     };
     if (two && a->temperature == 2.0f) go(std::integral_constant<int, kSquare>{});

@@ -491,7 +491,7 @@ inline EmbedGradPlan embed_grad_plan(const musapy_embedding_grad_args* a) {
     pl.tile = uint32_t((steps + kSortTiles - 1) / kSortTiles * kSortStep);
     pl.tiles = uint32_t((n + pl.tile - 1) / pl.tile);
   }
-  // Chunks of 8 to 64 tokens, some 500 of them: shorter ones keep more rows in flight (5003 tokens of 1111 f32 57 us with 8 or 16, 67
+  // Chunks of 8 to 64 tokens, some 500 of them, and of more from 131072 on: shorter ones keep more rows in flight (5003 tokens of 1111 f32 57 us with 8 or 16, 67
   // with 64), longer ones have fewer tokens that cross (65536 of 2048 bf16 280 us with 64, 311 with 8).
   pl.chunk = 8;
   while (n / pl.chunk > (pl.chunk < 64 ? 600 : 2048)) pl.chunk *= 2;
@@ -596,11 +596,9 @@ int launch_embedding_grad(const musapy_embedding_grad_args* a, char* ws, hipStre
   p.chunks = pl.chunks;
   p.tiles = uint32_t((a->width + 64 * n - 1) / (64 * n));
   p.scale = a->scale;
-  const uint64_t units = uint64_t(p.chunks) * p.tiles, grid = (units + 3) / 4;
-  const uint64_t joins = (pl.padded + 255) / 256;
-  if (units >= kVocabLimit || !grid_fits(grid, kEmbedBlock) || joins > 65535) return vocab_bad();
+  const uint64_t units = uint64_t(p.chunks) * p.tiles, grid = (units + 3) / 4;  // (at most 2049 by 2^14)
   launch_order(a, pl, ws, st);
-  const dim3 join(pl.chunks, unsigned(joins));
+  const dim3 join(pl.chunks, (pl.padded + 255) / 256);
   auto go = [&](auto N, auto ADD) {
     if (grid > 0) k_embed_sum<T, O, N.value, ADD.value><<<unsigned(grid), kEmbedBlock, 0, st>>>(p);
     if (pl.chunks > 1) k_embed_join<O, ADD.value><<<join, kEmbedBlock, 0, st>>>(p);
@@ -633,10 +631,13 @@ int musapy_embedding_v1(const musapy_embedding_args* a, hipStream_t st) {
   return rc;
 }
 
+// A row's columns, so that launches stay within a grid.
+constexpr uint64_t kGradColumns = uint64_t(1) << 22;
+
 static bool embedding_grad_ok(const musapy_embedding_grad_args* a) {
   return a != nullptr && vocab_float(a->dy_dtype) && vocab_float(a->out_dtype) && vocab_id(a->id_dtype) &&
          (a->accumulate == 0 || a->accumulate == 1) && a->tokens < kVocabLimit && a->rows < kVocabLimit &&
-         a->width < kVocabLimit;
+         a->width <= kGradColumns;
 }
 
 size_t musapy_embedding_grad_scratch_v1(const musapy_embedding_grad_args* a) {

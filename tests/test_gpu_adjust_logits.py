@@ -166,6 +166,21 @@ def test_no_rows_or_columns():
     assert ms.adjust_logits(ms.from_numpy(np.zeros((5, 0), np.float32))).shape == (5, 0)
 
 
+def test_offsets_past_32_bits():
+    """Logits and results past 2^32 elements: 8 GiB each."""
+    rows, width, kinds = 65601, 65544, 3
+    rng = np.random.default_rng(12)
+    z = R.draw(rng, (kinds, width), "bf16", 3.0)
+    kind = np.arange(rows) % kinds
+    Z = ms.embedding(R.to_device(z, "bf16"), R.ids(kind))
+    kw = some(rng, kinds, width, 40)
+    near = check(z, "bf16", **kw)
+    got = ms.adjust_logits(Z, **{k: ms.from_numpy(v[kind]) for k, v in kw.items()})
+    front = R.values(near)
+    for r in (0, 1, 2, 32767, 32768, 65527, 65528, 65529, rows - 2, rows - 1):
+        assert np.array_equal(R.values(got[r]), front[r % kinds]), r
+
+
 def test_refusals():
     z = ms.from_numpy(np.zeros((4, 40), np.float32))
     h, n = R.ids(np.zeros((4, 6), np.int64)), R.ids(np.zeros(4, np.int64))

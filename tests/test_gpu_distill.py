@@ -274,3 +274,32 @@ def test_few_long_rows(rows, width):
         rep = np.arange(rows) % few
         check(z[rep], index[rep], teacher[rep], label[rep], dt, "f32", 2.0, 0.5)
         check(z[rep], index[rep], teacher[rep], None, dt, "f32", 1.0, 1.0)
+
+
+def test_offsets_past_32_bits():
+    """Logits, and a gradient, that lie past 2^32 elements: two of 8 GiB.  Every row has the bits of the row of its kind near
+    the front: each is summed alike, as all begin on a multiple of 16 bytes."""
+    rows, width, kinds = 65601, 65544, 3
+    rng = np.random.default_rng(11)
+    z, index, teacher, label = inputs(rng, kinds, width, 7, "bf16", "f32")
+    kind = np.arange(rows) % kinds
+    Z = ms.embedding(R.to_device(z, "bf16"), R.ids(kind))
+    I, T, L = R.ids(index[kind]), R.to_device(teacher[kind], "f32"), R.ids(label[kind])
+    dl = np.linspace(0.5, 1.5, kinds, dtype=np.float32)
+    loss, sums = ms.distill_loss(Z, I, T, L, weight=0.5, temperature=2.0)
+    grad = ms.distill_loss_grad(ms.from_numpy(dl[kind]), Z, sums, I, T, L, weight=0.5, temperature=2.0)
+    assert np.array_equal(loss.numpy(), loss.numpy()[kind]) and np.array_equal(sums.numpy(), sums.numpy()[kind])
+    top = np.array([R.distill(z[r], index[r], teacher[r], label[r], 2.0, 0.5) for r in range(kinds)])
+    bound = np.array([R.distill_bound(z[r], index[r], teacher[r], label[r], 2.0, 0.5) for r in range(kinds)])
+    R.within(loss[:kinds], top[:, 0], bound[:, 0], "f32", "loss")
+    got = sums.numpy().astype(np.float64)
+    want = [R.distill_grad(dl[r], z[r], got[r], index[r], teacher[r], label[r], 2.0, 0.5) for r in range(kinds)]
+    room = [R.distill_grad_bound(dl[r], z[r], got[r], index[r], teacher[r], label[r], 2.0, 0.5) for r in range(kinds)]
+    R.within(grad[:kinds], np.stack(want), np.stack(room), "bf16", "gradient")
+    front = R.values(grad[:kinds])
+    for r in (32767, 32768, 65527, 65528, 65529, rows - 2, rows - 1):
+        assert np.array_equal(R.values(grad[r]), front[r % kinds]), r
+    # the same rows apart by a stride: two that lie 2^32 elements from each other
+    far = Z[::65529]
+    assert np.array_equal(ms.distill_loss(far, I[::65529], T[::65529], L[::65529], weight=0.5, temperature=2.0)[0].numpy(),
+                          loss.numpy()[[0, 65529]])

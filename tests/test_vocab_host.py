@@ -121,7 +121,7 @@ def test_embedding_grad_refusals():
     L = lib()
     base = dict(dy_dtype=F32, out_dtype=BF16, id_dtype=I64, scale=1, tokens=40, rows=8, width=16, dy=64, dy_pitch=16, ids=64, out=64)
     for kw in (dict(dy_dtype=F64), dict(out_dtype=I32), dict(id_dtype=F32), dict(accumulate=2), dict(tokens=1 << 31),
-               dict(rows=1 << 31), dict(width=1 << 31), dict(dy=None), dict(ids=None), dict(out=None)):
+               dict(rows=1 << 31), dict(width=(1 << 22) + 1), dict(width=1 << 31), dict(dy=None), dict(ids=None), dict(out=None)):
         refused(L.musapy_embedding_grad_v1, L, made(EmbedGradArgs, base, kw), 64, 1 << 40)
     refused(L.musapy_embedding_grad_v1, L, None, None, 0)
     a = made(EmbedGradArgs, base, {})
@@ -153,6 +153,10 @@ def test_distill_refusals():
         refused(fn, L, None, *scratch)
         assert fn(ctypes.byref(made(DistillArgs, base, dict(rows=0, logits=None))), *scratch, None) == 0
     refused(L.musapy_distill_loss_v1, L, made(DistillArgs, base, dict(loss=None)), None, 0)
+    # more workgroups than a launch has: a wave a row, eight a row, one for each 4 KB and one more
+    for kw in (dict(rows=1 << 26), dict(rows=1 << 23, width=40000)):
+        refused(L.musapy_distill_loss_v1, L, made(DistillArgs, base, kw), None, 0)
+    refused(L.musapy_distill_loss_grad_v1, L, made(DistillArgs, base, dict(rows=1 << 25)))
     # few long rows go through scratch
     assert L.musapy_distill_loss_scratch_v1(ctypes.byref(made(DistillArgs, base, {}))) == 0
     long = made(DistillArgs, base, dict(width=1 << 20, pitch=1 << 20))
@@ -172,7 +176,7 @@ def test_adjust_refusals():
                 rows=4, width=100, length=10, entries=3, logits=64, pitch=100, history=64, history_pitch=10, lengths=64,
                 repetition_value=1, bias=64, bias_pitch=3, bias_index=64, index_pitch=3, allowed=64, allowed_pitch=100, out=64)
     fn = L.musapy_adjust_logits_v1
-    for kw in (dict(dtype=F64), dict(out_dtype=9), dict(history_dtype=F32), dict(lengths_dtype=F32), dict(bias_dtype=I32),
+    for kw in (dict(dtype=F64), dict(out_dtype=9), dict(history_dtype=F32), dict(lengths_dtype=F32), dict(bias_dtype=I32), dict(dtype=F32, bias_dtype=BF16), dict(rows=1 << 23),
                dict(index_dtype=F32), dict(allowed_kind=2), dict(rows=1 << 31), dict(width=1 << 31), dict(length=1 << 31),
                dict(entries=1025), dict(logits=None), dict(out=None), dict(bias=None), dict(bias_index=None)):
         refused(fn, L, made(AdjustArgs, base, kw))
