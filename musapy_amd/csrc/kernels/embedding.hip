@@ -141,6 +141,54 @@ __device__ inline void order_clear(const OrderArgs& p, uint32_t block) {
   if (threadIdx.x < 16 ? edge < head : edge < p.zero_bytes) p.zero[edge] = 0;
 }
 
+// Up to kRankMost tokens, in one launch: a token's place is the number of tokens in front of it, counted against all others.  All
+// lie in LDS; a workgroup places 16 tokens, and sixteen threads to each count a sixteenth of the others, four at a time.  (With the
+// order in two launches, as below, the gradient of 1584 tokens took 20 us, so 14, and of 4096 25.2, so 21.2.)
+constexpr int kRankBlock = 256, kRankTokens = 16, kRankMost = 4096;
+
+__global__ __launch_bounds__(kRankBlock) void k_embed_rank(OrderArgs p) {
+  if (blockIdx.x >= p.order_blocks) return order_clear<kRankBlock>(p, blockIdx.x - p.order_blocks);
+  typedef uint32_t W __attribute__((ext_vector_type(4)));
+  extern __shared__ W groups[];  // four tokens each
+  __shared__ uint32_t part[kRankBlock / 64][kRankTokens];
+  uint32_t* all = reinterpret_cast<uint32_t*>(groups);
+  const uint32_t most = (p.n + 63) / 64 * 64;
+  for (uint32_t base = threadIdx.x; base < most; base += 8 * kRankBlock) {
+    RawId raw[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint32_t i = base + u * kRankBlock;
+      raw[u] = id_load(p.ids, i < p.n ? i : p.n - 1);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint32_t i = base + u * kRankBlock;
+      if (i < most) all[i] = i < p.n ? id_of(raw[u], p.rows) : ~0u;
+    }
+  }
+  __syncthreads();
+  const uint32_t item = threadIdx.x % kRankTokens, share = threadIdx.x / kRankTokens;
+  const uint32_t at = blockIdx.x * kRankTokens + item, own = at / 4;
+  const uint32_t key = all[at];
+  uint32_t count = 0;
+#pragma unroll 4
+  for (uint32_t g = share; g < most / 4; g += kRankBlock / kRankTokens) {
+    const W k = groups[g];
+    const uint32_t limit = g < own ? key + 1 : key;  // equals count in front of the token
+#pragma unroll
+    for (int e = 0; e < 4; ++e) count += k[e] < limit ? 1 : 0;
+  }
+  count += uint32_t(__shfl_xor(int(count), 16, kWave));
+  count += uint32_t(__shfl_xor(int(count), 32, kWave));
+  if (threadIdx.x % 64 < kRankTokens) part[threadIdx.x / 64][item] = count;
+  __syncthreads();
+  if (threadIdx.x >= kRankTokens || at >= p.n) return;
+  for (int w = 1; w < kRankBlock / 64; ++w) count += part[w][item];
+  for (uint32_t e = 0; e < at % 4; ++e) count += all[own * 4 + e] == key ? 1 : 0;
+  p.keys[count] = key;
+  p.pos[count] = at;
+}
+
 // Up to 16384 tokens, in two launches.  First, blocks of 256 tokens: a token's place in its block is the number of tokens
 // in front of it, counted against all others of the block.
 constexpr int kBlockTokens = 256, kOrderBlock = 1024, kOrderWaves = kOrderBlock / 64;
@@ -470,9 +518,155 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embed_join(EmbedGradArgs p) {
   }
 }
 
+// ---- gradient: few tokens --------------------------------------------------------------------------------
+// In one launch: a wave takes 1 KB of the table's gradient, a vector a lane, finds the tokens of its rows among all, and adds up
+// their rows of dy; most find none and clear.
+constexpr int kGatherMost = 256;
+
+struct EmbedGatherArgs {
+  Ids ids;
+  uint32_t n, rows, width;
+  const void* dy;
+  uint64_t pitch;
+  void* out;
+  uint32_t total, head, vectors;  // values, those in front of the first address that is a multiple of 16 bytes, vectors behind them
+  FastDiv wdiv;                   // divides by the width
+  float scale;
+};
+
+// K: tokens a lane looks at.  EVEN: every vector lies in one row.  Else one may end a row and begin the next (width >= N): its first
+// values are summed as the last N of its row, the others as the first N of the next.
+template <class T, class O, int K, bool EVEN>
+__global__ __launch_bounds__(kEmbedBlock) void k_embed_gather(EmbedGatherArgs p) {
+  constexpr int N = 16 / int(sizeof(O)), kRows = 128 / int(sizeof(T) * N);  // rows of dy in flight, in 32 registers
+  __shared__ uint2 lists[kEmbedBlock / 64][K * 64];  // token and place of each that is found, in order of places
+  const uint32_t lane = threadIdx.x % 64, wave = wave_uniform(threadIdx.x / 64);
+  RawId raw[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const uint32_t i = k * 64 + lane;
+    raw[k] = p.n > 0 ? id_load(p.ids, i < p.n ? i : p.n - 1) : RawId{0, 1};
+  }
+  const uint32_t base = blockIdx.x * kEmbedBlock + wave * 64, at = base + lane;
+  if (base > 0 && base >= p.vectors) return;
+  const bool ends = base + 64 >= p.vectors;
+  const uint32_t first = base == 0 ? 0 : p.head + base * N, past = ends ? p.total : p.head + (base + 64) * N;
+  const uint32_t low = fd_div(p.wdiv, first), high = fd_div(p.wdiv, past - 1);
+  uint2* list = lists[wave];
+  uint32_t count = 0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const uint32_t token = id_of(raw[k], p.rows);
+    const uint64_t here = __ballot(k * 64 + lane < p.n && token >= low && token <= high);
+    if (here == 0) continue;
+    if ((here >> lane) & 1) list[count + uint32_t(__popcll(here & ((uint64_t(1) << lane) - 1)))] = uint2{token, k * 64 + lane};
+    count += uint32_t(__popcll(here));
+  }
+  O* out = static_cast<O*>(p.out);
+  // a value of its own in front of the vectors (the first wave's) or behind them (the last one's)
+  uint32_t lone = p.total;
+  if (base == 0 && lane < p.head) lone = lane;
+  if (ends && lane >= 32 && lane < 32 + N) lone = p.head + p.vectors * N + lane - 32;
+  if (count == 0) {
+    if (at < p.vectors) vstore_el<false, O, N>(out + p.head + at * N, Vec<O, N>{});
+    if (lone < p.total) out[lone] = O(0.0f);
+    return;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  const T* dy = static_cast<const T*>(p.dy);
+  if (at < p.vectors) {
+    const uint32_t value = p.head + at * N, row = fd_div(p.wdiv, value), col = value - row * p.width;
+    const uint32_t cut = EVEN || p.width - col > uint32_t(N) ? uint32_t(N) : p.width - col;  // values of `row`
+    const uint32_t next = EVEN || cut == uint32_t(N) ? row : row + 1, from = EVEN || cut == uint32_t(N) ? col : p.width - N;
+    float sum[N] = {}, sum2[N] = {};
+    for (uint32_t b = 0; b < count; b += kRows) {
+      Vec<T, N> v[kRows];
+      uint32_t whose[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const uint2 l = list[b + i < count ? b + i : count - 1];
+        whose[i] = b + i < count ? l.x : p.rows;
+        v[i] = vload_el<T, N, true>(dy + l.y * p.pitch + (EVEN || l.x == row ? from : 0));
+      }
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          sum[e] += whose[i] == row ? float(v[i].v[e]) : 0.0f;
+          if (!EVEN) sum2[e] += whose[i] == next ? float(v[i].v[e]) : 0.0f;
+        }
+      }
+    }
+    Vec<O, N> o;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      float x = sum[e];
+      if (!EVEN && cut < uint32_t(N)) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if (uint32_t(e) < cut ? e + N == int(cut) + j : e == int(cut) + j) x = uint32_t(e) < cut ? sum[j] : sum2[j];
+        }
+      }
+      o.v[e] = O(x * p.scale);
+    }
+    vstore_el<false, O, N>(out + value, o);
+  }
+  if (lone < p.total) {
+    const uint32_t row = fd_div(p.wdiv, lone), col = lone - row * p.width;
+    float sum = 0.0f;
+#pragma unroll 8
+    for (uint32_t b = 0; b < count; ++b) {
+      const uint2 l = list[b];
+      const float x = float(dy[l.y * p.pitch + col]);
+      sum += l.x == row ? x : 0.0f;
+    }
+    out[lone] = O(sum * p.scale);
+  }
+}
+
+// Whether a gradient goes that way: not one that is added to what is there, whose rows without tokens are not touched.  Up to 64
+// tokens, one a lane, (131072, 1024) f32 takes 79 us at 6.8 TB/s, by an order and sums 87, and a table of a few MB 6, so 10 to 14.  With 250
+// tokens a wave's search costs more than a launch where the table is large ((131072, 2048) f32 209 us, so 165; (16384, 1024) 20.4 and
+// 18.7; (8704, 232) 6.6 and 14.7).  A wave's time grows by 0.12 us for every row that one token has (256 rows of one 32 us, so 16).
+constexpr uint64_t kGatherBytes = uint64_t(32) << 20;
+inline bool embed_gathers(const musapy_embedding_grad_args* a) {
+  const uint64_t size = a->out_dtype == MUSAPY_DT_F32 ? 4 : 2, values = a->rows * a->width;
+  return !a->accumulate && a->width >= 16 / size && values < kVocabLimit &&
+         (a->tokens <= 64 || (a->tokens <= uint64_t(kGatherMost) && values * size <= kGatherBytes));
+}
+
+template <class T, class O>
+int launch_embedding_gather(const musapy_embedding_grad_args* a, hipStream_t st) {
+  constexpr uint32_t kN = 16 / sizeof(O);
+  EmbedGatherArgs p{};
+  p.ids = vocab_ids(a->ids, a->id_dtype);
+  p.n = uint32_t(a->tokens);
+  p.rows = uint32_t(a->rows);
+  p.width = uint32_t(a->width);
+  p.dy = a->dy;
+  p.pitch = a->dy_pitch;
+  p.out = a->out;
+  p.total = uint32_t(a->rows * a->width);
+  const uint32_t past = uint32_t(reinterpret_cast<uintptr_t>(a->out) / sizeof(O) % kN);
+  p.head = past == 0 ? 0 : kN - past;  // (a row has as many)
+  p.vectors = (p.total - p.head) / kN;
+  p.wdiv = make_fastdiv(p.width);
+  p.scale = a->scale;
+  const unsigned grid = p.vectors == 0 ? 1 : (p.vectors + kEmbedBlock - 1) / kEmbedBlock;
+  auto go = [&](auto K, auto EVEN) { k_embed_gather<T, O, K.value, EVEN.value><<<grid, kEmbedBlock, 0, st>>>(p); };
+  using All = std::integral_constant<int, kGatherMost / 64>;
+  using One = std::integral_constant<int, 1>;
+  const bool even = p.head == 0 && p.width % kN == 0;
+  if (p.n <= 64 && even) go(One{}, std::true_type{});
+  else if (p.n <= 64) go(One{}, std::false_type{});
+  else if (even) go(All{}, std::true_type{});
+  else go(All{}, std::false_type{});
+  return 0;
+}
+
 // ---- launches -------------------------------------------------------------------------------------------
 struct EmbedGradPlan {
-  int passes, bits;         // 0 passes: by blocks
+  int passes, bits;         // 0 passes: by rank or by blocks
   uint32_t tile, tiles;     // of a pass
   uint32_t chunk, chunks;
   uint32_t padded;
@@ -504,7 +698,7 @@ inline EmbedGradPlan embed_grad_plan(const musapy_embedding_grad_args* a) {
   };
   pl.keys = take(n * 4);
   pl.pos = take(n * 4);
-  if (n > uint64_t(kBlockTokens)) {
+  if (n > uint64_t(kRankMost)) {
     pl.keys2 = take(n * 4);
     pl.pos2 = take(n * 4);
   }
@@ -541,13 +735,17 @@ inline void launch_order(const musapy_embedding_grad_args* a, const EmbedGradPla
     return unsigned(order + (pieces + o.zero_pieces - 1) / o.zero_pieces);
   };
   const uint64_t most = bytes - beside * uint64_t(launches - 1);  // of the first launch
+  if (o.n <= uint32_t(kRankMost)) {
+    o.keys = keys[0];
+    o.pos = pos[0];
+    const unsigned count = grid((o.n + kRankTokens - 1) / kRankTokens, kRankBlock, most);
+    if (count > 0) k_embed_rank<<<count, kRankBlock, (o.n + 63) / 64 * 256, st>>>(o);
+    return;
+  }
   if (pl.passes == 0) {
-    const bool one = blocks <= 1;
-    o.keys = keys[one ? 0 : 1];
-    o.pos = pos[one ? 0 : 1];
-    const unsigned first = grid(blocks, kBlockTokens, most);
-    if (first > 0) k_embed_blocks<<<first, kBlockTokens, 0, st>>>(o);
-    if (one) return;
+    o.keys = keys[1];
+    o.pos = pos[1];
+    k_embed_blocks<<<grid(blocks, kBlockTokens, most), kBlockTokens, 0, st>>>(o);
     o.keys_in = o.keys;
     o.pos_in = o.pos;
     o.keys = keys[0];
@@ -641,7 +839,7 @@ static bool embedding_grad_ok(const musapy_embedding_grad_args* a) {
 }
 
 size_t musapy_embedding_grad_scratch_v1(const musapy_embedding_grad_args* a) {
-  if (!embedding_grad_ok(a) || a->tokens == 0 || a->rows == 0 || a->width == 0) return 0;
+  if (!embedding_grad_ok(a) || a->tokens == 0 || a->rows == 0 || a->width == 0 || embed_gathers(a)) return 0;
   return embed_grad_plan(a).bytes;
 }
 
@@ -655,7 +853,8 @@ int musapy_embedding_grad_v1(const musapy_embedding_grad_args* a, void* scratch,
   int rc = 0;
   vocab_type(a->dy_dtype, [&](auto t) {
     vocab_type(a->out_dtype, [&](auto o) {
-      rc = launch_embedding_grad<decltype(t), decltype(o)>(a, static_cast<char*>(scratch), st);
+      if (embed_gathers(a)) rc = launch_embedding_gather<decltype(t), decltype(o)>(a, st);
+      else rc = launch_embedding_grad<decltype(t), decltype(o)>(a, static_cast<char*>(scratch), st);
     });
   });
   return rc;

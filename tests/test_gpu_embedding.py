@@ -90,6 +90,35 @@ def test_gradient_numbers_of_tokens(n, rows):
     grad(R.draw(rng, (n, 9), "f32"), tokens, rows, 0.5, "f32", "f32")
 
 
+@pytest.mark.parametrize("n,rows,width", [(255, 300, 40), (256, 300, 40), (257, 300, 40), (64, 20, 2100), (65, 20, 2100), (64, 8200, 1030),
+                                          (200, 8200, 1030), (200, 5, 4), (4095, 50, 24), (4096, 5000, 24), (4097, 50, 24)])
+@pytest.mark.parametrize("dt,to", [("bf16", "f32"), ("f32", "bf16"), ("f32", "f32"), ("f16", "f16")])
+def test_gradient_from_way_to_way(n, rows, width, dt, to):
+    """At the numbers of tokens, and the sizes of a table, where one way ends and the next begins."""
+    rng = np.random.default_rng(n + width)
+    tokens = (rows ** rng.random(n)).astype(np.int64) - rng.integers(0, 2, n)
+    grad(R.draw(rng, (n, width), dt), tokens, rows, 0.5, dt, to, "i32")
+
+
+@pytest.mark.parametrize("to", ["f32", "bf16"])
+@pytest.mark.parametrize("width", [4, 8, 9, 13, 64, 255, 1001])
+@pytest.mark.parametrize("n", [0, 1, 30, 150, 600])
+def test_gradient_into_part_of_an_array(n, width, to):
+    """Rows that begin and end between two multiples of 16 bytes, with other rows around them."""
+    rng = np.random.default_rng(n + width)
+    dy = R.draw(rng, (n, width), "f32")
+    for before in (1, 2, 3):
+        rows = 41
+        tokens = np.sort((rows ** rng.random(n)).astype(np.int64) - 1)[::-1].copy()
+        whole = R.to_device(np.full((before + rows + 2, width), 7.0), to)
+        part = whole[before:before + rows]
+        got = ms.embedding_grad(R.to_device(dy, "f32"), R.ids(tokens), rows, 1.0, out=part)
+        want, bound = R.embedding_grad(dy, tokens, rows, 1.0)
+        R.within(got, want, bound, to)
+        v = R.values(whole)
+        assert (v[:before] == 7).all() and (v[before + rows:] == 7).all()
+
+
 def test_gradient_three_passes():
     rng = np.random.default_rng(5)
     grad(R.draw(rng, (20000, 4), "bf16"), rng.integers(0, 300001, 20000), 300001, 1.0, "bf16", "bf16")
@@ -165,6 +194,19 @@ def test_offsets_past_32_bits():
     assert not R.values(out[rows - 2]).any() and not R.values(out[6]).any()
     got = ms.embedding(out, R.ids([rows - 1, 0, 5, rows]), 3.0)
     assert np.array_equal(R.values(got), np.repeat([[6.0], [0.0], [3.0], [0.0]], width, 1))
+
+
+def test_offsets_near_31_bits():
+    """Few tokens and a gradient of just below 2^31 values: 8 GiB of f32, begun 8 bytes off."""
+    rows, width = 65524, 32774
+    assert rows * width < 1 << 31 < (rows + 1) * width
+    whole = ms.embedding(R.to_device(np.ones((1, width)), "f32"), R.ids(np.zeros(rows + 1)))
+    out = whole[1:]
+    ms.embedding_grad(R.to_device(np.ones((3, width)), "f32"), R.ids([rows - 1, 5, rows - 1]), rows, out=out)
+    assert R.values(out[rows - 1]).tolist() == [2.0] * width and R.values(out[5]).tolist() == [1.0] * width
+    assert not R.values(out[rows - 2]).any() and not R.values(out[6]).any() and not R.values(out[0]).any()
+    assert R.values(whole[0]).tolist() == [1.0] * width
+    assert R.values(ms.max(out[6:rows - 1])) == 0.0
 
 
 def test_refusals():

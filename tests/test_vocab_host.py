@@ -119,7 +119,7 @@ def test_embedding_refusals():
 @no_gpu
 def test_embedding_grad_refusals():
     L = lib()
-    base = dict(dy_dtype=F32, out_dtype=BF16, id_dtype=I64, scale=1, tokens=40, rows=8, width=16, dy=64, dy_pitch=16, ids=64, out=64)
+    base = dict(dy_dtype=F32, out_dtype=BF16, id_dtype=I64, scale=1, tokens=600, rows=8, width=16, dy=64, dy_pitch=16, ids=64, out=64)
     for kw in (dict(dy_dtype=F64), dict(out_dtype=I32), dict(id_dtype=F32), dict(accumulate=2), dict(tokens=1 << 31),
                dict(rows=1 << 31), dict(width=(1 << 22) + 1), dict(width=1 << 31), dict(dy=None), dict(ids=None), dict(out=None)):
         refused(L.musapy_embedding_grad_v1, L, made(EmbedGradArgs, base, kw), 64, 1 << 40)
