@@ -189,70 +189,95 @@ __global__ __launch_bounds__(kRankBlock) void k_embed_rank(OrderArgs p) {
   p.pos[count] = at;
 }
 
-// Up to 16384 tokens, in two launches.  First, blocks of 256 tokens: a token's place in its block is the number of tokens
-// in front of it, counted against all others of the block.
+// Up to kOrderMost tokens, in two launches.  First, blocks of 256 tokens, a quarter of one a workgroup: a token's place in its block
+// is the number of tokens in front of it, counted by each wave against a quarter of the block.
 constexpr int kBlockTokens = 256, kOrderBlock = 1024, kOrderWaves = kOrderBlock / 64;
-constexpr int kOrderMost = 16384;
+constexpr int kOrderMost = 32768;
 
 __global__ __launch_bounds__(kBlockTokens) void k_embed_blocks(OrderArgs p) {
   if (blockIdx.x >= p.order_blocks) return order_clear<kBlockTokens>(p, blockIdx.x - p.order_blocks);
-  __shared__ uint32_t all[kBlockTokens];
-  const uint32_t item = threadIdx.x, wave = wave_uniform(threadIdx.x / 64);
-  const uint32_t first = blockIdx.x * kBlockTokens;
-  const uint32_t key = first + item < p.n ? id_at(p.ids, first + item, p.rows) : ~0u;
-  all[item] = key;
+  typedef uint32_t W __attribute__((ext_vector_type(4)));
+  __shared__ W groups[kBlockTokens / 4];
+  __shared__ uint32_t part[kBlockTokens / 64][64];
+  uint32_t* all = reinterpret_cast<uint32_t*>(groups);
+  const uint32_t lane = threadIdx.x % 64, wave = wave_uniform(threadIdx.x / 64), quarter = blockIdx.x % 4;
+  const uint32_t first = blockIdx.x / 4 * kBlockTokens, at = first + quarter * 64 + lane;
+  all[threadIdx.x] = first + threadIdx.x < p.n ? id_at(p.ids, first + threadIdx.x, p.rows) : ~0u;
   __syncthreads();
+  const uint32_t key = all[quarter * 64 + lane];
+  const uint32_t limit = wave < quarter ? key + 1 : key;  // equals count in front of the token (a missing one's limit is not used)
   uint32_t count = 0;
-#pragma unroll 1
-  for (uint32_t w = 0; w < kBlockTokens / 64; ++w) {
-    const uint32_t limit = w < wave ? key + 1 : key;  // equals count in front of the token (a missing one's limit is not used)
-#pragma unroll 16
-    for (uint32_t j = 0; j < 64; ++j) count += all[w * 64 + j] < limit ? 1 : 0;
-  }
-#pragma unroll 16
-  for (uint32_t j = 0; j < 64; ++j) count += all[wave * 64 + j] == key && j < item % 64 ? 1 : 0;
-  if (first + item >= p.n) return;
-  p.keys[first + count] = key;
-  p.pos[first + count] = first + item;
-}
-
-// Then a token's place among all is its place in its block and, of every other block, the number of keys below
-// its own (or not above it, of the blocks in front), each found by halving.  All keys lie in LDS; a workgroup places 64
-// tokens, and each of its 16 waves searches every sixteenth block, four at a time.
-__global__ __launch_bounds__(kOrderBlock) void k_embed_merge(OrderArgs p) {
-  extern __shared__ uint32_t all[];
-  __shared__ uint32_t part[kOrderWaves][64];
-  const uint32_t blocks = (p.n + kBlockTokens - 1) / kBlockTokens;
-  for (uint32_t i = threadIdx.x; i < blocks * kBlockTokens; i += kOrderBlock) all[i] = i < p.n ? p.keys_in[i] : ~0u;
-  __syncthreads();
-  const int lane = threadIdx.x % 64;
-  const uint32_t wave = wave_uniform(threadIdx.x / 64);
-  const uint32_t at = blockIdx.x * 64 + lane, own = blockIdx.x * 64 / kBlockTokens;
-  const uint32_t key = all[at];
-  uint32_t count = 0;
-  for (uint32_t b0 = wave; b0 < blocks; b0 += 4 * kOrderWaves) {
-    uint32_t base[4], limit[4], c[4] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t b = b0 + i * kOrderWaves;
-      base[i] = b < blocks ? b * kBlockTokens : 0;
-      limit[i] = b < blocks && b != own ? key + (b < own ? 1 : 0) : 0;  // nothing is below 0
+  for (uint32_t g = 0; g < 16; ++g) {
+    const W k = groups[wave * 16 + g];
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+      count += k[e] < limit ? 1 : 0;
+      if (wave == quarter) count += k[e] == key && g * 4 + e < lane ? 1 : 0;
     }
-#pragma unroll
-    for (uint32_t step = kBlockTokens / 2; step > 0; step /= 2)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] += all[base[i] + c[i] + step - 1] < limit[i] ? step : 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) count += c[i] + (all[base[i] + c[i]] < limit[i] ? 1 : 0);
   }
   part[wave][lane] = count;
   __syncthreads();
   if (wave != 0 || at >= p.n) return;
-  uint32_t to = at - own * kBlockTokens;
+  count = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+  p.keys[first + count] = key;
+  p.pos[first + count] = at;
+}
+
+// Then a token's place among all is its place in its block and, of every other block, the number of keys below
+// its own (or not above it, of the blocks in front), each found by halving.  All keys lie in LDS; a workgroup places 64
+// tokens at a time, 128 in all beyond 16384, where one workgroup has a CU for itself, and each of its 16 waves searches every sixteenth
+// block, four at a time.  (26784 tokens 9.8 us behind some 4 for the blocks; in passes over their digits 33.)
+__global__ __launch_bounds__(kOrderBlock) void k_embed_merge(OrderArgs p) {
+  typedef uint32_t W __attribute__((ext_vector_type(4)));
+  extern __shared__ W sorted[];
+  __shared__ uint32_t part[kOrderWaves][64];
+  uint32_t* all = reinterpret_cast<uint32_t*>(sorted);
+  const uint32_t blocks = (p.n + kBlockTokens - 1) / kBlockTokens, vectors = p.n / 4;
+  for (uint32_t base = threadIdx.x; base < vectors; base += 4 * kOrderBlock) {
+    W k[4];
 #pragma unroll
-  for (int w = 0; w < kOrderWaves; ++w) to += part[w][lane];
-  p.keys[to] = key;
-  p.pos[to] = p.pos_in[at];
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t i = base + u * kOrderBlock;
+      k[u] = reinterpret_cast<const W*>(p.keys_in)[i < vectors ? i : vectors - 1];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (base + u * kOrderBlock < vectors) sorted[base + u * kOrderBlock] = k[u];
+  }
+  for (uint32_t i = vectors * 4 + threadIdx.x; i < blocks * kBlockTokens; i += kOrderBlock) all[i] = i < p.n ? p.keys_in[i] : ~0u;
+  __syncthreads();
+  const int lane = threadIdx.x % 64;
+  const uint32_t wave = wave_uniform(threadIdx.x / 64);
+  for (uint32_t set = blockIdx.x; set * 64 < p.n; set += gridDim.x) {
+    const uint32_t at = set * 64 + lane, own = set * 64 / kBlockTokens;
+    const uint32_t key = all[at];
+    uint32_t count = 0;
+    for (uint32_t b0 = wave; b0 < blocks; b0 += 4 * kOrderWaves) {
+      uint32_t base[4], limit[4], c[4] = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t b = b0 + i * kOrderWaves;
+        base[i] = b < blocks ? b * kBlockTokens : 0;
+        limit[i] = b < blocks && b != own ? key + (b < own ? 1 : 0) : 0;  // nothing is below 0
+      }
+#pragma unroll
+      for (uint32_t step = kBlockTokens / 2; step > 0; step /= 2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] += all[base[i] + c[i] + step - 1] < limit[i] ? step : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) count += c[i] + (all[base[i] + c[i]] < limit[i] ? 1 : 0);
+    }
+    if (set != blockIdx.x) __syncthreads();
+    part[wave][lane] = count;
+    __syncthreads();
+    if (wave != 0 || at >= p.n) continue;
+    uint32_t to = at - own * kBlockTokens;
+#pragma unroll
+    for (int w = 0; w < kOrderWaves; ++w) to += part[w][lane];
+    p.keys[to] = key;
+    p.pos[to] = p.pos_in[at];
+  }
 }
 
 // More tokens: passes over up to nine bits each, lowest first; a pass counts its digits in every tile of
@@ -401,14 +426,15 @@ __device__ inline void embed_store(O* at, int skip, const float (&sum)[N], float
   }
 }
 
-// A wave sums a chunk of the order over 64 * N columns, eight rows of dy in flight, and stores a row of the
+// A wave sums a chunk of the order over 64 * N columns and stores a row of the
 // table wherever the token changes.  What belongs to a token that the chunk shares with a neighbour goes to a
 // slot in f32.  A row's last columns overlap as in the lookup; `skip` of them are the neighbour's where the
 // store adds to what is there.
-constexpr int kEmbedRows = 8;
+
 
 template <class T, class O, int N, bool ADD>
 __global__ __launch_bounds__(kEmbedBlock) void k_embed_sum(EmbedGradArgs p) {
+  constexpr int kEmbedRows = N * sizeof(T) > 16 ? 4 : 8;
   const int lane = threadIdx.x % 64;
   const uint32_t unit = blockIdx.x * (kEmbedBlock / 64) + wave_uniform(threadIdx.x / 64);
   const uint32_t chunk = unit / p.tiles;
@@ -419,10 +445,13 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embed_sum(EmbedGradArgs p) {
   const int skip = active ? int(c - col) : 0;
   const uint32_t first = chunk * p.chunk;
   const uint32_t last = p.n - first < p.chunk ? p.n : first + p.chunk;
-  uint32_t cur = wave_uniform(p.keys[first]);
+  // the first 64 tokens of the chunk and its neighbours, all on their way at once
+  uint32_t key = p.keys[first + lane < last ? first + lane : last - 1], place = p.pos[first + lane < last ? first + lane : last - 1];
+  const uint32_t before = p.keys[first > 0 ? first - 1 : 0], behind = p.keys[last < p.n ? last : p.n - 1];
+  uint32_t cur = wave_uniform(key);
   if (cur >= p.rows) return;
-  bool shared = first > 0 && wave_uniform(p.keys[first - 1]) == cur;  // the run began in front of the chunk
-  const uint32_t next = last < p.n ? wave_uniform(p.keys[last]) : ~0u;
+  bool shared = first > 0 && wave_uniform(before) == cur;  // the run began in front of the chunk
+  const uint32_t next = last < p.n ? wave_uniform(behind) : ~0u;
   const T* dy = static_cast<const T*>(p.dy) + col;
   float sum[N] = {};
 
@@ -442,17 +471,25 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embed_sum(EmbedGradArgs p) {
     for (int e = 0; e < N; ++e) sum[e] = 0.0f;
   };
 
+  // As many rows are added up while the next are on their way: a load behind a store is waited for with it, and stores are slow (100000
+  // tokens of 1024 bf16 113.8 us, so 118.9).
+  Vec<T, N> va[kEmbedRows], vb[kEmbedRows];
   for (uint32_t base = first; base < last; base += 64) {
-    const uint32_t at = base + lane;
-    const uint32_t key = at < last ? p.keys[at] : ~0u, place = at < last ? p.pos[at] : 0;
+    if (base > first) {
+      const uint32_t at = base + lane < last ? base + lane : last - 1;
+      key = p.keys[at];
+      place = p.pos[at];
+    }
     const int count = last - base < 64 ? int(last - base) : 64;
-    for (int i = 0; i < count; i += kEmbedRows) {
-      Vec<T, N> v[kEmbedRows];
+    auto fetch = [&](Vec<T, N>(&v)[kEmbedRows], int i) {
+      if (i >= count) return;
 #pragma unroll
       for (int u = 0; u < kEmbedRows; ++u) {
         const int j = i + u < count ? i + u : count - 1;
         v[u] = vload_el<T, N, true>(dy + uint64_t(uint32_t(__builtin_amdgcn_readlane(int(place), j))) * p.pitch);
       }
+    };
+    auto add = [&](const Vec<T, N>(&v)[kEmbedRows], int i) {
 #pragma unroll
       for (int u = 0; u < kEmbedRows; ++u) {
         if (i + u >= count) continue;
@@ -465,6 +502,13 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embed_sum(EmbedGradArgs p) {
 #pragma unroll
         for (int e = 0; e < N; ++e) sum[e] += float(v[u].v[e]);
       }
+    };
+    fetch(va, 0);
+    for (int i = 0; i < count; i += 2 * kEmbedRows) {
+      fetch(vb, i + kEmbedRows);
+      add(va, i);
+      fetch(va, i + 2 * kEmbedRows);
+      add(vb, i + kEmbedRows);
     }
   }
   store(next == cur);
@@ -685,10 +729,11 @@ inline EmbedGradPlan embed_grad_plan(const musapy_embedding_grad_args* a) {
     pl.tile = uint32_t((steps + kSortTiles - 1) / kSortTiles * kSortStep);
     pl.tiles = uint32_t((n + pl.tile - 1) / pl.tile);
   }
-  // Chunks of 8 to 64 tokens, some 500 of them, and of more from 131072 on: shorter ones keep more rows in flight (5003 tokens of 1111 f32 57 us with 8 or 16, 67
-  // with 64), longer ones have fewer tokens that cross (65536 of 2048 bf16 280 us with 64, 311 with 8).
+  // Chunks of 8 to 64 tokens that give some 4096 waves (longer ones beyond 131072 tokens): shorter ones keep more rows in flight (20000
+  // tokens of 512 bf16 47 us, so 57 with chunks of 64; 5003 of 1111 f32 57 and 67), longer ones have fewer tokens that cross.
   pl.chunk = 8;
-  while (n / pl.chunk > (pl.chunk < 64 ? 600 : 2048)) pl.chunk *= 2;
+  const uint64_t tiles = (a->width + 255) / 256;
+  while ((pl.chunk < 64 && n / pl.chunk * tiles > 4096) || n / pl.chunk > 2048) pl.chunk *= 2;
   pl.chunks = uint32_t((n + pl.chunk - 1) / pl.chunk);
   pl.padded = uint32_t((a->width + 3) / 4 * 4);
   auto take = [&](size_t bytes) {
@@ -745,12 +790,13 @@ inline void launch_order(const musapy_embedding_grad_args* a, const EmbedGradPla
   if (pl.passes == 0) {
     o.keys = keys[1];
     o.pos = pos[1];
-    k_embed_blocks<<<grid(blocks, kBlockTokens, most), kBlockTokens, 0, st>>>(o);
+    k_embed_blocks<<<grid((o.n + 63) / 64, kBlockTokens, most), kBlockTokens, 0, st>>>(o);
     o.keys_in = o.keys;
     o.pos_in = o.pos;
     o.keys = keys[0];
     o.pos = pos[0];
-    k_embed_merge<<<(o.n + 63) / 64, kOrderBlock, blocks * kBlockTokens * 4, st>>>(o);
+    const unsigned sets = (o.n + 63) / 64;
+    k_embed_merge<<<o.n > 16384 ? (sets + 1) / 2 : sets, kOrderBlock, blocks * kBlockTokens * 4, st>>>(o);
     return;
   }
   o.hist = reinterpret_cast<uint32_t*>(ws + pl.hist);

@@ -81,7 +81,7 @@ def test_gradient(dt, to, width):
         grad(R.draw(rng, (n, width), dt), rng.integers(-2, rows + 2, n), rows, 1.7, dt, to, "i32" if n > 1 else "i64")
 
 
-@pytest.mark.parametrize("n", [0, 1, 2, 31, 32, 33, 63, 64, 65, 1024, 1025, 2049, 5000, 8193, 16384, 16385, 40001])
+@pytest.mark.parametrize("n", [0, 1, 2, 31, 32, 33, 63, 64, 65, 1024, 1025, 2049, 5000, 8193, 16384, 16385, 24001, 32768, 32769, 40001])
 @pytest.mark.parametrize("rows", [1, 2, 511, 512, 70000])
 def test_gradient_numbers_of_tokens(n, rows):
     """Orders by rank and in one and two passes; runs within a chunk, over its end, over many chunks."""
