@@ -640,7 +640,7 @@ size_t musapy_distill_loss_scratch_v1(const musapy_distill_args* args);
 int musapy_distill_loss_v1(const musapy_distill_args* args, void* scratch, size_t scratch_bytes, hipStream_t stream);
 int musapy_distill_loss_grad_v1(const musapy_distill_args* args, hipStream_t stream);
 
-/* Logits of the next token, made ready for its choice (fewer than 2^23 tiles of 2048 columns in all rows).  For each row, with c the number of times that a column is among the
+/* Logits of the next token, made ready for its choice.  For each row, with c the number of times that a column is among the
  * first `lengths[row]` (NULL: `length`; cut to 0 .. length) numbers of its history:
  *   z = (z > 0 ? z / repetition : z * repetition) - (frequency * c + presence) where c > 0
  *   z = z + bias
@@ -649,7 +649,7 @@ int musapy_distill_loss_grad_v1(const musapy_distill_args* args, hipStream_t str
  * (NULL) its `_value`.  The bias is a row of `width` values, bias_pitch apart (0: one row for all), or, with `entries`
  * (at most 1024), values for the columns bias_index of each row: an index that is no column has no effect, and
  * biases of one column add up; bias_dtype is `dtype` or F32.  `allowed` is bytes, or 32-bit words whose lowest bits come first, in rows
- * allowed_pitch bytes or words apart (0: one row for all). */
+ * allowed_pitch bytes or words apart (0: one row for all).  Fewer than 2^22 tiles of 2048 columns in all rows. */
 enum { MUSAPY_ALLOWED_BYTES = 0, MUSAPY_ALLOWED_BITS = 1 };
 typedef struct {
   int dtype, out_dtype; /* out_dtype: dtype or F32 */

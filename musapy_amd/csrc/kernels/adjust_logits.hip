@@ -234,7 +234,9 @@ __global__ __launch_bounds__(BLOCK) void k_adjust(AdjustArgs p) {
 
 // The tile: 2048 columns without a history ((256, 131072) bf16 with packed masks and biases into f32 34.6 us, 35.1 with 8192); with one, which
 // every tile reads, 8192 (42.4, with 2048 54.6, for 4096 tokens each), and 4096 where that leaves the chip's 256 CUs few
-// ((4, 32768) f32 4.2 us, with 8192 4.9; (32, 50001) with 30000 tokens 13.8, with 2048 18.1).
+// ((4, 32768) f32 4.2 us, with 8192 4.9; (32, 50001) with 30000 tokens 13.8, with 2048 18.1).  Histories of 128 KB and more are read from
+// the L2 longer than the logits: 16384 there, if that is a workgroup for every CU ((256, 50001) f16 with 30000 tokens of 64 bits
+// 46.5 us, with 8192 63; but with 5000 27.2 and 26.8, and (256, 131072) with 4096 of 32 bits 45.4 and 42.4).
 template <class T, class O>
 int launch_adjust(AdjustArgs& p, bool history, hipStream_t st) {
   auto go = [&](auto HISTORY, auto BLOCK, auto TILE) {
@@ -248,10 +250,13 @@ int launch_adjust(AdjustArgs& p, bool history, hipStream_t st) {
   };
   using Few = std::integral_constant<int, 256>;
   using Many = std::integral_constant<int, 512>;
+  using Most = std::integral_constant<int, 1024>;
   if (!history) {
     p.length = 0;
     return go(std::false_type{}, Few{}, std::integral_constant<int, 2048>{});
   }
+  if (uint64_t(p.length) * (p.history.wide ? 8 : 4) >= 128 * 1024 && p.rows * ((uint64_t(p.width) + 16383) / 16384) >= 256)
+    return go(std::true_type{}, Most{}, std::integral_constant<int, 16384>{});
   if (p.rows * ((uint64_t(p.width) + 8191) / 8192) >= 512) return go(std::true_type{}, Many{}, std::integral_constant<int, 8192>{});
   return go(std::true_type{}, Many{}, std::integral_constant<int, 4096>{});
 }

@@ -76,6 +76,16 @@ def test_numbers_of_rows(rows):
     check(z, "bf16", "f32", allowed=rng.random((rows, 4500)) < 0.5, packed=True, **some(rng, rows, 4500, 20))
 
 
+@pytest.mark.parametrize("dt,to,length,id_dt", [("bf16", "f32", 16384, "i64"), ("f32", "f32", 32768, "i32"), ("f16", "f16", 66000, "i32")])
+def test_many_long_histories(dt, to, length, id_dt):
+    rng = np.random.default_rng(length)
+    rows, width = 130, 16390
+    kw = some(rng, rows, width, length)
+    kw["lengths"][:3] = 0, 1, length
+    check(R.draw(rng, (rows, width), dt, 3.0), dt, to, id_dt=id_dt, allowed=rng.random((rows, width)) < 0.7, packed=True,
+          bias=R.draw(rng, (rows, 5), "f32"), bias_index=rng.integers(-1, width, (rows, 5)), **kw)
+
+
 def test_each_alone():
     rng = np.random.default_rng(1)
     z = R.draw(rng, (4, 999), "f32", 3.0)

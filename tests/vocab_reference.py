@@ -179,10 +179,9 @@ def adjust(z, history=None, repetition=1.0, presence=0.0, frequency=0.0, bias=No
     z = z.astype(np.float64).copy()
     size = np.abs(np.where(np.isfinite(z), z, 0.0))
     if history is not None:
-        for v in np.unique(history):
+        for v, c in zip(*np.unique(history, return_counts=True)):
             if not 0 <= v < len(z):
                 continue
-            c = int((history == v).sum())
             z[v] = z[v] / repetition if z[v] > 0 else z[v] * repetition
             z[v] -= frequency * c + presence
             size[v] = max(size[v], size[v] * repetition, size[v] / repetition) + 2 * (abs(frequency) * c + abs(presence))
