@@ -141,10 +141,12 @@ __device__ inline void order_clear(const OrderArgs& p, uint32_t block) {
   if (threadIdx.x < 16 ? edge < head : edge < p.zero_bytes) p.zero[edge] = 0;
 }
 
-// Up to kRankMost tokens, in one launch: a token's place is the number of tokens in front of it, counted against all others.  All
-// lie in LDS; a workgroup places 16 tokens, and sixteen threads to each count a sixteenth of the others, four at a time.  (With the
-// order in two launches, as below, the gradient of 1584 tokens took 20 us, so 14, and of 4096 25.2, so 21.2.)
-constexpr int kRankBlock = 256, kRankTokens = 16, kRankMost = 4096;
+// Up to 5120 tokens, in one launch: a token's place is the number of tokens in front of it, counted against all others.  All lie in
+// LDS (20 KB a workgroup, so that eight that clear fit a CU); a workgroup places 16 tokens, and sixteen threads to each count a
+// sixteenth of the others, four at a time.  Against two launches, as below: 1584 tokens 20 us, so 14; 5120 of 1024 into (50000,
+// 1024) f32 50.2 and 46.6, but numbers of 64 bits, which every workgroup reads, 52.4, and 4096 of them level.
+constexpr int kRankBlock = 256, kRankTokens = 16;
+inline bool embed_ranks(uint64_t tokens, int id_dtype) { return tokens <= (id_dtype == MUSAPY_DT_I64 ? 4096u : 5120u); }
 
 __global__ __launch_bounds__(kRankBlock) void k_embed_rank(OrderArgs p) {
   if (blockIdx.x >= p.order_blocks) return order_clear<kRankBlock>(p, blockIdx.x - p.order_blocks);
@@ -730,7 +732,7 @@ inline EmbedGradPlan embed_grad_plan(const musapy_embedding_grad_args* a) {
     pl.tiles = uint32_t((n + pl.tile - 1) / pl.tile);
   }
   // Chunks of 8 to 64 tokens that give some 4096 waves (longer ones beyond 131072 tokens): shorter ones keep more rows in flight (20000
-  // tokens of 512 bf16 47 us, so 57 with chunks of 64; 5003 of 1111 f32 57 and 67), longer ones have fewer tokens that cross.
+  // tokens of 512 bf16 take 10 us less than with chunks of 64), longer ones have fewer tokens that cross.
   pl.chunk = 8;
   const uint64_t tiles = (a->width + 255) / 256;
   while ((pl.chunk < 64 && n / pl.chunk * tiles > 4096) || n / pl.chunk > 2048) pl.chunk *= 2;
@@ -743,7 +745,7 @@ inline EmbedGradPlan embed_grad_plan(const musapy_embedding_grad_args* a) {
   };
   pl.keys = take(n * 4);
   pl.pos = take(n * 4);
-  if (n > uint64_t(kRankMost)) {
+  if (!embed_ranks(n, a->id_dtype)) {
     pl.keys2 = take(n * 4);
     pl.pos2 = take(n * 4);
   }
@@ -780,7 +782,7 @@ inline void launch_order(const musapy_embedding_grad_args* a, const EmbedGradPla
     return unsigned(order + (pieces + o.zero_pieces - 1) / o.zero_pieces);
   };
   const uint64_t most = bytes - beside * uint64_t(launches - 1);  // of the first launch
-  if (o.n <= uint32_t(kRankMost)) {
+  if (embed_ranks(o.n, a->id_dtype)) {
     o.keys = keys[0];
     o.pos = pos[0];
     const unsigned count = grid((o.n + kRankTokens - 1) / kRankTokens, kRankBlock, most);

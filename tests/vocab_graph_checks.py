@@ -76,7 +76,7 @@ def same(a, b):
 def check_replays():
     """Replays on new inputs, with eager work between them, give bit for bit what the eager calls give."""
     L = lib()
-    for tokens in (100, N, 17000):  # one block of tokens, several, orders by digits
+    for tokens in (50, 100, N, 9000, 17000, 40000):  # without an order, by rank, by blocks, by digits
         step = Step(L, tokens, tokens)
         graph = captured(step)
         for k in range(4):
@@ -94,7 +94,7 @@ def check_replays():
 def check_two_graphs_on_one_scratch():
     """Graphs of a stream that share the gradient's scratch: it may hold anything."""
     L = lib()
-    a = Step(L, 1, 17000)
+    a = Step(L, 1, 40000)
     b = Step(L, 2, N, a.scratch)
     graphs = captured(a), captured(b)
     for k in range(4):
