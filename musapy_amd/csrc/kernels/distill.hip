@@ -103,20 +103,34 @@ __device__ inline void row_unused(const DistillArgs& p, uint32_t row) {
   for (int i = 0; i < 3; ++i) p.sums[uint64_t(row) * 3 + i] = 0.0f;
 }
 
-// The row's results, by one wave, from its maximum and sums; z0: the logits of the first 64 entries.
-template <class T, int SUMS>
+// The row's results, by one wave, from its maximum and sums; z0: the logits of the first 64 entries.  KR: entries that a lane
+// loads at once ((16384, 4000) with 128 entries 47.5 us, 64 at a time 55.5).
+template <class T, int SUMS, int KR>
 __device__ inline void row_finish(const DistillArgs& p, uint32_t row, int lane, const T* z, const RowTerms& t, float z0, float most, float s, float s1) {
   float a = 0.0f, b = 0.0f, r = -__builtin_inff();
   if (t.soft) {
+    RawEntry raw[KR];
+    uint32_t ki[KR];
+    float kx[KR], ky[KR];
+#pragma unroll
+    for (int k = 1; k < KR; ++k) raw[k] = entry_load(p, row, k * 64 + lane);
+    ki[0] = t.i0;
+    kx[0] = t.x0;
+    ky[0] = z0;
+#pragma unroll
+    for (int k = 1; k < KR; ++k) {
+      entry_of(p, raw[k], k * 64 + lane, ki[k], kx[k]);
+      ky[k] = float(z[ki[k] < p.width ? ki[k] : 0]);
+    }
     auto each = [&](auto fn) {
-      for (uint32_t k0 = 0; k0 < p.entries; k0 += 64) {
-        uint32_t i = t.i0;
-        float x = t.x0, y = z0;
-        if (k0 > 0) {
-          teacher_entry(p, row, k0 + lane, i, x);
-          if (i < p.width) y = float(z[i]);
-        }
-        if (i < p.width) fn(x, y);
+#pragma unroll
+      for (int k = 0; k < KR; ++k)
+        if (ki[k] < p.width) fn(kx[k], ky[k]);
+      for (uint32_t k0 = KR * 64; k0 < p.entries; k0 += 64) {
+        uint32_t i;
+        float x;
+        teacher_entry(p, row, k0 + lane, i, x);
+        if (i < p.width) fn(x, float(z[i]));
       }
     };
     float top = -__builtin_inff();
@@ -151,7 +165,7 @@ __device__ inline void row_finish(const DistillArgs& p, uint32_t row, int lane, 
   sums[2] = t.hard ? ls1 : 0.0f;
 }
 
-template <class T, int BLOCK, int SUMS, bool PART>
+template <class T, int BLOCK, int SUMS, bool PART, int KR>
 __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
   constexpr int N = 16 / int(sizeof(T)), U = 4, kWaves = BLOCK / 64;
   constexpr bool TWO = SUMS != kOne;
@@ -263,12 +277,12 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
     to[1] = s;
     to[2] = s1;
   } else {
-    row_finish<T, SUMS>(p, row, lane, z, terms, z0, most, s, s1);
+    row_finish<T, SUMS, KR>(p, row, lane, z, terms, z0, most, s, s1);
   }
 }
 
 // The segments of a row, at most 64, to a wave.
-template <class T, int SUMS>
+template <class T, int SUMS, int KR>
 __global__ __launch_bounds__(64) void k_distill_join(DistillArgs p) {
   const uint32_t row = blockIdx.x;
   const int lane = threadIdx.x;
@@ -287,7 +301,7 @@ __global__ __launch_bounds__(64) void k_distill_join(DistillArgs p) {
   const float m = there ? m0 : -__FLT_MAX__, most = wave_max(m);
   const float s = wave_sum(there ? s0 * sum_change(m, most, p.c) : 0.0f);
   const float s1 = SUMS != kOne ? wave_sum(there ? s10 * sum_change(m, most, kLog2e) : 0.0f) : 0.0f;
-  row_finish<T, SUMS>(p, row, lane, z, terms, z0, most, s, s1);
+  row_finish<T, SUMS, KR>(p, row, lane, z, terms, z0, most, s, s1);
 }
 
 // A workgroup of one wave takes a segment of a row, four vectors of 16 bytes to a lane: dloss (weight T softmax(z / T) +
@@ -298,8 +312,9 @@ __global__ __launch_bounds__(64) void k_distill_join(DistillArgs p) {
 constexpr int kGradVectors = 4;
 constexpr unsigned grad_lds(uint32_t entries) { return (entries + 1) * 12; }
 
-template <class T, bool SQUARE>
-__global__ __launch_bounds__(64, 8) void k_distill_grad(DistillArgs p) {
+// KR: entries that a lane loads at once, before everything else ((3000, 32000) with 200 entries 101 us, 64 at a time 115).
+template <class T, bool SQUARE, int KR>
+__global__ __launch_bounds__(64, KR > 2 ? 7 : 8) void k_distill_grad(DistillArgs p) {
   constexpr int N = 16 / int(sizeof(T)), U = kGradVectors, kColumns = 64 * U * N;
   __shared__ Vec<uint16_t, N> map[64 * U];  // of the vectors' columns: 0, or 1 + the place in the list
   extern __shared__ uint32_t column[];      // [entries + 1] the list: columns, the entries' exponentials, what is taken off
@@ -323,13 +338,16 @@ __global__ __launch_bounds__(64, 8) void k_distill_grad(DistillArgs p) {
   uint32_t lone = lane < before ? lane : head + vectors * N + (lane - before);
   if (lane >= before && to < vectors) lone = p.width;
   auto vector = [&](int u) { return uint32_t(start + u * 64) + lane; };
-  // The first 64 entries, which are waited for before the logits are asked for: with all loads under way at once (4096, 131072) bf16
+  // The first entries, which are waited for before the logits are asked for: with all loads under way at once (4096, 131072) bf16
   // took 350 us, so 342.
-  const RawEntry e0 = entry_load(p, row, lane);
+  RawEntry raw[KR];
+#pragma unroll
+  for (int k = 0; k < KR; ++k) raw[k] = entry_load(p, row, k * 64 + lane);
   const RawId raw_label = p.labels.at ? id_load(p.labels, row) : RawId{0, 1};
-  uint32_t i0;
-  float x0;
-  entry_of(p, e0, lane, i0, x0);
+  uint32_t ki[KR];
+  float kx[KR];
+#pragma unroll
+  for (int k = 0; k < KR; ++k) entry_of(p, raw[k], k * 64 + lane, ki[k], kx[k]);
   const float dl = p.dloss[int64_t(row) * p.dloss_stride];
   const float m = p.sums[uint64_t(row) * 3];
   const float ls = p.sums[uint64_t(row) * 3 + 1], ls1 = p.sums[uint64_t(row) * 3 + 2];
@@ -345,10 +363,13 @@ __global__ __launch_bounds__(64, 8) void k_distill_grad(DistillArgs p) {
   const bool hard = label < p.width;
   const float ka = dl * p.soft, kb = dl * p.hard, la = ls * kLog2e, lb = ls1 * kLog2e;
   auto each = [&](auto fn) {  // an entry that counts to a lane, or the width in its place
-    for (uint32_t k0 = 0; k0 < p.entries; k0 += 64) {
-      uint32_t i = i0;
-      float x = x0;
-      if (k0 > 0) teacher_entry(p, row, k0 + lane, i, x);
+#pragma unroll
+    for (int k = 0; k < KR; ++k)
+      if (k == 0 || k * 64 < int(p.entries)) fn(ki[k], kx[k]);
+    for (uint32_t k0 = KR * 64; k0 < p.entries; k0 += 64) {
+      uint32_t i;
+      float x;
+      teacher_entry(p, row, k0 + lane, i, x);
       fn(i, x);
     }
   };
@@ -381,14 +402,27 @@ __global__ __launch_bounds__(64, 8) void k_distill_grad(DistillArgs p) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
     uint16_t* place = reinterpret_cast<uint16_t*>(map);
     bool labelled = false;  // whether an entry's column is the label's
+    // Every entry writes its place; one that finds another's there, or has no vector, has the list searched for columns that are
+    // named more than once ((16384, 4000) with 128 entries 68 us, with a search each time 112).
+    for (uint32_t k = lane; k < listed; k += 64)
+      if (column[k] - base < uint32_t(kColumns)) place[column[k] - base] = uint16_t(k + 1);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    bool again = false;
+    for (uint32_t k = lane; k < listed; k += 64)
+      if (column[k] - base >= uint32_t(kColumns) || place[column[k] - base] != k + 1) again = true;
+    const bool search = __ballot(again) != 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
     for (uint32_t k = lane; k < listed; k += 64) {
       const uint32_t i = column[k];
-      float sum = 0.0f;
+      float sum = part[k];
       bool leads = true;
-      for (uint32_t j = 0; j < listed; ++j) {
-        if (column[j] != i) continue;
-        if (j < k) leads = false;
-        sum += part[j];
+      if (search) {
+        sum = 0.0f;
+        for (uint32_t j = 0; j < listed; ++j) {
+          if (column[j] != i) continue;
+          if (j < k) leads = false;
+          sum += part[j];
+        }
       }
       sum = ka * (sum / a);
       if (hard && i == label) {
@@ -531,24 +565,28 @@ int musapy_distill_loss_v1(const musapy_distill_args* a, void* scratch, size_t s
   const bool two = p.labels.at != nullptr && a->temperature != 1.0f;
   vocab_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    auto go = [&](auto SUMS) {
-      constexpr int kS = SUMS.value;
+    auto go = [&](auto SUMS, auto KEPT) {
+      constexpr int kS = SUMS.value, kK = KEPT.value;
       p.segments = distill_segments(p.rows, p.width, sizeof(T));
       if (p.segments > 1) {
         p.parts = static_cast<float*>(scratch);
         p.segment = (p.width / p.segments + 64) / 64 * 64;  // at least width / segments: no more segments than asked for
         p.segments = (p.width + p.segment - 1) / p.segment;
-        k_distill_loss<T, 512, kS, true><<<p.rows * p.segments, 512, 0, st>>>(p);
-        k_distill_join<T, kS><<<p.rows, 64, 0, st>>>(p);
+        k_distill_loss<T, 512, kS, true, 1><<<p.rows * p.segments, 512, 0, st>>>(p);
+        k_distill_join<T, kS, kK><<<p.rows, 64, 0, st>>>(p);
         return;
       }
-      if (block == 64) k_distill_loss<T, 64, kS, false><<<p.rows, 64, 0, st>>>(p);
-      else if (block == 256) k_distill_loss<T, 256, kS, false><<<p.rows, 256, 0, st>>>(p);
-      else k_distill_loss<T, 512, kS, false><<<p.rows, 512, 0, st>>>(p);
+      if (block == 64) k_distill_loss<T, 64, kS, false, kK><<<p.rows, 64, 0, st>>>(p);
+      else if (block == 256) k_distill_loss<T, 256, kS, false, kK><<<p.rows, 256, 0, st>>>(p);
+      else k_distill_loss<T, 512, kS, false, kK><<<p.rows, 512, 0, st>>>(p);
     };
-    if (two && a->temperature == 2.0f) go(std::integral_constant<int, kSquare>{});
-    else if (two) go(std::integral_constant<int, kTwo>{});
-    else go(std::integral_constant<int, kOne>{});
+    auto sums = [&](auto KEPT) {
+      if (two && a->temperature == 2.0f) go(std::integral_constant<int, kSquare>{}, KEPT);
+      else if (two) go(std::integral_constant<int, kTwo>{}, KEPT);
+      else go(std::integral_constant<int, kOne>{}, KEPT);
+    };
+    if (p.entries <= 64) sums(std::integral_constant<int, 1>{});
+    else sums(std::integral_constant<int, 4>{});
   });
   return 0;
 }
@@ -572,8 +610,16 @@ int musapy_distill_loss_grad_v1(const musapy_distill_args* a, hipStream_t st) {
       p.segments = 0;
       return;
     }
-    if (a->temperature == 2.0f) k_distill_grad<T, true><<<unsigned(grid), 64, grad_lds(p.entries), st>>>(p);
-    else k_distill_grad<T, false><<<unsigned(grid), 64, grad_lds(p.entries), st>>>(p);
+    auto go = [&](auto SQUARE, auto KR) {
+      k_distill_grad<T, SQUARE.value, KR.value><<<unsigned(grid), 64, grad_lds(p.entries), st>>>(p);
+    };
+    auto entries = [&](auto SQUARE) {
+      if (p.entries <= 64) go(SQUARE, std::integral_constant<int, 1>{});
+      else if (p.entries <= 128) go(SQUARE, std::integral_constant<int, 2>{});
+      else go(SQUARE, std::integral_constant<int, 4>{});
+    };
+    if (a->temperature == 2.0f) entries(std::true_type{});
+    else entries(std::false_type{});
   });
   if (p.segments == 0) return vocab_bad();
   return 0;

@@ -71,6 +71,20 @@ def test_numbers_of_entries(k):
     check(*inputs(rng, 2, 5000, k, "bf16", "bf16", labelled=False), "bf16", "bf16")
 
 
+@pytest.mark.parametrize("k", [2, 40, 130, 300])
+@pytest.mark.parametrize("dt,width", [("bf16", 4001), ("f32", 4001), ("f16", 2100), ("bf16", 9), ("f32", 5)])
+def test_columns_that_several_entries_name(k, dt, width):
+    """A few columns in all entries, the first and last of the row among them, and the label one of them."""
+    rng = np.random.default_rng(k + width)
+    rows = 9
+    z, _, teacher, label = inputs(rng, rows, width, k, dt, "f32")
+    few = np.stack([rng.choice(np.r_[0, 1, 2, width - 3, width - 2, width - 1, rng.integers(0, width, 20)], 6) for _ in range(rows)])
+    index = np.take_along_axis(few, rng.integers(0, 6, (rows, k)), 1)
+    index[4] = rng.permutation(max(width, k))[:k]  # a row without any, or with some past the width
+    label[::2] = index[::2, 0] % width
+    check(z, index, teacher, label, dt, "f32", 1.5, 0.6)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 600, 2100])
 def test_numbers_of_rows(rows):
     rng = np.random.default_rng(rows)
