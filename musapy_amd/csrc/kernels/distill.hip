@@ -553,10 +553,12 @@ int musapy_distill_loss_v1(const musapy_distill_args* a, void* scratch, size_t s
   DistillArgs p{};
   if (!distill_args(a, false, p)) return vocab_bad();
   if (p.rows == 0) return 0;
-  // The fewest waves a row that fill the chip's 8192, since a row takes some 6 us however short it is ((16384, 4000) bf16 29 us, with
-  // 256 threads a row 45, with 512 91).  But with more than 32 vectors a thread the larger workgroups are level or better.
+  // The fewest waves a row that still fill the chip, since a row takes some 6 us however short it is: one with 2048 rows of up to 16 KB
+  // or 8192 of up to 32 KB (bf16, (5000, 1408) 9.8 us, with four waves 17.0, with eight 30.2; (7500, 8000) 24.5, 25.5 and 42.9), four
+  // with 2048 of up to 128 KB.  With more than 32 vectors a thread the larger workgroups are level or better, and with 1000 rows all are.
   const uint64_t vectors = uint64_t(p.width) * (a->dtype == MUSAPY_DT_F32 ? 4 : 2) / 16;
-  const unsigned block = p.rows >= 8192 && vectors <= 32 * 64 ? 64 : p.rows >= 2048 && vectors <= 32 * 256 ? 256 : 512;
+  const bool one_wave = (p.rows >= 2048 && vectors <= 16 * 64) || (p.rows >= 8192 && vectors <= 32 * 64);
+  const unsigned block = one_wave ? 64 : p.rows >= 2048 && vectors <= 32 * 256 ? 256 : 512;
   if (p.loss == nullptr || p.sums == nullptr || (p.width > 0 && p.logits == nullptr) ||
       (p.entries > 0 && (p.index.at == nullptr || p.teacher == nullptr)) || !grid_fits(p.rows, block))
     return vocab_bad();

@@ -91,6 +91,24 @@ def test_numbers_of_rows(rows):
     check(*inputs(rng, rows, 777, 5, "bf16", "f32"), "bf16", "f32", 1.5, 0.5)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,width", [(2047, 300), (2048, 1), (2048, 9), (2049, 300), (2049, 4003), (2048, 8197), (2048, 33000), (8192, 12001)])
+def test_many_rows(rows, width, dt):
+    """Rows of five kinds, by a wave, four and eight each."""
+    rng = np.random.default_rng(rows + width)
+    k = min(width, 70)
+    z, index, teacher, label = inputs(rng, 5, width, k, dt, "f32")
+    label[1], index[2] = -100, -1
+    kind = rng.integers(0, 5, rows)
+    loss, sums = ms.distill_loss(ms.embedding(R.to_device(z, dt), R.ids(kind)), R.ids(index[kind]), R.to_device(teacher[kind], "f32"),
+                                 R.ids(label[kind]), temperature=1.5, weight=0.5)
+    want = np.array([R.distill(z[r], index[r], teacher[r], label[r], 1.5, 0.5) for r in range(5)])
+    bound = np.array([R.distill_bound(z[r], index[r], teacher[r], label[r], 1.5, 0.5) for r in range(5)])
+    R.within(loss, want[kind, 0], bound[kind, 0], "f32", "loss")
+    for j in (0, 1, 2):
+        R.within(sums.numpy()[:, j].astype(np.float64), want[kind, 1 + j], bound[kind, 1 + j], "f32", f"sums {j}")
+
+
 def test_no_rows():
     z = ms.from_numpy(np.zeros((0, 10), np.float32))
     i, t = ms.from_numpy(np.zeros((0, 2), np.int64)), ms.from_numpy(np.zeros((0, 2), np.float32))

@@ -142,7 +142,7 @@ def test_gradient_is_the_same_from_call_to_call():
 
 @pytest.mark.parametrize("dt,to", [("bf16", "f32"), ("f32", "f32"), ("bf16", "bf16"), ("f16", "f16")])
 @pytest.mark.parametrize("width", [3, 64, 101])
-@pytest.mark.parametrize("n", [0, 300, 20000])
+@pytest.mark.parametrize("n", [0, 40, 300, 6000, 20000])
 def test_gradient_added(dt, to, width, n):
     rng = np.random.default_rng(8)
     rows = 90
