@@ -18,6 +18,7 @@ struct DistillArgs {
   uint32_t rows, width, entries;
   float inv_t;             // 1 / T
   float c;                 // log2(e) / T
+  float near;              // of the loss: logits below it in size take one multiply-add an exponent
   float soft;              // weight T^2; of the gradient, weight T
   float hard;              // 1 - weight
   int use_soft;            // weight is not 0
@@ -67,15 +68,19 @@ __device__ inline uint32_t row_head(const T* row, uint32_t width) {
 //   e_k = exp((v_k - max v) / T),  A = sum e_k,  B = sum e_k ((v_k - max v) - (z_k - r)) / T
 // with r the highest of the entries' logits: all differences are of near numbers, so that logits far from 0 lose nothing.
 //
-// Below kNear, exponents are one multiply-add, x c - round(m c): the sums are then relative to 2^round(m c), and the rounding
-// itself, the same for all terms, is taken off at the end.  Beyond it, where m c or x c may leave f32's range (rows and
-// threads with nothing but -inf or the types' lowest values among them), (x - m) c.
+// For maxima below `near` in size, exponents are one multiply-add, x c - round(m c): the sums are then relative to 2^round(m c), and
+// what m c was rounded by, the same for all terms, is taken off at the end.  That lies in the terms' exponents meanwhile, half a unit of
+// m c's last place at most: `near` is where m c, at T and at 1, reaches 2^24, so that it is 1/2 at most there.  For maxima beyond (rows
+// that a mask of -1e10, the types' lowest value or -inf leaves nothing else, T of 2^-20 with logits above 11) exponents are (x - m) c, a
+// subtraction more, and sums are relative to 2^(m c) itself.
 enum { kOne = 0, kTwo = 1, kSquare = 2 };  // one sum; two; two at T = 2, where exp(z - m) is the square of exp((z - m) / 2)
 
-constexpr float kNear = 1e30f;
+constexpr float kNearExponent = 0x1p24f;
 // what sums relative to the maximum `from` are multiplied with to be relative to `to`
-__device__ inline float sum_change(float from, float to, float c) {
-  return exp2_fast(__builtin_fabsf(to) < kNear ? from * c - to * c : (from - to) * c);
+__device__ inline float sum_change(float from, float to, float c, float near) {
+  const bool a = __builtin_fabsf(from) < near, b = __builtin_fabsf(to) < near;
+  if (a == b) return exp2_fast(b ? from * c - to * c : (from - to) * c);
+  return exp2_fast(b ? __builtin_fmaf(from, c, -(to * c)) : -__builtin_fmaf(to, c, -(from * c)));
 }
 
 // What a wave knows of a row before its logits: the first 64 entries and the label, and which terms the row has.
@@ -151,7 +156,7 @@ __device__ inline void row_finish(const DistillArgs& p, uint32_t row, int lane, 
   }
   if (lane != 0) return;
   auto log_sum = [&](float sum, float c) {
-    const float off = __builtin_fabsf(most) < kNear ? __builtin_fmaf(most, c, -(most * c)) : 0.0f;
+    const float off = __builtin_fabsf(most) < p.near ? __builtin_fmaf(most, c, -(most * c)) : 0.0f;
     return kLn2 * (__builtin_amdgcn_logf(sum) - off);
   };
   const float ls = log_sum(s, p.c), ls1 = SUMS != kOne ? log_sum(s1, kLog2e) : ls;
@@ -207,8 +212,8 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
 
   float m = -__FLT_MAX__, s = 0.0f, s1 = 0.0f;
   auto raise = [&](float high) {
-    s *= sum_change(m, high, p.c);
-    if (TWO) s1 *= sum_change(m, high, kLog2e);
+    s *= sum_change(m, high, p.c, p.near);
+    if (TWO) s1 *= sum_change(m, high, kLog2e, p.near);
     m = high;
   };
   auto one = [&](float w, float w1) {
@@ -217,7 +222,7 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
     if (SUMS == kSquare) s1 = __builtin_fmaf(w, w, s1);
   };
   auto sum = [&](const auto& x, auto COUNT) {
-    if (__builtin_fabsf(m) < kNear) {
+    if (__builtin_fabsf(m) < p.near) {
       const float mc = -(m * p.c), mc1 = -(m * kLog2e);
 #pragma unroll
       for (int e = 0; e < COUNT.value; ++e)
@@ -255,8 +260,8 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
     sum(x, std::integral_constant<int, 1>{});
   }
   float most = wave_max(m);
-  s = wave_sum(s * sum_change(m, most, p.c));
-  if (TWO) s1 = wave_sum(s1 * sum_change(m, most, kLog2e));
+  s = wave_sum(s * sum_change(m, most, p.c, p.near));
+  if (TWO) s1 = wave_sum(s1 * sum_change(m, most, kLog2e, p.near));
   if constexpr (kWaves > 1) {
     if (lane == 0) {
       part[wave][0] = most;
@@ -267,8 +272,8 @@ __global__ __launch_bounds__(BLOCK) void k_distill_loss(DistillArgs p) {
     if (wave != 0) return;
     m = lane < kWaves ? part[lane][0] : -__FLT_MAX__;
     most = wave_max(m);
-    s = wave_sum(lane < kWaves ? part[lane][1] * sum_change(m, most, p.c) : 0.0f);
-    if (TWO) s1 = wave_sum(lane < kWaves ? part[lane][2] * sum_change(m, most, kLog2e) : 0.0f);
+    s = wave_sum(lane < kWaves ? part[lane][1] * sum_change(m, most, p.c, p.near) : 0.0f);
+    if (TWO) s1 = wave_sum(lane < kWaves ? part[lane][2] * sum_change(m, most, kLog2e, p.near) : 0.0f);
   }
   if constexpr (PART) {
     if (lane != 0) return;
@@ -299,8 +304,8 @@ __global__ __launch_bounds__(64) void k_distill_join(DistillArgs p) {
   const float z0 = terms.i0 < p.width ? float(z[terms.i0]) : 0.0f;
   const bool there = uint32_t(lane) < p.segments;
   const float m = there ? m0 : -__FLT_MAX__, most = wave_max(m);
-  const float s = wave_sum(there ? s0 * sum_change(m, most, p.c) : 0.0f);
-  const float s1 = SUMS != kOne ? wave_sum(there ? s10 * sum_change(m, most, kLog2e) : 0.0f) : 0.0f;
+  const float s = wave_sum(there ? s0 * sum_change(m, most, p.c, p.near) : 0.0f);
+  const float s1 = SUMS != kOne ? wave_sum(there ? s10 * sum_change(m, most, kLog2e, p.near) : 0.0f) : 0.0f;
   row_finish<T, SUMS, KR>(p, row, lane, z, terms, z0, most, s, s1);
 }
 
@@ -526,6 +531,7 @@ static bool distill_args(const musapy_distill_args* a, bool grad, DistillArgs& p
   p.entries = uint32_t(a->entries);
   p.inv_t = 1.0f / a->temperature;
   p.c = kLog2e / a->temperature;
+  p.near = kNearExponent / (p.c > kLog2e ? p.c : kLog2e);
   p.soft = a->weight * a->temperature * (grad ? 1.0f : a->temperature);
   p.hard = 1.0f - a->weight;
   p.loss = a->loss;
