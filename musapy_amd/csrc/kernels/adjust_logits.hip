@@ -47,7 +47,7 @@ __device__ inline void count_one(uint32_t* count, uint32_t at) {
 // once.
 constexpr int kPast = 4;
 
-template <class T, class O, class C, bool HISTORY, int BLOCK, int TILE>
+template <class T, class O, class C, bool HISTORY, int BLOCK, int TILE, bool NT>
 __global__ __launch_bounds__(BLOCK) void k_adjust(AdjustArgs p) {
   constexpr int N = 16 / int(sizeof(O)), U = TILE / BLOCK / N;
   static_assert(U > 0 && U * BLOCK * N == TILE, "whole vectors");
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(BLOCK) void k_adjust(AdjustArgs p) {
     Vec<O, N> o;
 #pragma unroll
     for (int e = 0; e < N; ++e) o.v[e] = O((ok >> e) & 1 ? x[u][e] : -__builtin_inff());
-    vstore_el<true, O, N>(out + i, o);
+    vstore_el<NT, O, N>(out + i, o);
   }
   if (behind >= columns) return;
   const bool ok = words ? (words[(first + behind) / 32] >> ((first + behind) % 32)) & 1 : bytes ? bytes[behind] != 0 : true;
@@ -237,6 +237,11 @@ __global__ __launch_bounds__(BLOCK) void k_adjust(AdjustArgs p) {
 // ((4, 32768) f32 4.2 us, with 8192 4.9; (32, 50001) with 30000 tokens 13.8, with 2048 18.1).  Histories of 128 KB and more are read from
 // the L2 longer than the logits: 16384 there, if that is a workgroup for every CU ((256, 50001) f16 with 30000 tokens of 64 bits
 // 46.5 us, with 8192 63; but with 5000 27.2 and 26.8, and (256, 131072) with 4096 of 32 bits 45.4 and 42.4).
+//
+// Results stream from kStreamStoreBytes on, as elsewhere: a smaller one is read by whatever chooses the token while the caches hold it.
+// Alone, the call is as long either way up to some 8 MB and up to a fifth longer with default stores from there; with a reader of
+// the result behind it (a maximum of each row), both together take 13.0 us, streamed 15.8, for (4, 32768) f32 with 500 tokens; 29.6
+// and 41.5 for (16, 131072) bf16 into f32; 35.8 and 48.8 for 64 of them with 500 tokens.
 template <class T, class O>
 int launch_adjust(AdjustArgs& p, bool history, hipStream_t st) {
   auto go = [&](auto HISTORY, auto BLOCK, auto TILE) {
@@ -244,8 +249,10 @@ int launch_adjust(AdjustArgs& p, bool history, hipStream_t st) {
     p.tiles = (p.width + kTile - 1) / kTile;
     const uint64_t grid = uint64_t(p.rows) * p.tiles;
     if (!grid_fits(grid, BLOCK.value)) return vocab_bad();
-    if (p.length < 65536) k_adjust<T, O, uint16_t, HISTORY.value, BLOCK.value, kTile><<<unsigned(grid), BLOCK.value, 0, st>>>(p);
-    else if constexpr (HISTORY.value) k_adjust<T, O, uint32_t, true, BLOCK.value, kTile><<<unsigned(grid), BLOCK.value, 0, st>>>(p);
+    with_store_policy(uint64_t(p.rows) * p.width * sizeof(O) >= kStreamStoreBytes, [&](auto NT) {
+      if (p.length < 65536) k_adjust<T, O, uint16_t, HISTORY.value, BLOCK.value, kTile, NT.value><<<unsigned(grid), BLOCK.value, 0, st>>>(p);
+      else if constexpr (HISTORY.value) k_adjust<T, O, uint32_t, true, BLOCK.value, kTile, NT.value><<<unsigned(grid), BLOCK.value, 0, st>>>(p);
+    });
     return 0;
   };
   using Few = std::integral_constant<int, 256>;

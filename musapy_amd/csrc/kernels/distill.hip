@@ -318,7 +318,10 @@ constexpr int kGradVectors = 4;
 constexpr unsigned grad_lds(uint32_t entries) { return (entries + 1) * 12; }
 
 // KR: entries that a lane loads at once, before everything else ((3000, 32000) with 200 entries 101 us, 64 at a time 115).
-template <class T, bool SQUARE, int KR>
+// NT: streaming stores, from kStreamStoreBytes on, as elsewhere.  Alone, smaller gradients take up to an eighth longer without ((128,
+// 32768) bf16 8.9 us, streamed 7.9; (512, 32768) 15.2 and 14.0), but whatever reads them next finds them in the caches (the two
+// together with a maximum of each row 18.7 and 21.0, 26.9 and 29.3).
+template <class T, bool SQUARE, int KR, bool NT>
 __global__ __launch_bounds__(64, KR > 2 ? 7 : 8) void k_distill_grad(DistillArgs p) {
   constexpr int N = 16 / int(sizeof(T)), U = kGradVectors, kColumns = 64 * U * N;
   __shared__ Vec<uint16_t, N> map[64 * U];  // of the vectors' columns: 0, or 1 + the place in the list
@@ -469,7 +472,7 @@ __global__ __launch_bounds__(64, KR > 2 ? 7 : 8) void k_distill_grad(DistillArgs
       Vec<T, N> o;
 #pragma unroll
       for (int e = 0; e < N; ++e) o.v[e] = T(g[e]);
-      vstore_el<true, T, N>(out + head + uint64_t(at) * N, o);
+      vstore_el<NT, T, N>(out + head + uint64_t(at) * N, o);
     }
     if (lone < p.width) {
       float g = fn(float(z[lone]));
@@ -619,7 +622,9 @@ int musapy_distill_loss_grad_v1(const musapy_distill_args* a, hipStream_t st) {
       return;
     }
     auto go = [&](auto SQUARE, auto KR) {
-      k_distill_grad<T, SQUARE.value, KR.value><<<unsigned(grid), 64, grad_lds(p.entries), st>>>(p);
+      with_store_policy(p.rows * bytes >= kStreamStoreBytes, [&](auto NT) {
+        k_distill_grad<T, SQUARE.value, KR.value, NT.value><<<unsigned(grid), 64, grad_lds(p.entries), st>>>(p);
+      });
     };
     auto entries = [&](auto SQUARE) {
       if (p.entries <= 64) go(SQUARE, std::integral_constant<int, 1>{});

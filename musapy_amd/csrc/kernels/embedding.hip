@@ -414,7 +414,7 @@ struct EmbedGradArgs {
   float scale;
 };
 
-template <class O, int N, bool ADD>
+template <class O, int N, bool ADD, bool NT>
 __device__ inline void embed_store(O* at, int skip, const float (&sum)[N], float scale) {
   if constexpr (ADD) {
 #pragma unroll
@@ -424,17 +424,16 @@ __device__ inline void embed_store(O* at, int skip, const float (&sum)[N], float
     Vec<O, N> v;
 #pragma unroll
     for (int e = 0; e < N; ++e) v.v[e] = O(sum[e] * scale);
-    vstore_el<true, O, N>(at, v);
+    vstore_el<NT, O, N>(at, v);
   }
 }
 
 // A wave sums a chunk of the order over 64 * N columns and stores a row of the
 // table wherever the token changes.  What belongs to a token that the chunk shares with a neighbour goes to a
 // slot in f32.  A row's last columns overlap as in the lookup; `skip` of them are the neighbour's where the
-// store adds to what is there.
-
-
-template <class T, class O, int N, bool ADD>
+// store adds to what is there.  NT: streaming stores, where the table's gradient has kStreamStoreBytes or more, as elsewhere (alone level;
+// 1000 tokens into (5000, 1024) f32 with a maximum of each row behind 22.6 us streamed, 21.5 not; 8000 into (32000, 512) 42.5 and 40.6).
+template <class T, class O, int N, bool ADD, bool NT>
 __global__ __launch_bounds__(kEmbedBlock) void k_embed_sum(EmbedGradArgs p) {
   constexpr int kEmbedRows = N * sizeof(T) > 16 ? 4 : 8;
   const int lane = threadIdx.x % 64;
@@ -460,7 +459,7 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embed_sum(EmbedGradArgs p) {
   auto store = [&](bool goes_on) {
     if (cur < p.rows && active) {
       if (!shared && !goes_on) {
-        embed_store<O, N, ADD>(static_cast<O*>(p.out) + uint64_t(cur) * p.width + col, skip, sum, p.scale);
+        embed_store<O, N, ADD, NT>(static_cast<O*>(p.out) + uint64_t(cur) * p.width + col, skip, sum, p.scale);
       } else {
         float* slot = p.slots + (uint64_t(chunk) * 2 + (shared ? 0 : 1)) * p.padded + col;
         Vec<float, N> v;
@@ -845,8 +844,12 @@ int launch_embedding_grad(const musapy_embedding_grad_args* a, char* ws, hipStre
   const uint64_t units = uint64_t(p.chunks) * p.tiles, grid = (units + 3) / 4;  // (at most 2049 by 2^14)
   launch_order(a, pl, ws, st);
   const dim3 join(pl.chunks, (pl.padded + 255) / 256);
+  const bool nt = a->rows * a->width * sizeof(O) >= kStreamStoreBytes;
   auto go = [&](auto N, auto ADD) {
-    if (grid > 0) k_embed_sum<T, O, N.value, ADD.value><<<unsigned(grid), kEmbedBlock, 0, st>>>(p);
+    if (grid > 0) {
+      if constexpr (ADD.value) k_embed_sum<T, O, N.value, true, false><<<unsigned(grid), kEmbedBlock, 0, st>>>(p);
+      else with_store_policy(nt, [&](auto NT) { k_embed_sum<T, O, N.value, false, NT.value><<<unsigned(grid), kEmbedBlock, 0, st>>>(p); });
+    }
     if (pl.chunks > 1) k_embed_join<O, ADD.value><<<join, kEmbedBlock, 0, st>>>(p);
   };
   using Full = std::integral_constant<int, kN>;
