@@ -576,11 +576,11 @@ int musapy_dropout_v1(const void* a, void* out, int dtype, int ndim, const size_
  *
  * Embedding: out[n] = scale * table[ids[n]]; a number outside [0, rows) is padding: its row is zeros.  `ids` has `tokens`
  * numbers, `out` (tokens, width) is C-contiguous; the table's strides are in elements (groups of 4 or 8 columns of all
- * tokens together fewer than 2^32).
+ * tokens together fewer than 2^32, the 4 or 8 that fill 16 bytes of `out`; in narrower rows every column is a group).
  *
  * Its gradient: out[v] = scale * sum of dy[n] over the n with ids[n] = v, for every row v of the table, zeros where no
  * token is v; with `accumulate` 1 the sums are added to `out` instead, and rows without a token stay as they are.  A row's
- * terms are added in one order that the tokens alone decide: results are the same from call to call.  dy's rows are
+ * terms are added in one order that the tokens, the sizes and the types decide: results are the same from call to call.  dy's rows are
  * unit-stride, dy_pitch elements apart, of at most 2^22 columns.  `scratch` (musapy_embedding_grad_scratch_v1 bytes, 16-byte
  * aligned) is the call's own, of any contents. */
 typedef struct {
@@ -611,7 +611,8 @@ int musapy_embedding_grad_v1(const musapy_embedding_grad_args* args, void* scrat
  *   dlogits = dloss (weight T (q - p) + (1 - weight) (s - one-hot(label)))
  * An entry whose index is no column, or whose value is -inf, does not count; the same index may stand in several
  * entries.  The first term is 0 in a row without entries that count, the second where the label is no column (and
- * both where their factor is 0); the logits of a row without either are not read.  sums (rows, 3) receives the highest
+ * both where their factor is 0); the logits of a row without either have no effect (they are read all the same: rows behind
+ * a batch's last one have to be there).  Temperature and weight are f32, and 1 - weight is that of the f32 weight.  sums (rows, 3) receives the highest
  * logit m, log(sum exp((z - m) / T)) and log(sum exp(z - m)), 0 where a row has no use for one, and the gradient reads it.  A
  * column of -inf has probability 0; a row of nothing else, and one with +inf or NaN, gives NaN.
  * At most 1024 entries; T from 2^-20 to 2^20, weight from 0 to 1.  Rows of logits, indices and values are unit-stride, `*_pitch`

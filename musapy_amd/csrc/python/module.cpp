@@ -683,7 +683,7 @@ PYBIND11_MODULE(_core, m) {
       py::arg("dout"), py::arg("tokens"), py::arg("rows"), py::arg("scale") = 1.0, py::kw_only(), py::arg("dtype") = py::none(),
       py::arg("accumulate") = false, py::arg("out") = nullptr,
       "Gradient of embedding's table, (rows, width): to each token's row, scale times the sum of its rows of dout, in f32 and\n"
-      "in an order that the tokens alone decide; zeros to the others.  accumulate: add to out= instead, rows of\n"
+      "in an order that the tokens, the sizes and the types decide; zeros to the others.  accumulate: add to out= instead, rows of\n"
       "tokens that do not occur stay as they are.  dtype: the result's, out's or dout's when None.");
   m.def(
       "distill_loss",
@@ -701,7 +701,8 @@ PYBIND11_MODULE(_core, m) {
       "A student's loss against a teacher's top entries, and labels: for each row of logits (..., columns), with\n"
       "p = softmax(teacher / T) over the row's entries (at most 1024) and q = softmax(logits / T),\n"
       "  weight T^2 sum_k p_k (log p_k - log q[indices_k]) - (1 - weight) log softmax(logits)[label].\n"
-      "indices (i32 or i64) and teacher (f32, f16 or bf16): (..., entries); an index that is no column and a value of\n"
+      "temperature and weight are taken as f32.  indices (i32 or i64) and teacher (f32, f16 or bf16): (..., entries); an index that is no\n"
+      "column and a value of\n"
       "-inf do not count.  labels (...): a label that is no column does not count.  Returns (loss (...), sums (..., 3)), f32;\n"
       "sums holds each row's highest logit m, log sum exp((z - m) / T) and log sum exp(z - m) for distill_loss_grad.\n"
       "out: a tuple of two arrays or Nones.");
